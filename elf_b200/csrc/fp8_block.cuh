@@ -1,0 +1,97 @@
+// Scaling and conversion of blocks of e4m3 values, shared by the kernels that write or read them.
+#pragma once
+
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace elfb {
+
+// Products by powers of two are exact as long as subnormal inputs and results survive, so they are
+// written out: the library is built with flush-to-zero arithmetic.
+__device__ __forceinline__ float mul_exact(float a, float b) {
+  float r;
+  asm("mul.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+constexpr uint32_t kInfBits = 0x7f800000u;
+
+// Exponent byte of a block whose largest finite magnitude has the bits `amax` (an fp32 pattern):
+// the smallest power of two s with amax <= 448 s.  448 = 1.75 * 2^8, so with amax = m * 2^e the
+// exponent is e - 8 where m <= 1.75 and e - 7 above; subnormal and zero blocks get the smallest
+// scale that is itself a normal number.
+__device__ __forceinline__ uint32_t block_exponent(uint32_t amax) {
+  const int e = int(amax >> 23) - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return uint32_t(e < 1 ? 1 : e);
+}
+// 2^(byte - 127); bytes 0 and 255 (never written here, legal in a tensor from elsewhere) are 2^-127 and NaN
+__device__ __forceinline__ float exponent_value(uint32_t byte) {
+  return __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7fc00000u : byte << 23);
+}
+// 2^(127 - byte) for bytes 1 to 253
+__device__ __forceinline__ float inverse_exponent_value(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+
+// two values to e4m3, round to nearest even: lo in bits 0-7, hi in bits 8-15
+__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d) { return to_e4m3x2(a, b) | (to_e4m3x2(c, d) << 16); }
+__device__ __forceinline__ float2 from_e4m3x2(uint32_t v) {  // exact
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(v)));
+  return __half22float2(*reinterpret_cast<__half2*>(&h));
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// magnitude that counts towards a block's maximum: what is not finite does not
+__device__ __forceinline__ uint32_t finite_bits(float v) {
+  const uint32_t b = abs_bits(v);
+  return b < kInfBits ? b : 0u;
+}
+// a value that is not finite becomes NaN (an infinity would otherwise saturate to a finite 448)
+__device__ __forceinline__ float nan_unless_finite(float scaled, float v) { return abs_bits(v) < kInfBits ? scaled : __uint_as_float(0x7fc00000u); }
+
+// maximum over groups of W consecutive lanes
+template <int W>
+__device__ __forceinline__ uint32_t group_max(uint32_t v) {
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// Scales and converts the N values a lane holds of a 128-column block shared by W consecutive lanes
+// (all 32 lanes of the warp call this).  Returns the block's exponent byte.  Blocks without
+// infinities and NaN, practically all, take the branch without per-value tests.
+template <int N, int W>
+__device__ __forceinline__ uint32_t quantize_block(const float (&v)[N], uint32_t (&out)[N / 4]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) m = max(m, abs_bits(v[j]));
+  m = group_max<W>(m);
+  const bool odd = m >= kInfBits;
+  if (__any_sync(0xffffffffu, odd)) {
+    uint32_t f = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) f = max(f, finite_bits(v[j]));
+    f = group_max<W>(f);
+    const uint32_t byte = block_exponent(f);
+    const float inv = inverse_exponent_value(byte);
+    float s[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) s[j] = nan_unless_finite(mul_exact(v[j], inv), v[j]);
+#pragma unroll
+    for (int j = 0; j < N / 4; ++j) out[j] = to_e4m3x4(s[4 * j], s[4 * j + 1], s[4 * j + 2], s[4 * j + 3]);
+    return byte;
+  }
+  const uint32_t byte = block_exponent(m);
+  const float inv = inverse_exponent_value(byte);
+#pragma unroll
+  for (int j = 0; j < N / 4; ++j)
+    out[j] = to_e4m3x4(mul_exact(v[4 * j], inv), mul_exact(v[4 * j + 1], inv), mul_exact(v[4 * j + 2], inv), mul_exact(v[4 * j + 3], inv));
+  return byte;
+}
+
+}  // namespace elfb

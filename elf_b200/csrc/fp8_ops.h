@@ -1,0 +1,63 @@
+// Host entry points of the block-scaled 8-bit kernels (fp8_ops.cu, fp8_gemm_sm100.cu).
+//
+// A block-scaled matrix holds e4m3 values and one biased exponent byte per block of 128 columns
+// (and 1 or 128 rows): value = data * 2^(byte - 127).
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace elfb {
+
+enum class Elem : int { kBf16 = 0, kF16 = 1, kF32 = 2 };
+
+// x [rows][cols] (pitch ldx elements) -> data [rows][cols] (pitch ldq bytes), scale [rows][ceil(cols/128)] (pitch lds bytes)
+cudaError_t fp8_quantize_rows(const void* x, Elem type, long long ldx, uint8_t* data, long long ldq, uint8_t* scale, long long lds, long long rows,
+                              int cols, cudaStream_t stream);
+// the same with one scale per 128 x 128 tile: scale [ceil(rows/128)][ceil(cols/128)]
+cudaError_t fp8_quantize_tiles(const void* x, Elem type, long long ldx, uint8_t* data, long long ldq, uint8_t* scale, long long lds, long long rows,
+                               int cols, cudaStream_t stream);
+// scale row of matrix row r is r >> row_shift (0 or 7)
+cudaError_t fp8_dequantize(const uint8_t* data, long long ldq, const uint8_t* scale, long long lds, int row_shift, void* y, Elem type, long long ldy,
+                           long long rows, int cols, cudaStream_t stream);
+// h = x + residual (bf16, written when residual is given); data/scale = blocks of h * rstd * w
+cudaError_t fp8_rmsnorm(const void* x, const void* residual, const void* w, void* h, float* rstd, uint8_t* data, long long ldq, uint8_t* scale,
+                        long long lds, long long rows, int dim, float eps, cudaStream_t stream);
+// dact [rows][f] fp32; gu/dgu [rows][2f] block-scaled (f a multiple of 128): the gradient of silu(gate) * up
+cudaError_t fp8_swiglu_backward(const float* dact, long long lda, const uint8_t* gu, long long ldgu, const uint8_t* gu_scale, long long ldgs, uint8_t* dgu,
+                                long long ldd, uint8_t* dgu_scale, long long ldds, long long rows, int f, cudaStream_t stream);
+
+// One operand of a block-scaled product.  Its scale for (row of the product, block of the
+// reduction) is scale[(row >> row_shift) * row_stride + block * block_stride].
+struct Fp8Operand {
+  const uint8_t* data = nullptr;
+  long long ld = 0;  // bytes between consecutive rows in memory, a multiple of 16
+  const uint8_t* scale = nullptr;
+  long long row_stride = 0, block_stride = 0;
+  int row_shift = 0;
+  bool mn_major = false;  // stored [K][MN] instead of [MN][K]
+};
+
+struct Fp8GemmArgs {
+  Fp8Operand a, b;             // a: [M][K]; b: [N][K], or [K][N] when mn_major
+  void* d = nullptr;           // [M][N], pitch ldd elements
+  Elem out = Elem::kBf16;
+  long long ldd = 0;
+  const void* bias = nullptr;  // optional [N], type of d
+  int M = 0, N = 0, K = 0;
+  // gated form: b is [2F][K], N = 2F; d is unused, the activation and the two projections leave in 8 bits
+  bool gated = false;
+  uint8_t* act = nullptr;      // [M][F]
+  long long ld_act = 0;
+  uint8_t* act_scale = nullptr;
+  long long ld_act_scale = 0;
+  uint8_t* gu = nullptr;       // [M][2F], nullptr when no backward pass follows
+  long long ld_gu = 0;
+  uint8_t* gu_scale = nullptr;
+  long long ld_gu_scale = 0;
+  int* status = nullptr;
+};
+// Returns nullptr on success, otherwise a description of the failure.
+const char* fp8_gemm(const Fp8GemmArgs& args, int num_sms, cudaStream_t stream);
+
+}  // namespace elfb

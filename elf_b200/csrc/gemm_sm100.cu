@@ -336,6 +336,25 @@ const char* make_tmap_2d(CUtensorMap* out, const void* ptr, int fmt, uint64_t ro
   return msg;
 }
 
+// Row-major [rows][cols] matrix of bytes, pitch `ld`, for the 8-bit products: 128B swizzle, zero fill.
+const char* make_tmap_bytes(CUtensorMap* out, const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_cols, uint32_t box_rows) {
+  static thread_local bool context_ready = false;  // as in make_tmap_2d
+  if (!context_ready) {
+    cudaFree(nullptr);
+    context_ready = true;
+  }
+  EncodeFn enc = get_encode_fn();
+  if (!enc) return "cuTensorMapEncodeTiled entry point not found";
+  if (((reinterpret_cast<uintptr_t>(ptr) | ld) & 15) != 0) return "8-bit operands must be 16-byte aligned with a 16-byte multiple row pitch";
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {ld};
+  cuuint32_t box[2] = {box_cols, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? nullptr : "cuTensorMapEncodeTiled failed for an 8-bit operand";
+}
+
 // Row-major [rows][cols] output matrix of 16-bit (fmt 0/1) or fp32 (fmt 2) elements for TMA
 // stores / add-reductions: 128-byte swizzled boxes of box_cols x box_rows.
 const char* make_tmap_out(CUtensorMap* out, const void* ptr, int fmt, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_cols,

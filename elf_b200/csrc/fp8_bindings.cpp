@@ -1,6 +1,11 @@
-// torch glue for fp8_ops.cu and fp8_gemm_sm100.cu: checks and stream selection.  Outputs are allocated
-// by the caller (elf_b200/ops/fp8.py), which knows the row pitches the products need.
+// torch glue for fp8_ops.cu and fp8_gemm_sm100.cu: checks, output allocation, stream selection.  The small
+// calls of these operators are bound by what the host does per call, so shapes are taken apart here
+// and not in Python.
 #include <torch/extension.h>
+#include <climits>
+#include <tuple>
+#include <utility>
+#include <vector>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
@@ -20,117 +25,201 @@ elfb::Elem elem_of(const at::Tensor& t, const char* name) {
 }
 
 int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
+int64_t round_up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
-void need_matrix(const at::Tensor& t, const char* name, const at::Device& dev) {
-  TORCH_CHECK(t.is_cuda() && t.device() == dev, name, " must be a CUDA tensor on ", dev);
-  TORCH_CHECK(t.dim() == 2 && (t.stride(1) == 1 || t.size(1) <= 1), name, " must be a matrix with a contiguous last dimension");
-  TORCH_CHECK(t.size(0) <= 1 || t.stride(0) >= t.size(1), name, " must not overlap itself");
-  TORCH_CHECK(t.size(0) <= INT_MAX - 1024 && t.size(1) <= INT_MAX - 1024, name, " is too large");
+// A tensor [..., cols] seen as a matrix with a contiguous last dimension; a copy only where strides force one.
+struct Mat {
+  at::Tensor t;
+  int64_t rows, cols, pitch;  // pitch in elements
+  uint8_t* bytes() const { return static_cast<uint8_t*>(t.data_ptr()); }
+  bool aligned(int64_t to) const { return (reinterpret_cast<uintptr_t>(t.data_ptr()) | uintptr_t(pitch * t.element_size())) % to == 0; }
+};
+
+bool row_pitch(const at::Tensor& t, int64_t* pitch) {
+  const int64_t d = t.dim(), cols = t.size(d - 1);
+  if (cols > 1 && t.stride(d - 1) != 1) return false;
+  *pitch = cols;
+  int64_t expected = 0;  // stride the next dimension outwards must have
+  for (int64_t i = d - 2; i >= 0; --i) {
+    if (t.size(i) == 1) continue;
+    if (expected == 0) {
+      if (t.stride(i) < cols) return false;
+      *pitch = t.stride(i);
+    } else if (t.stride(i) != expected) {
+      return false;
+    }
+    expected = t.stride(i) * t.size(i);
+  }
+  if (expected == 0 && d >= 2 && t.stride(d - 2) > cols) *pitch = t.stride(d - 2);  // a single row
+  return true;
 }
 
-void need_scaled(const at::Tensor& data, const at::Tensor& scale, int64_t row_shift, const char* name, const at::Device& dev) {
-  need_matrix(data, name, dev);
-  need_matrix(scale, "scale", dev);
+Mat matrix(const at::Tensor& t, const char* name, const at::Device& dev, bool may_copy = true) {
+  TORCH_CHECK(t.is_cuda() && t.device() == dev, name, " must be a CUDA tensor on ", dev);
+  TORCH_CHECK(t.dim() >= 1, name, " must have at least one dimension");
+  Mat m{t, 0, t.size(-1), 0};
+  m.rows = 1;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) m.rows *= t.size(i);
+  TORCH_CHECK(m.cols <= INT_MAX - 1024, name, " is too wide");
+  if (t.numel() == 0) {
+    m.pitch = m.cols;
+  } else if (!row_pitch(t, &m.pitch)) {
+    TORCH_CHECK(may_copy, name, " must have a contiguous last dimension and rows that do not overlap");
+    m.t = t.contiguous();
+    m.pitch = m.cols;
+  }
+  return m;
+}
+
+// Block-scaled matrix; scales of rows (row_shift 0) or of tiles of 128 rows (7).
+struct Scaled {
+  Mat data, scale;
+};
+
+Scaled scaled(const at::Tensor& data, const at::Tensor& scale, int64_t row_shift, const char* name, const at::Device& dev, bool may_copy = true) {
   TORCH_CHECK(data.element_size() == 1 && scale.element_size() == 1, name, " must hold 8-bit values and exponents");
   TORCH_CHECK(row_shift == 0 || row_shift == 7, "scales belong to rows or to tiles of 128 rows");
-  const int64_t rows = row_shift ? blocks_of(data.size(0)) : data.size(0);
-  TORCH_CHECK(scale.size(0) == rows && scale.size(1) == blocks_of(data.size(1)), name, ": expected scales [", rows, ", ", blocks_of(data.size(1)), "], got ",
-              scale.sizes());
+  Scaled s{matrix(data, name, dev, may_copy), matrix(scale, "the scales", dev, may_copy)};
+  const int64_t rows = row_shift ? blocks_of(s.data.rows) : s.data.rows;
+  TORCH_CHECK(s.scale.rows == rows && s.scale.cols == blocks_of(s.data.cols), name, ": expected scales [", rows, ", ", blocks_of(s.data.cols), "], got [",
+              s.scale.rows, ", ", s.scale.cols, "]");
+  return s;
 }
 
-uint8_t* bytes(const at::Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
-int64_t pitch(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : std::max<int64_t>(t.stride(0), t.size(1)); }
-
-void quantize(const at::Tensor& x, at::Tensor& data, at::Tensor& scale, bool tiles) {
-  const auto dev = data.device();
-  need_matrix(x, "x", dev);
-  need_scaled(data, scale, tiles ? 7 : 0, "data", dev);
-  TORCH_CHECK(x.sizes() == data.sizes(), "x and data must have the same shape");
-  c10::cuda::CUDAGuard g(dev);
-  auto* fn = tiles ? elfb::fp8_quantize_tiles : elfb::fp8_quantize_rows;
-  check(fn(x.data_ptr(), elem_of(x, "x"), pitch(x), bytes(data), pitch(data), bytes(scale), pitch(scale), x.size(0), int(x.size(1)), cur()), "fp8_quantize");
-}
-
-void dequantize(const at::Tensor& data, const at::Tensor& scale, int64_t row_shift, at::Tensor& out) {
-  const auto dev = data.device();
-  need_scaled(data, scale, row_shift, "data", dev);
-  need_matrix(out, "out", dev);
-  TORCH_CHECK(out.sizes() == data.sizes(), "out and data must have the same shape");
-  c10::cuda::CUDAGuard g(dev);
-  check(elfb::fp8_dequantize(bytes(data), pitch(data), bytes(scale), pitch(scale), int(row_shift), out.data_ptr(), elem_of(out, "out"), pitch(out),
-                             data.size(0), int(data.size(1)), cur()),
-        "fp8_dequantize");
-}
-
-void need_dense_bf16(const at::Tensor& t, const char* name, const at::Device& dev) {
-  TORCH_CHECK(t.is_cuda() && t.device() == dev && t.scalar_type() == at::kBFloat16 && t.is_contiguous(), name, " must be a contiguous bf16 tensor on ", dev);
-  TORCH_CHECK((reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0, name, " must be 16-byte aligned");
-}
-
-// returns (rstd, h): h = x + residual, or x itself without one
-std::tuple<at::Tensor, at::Tensor> rmsnorm(const at::Tensor& x, const at::Tensor& w, double eps, const c10::optional<at::Tensor>& residual, at::Tensor& data,
-                                           at::Tensor& scale) {
-  const auto dev = x.device();
-  TORCH_CHECK(x.dim() == 2, "x must be a matrix");
-  need_dense_bf16(x, "x", dev);
-  need_dense_bf16(w, "weight", dev);
-  need_scaled(data, scale, 0, "data", dev);
-  TORCH_CHECK(x.sizes() == data.sizes() && w.numel() == x.size(1), "x, data and weight do not match");
-  TORCH_CHECK(x.size(1) % 8 == 0 && x.size(1) <= 8192, "the norm's width must be a multiple of 8, at most 8192");
-  TORCH_CHECK(pitch(data) % 8 == 0 && (reinterpret_cast<uintptr_t>(data.data_ptr()) & 7) == 0, "data must have 8-byte aligned rows");
-  c10::cuda::CUDAGuard g(dev);
-  at::Tensor h = x;
-  const void* res = nullptr;
-  if (residual.has_value() && residual->defined()) {
-    need_dense_bf16(*residual, "residual", dev);
-    TORCH_CHECK(residual->sizes() == x.sizes(), "residual must match x");
-    h = at::empty_like(x);
-    res = residual->data_ptr();
+// New tensor whose rows are `pitch` elements apart.
+at::Tensor new_rows(at::IntArrayRef lead, int64_t cols, int64_t pitch, const at::TensorOptions& opt) {
+  std::vector<int64_t> sizes(lead.begin(), lead.end()), strides(lead.size() + 1);
+  sizes.push_back(cols);
+  strides.back() = 1;
+  int64_t step = pitch;
+  for (int64_t i = int64_t(lead.size()) - 1; i >= 0; --i) {
+    strides[i] = step;
+    step *= std::max<int64_t>(sizes[i], 1);
   }
-  auto rstd = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
-  check(elfb::fp8_rmsnorm(x.data_ptr(), res, w.data_ptr(), res ? h.data_ptr() : nullptr, rstd.data_ptr<float>(), bytes(data), pitch(data), bytes(scale),
-                          pitch(scale), x.size(0), int(x.size(1)), float(eps), cur()),
-        "fp8_rmsnorm");
-  return {rstd, h};
+  return at::empty_strided(sizes, strides, opt);
 }
 
-void swiglu_bwd(const at::Tensor& dact, const at::Tensor& gu, const at::Tensor& gu_scale, at::Tensor& dgu, at::Tensor& dgu_scale) {
-  const auto dev = dact.device();
-  need_matrix(dact, "dact", dev);
-  need_scaled(gu, gu_scale, 0, "gate_up", dev);
-  need_scaled(dgu, dgu_scale, 0, "d_gate_up", dev);
-  const int64_t f = dact.size(1);
-  TORCH_CHECK(dact.scalar_type() == at::kFloat && f % 128 == 0, "dact must be fp32, its width a multiple of 128");
-  TORCH_CHECK(gu.size(0) == dact.size(0) && gu.size(1) == 2 * f && gu.sizes() == dgu.sizes(), "gate_up does not match dact");
-  for (const at::Tensor* t : {&dact, &gu, &static_cast<const at::Tensor&>(dgu)})
-    TORCH_CHECK((pitch(*t) * t->element_size()) % 16 == 0 && (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) == 0, "rows must be 16-byte aligned");
+// Block-scaled tensor [*lead, cols] with the row pitches the products want.
+std::pair<at::Tensor, at::Tensor> new_scaled(at::IntArrayRef lead, int64_t cols, bool tiles, const at::Device& dev) {
+  const auto opt = at::TensorOptions().device(dev);
+  const int64_t tile_rows[1] = {tiles ? blocks_of(lead[0]) : 0};
+  return {new_rows(lead, cols, round_up(cols, 16), opt.dtype(at::kFloat8_e4m3fn)),
+          new_rows(tiles ? at::IntArrayRef(tile_rows, 1) : lead, blocks_of(cols), round_up(blocks_of(cols), 4), opt.dtype(at::kByte))};
+}
+
+at::IntArrayRef lead_of(const at::Tensor& t) { return t.sizes().slice(0, t.dim() - 1); }
+
+std::pair<at::Tensor, at::Tensor> quantize(const at::Tensor& x, bool tiles, const c10::optional<at::Tensor>& data_out, const c10::optional<at::Tensor>& scale_out) {
+  const auto dev = x.device();
+  const Mat m = matrix(x, "x", dev);
+  TORCH_CHECK(!tiles || x.dim() == 2, "only matrices have tiles");
   c10::cuda::CUDAGuard g(dev);
-  check(elfb::fp8_swiglu_backward(dact.data_ptr<float>(), pitch(dact), bytes(gu), pitch(gu), bytes(gu_scale), pitch(gu_scale), bytes(dgu), pitch(dgu),
-                                  bytes(dgu_scale), pitch(dgu_scale), dact.size(0), int(f), cur()),
-        "fp8_swiglu_backward");
+  std::pair<at::Tensor, at::Tensor> q;
+  if (data_out.has_value()) {
+    TORCH_CHECK(scale_out.has_value() && data_out->sizes() == x.sizes(), "data must have the shape of x and come with its scales");
+    q = {*data_out, *scale_out};
+  } else {
+    q = new_scaled(lead_of(x), m.cols, tiles, dev);
+  }
+  const Scaled s = scaled(q.first, q.second, tiles ? 7 : 0, "data", dev, false);
+  auto* fn = tiles ? elfb::fp8_quantize_tiles : elfb::fp8_quantize_rows;
+  check(fn(m.t.data_ptr(), elem_of(x, "x"), m.pitch, s.data.bytes(), s.data.pitch, s.scale.bytes(), s.scale.pitch, m.rows, int(m.cols), cur()), "fp8_quantize");
+  return q;
 }
 
-elfb::Fp8Operand operand(const at::Tensor& data, const at::Tensor& scale, int64_t row_shift, bool mn_major, const char* name, const at::Device& dev) {
-  need_scaled(data, scale, row_shift, name, dev);
+at::Tensor dequantize(const at::Tensor& data, const at::Tensor& scale, int64_t row_shift, at::ScalarType dtype, const c10::optional<at::Tensor>& out) {
+  const auto dev = data.device();
+  const Scaled s = scaled(data, scale, row_shift, "data", dev);
+  c10::cuda::CUDAGuard g(dev);
+  at::Tensor y = out.has_value() ? *out : at::empty(data.sizes(), at::TensorOptions().device(dev).dtype(dtype));
+  TORCH_CHECK(y.sizes() == data.sizes(), "out must have the shape of data");
+  const Mat m = matrix(y, "out", dev, false);
+  check(elfb::fp8_dequantize(s.data.bytes(), s.data.pitch, s.scale.bytes(), s.scale.pitch, int(row_shift), y.data_ptr(), elem_of(y, "out"), m.pitch,
+                             s.data.rows, int(s.data.cols), cur()),
+        "fp8_dequantize");
+  return y;
+}
+
+at::Tensor dense_bf16(const at::Tensor& t, const char* name, const at::Device& dev) {
+  TORCH_CHECK(t.is_cuda() && t.device() == dev && t.scalar_type() == at::kBFloat16, name, " must be a bf16 tensor on ", dev);
+  const at::Tensor c = t.contiguous();
+  return (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15) == 0 ? c : c.clone();
+}
+
+// returns (data, scale, rstd, h): h = x + residual, or x itself without one
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> rmsnorm(const at::Tensor& x_in, const at::Tensor& w_in, double eps,
+                                                                   const c10::optional<at::Tensor>& residual) {
+  const auto dev = x_in.device();
+  c10::cuda::CUDAGuard g(dev);
+  TORCH_CHECK(x_in.dim() >= 1, "x must have at least one dimension");
+  const at::Tensor x = dense_bf16(x_in, "x", dev), w = dense_bf16(w_in, "weight", dev);
+  const int64_t dim = x.size(-1);
+  TORCH_CHECK(w.numel() == dim && dim % 8 == 0 && dim > 0 && dim <= 8192, "the norm's width must match the weight's and be a multiple of 8, at most 8192");
+  const int64_t rows = x.numel() / dim;
+  at::Tensor h = x_in, res;
+  if (residual.has_value()) {
+    TORCH_CHECK(residual->sizes() == x.sizes(), "residual must match x");
+    res = dense_bf16(*residual, "residual", dev);
+    h = at::empty(x.sizes(), x.options());
+  }
+  auto q = new_scaled(lead_of(x), dim, false, dev);
+  auto rstd = at::empty(lead_of(x), x.options().dtype(at::kFloat));
+  const Scaled s = scaled(q.first, q.second, 0, "data", dev, false);
+  check(elfb::fp8_rmsnorm(x.data_ptr(), res.defined() ? res.data_ptr() : nullptr, w.data_ptr(), res.defined() ? h.data_ptr() : nullptr, rstd.data_ptr<float>(),
+                          s.data.bytes(), s.data.pitch, s.scale.bytes(), s.scale.pitch, rows, int(dim), float(eps), cur()),
+        "fp8_rmsnorm");
+  return {q.first, q.second, rstd, h};
+}
+
+// d silu(gate) up for dact [..., F] fp32 and gate | up = gu [..., 2F]
+std::pair<at::Tensor, at::Tensor> swiglu_bwd(const at::Tensor& dact, const at::Tensor& gu, const at::Tensor& gu_scale) {
+  const auto dev = dact.device();
+  c10::cuda::CUDAGuard g(dev);
+  const Mat d = matrix(dact, "dact", dev);
+  const Scaled s = scaled(gu, gu_scale, 0, "gate_up", dev);
+  TORCH_CHECK(dact.scalar_type() == at::kFloat && d.cols % 128 == 0, "dact must be fp32, its width a multiple of 128");
+  TORCH_CHECK(s.data.rows == d.rows && s.data.cols == 2 * d.cols, "gate_up does not match dact");
+  TORCH_CHECK(d.aligned(16) && s.data.aligned(16), "rows must be 16-byte aligned");
+  auto q = new_scaled(lead_of(gu), s.data.cols, false, dev);
+  const Scaled o = scaled(q.first, q.second, 0, "d_gate_up", dev, false);
+  check(elfb::fp8_swiglu_backward(static_cast<const float*>(d.t.data_ptr()), d.pitch, s.data.bytes(), s.data.pitch, s.scale.bytes(), s.scale.pitch, o.data.bytes(),
+                                  o.data.pitch, o.scale.bytes(), o.scale.pitch, d.rows, int(d.cols), cur()),
+        "fp8_swiglu_backward");
+  return q;
+}
+
+// An operand of a product and the tensors that keep its memory alive until the launch is queued.
+struct Operand {
+  Scaled s;
   elfb::Fp8Operand o;
-  o.data = bytes(data);
-  o.ld = pitch(data);
-  TORCH_CHECK(o.ld % 16 == 0 && (reinterpret_cast<uintptr_t>(o.data) & 15) == 0, name, " must have 16-byte aligned rows");
-  o.scale = bytes(scale);
-  o.mn_major = mn_major;
+};
+
+Operand operand(const at::Tensor& data, const at::Tensor& scale, int64_t row_shift, bool mn_major, const char* name, const at::Device& dev) {
+  Operand r{scaled(data, scale, row_shift, name, dev), {}};
+  TORCH_CHECK(r.s.data.rows <= INT_MAX - 1024, name, " has too many rows");
+  if (!r.s.data.aligned(16)) {  // TMA wants rows on 16-byte boundaries: a copy with padded rows
+    const int64_t lead[1] = {r.s.data.rows};
+    at::Tensor padded = new_rows(at::IntArrayRef(lead, 1), r.s.data.cols, round_up(r.s.data.cols, 16), data.options());
+    padded.copy_(r.s.data.t.dim() == 2 ? r.s.data.t : r.s.data.t.reshape({r.s.data.rows, r.s.data.cols}));
+    r.s.data = matrix(padded, name, dev, false);
+  }
+  r.o.data = r.s.data.bytes();
+  r.o.ld = round_up(r.s.data.pitch, 16);  // (a single row may have any pitch)
+  r.o.scale = r.s.scale.bytes();
+  r.o.mn_major = mn_major;
   if (mn_major) {
     // stored [K][MN]: a row of the product is a column of the matrix, so scales of single rows would
     // change inside a block of the reduction
     TORCH_CHECK(row_shift == 7, name, " must be scaled in tiles of 128 x 128 to be used transposed");
-    o.row_shift = 7;
-    o.row_stride = 1;
-    o.block_stride = pitch(scale);
+    r.o.row_shift = 7;
+    r.o.row_stride = 1;
+    r.o.block_stride = r.s.scale.pitch;
   } else {
-    o.row_shift = int(row_shift);
-    o.row_stride = pitch(scale);
-    o.block_stride = 1;
+    r.o.row_shift = int(row_shift);
+    r.o.row_stride = r.s.scale.pitch;
+    r.o.block_stride = 1;
   }
-  return o;
+  return r;
 }
 
 int sm_count(const at::Device& dev) { return at::cuda::getDeviceProperties(dev.index())->multiProcessorCount; }
@@ -140,73 +229,95 @@ int* status_ptr(const at::Tensor& status, const at::Device& dev) {
   return status.data_ptr<int>();
 }
 
-// d = a . b^T (b [N, K]), or a . b (b_mn_major, b [K, N])
-void gemm(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& b, const at::Tensor& b_scale, int64_t b_row_shift, bool b_mn_major, at::Tensor& d,
-          const c10::optional<at::Tensor>& bias, const at::Tensor& status) {
-  const auto dev = d.device();
+// a . b^T (b [N, K]), or a . b (b_mn_major, b [K, N]); a [..., K]
+at::Tensor gemm(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& b, const at::Tensor& b_scale, int64_t b_row_shift, bool b_mn_major,
+                at::ScalarType dtype, const c10::optional<at::Tensor>& bias, const at::Tensor& status) {
+  const auto dev = a.device();
   c10::cuda::CUDAGuard guard(dev);
-  need_matrix(d, "out", dev);
+  const Operand oa = operand(a, a_scale, 0, false, "the activation", dev), ob = operand(b, b_scale, b_row_shift, b_mn_major, "the weight", dev);
   elfb::Fp8GemmArgs g;
-  g.a = operand(a, a_scale, 0, false, "a", dev);
-  g.b = operand(b, b_scale, b_row_shift, b_mn_major, "b", dev);
-  g.M = int(d.size(0));
-  g.N = int(d.size(1));
-  g.K = int(a.size(1));
-  TORCH_CHECK(a.size(0) == g.M && b.size(b_mn_major ? 1 : 0) == g.N && b.size(b_mn_major ? 0 : 1) == g.K, "shapes do not match");
+  g.a = oa.o;
+  g.b = ob.o;
+  g.M = int(oa.s.data.rows);
+  g.K = int(oa.s.data.cols);
+  g.N = int(b_mn_major ? ob.s.data.cols : ob.s.data.rows);
+  TORCH_CHECK(g.K == (b_mn_major ? ob.s.data.rows : ob.s.data.cols), "the operands disagree on the reduction length");
+  auto sizes = a.sizes().vec();
+  sizes.back() = g.N;
+  at::Tensor d = at::empty(sizes, at::TensorOptions().device(dev).dtype(dtype));
   g.d = d.data_ptr();
-  g.ldd = pitch(d);
-  g.out = elem_of(d, "out");
-  if (bias.has_value() && bias->defined()) {
-    TORCH_CHECK(bias->device() == dev && bias->scalar_type() == d.scalar_type() && bias->dim() == 1 && bias->numel() == g.N && bias->is_contiguous(),
-                "bias must be a contiguous [N] tensor of the output's dtype");
+  g.ldd = g.N;
+  g.out = elem_of(d, "the product");
+  if (bias.has_value()) {
+    TORCH_CHECK(bias->device() == dev && bias->scalar_type() == dtype && bias->dim() == 1 && bias->numel() == g.N && bias->is_contiguous(),
+                "the bias must be a contiguous [N] tensor of the product's dtype");
     g.bias = bias->data_ptr();
   }
   g.status = status_ptr(status, dev);
+  // from the caching allocator, call by call: two streams or two captured graphs never share it
+  at::Tensor workspace;
+  if (const size_t bytes = elfb::fp8_gemm_workspace(g, sm_count(dev))) {
+    workspace = at::empty({int64_t(bytes)}, at::TensorOptions().device(dev).dtype(at::kByte));
+    g.workspace = workspace.data_ptr();
+  }
   const char* err = elfb::fp8_gemm(g, sm_count(dev), cur());
   TORCH_CHECK(err == nullptr, "elf_b200 fp8_gemm: ", err);
+  return d;
 }
 
-// act [M, F] = silu(gate) * up for gate | up = a . b^T (b [2F, K]); gu (and its scales) may be None
-void gated(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& b, const at::Tensor& b_scale, int64_t b_row_shift, at::Tensor& act,
-           at::Tensor& act_scale, const c10::optional<at::Tensor>& gu, const c10::optional<at::Tensor>& gu_scale, const at::Tensor& status) {
-  const auto dev = act.device();
+// act [..., F] = silu(gate) * up for gate | up = a . b^T (b [2F, K]); returns (act, act_scale, gate_up, its scales), the last two undefined unless `keep`
+std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>> gated(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& b,
+                                                                                               const at::Tensor& b_scale, int64_t b_row_shift, bool keep,
+                                                                                               const at::Tensor& status) {
+  const auto dev = a.device();
   c10::cuda::CUDAGuard guard(dev);
-  need_scaled(act, act_scale, 0, "act", dev);
+  const Operand oa = operand(a, a_scale, 0, false, "the activation", dev), ob = operand(b, b_scale, b_row_shift, false, "the weight", dev);
   elfb::Fp8GemmArgs g;
-  g.a = operand(a, a_scale, 0, false, "a", dev);
-  g.b = operand(b, b_scale, b_row_shift, false, "b", dev);
-  g.M = int(act.size(0));
-  g.N = int(b.size(0));
-  g.K = int(a.size(1));
-  TORCH_CHECK(a.size(0) == g.M && b.size(1) == g.K && 2 * act.size(1) == g.N, "shapes do not match");
+  g.a = oa.o;
+  g.b = ob.o;
+  g.M = int(oa.s.data.rows);
+  g.K = int(oa.s.data.cols);
+  g.N = int(ob.s.data.rows);
+  TORCH_CHECK(g.K == ob.s.data.cols, "the operands disagree on the reduction length");
+  TORCH_CHECK(g.N % 256 == 0, "the width of gate and of up must be a multiple of 128");
+  auto act = new_scaled(lead_of(a), g.N / 2, false, dev);
+  const Scaled sa = scaled(act.first, act.second, 0, "act", dev, false);
   g.gated = true;
-  g.act = bytes(act);
-  g.ld_act = pitch(act);
-  g.act_scale = bytes(act_scale);
-  g.ld_act_scale = pitch(act_scale);
-  if (gu.has_value() && gu->defined()) {
-    TORCH_CHECK(gu_scale.has_value(), "gate_up needs its scales");
-    need_scaled(*gu, *gu_scale, 0, "gate_up", dev);
-    TORCH_CHECK(gu->size(0) == g.M && gu->size(1) == g.N, "gate_up does not match the weights");
-    g.gu = bytes(*gu);
-    g.ld_gu = pitch(*gu);
-    g.gu_scale = bytes(*gu_scale);
-    g.ld_gu_scale = pitch(*gu_scale);
+  g.act = sa.data.bytes();
+  g.ld_act = sa.data.pitch;
+  g.act_scale = sa.scale.bytes();
+  g.ld_act_scale = sa.scale.pitch;
+  c10::optional<at::Tensor> gu_data, gu_scale;
+  if (keep) {
+    auto gu = new_scaled(lead_of(a), g.N, false, dev);
+    const Scaled sg = scaled(gu.first, gu.second, 0, "gate_up", dev, false);
+    g.gu = sg.data.bytes();
+    g.ld_gu = sg.data.pitch;
+    g.gu_scale = sg.scale.bytes();
+    g.ld_gu_scale = sg.scale.pitch;
+    gu_data = gu.first;
+    gu_scale = gu.second;
   }
   g.status = status_ptr(status, dev);
+  // from the caching allocator, call by call: two streams or two captured graphs never share it
+  at::Tensor workspace;
+  if (const size_t bytes = elfb::fp8_gemm_workspace(g, sm_count(dev))) {
+    workspace = at::empty({int64_t(bytes)}, at::TensorOptions().device(dev).dtype(at::kByte));
+    g.workspace = workspace.data_ptr();
+  }
   const char* err = elfb::fp8_gemm(g, sm_count(dev), cur());
   TORCH_CHECK(err == nullptr, "elf_b200 fp8_gated: ", err);
+  return {act.first, act.second, gu_data, gu_scale};
 }
 
 }  // namespace
 
 void register_fp8(pybind11::module_& m) {
-  m.def("fp8_quantize", &quantize, py::arg("x"), py::arg("data"), py::arg("scale"), py::arg("tiles"));
-  m.def("fp8_dequantize", &dequantize, py::arg("data"), py::arg("scale"), py::arg("row_shift"), py::arg("out"));
-  m.def("fp8_rmsnorm", &rmsnorm, py::arg("x"), py::arg("w"), py::arg("eps"), py::arg("residual"), py::arg("data"), py::arg("scale"));
-  m.def("fp8_swiglu_bwd", &swiglu_bwd, py::arg("dact"), py::arg("gu"), py::arg("gu_scale"), py::arg("dgu"), py::arg("dgu_scale"));
-  m.def("fp8_gemm", &gemm, py::arg("a"), py::arg("a_scale"), py::arg("b"), py::arg("b_scale"), py::arg("b_row_shift"), py::arg("b_mn_major"), py::arg("d"),
+  m.def("fp8_quantize", &quantize, py::arg("x"), py::arg("tiles"), py::arg("data") = c10::nullopt, py::arg("scale") = c10::nullopt);
+  m.def("fp8_dequantize", &dequantize, py::arg("data"), py::arg("scale"), py::arg("row_shift"), py::arg("dtype"), py::arg("out") = c10::nullopt);
+  m.def("fp8_rmsnorm", &rmsnorm, py::arg("x"), py::arg("w"), py::arg("eps"), py::arg("residual") = c10::nullopt);
+  m.def("fp8_swiglu_bwd", &swiglu_bwd, py::arg("dact"), py::arg("gu"), py::arg("gu_scale"));
+  m.def("fp8_gemm", &gemm, py::arg("a"), py::arg("a_scale"), py::arg("b"), py::arg("b_scale"), py::arg("b_row_shift"), py::arg("b_mn_major"), py::arg("dtype"),
         py::arg("bias"), py::arg("status"));
-  m.def("fp8_gated", &gated, py::arg("a"), py::arg("a_scale"), py::arg("b"), py::arg("b_scale"), py::arg("b_row_shift"), py::arg("act"), py::arg("act_scale"),
-        py::arg("gu"), py::arg("gu_scale"), py::arg("status"));
+  m.def("fp8_gated", &gated, py::arg("a"), py::arg("a_scale"), py::arg("b"), py::arg("b_scale"), py::arg("b_row_shift"), py::arg("keep"), py::arg("status"));
 }

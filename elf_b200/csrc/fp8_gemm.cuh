@@ -1,0 +1,213 @@
+// What the two kernels of the block-scaled products (one CTA, CTA pair) share: scale words, epilogues.
+#pragma once
+
+#include <type_traits>
+
+#include "fp8_block.cuh"
+#include "fp8_ops.h"
+#include "sm100_ptx.cuh"
+
+namespace elfb {
+namespace fp8 {
+
+constexpr int BM = 128;  // rows per CTA
+constexpr int BK = 128;  // bytes = values; one scale block
+constexpr int UMMA_K = 32;
+constexpr int BOX_BYTES = 128 * BK;  // 16 KiB: 128 rows of an operand
+constexpr int TMEM_COLS = 512;
+constexpr int SF_COL = 480;  // two 16-column scale slots: A's 4 columns, then B's
+
+struct Scales {
+  const uint8_t* p;
+  long long row_stride, block_stride;
+  int row_shift;
+  bool words;  // the bytes of four consecutive blocks can be read as one aligned word
+  explicit Scales(const Fp8Operand& o)
+      : p(o.scale), row_stride(o.row_stride), block_stride(o.block_stride), row_shift(o.row_shift),
+        words(o.block_stride == 1 && o.row_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(o.scale) & 3) == 0) {}
+};
+
+struct Params {
+  int M, N, K;
+  Scales sa, sb;
+  void* d;
+  long long ldd;
+  const void* bias;
+  bool vec;  // D may be stored in 16-byte pieces
+  // gated form
+  uint8_t *act, *act_scale, *gu, *gu_scale;
+  long long ld_act, ld_act_scale, ld_gu, ld_gu_scale;
+  int* status;
+};
+
+// Exponent bytes of blocks 4g .. 4g+3 for rows row0 + lane, + 32, + 64, + 96 of an operand, as they come from
+// memory: nothing here looks at a loaded value, so a warp issues the loads of all operands and goes on
+// (combining them at once cost the products 10 to 30 % of their time, waiting for this warp).
+struct RawScales {
+  uint32_t v[4][4];  // [row][byte]; aligned words: [row][0]; one scale for all 128 rows: [0]
+};
+// Rows and blocks that do not exist read the last that does: what they scale is zero, or never used.
+__device__ __forceinline__ void load_scales(const Scales& s, int row0, int rows, int g, int blocks, int lane, RawScales& r) {
+  const bool word = s.words && 4 * g + 4 <= blocks;
+  const int n = s.row_shift ? 1 : 4;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (j < n) {
+      const int row = s.row_shift ? min(row0, rows - 1) >> 7 : min(row0 + 32 * j + lane, rows - 1);
+      const uint8_t* p = s.p + (long long)row * s.row_stride;
+      if (word) {
+        r.v[j][0] = *reinterpret_cast<const uint32_t*>(p + 4 * g);
+      } else {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) r.v[j][b] = p[(long long)min(4 * g + b, blocks - 1) * s.block_stride];
+      }
+    }
+  }
+}
+__device__ __forceinline__ void combine_scales(const Scales& s, int g, int blocks, const RawScales& r, uint32_t (&w)[4]) {
+  const bool word = s.words && 4 * g + 4 <= blocks;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t(&v)[4] = r.v[s.row_shift ? 0 : j];
+    w[j] = word ? v[0] : v[0] | v[1] << 8 | v[2] << 16 | v[3] << 24;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float bias_at(const void* bias, int col) {
+  const T v = static_cast<const T*>(bias)[col];
+  if constexpr (sizeof(T) == 4) return v;
+  else if constexpr (std::is_same<T, __half>::value) return __half2float(v);
+  else return __bfloat162float(v);
+}
+
+// D[row, col .. col+32) = v (+ bias)
+template <typename T>
+__device__ __forceinline__ void store_chunk(const uint32_t (&v)[32], int row, int col, const Params& p) {
+  if (row >= p.M) return;
+  T* dst = static_cast<T*>(p.d) + (long long)row * p.ldd + col;
+  float f[32];
+#pragma unroll
+  for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
+  if (p.bias != nullptr) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (col + j < p.N) f[j] += bias_at<T>(p.bias, col + j);
+  }
+  if (p.vec && col + 32 <= p.N) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(dst + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; j += 8) {
+        uint4 o;
+        if constexpr (std::is_same<T, __half>::value)
+          o = make_uint4(pack_f16x2(f[j], f[j + 1]), pack_f16x2(f[j + 2], f[j + 3]), pack_f16x2(f[j + 4], f[j + 5]), pack_f16x2(f[j + 6], f[j + 7]));
+        else
+          o = make_uint4(pack_bf16x2(f[j], f[j + 1]), pack_bf16x2(f[j + 2], f[j + 3]), pack_bf16x2(f[j + 4], f[j + 5]), pack_bf16x2(f[j + 6], f[j + 7]));
+        *reinterpret_cast<uint4*>(dst + j) = o;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      if (col + j < p.N) {
+        if constexpr (sizeof(T) == 4) dst[j] = f[j];
+        else if constexpr (std::is_same<T, __half>::value) dst[j] = __float2half_rn(f[j]);
+        else dst[j] = __float2bfloat16_rn(f[j]);
+      }
+    }
+  }
+}
+
+// 16 values times 2^(127 - byte) to e4m3
+__device__ __forceinline__ void scale_and_store(const uint32_t (&v)[16], float inv, uint8_t* dst) {
+  uint32_t q[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float s[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float x = __uint_as_float(v[4 * j + k]);
+      s[k] = nan_unless_finite(mul_exact(x, inv), x);
+    }
+    q[j] = to_e4m3x4(s[0], s[1], s[2], s[3]);
+  }
+  *reinterpret_cast<uint4*>(dst) = make_uint4(q[0], q[1], q[2], q[3]);
+}
+
+// One tile of the gated form: columns 0..127 of the accumulator are gate, 128..255 up.  One thread per
+// row.  `release` is called once the 32 columns shared with the other accumulator have been read for
+// the last time (ACC 0: the end of up, ACC 1: the beginning of gate).
+//   first sweep (with a checkpoint): the maxima of the row's gate and up blocks
+//   second sweep: gate and up leave in 8 bits, silu(gate) * up collects in 128 registers
+//   then the activation's block is scaled and leaves
+template <int ACC, typename Release>
+__device__ __forceinline__ void gated_tile(uint32_t taddr, int row, int f0, int f, const Params& p, Release&& release) {
+  const bool live = row < p.M;
+  const bool keep = p.gu != nullptr;
+  uint32_t top[2] = {0, 0};
+  uint32_t v[16];
+  if (keep) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        tmem_ld_32x32b_x16(taddr + half * 128 + c * 16, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) top[half] = max(top[half], finite_bits(__uint_as_float(v[j])));
+      }
+    }
+  }
+  const uint32_t byte_g = block_exponent(top[0]), byte_u = block_exponent(top[1]);
+  const float inv_g = inverse_exponent_value(byte_g), inv_u = inverse_exponent_value(byte_u);
+  uint8_t* gate_dst = p.gu + (long long)row * p.ld_gu + f0;
+  float act[128];
+  uint32_t top_act = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    constexpr int kFirst = ACC == 0 ? 7 : 0, kStep = ACC == 0 ? -1 : 1;
+    const int c = kFirst + kStep * i;
+    tmem_ld_32x32b_x16(taddr + c * 16, v);
+    tmem_ld_wait();
+    if (live && keep) scale_and_store(v, inv_g, gate_dst + c * 16);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float g = __uint_as_float(v[j]);
+      act[c * 16 + j] = g * __fdividef(1.f, 1.f + __expf(-g));
+    }
+    tmem_ld_32x32b_x16(taddr + 128 + c * 16, v);
+    tmem_ld_wait();
+    if (i == 1) release();
+    if (live && keep) scale_and_store(v, inv_u, gate_dst + f + c * 16);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      act[c * 16 + j] *= __uint_as_float(v[j]);
+      top_act = max(top_act, finite_bits(act[c * 16 + j]));
+    }
+  }
+  const uint32_t byte = block_exponent(top_act);
+  if (!live) return;
+  uint8_t* dst = p.act + (long long)row * p.ld_act + f0;
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(act[c * 16 + j]);
+    scale_and_store(v, inverse_exponent_value(byte), dst + c * 16);
+  }
+  p.act_scale[(long long)row * p.ld_act_scale + f0 / 128] = uint8_t(byte);
+  if (keep) {
+    uint8_t* s = p.gu_scale + (long long)row * p.ld_gu_scale;
+    s[f0 / 128] = uint8_t(byte_g);
+    s[(f + f0) / 128] = uint8_t(byte_u);
+  }
+}
+
+// The layout tcgen05.cp wants: 16 bytes per lane, word j for row 32 j + lane.
+__device__ __forceinline__ void store_scale_words(uint32_t smem, int lane, const uint32_t (&w)[4]) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(smem + lane * 16), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+}
+}  // namespace fp8
+}  // namespace elfb

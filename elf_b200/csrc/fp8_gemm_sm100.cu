@@ -21,50 +21,20 @@
 // TMEM has 512 columns; two 256-column accumulators would leave none for the scales.  The second one
 // therefore starts 32 columns early and shares them with the first; the epilogue reads the shared
 // columns first and the next tile's products start as soon as it has.
-#include <cstdio>
-
-#include "fp8_block.cuh"
-#include "fp8_ops.h"
-#include "gemm_sm100.h"
-#include "sm100_ptx.cuh"
+#include "fp8_gemm.cuh"
 
 namespace elfb {
 
 namespace fp8 {
 
-constexpr int BM = 128;
-constexpr int BK = 128;  // bytes = values; one scale block
 constexpr int STAGES = 4;
-constexpr int UMMA_K = 32;
-constexpr int BOX_BYTES = 128 * BK;  // 16 KiB: 128 rows of A, or of one half of B
 constexpr int NUM_THREADS = 320;
-constexpr int TMEM_COLS = 512;
-constexpr int SF_COL = 480;  // two 16-column scale slots: A's 4 columns, then B's
-constexpr int GROUP_M = 8;   // tiles of GROUP_M consecutive M-blocks share B panels in L2
+constexpr int GROUP_M = 8;  // tiles of GROUP_M consecutive M-blocks share B panels in L2
 
 template <int BN>
 constexpr int kStageBytes = BOX_BYTES * (1 + BN / 128);
 template <int BN>
 constexpr size_t kSmemBytes = size_t(STAGES) * kStageBytes<BN> + 1024 /*align slack*/ + 256 /*barriers*/;
-
-struct Scales {
-  const uint8_t* p;
-  long long row_stride, block_stride;
-  int row_shift;
-};
-
-struct Params {
-  int M, N, K;
-  Scales sa, sb;
-  void* d;
-  long long ldd;
-  const void* bias;
-  bool vec;  // D may be stored in 16-byte pieces
-  // gated form
-  uint8_t *act, *act_scale, *gu, *gu_scale;
-  long long ld_act, ld_act_scale, ld_gu, ld_gu_scale;
-  int* status;
-};
 
 struct Tile {
   int m0, n0, n1;  // first row of A; first rows of B's two 128-row halves
@@ -87,149 +57,6 @@ __device__ __forceinline__ Tile tile_at(int t, int tiles_m, int tiles_n, int f) 
     r.n1 = r.n0 + 128;
   }
   return r;
-}
-
-// exponent bytes of blocks 4g .. 4g+3 for one row; rows and blocks that do not exist get 2^0
-__device__ __forceinline__ uint32_t scale_word(const Scales& s, int row, int rows, int g, int blocks) {
-  if (row >= rows) return 0x7f7f7f7fu;
-  const uint8_t* p = s.p + (long long)(row >> s.row_shift) * s.row_stride + (long long)(4 * g) * s.block_stride;
-  if (s.block_stride == 1 && 4 * g + 4 <= blocks && (reinterpret_cast<uintptr_t>(p) & 3) == 0) return *reinterpret_cast<const uint32_t*>(p);
-  uint32_t w = 0;
-#pragma unroll
-  for (int b = 0; b < 4; ++b) w |= (4 * g + b < blocks ? uint32_t(p[b * s.block_stride]) : 0x7fu) << (8 * b);
-  return w;
-}
-
-template <typename T>
-__device__ __forceinline__ float bias_at(const void* bias, int col) {
-  const T v = static_cast<const T*>(bias)[col];
-  if constexpr (sizeof(T) == 4) return v;
-  else if constexpr (std::is_same<T, __half>::value) return __half2float(v);
-  else return __bfloat162float(v);
-}
-
-// D[row, col .. col+32) = v (+ bias)
-template <typename T>
-__device__ __forceinline__ void store_chunk(const uint32_t (&v)[32], int row, int col, const Params& p) {
-  if (row >= p.M) return;
-  T* dst = static_cast<T*>(p.d) + (long long)row * p.ldd + col;
-  float f[32];
-#pragma unroll
-  for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
-  if (p.bias != nullptr) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (col + j < p.N) f[j] += bias_at<T>(p.bias, col + j);
-  }
-  if (p.vec && col + 32 <= p.N) {
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(dst + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; j += 8) {
-        uint4 o;
-        if constexpr (std::is_same<T, __half>::value)
-          o = make_uint4(pack_f16x2(f[j], f[j + 1]), pack_f16x2(f[j + 2], f[j + 3]), pack_f16x2(f[j + 4], f[j + 5]), pack_f16x2(f[j + 6], f[j + 7]));
-        else
-          o = make_uint4(pack_bf16x2(f[j], f[j + 1]), pack_bf16x2(f[j + 2], f[j + 3]), pack_bf16x2(f[j + 4], f[j + 5]), pack_bf16x2(f[j + 6], f[j + 7]));
-        *reinterpret_cast<uint4*>(dst + j) = o;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      if (col + j < p.N) {
-        if constexpr (sizeof(T) == 4) dst[j] = f[j];
-        else if constexpr (std::is_same<T, __half>::value) dst[j] = __float2half_rn(f[j]);
-        else dst[j] = __float2bfloat16_rn(f[j]);
-      }
-    }
-  }
-}
-
-// 16 values times 2^(127 - byte) to e4m3
-__device__ __forceinline__ void scale_and_store(const uint32_t (&v)[16], float inv, uint8_t* dst) {
-  uint32_t q[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    float s[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float x = __uint_as_float(v[4 * j + k]);
-      s[k] = nan_unless_finite(mul_exact(x, inv), x);
-    }
-    q[j] = to_e4m3x4(s[0], s[1], s[2], s[3]);
-  }
-  *reinterpret_cast<uint4*>(dst) = make_uint4(q[0], q[1], q[2], q[3]);
-}
-
-// One tile of the gated form: columns 0..127 of the accumulator are gate, 128..255 up.  One thread per
-// row.  `release` is called once the 32 columns shared with the other accumulator have been read for
-// the last time (ACC 0: the end of up, ACC 1: the beginning of gate).
-//   first sweep (with a checkpoint): the maxima of the row's gate and up blocks
-//   second sweep: gate and up leave in 8 bits, silu(gate) * up collects in 128 registers
-//   then the activation's block is scaled and leaves
-template <int ACC, typename Release>
-__device__ __forceinline__ void gated_tile(uint32_t taddr, int row, int f0, int f, const Params& p, Release&& release) {
-  const bool live = row < p.M;
-  const bool keep = p.gu != nullptr;
-  uint32_t top[2] = {0, 0};
-  uint32_t v[16];
-  if (keep) {
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        tmem_ld_32x32b_x16(taddr + half * 128 + c * 16, v);
-        tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < 16; ++j) top[half] = max(top[half], finite_bits(__uint_as_float(v[j])));
-      }
-    }
-  }
-  const uint32_t byte_g = block_exponent(top[0]), byte_u = block_exponent(top[1]);
-  const float inv_g = inverse_exponent_value(byte_g), inv_u = inverse_exponent_value(byte_u);
-  uint8_t* gate_dst = p.gu + (long long)row * p.ld_gu + f0;
-  float act[128];
-  uint32_t top_act = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    constexpr int kFirst = ACC == 0 ? 7 : 0, kStep = ACC == 0 ? -1 : 1;
-    const int c = kFirst + kStep * i;
-    tmem_ld_32x32b_x16(taddr + c * 16, v);
-    tmem_ld_wait();
-    if (live && keep) scale_and_store(v, inv_g, gate_dst + c * 16);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float g = __uint_as_float(v[j]);
-      act[c * 16 + j] = g * __fdividef(1.f, 1.f + __expf(-g));
-    }
-    tmem_ld_32x32b_x16(taddr + 128 + c * 16, v);
-    tmem_ld_wait();
-    if (i == 1) release();
-    if (live && keep) scale_and_store(v, inv_u, gate_dst + f + c * 16);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      act[c * 16 + j] *= __uint_as_float(v[j]);
-      top_act = max(top_act, finite_bits(act[c * 16 + j]));
-    }
-  }
-  const uint32_t byte = block_exponent(top_act);
-  if (!live) return;
-  uint8_t* dst = p.act + (long long)row * p.ld_act + f0;
-#pragma unroll
-  for (int c = 0; c < 8; ++c) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(act[c * 16 + j]);
-    scale_and_store(v, inverse_exponent_value(byte), dst + c * 16);
-  }
-  p.act_scale[(long long)row * p.ld_act_scale + f0 / 128] = uint8_t(byte);
-  if (keep) {
-    uint8_t* s = p.gu_scale + (long long)row * p.ld_gu_scale;
-    s[f0 / 128] = uint8_t(byte_g);
-    s[(f + f0) / 128] = uint8_t(byte_u);
-  }
 }
 
 template <int BN, bool B_MN, bool GATED, typename T>
@@ -409,34 +236,39 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     }
   } else {
     // ------------------------------------------------------------------ scale writers (warps 6..9)
-    const uint32_t quarter = uint32_t(warp & 3);
-    uint32_t count = 0;
-    bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const Tile tile = tile_at<BN, GATED>(t, tiles_m, tiles_n, f);
-      for (int g = 0; 4 * g < k_blocks; ++g, ++count) {
-        uint32_t a[4], b0[4], b1[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          a[j] = scale_word(p.sa, tile.m0 + 32 * j + lane, p.M, g, k_blocks);
-          b0[j] = scale_word(p.sb, tile.n0 + 32 * j + lane, p.N, g, k_blocks);
-          b1[j] = BN == 256 ? scale_word(p.sb, tile.n1 + 32 * j + lane, p.N, g, k_blocks) : 0u;
-        }
-        const int slot = count & 1;
-        if (!mbar_wait(sf_empty_bar(slot), ((count >> 1) & 1u) ^ 1u, abort_flag)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after_sync();
-        const uint32_t dst = tmem_base + (quarter * 32u << 16) + SF_COL + slot * 16;
-        tmem_st_32x32b_x4(dst, a);
-        tmem_st_32x32b_x4(dst + 4, b0);
-        if (BN == 256) tmem_st_32x32b_x4(dst + 8, b1);
-        tmem_st_wait();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(sf_full_bar(slot));
+    // The words of the next group are fetched before the slot of this one is waited for.
+    const int quarter = warp & 3;
+    int t = blockIdx.x, g = 0;
+    Tile tile = tile_at<BN, GATED>(t, tiles_m, tiles_n, f);
+    RawScales ra, rb0, rb1;
+    auto load = [&] {
+      load_scales(p.sa, tile.m0, p.M, g, k_blocks, lane, ra);
+      load_scales(p.sb, tile.n0, p.N, g, k_blocks, lane, rb0);
+      if (BN == 256) load_scales(p.sb, tile.n1, p.N, g, k_blocks, lane, rb1);
+    };
+    if (t < tiles) load();
+    for (uint32_t count = 0; t < tiles; ++count) {
+      uint32_t a[4], b0[4], b1[4];
+      combine_scales(p.sa, g, k_blocks, ra, a);
+      combine_scales(p.sb, g, k_blocks, rb0, b0);
+      if (BN == 256) combine_scales(p.sb, g, k_blocks, rb1, b1);
+      if (4 * ++g >= k_blocks) {
+        g = 0;
+        t += gridDim.x;
+        if (t < tiles) tile = tile_at<BN, GATED>(t, tiles_m, tiles_n, f);
       }
+      if (t < tiles) load();
+      const int slot = count & 1;
+      if (!mbar_wait(sf_empty_bar(slot), ((count >> 1) & 1u) ^ 1u, abort_flag)) break;
+      tc_fence_after_sync();
+      const uint32_t dst = tmem_base + (uint32_t(quarter) * 32u << 16) + SF_COL + slot * 16;
+      tmem_st_32x32b_x4(dst, a);
+      tmem_st_32x32b_x4(dst + 4, b0);
+      if (BN == 256) tmem_st_32x32b_x4(dst + 8, b1);
+      tmem_st_wait();
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sf_full_bar(slot));
     }
   }
 
@@ -494,7 +326,18 @@ cudaError_t dispatch(const Fp8GemmArgs& g, const CUtensorMap& ta, const CUtensor
   return launch<BN, false, false, float>(ta, tb, p, num_sms, s);
 }
 
+cudaError_t launch_pair(const Fp8GemmArgs& g, const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int num_sms, cudaStream_t stream);
+size_t pair_workspace(int M, int N, int K, bool gated, int num_sms);
+
+// Few rows leave most of a 256-row tile empty.
+bool use_pair(const Fp8GemmArgs& g, int num_sms) { return num_sms >= 2 && g.M > 128; }
+
 }  // namespace fp8
+
+size_t fp8_gemm_workspace(const Fp8GemmArgs& g, int num_sms) {
+  if (g.M <= 0 || g.N <= 0 || g.K <= 0 || !fp8::use_pair(g, num_sms)) return 0;
+  return fp8::pair_workspace(g.M, g.N, g.K, g.gated, num_sms);
+}
 
 const char* make_tmap_bytes(CUtensorMap* out, const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_cols, uint32_t box_rows);
 
@@ -507,10 +350,7 @@ const char* fp8_gemm(const Fp8GemmArgs& g, int num_sms, cudaStream_t stream) {
   if (g.b.mn_major) err = make_tmap_bytes(&tb, g.b.data, uint64_t(g.K), uint64_t(g.N), uint64_t(g.b.ld), 128, BK);
   else              err = make_tmap_bytes(&tb, g.b.data, uint64_t(g.N), uint64_t(g.K), uint64_t(g.b.ld), BK, 128);
   if (err) return err;
-  Params p{};
-  p.M = g.M, p.N = g.N, p.K = g.K;
-  p.sa = {g.a.scale, g.a.row_stride, g.a.block_stride, g.a.row_shift};
-  p.sb = {g.b.scale, g.b.row_stride, g.b.block_stride, g.b.row_shift};
+  Params p{g.M, g.N, g.K, Scales(g.a), Scales(g.b)};
   p.status = g.status;
   cudaError_t e;
   if (g.gated) {
@@ -519,12 +359,13 @@ const char* fp8_gemm(const Fp8GemmArgs& g, int num_sms, cudaStream_t stream) {
     if (!aligned(g.act, g.ld_act) || (g.gu && !aligned(g.gu, g.ld_gu))) return "8-bit outputs must be 16-byte aligned with a 16-byte multiple row pitch";
     p.act = g.act, p.act_scale = g.act_scale, p.gu = g.gu, p.gu_scale = g.gu_scale;
     p.ld_act = g.ld_act, p.ld_act_scale = g.ld_act_scale, p.ld_gu = g.ld_gu, p.ld_gu_scale = g.ld_gu_scale;
-    e = launch<256, false, true, __nv_bfloat16>(ta, tb, p, num_sms, stream);
+    e = use_pair(g, num_sms) ? launch_pair(g, ta, tb, p, num_sms, stream) : launch<256, false, true, __nv_bfloat16>(ta, tb, p, num_sms, stream);
   } else {
     const long long esz = g.out == Elem::kF32 ? 4 : 2;
     p.d = g.d, p.ldd = g.ldd, p.bias = g.bias;
     p.vec = ((reinterpret_cast<uintptr_t>(g.d) | uintptr_t(g.ldd * esz)) & 15) == 0;
-    e = g.N > 128 ? dispatch<256>(g, ta, tb, p, num_sms, stream) : dispatch<128>(g, ta, tb, p, num_sms, stream);
+    if (use_pair(g, num_sms)) e = launch_pair(g, ta, tb, p, num_sms, stream);
+    else e = g.N > 128 ? dispatch<256>(g, ta, tb, p, num_sms, stream) : dispatch<128>(g, ta, tb, p, num_sms, stream);
   }
   return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
 }

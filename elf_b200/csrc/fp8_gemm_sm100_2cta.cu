@@ -1,0 +1,493 @@
+// CTA-pair kernel of the block-scaled products: two CTAs on neighbouring SMs share a 256 x 256 tile
+// through tcgen05.mma.cta_group::2.
+//
+// Why pairs: a 128 x 256 tile on one CTA fetches 48 KiB for 512 cycles of 8-bit MMA, 25 TB/s over the chip,
+// which is more than L2 delivers; the pair fetches 32 KiB per CTA in the same time (each its own 128 rows
+// of A and half of B).  4096 x 4096 x 14336: 249 us with single CTAs.
+//
+// Roles per CTA as in fp8_gemm_sm100.cu.  The even CTA's MMA thread issues for both.  Barriers:
+//   full[s]      even CTA: armed with both CTAs' bytes, both CTAs' copies complete on it; for the first of two
+//                stages both CTAs' scale warps arrive too, when their words lie in shared memory
+//   empty[s/2]   one per CTA, committed to both once for two stages: a commit costs about as much as a step
+//                of MMA (two single commits per stage instead: 218 us against 200 in the loop alone)
+//   acc_full[a]  one per CTA, committed to both
+//   acc_free     even CTA: the epilogue warps of both arrive once the columns the two accumulators share
+//                have been read (8 arrivals per unit)
+//
+// The tiles of a last, partly filled wave are split along K into units on different pairs.  Every unit but
+// the last to finish leaves its fp32 sums in a workspace; the last one adds all parts in their order, so
+// results do not depend on who that is.  Nobody waits for another unit.
+#include "fp8_gemm.cuh"
+
+namespace elfb {
+namespace fp8 {
+namespace pair {
+
+constexpr int BN = 256;
+constexpr int STAGES = 6;
+constexpr int STAGE_BYTES = 2 * BOX_BYTES;  // per CTA: 128 rows of A, 128 rows of B
+constexpr int SLOTS = STAGES / 2;           // two consecutive stages are freed by one commit
+constexpr int NUM_THREADS = 224;
+constexpr int SF_BYTES = 3 * 512;           // scale words of a slot: 128 rows of A, 256 columns of B
+constexpr int GROUP_M = 4;  // tile rows (of 256) that are swept together before moving to the next columns
+constexpr int ACC1 = 224;   // first column of the second accumulator: shares 32 with the first
+constexpr size_t SMEM_BYTES = size_t(STAGES) * STAGE_BYTES + SLOTS * SF_BYTES + 1024 /*align slack*/ + 256 /*barriers*/;
+constexpr int PART_FLOATS = BM * BN;  // one CTA's half of a tile in the workspace
+
+struct Schedule {
+  int tiles_m, tiles_n, full_tiles, ksplit, total_units;
+};
+
+struct Unit {
+  int m0, n0;    // first row of this pair's tile; first column (gated: of gate)
+  int kb0, kb1;  // blocks of the reduction
+  int part;      // index among the parts of its tile
+  int rest;      // index of its tile among the split tiles, -1 for a whole one
+};
+
+__device__ __forceinline__ Unit unit_at(int u, const Schedule& s, int k_blocks, int width) {
+  Unit r;
+  int tile = u;
+  r.kb0 = 0, r.kb1 = k_blocks, r.part = 0, r.rest = -1;
+  if (u >= s.full_tiles) {
+    const int rem = (s.total_units - s.full_tiles) / s.ksplit;  // parts of one tile are `rem` units apart: other pairs
+    const int v = u - s.full_tiles;
+    r.rest = v % rem;
+    r.part = v / rem;
+    tile = s.full_tiles + r.rest;
+    if (s.ksplit == 1) {
+      r.rest = -1;
+    } else {  // whole groups of four blocks, which share scale words
+      const int groups = (k_blocks + 3) / 4;
+      r.kb0 = 4 * int((long long)groups * r.part / s.ksplit);
+      r.kb1 = min(k_blocks, 4 * int((long long)groups * (r.part + 1) / s.ksplit));
+    }
+  }
+  const int per_group = GROUP_M * s.tiles_n;
+  const int group = tile / per_group;
+  const int first_m = group * GROUP_M;
+  const int rows = min(GROUP_M, s.tiles_m - first_m);
+  const int in_group = tile - group * per_group;
+  r.m0 = (first_m + in_group % rows) * 2 * BM;
+  r.n0 = (in_group / rows) * width;
+  return r;
+}
+
+// whether `ok` holds for all `threads` threads at the barrier
+__device__ __forceinline__ bool named_barrier_all(uint32_t id, uint32_t threads, bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred P, Q;\n\t"
+      "setp.ne.u32 P, %3, 0;\n\t"
+      "barrier.cta.red.and.pred Q, %1, %2, P;\n\t"
+      "selp.u32 %0, 1, 0, Q;\n\t"
+      "}\n"
+      : "=r"(r)
+      : "r"(id), "r"(threads), "r"(uint32_t(ok))
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void umma_ss_mxf8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+      "}\n"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+
+// Arrival on a barrier of the other CTA without the release, which waits for every earlier memory operation of
+// the thread at cluster scope: 1250 cycles, against the 1024 that the MMAs of a slot take.  The words it
+// announces are shared memory of this CTA, made visible to the tensor core's copy by the proxy fence before it.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// arrive on the barrier at this offset in both CTAs once all MMAs issued so far have completed
+__device__ __forceinline__ void umma_commit_both(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(uint16_t(3)) : "memory");
+}
+
+template <bool B_MN, bool GATED, typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
+fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ Params p,
+                     const __grid_constant__ Schedule sched, float* __restrict__ parts, unsigned int* __restrict__ parts_done) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem_aligned = smem_raw + (smem_base - smem_u32(smem_raw));
+  const uint32_t sf_base = smem_base + STAGES * STAGE_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_aligned + size_t(STAGES) * STAGE_BYTES + SLOTS * SF_BYTES);
+  const uint32_t bar0 = smem_u32(bars);
+  auto full_bar = [&](int s) { return bar0 + 8u * s; };
+  auto empty_bar = [&](int slot) { return bar0 + 8u * (STAGES + slot); };
+  auto acc_full_bar = [&](int a) { return bar0 + 8u * (2 * STAGES + a); };
+  const uint32_t acc_free_bar = bar0 + 8u * (2 * STAGES + 2);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 3);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile unsigned int* arrived = tmem_slot + 2;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t cta = cluster_ctarank();  // 0 = leader
+  const bool leader = cta == 0;
+  const int pair_id = blockIdx.x >> 1;
+  const int num_pairs = gridDim.x >> 1;
+  const int f = p.N / 2;  // gated: width of the activation
+  const int width = GATED ? 128 : BN;
+  const int k_blocks = (p.K + BK - 1) / BK;
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < STAGES; ++s) mbar_init(full_bar(s), s & 1 ? 1 : 3);  // a slot's first stage also waits for both scale warps
+    for (int s = 0; s < SLOTS; ++s) mbar_init(empty_bar(s), 1);
+    mbar_init(acc_free_bar, 8);
+    for (int a = 0; a < 2; ++a) mbar_init(acc_full_bar(a), 1);
+    fence_barrier_init();
+    prefetch_tensormap(&tmap_a);
+    prefetch_tensormap(&tmap_b);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(tmem_slot), TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers are initialised before anyone touches the peer's
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer (both CTAs)
+    if (lane == 0) {
+      int slot = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int u = pair_id; u < sched.total_units && ok; u += num_pairs) {
+        const Unit unit = unit_at(u, sched, k_blocks, width);
+        const int m0 = unit.m0 + int(cta) * BM;
+        // this CTA's 128 rows of B; gated: gate in the even CTA, up in the odd one.  Boxes behind the last row arrive as zeros.
+        const int n0 = unit.n0 + int(cta) * (GATED ? f : 128);
+        for (int kb2 = unit.kb0; kb2 < unit.kb1; kb2 += 2) {
+          if (!mbar_wait(empty_bar(slot), phase ^ 1u, abort_flag)) {
+            ok = false;
+            break;
+          }
+          for (int kb = kb2; kb < min(kb2 + 2, unit.kb1); ++kb) {
+            const int stage = 2 * slot + (kb - kb2);
+            const uint32_t sa = smem_base + stage * STAGE_BYTES, sb = sa + BOX_BYTES;
+            const uint32_t bar = map_to_cta(full_bar(stage), 0);
+            if (leader) mbar_arrive_expect_tx(full_bar(stage), 2 * STAGE_BYTES);
+            const int k0 = kb * BK;
+            tma_load_2d_pair(sa, &tmap_a, bar, k0, m0);
+            if (B_MN) tma_load_2d_pair(sb, &tmap_b, bar, n0, k0);
+            else tma_load_2d_pair(sb, &tmap_b, bar, k0, n0);
+          }
+          if (++slot == SLOTS) {
+            slot = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer (leader only)
+    if (leader && lane == 0) {
+      constexpr uint32_t B_KSTEP = B_MN ? UMMA_K * 128 : UMMA_K;  // see fp8_gemm_sm100.cu; one 128-wide box per CTA
+      int slot = 0;
+      uint32_t sf_count = 0;
+      bool ok = true;
+      int i = 0;  // units of this pair so far
+      uint32_t stage_phase = 0;  // bit s: parity of stage s (a unit with an odd number of blocks leaves half a slot unused)
+      for (int u = pair_id; u < sched.total_units && ok; u += num_pairs, ++i) {
+        const Unit unit = unit_at(u, sched, k_blocks, width);
+        const int acc = i & 1;
+        if (i > 0 && !mbar_wait(acc_free_bar, uint32_t(i - 1) & 1u, abort_flag)) break;
+        tc_fence_after_sync();
+        const uint32_t tmem_d = tmem_base + acc * ACC1;
+        for (int kb2 = unit.kb0; kb2 < unit.kb1 && ok; kb2 += 2) {
+          const uint32_t sfa = tmem_base + SF_COL + (sf_count++ & 1) * 16, sfb = sfa + 4;
+          for (int kb = kb2; kb < min(kb2 + 2, unit.kb1); ++kb) {
+            const int stage = 2 * slot + (kb - kb2);
+            if (!mbar_wait(full_bar(stage), (stage_phase >> stage) & 1u, abort_flag)) {
+              ok = false;
+              break;
+            }
+            stage_phase ^= 1u << stage;
+            tc_fence_after_sync();
+            const uint32_t sa = smem_base + stage * STAGE_BYTES, sb = sa + BOX_BYTES;
+            if (kb == kb2) {
+              const uint32_t sf = sf_base + slot * SF_BYTES;
+#pragma unroll
+              for (int j = 0; j < 3; ++j) tmem_cp_32x128b_pair(sfa + 4 * j, make_smem_desc_rows16(sf + 512 * j));
+            }
+            const uint32_t idesc = make_idesc_mxf8(2 * BM, BN, 0u, B_MN ? 1u : 0u, kb & 3);
+#pragma unroll
+            for (int k = 0; k < BK / UMMA_K; ++k) {
+              const uint64_t da = make_smem_desc_sw128(sa + k * UMMA_K, 0, 1024);
+              const uint64_t db = make_smem_desc_sw128(sb + k * B_KSTEP, 0, 1024);
+              umma_ss_mxf8_pair(tmem_d, da, db, idesc, sfa, sfb, (kb > unit.kb0 || k) ? 1u : 0u);
+            }
+          }
+          if (!ok) break;
+          umma_commit_both(empty_bar(slot));
+          if (++slot == SLOTS) slot = 0;
+        }
+        if (!ok) break;
+        umma_commit_both(acc_full_bar(acc));
+      }
+    }
+    __syncwarp();
+  } else if (warp < 6) {
+    // ------------------------------------------------------------------ epilogue (warps 2..5 of both CTAs)
+    const int quarter = warp & 3;  // TMEM lanes [32*quarter, 32*quarter+32) belong to this warp
+    const uint32_t free_bar = map_to_cta(acc_free_bar, 0);
+    int i = 0;
+    for (int u = pair_id; u < sched.total_units; u += num_pairs, ++i) {
+      const Unit unit = unit_at(u, sched, k_blocks, width);
+      const int acc = i & 1;
+      const int row = unit.m0 + int(cta) * BM + quarter * 32 + lane;
+      // all four warps go on or none does: they meet at barriers below
+      if (!named_barrier_all(1, 128, mbar_wait(acc_full_bar(acc), uint32_t(i >> 1) & 1u, abort_flag))) break;
+      tc_fence_after_sync();
+      const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + acc * ACC1;
+      auto release = [&] {
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(free_bar);
+      };
+      if constexpr (GATED) {
+        if (acc == 0) gated_tile<0>(taddr, row, unit.n0, f, p, release);
+        else gated_tile<1>(taddr, row, unit.n0, f, p, release);
+      } else {
+        constexpr int CHUNKS = BN / 32;
+        if (unit.rest < 0) {
+#pragma unroll 1
+          for (int j = 0; j < CHUNKS; ++j) {
+            const int c = acc == 0 ? CHUNKS - 1 - j : j;  // the shared columns first
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(taddr + c * 32, v);
+            tmem_ld_wait();
+            if (j == 0) release();
+            const int col = unit.n0 + c * 32;
+            if (col < p.N) store_chunk<T>(v, row, col, p);
+          }
+        } else {
+          // A part of a split tile.  Workspace layout [part][CTA][chunk][4 columns][row]: a warp's access covers
+          // 512 consecutive bytes.  The part that finds all others done keeps its own sums in TMEM.
+          const int others = sched.ksplit - 1;
+          unsigned int* done = parts_done + unit.rest * 2 + cta;
+          float4* tile = reinterpret_cast<float4*>(parts) + ((long long)unit.rest * sched.ksplit * 2 + cta) * (PART_FLOATS / 4) + quarter * 32 + lane;
+          constexpr long long PART_STEP = 2 * (PART_FLOATS / 4);
+          if (threadIdx.x == 64) *arrived = *reinterpret_cast<volatile unsigned int*>(done);
+          named_barrier_sync(1, 128);
+          bool last = *arrived == unsigned(others);
+          if (!last) {
+            float4* mine = tile + unit.part * PART_STEP;
+#pragma unroll 1
+            for (int c = 0; c < CHUNKS; ++c) {
+              uint32_t v[32];
+              tmem_ld_32x32b_x32(taddr + c * 32, v);
+              tmem_ld_wait();
+              if (unit.n0 + c * 32 < p.N && row < p.M) {
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                  mine[(c * 8 + q) * BM] = make_float4(__uint_as_float(v[4 * q]), __uint_as_float(v[4 * q + 1]), __uint_as_float(v[4 * q + 2]), __uint_as_float(v[4 * q + 3]));
+              }
+            }
+            __threadfence();
+            named_barrier_sync(1, 128);  // every thread has also read `arrived`
+            if (threadIdx.x == 64) *arrived = atomicAdd(done, 1u);
+            named_barrier_sync(1, 128);
+            last = *arrived == unsigned(others);
+          }
+          if (last) {
+            __threadfence();
+#pragma unroll 1
+            for (int c = 0; c < CHUNKS; ++c) {
+              uint32_t v[32];
+              tmem_ld_32x32b_x32(taddr + c * 32, v);
+              tmem_ld_wait();
+              const int col = unit.n0 + c * 32;
+              if (col >= p.N || row >= p.M) continue;
+              float s[32];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) s[j] = 0.f;
+#pragma unroll 2
+              for (int part = 0; part <= others; ++part) {  // in this order whoever is last
+                if (part == unit.part) {
+#pragma unroll
+                  for (int j = 0; j < 32; ++j) s[j] += __uint_as_float(v[j]);
+                } else {
+                  float4 t[8];
+#pragma unroll
+                  for (int q = 0; q < 8; ++q) t[q] = __ldcg(tile + part * PART_STEP + (c * 8 + q) * BM);
+#pragma unroll
+                  for (int q = 0; q < 8; ++q) s[4 * q] += t[q].x, s[4 * q + 1] += t[q].y, s[4 * q + 2] += t[q].z, s[4 * q + 3] += t[q].w;
+                }
+              }
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(s[j]);
+              store_chunk<T>(v, row, col, p);
+            }
+          }
+          named_barrier_sync(1, 128);  // `arrived` may be written again
+          release();
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ scale words (warp 6 of both CTAs)
+    // A second producer of the ring: the words of a group of four blocks go to both slots of the group.  Those
+    // of the next group are fetched from global memory before a slot is waited for.
+    int u = pair_id, g = 0, slot = 0;
+    uint32_t phase = 0;
+    Unit unit{};
+    RawScales ra, rb0, rb1;
+    auto load = [&] {
+      load_scales(p.sa, unit.m0 + int(cta) * BM, p.M, g, k_blocks, lane, ra);
+      load_scales(p.sb, unit.n0, p.N, g, k_blocks, lane, rb0);
+      load_scales(p.sb, unit.n0 + (GATED ? f : 128), p.N, g, k_blocks, lane, rb1);
+    };
+    auto begin = [&] {
+      unit = unit_at(u, sched, k_blocks, width);
+      g = unit.kb0 / 4;
+    };
+    if (u < sched.total_units) {
+      begin();
+      load();
+    }
+    bool ok = true;
+    while (ok && u < sched.total_units) {
+      uint32_t a[4], b0[4], b1[4];
+      combine_scales(p.sa, g, k_blocks, ra, a);
+      combine_scales(p.sb, g, k_blocks, rb0, b0);
+      combine_scales(p.sb, g, k_blocks, rb1, b1);
+      const int slots = unit.kb1 - 4 * g > 2 ? 2 : 1;
+      if (4 * ++g >= unit.kb1) {
+        u += num_pairs;
+        if (u < sched.total_units) begin();
+      }
+      for (int i = 0; i < slots; ++i) {
+        if (!mbar_wait(empty_bar(slot), phase ^ 1u, abort_flag)) {
+          ok = false;
+          break;
+        }
+        store_scale_words(sf_base + slot * SF_BYTES, lane, a);
+        store_scale_words(sf_base + slot * SF_BYTES + 512, lane, b0);
+        store_scale_words(sf_base + slot * SF_BYTES + 1024, lane, b1);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(full_bar(2 * slot), 0));
+        if (++slot == SLOTS) {
+          slot = 0;
+          phase ^= 1u;
+        }
+      }
+      if (u < sched.total_units) load();
+    }
+  }
+
+  // ------------------------------------------------------------------ common exit
+  tc_fence_before_sync();
+  __syncthreads();
+  if (*abort_flag) {
+    if (threadIdx.x == 0) {
+      // let TMA copies that are still in flight land before the CTA's shared memory goes away
+      const unsigned long long t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 200000ull) {
+      }
+      if (p.status != nullptr && atomicCAS(p.status, kOk, kErrBarrierTimeout) == kOk) {
+        p.status[1] = 3000000 + blockIdx.x;
+        p.status[2] = p.M;
+        p.status[3] = p.N;
+      }
+    }
+    __syncthreads();
+  }
+  cluster_sync_all();  // the peer may still be signalling barriers in this CTA's shared memory
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem_base, TMEM_COLS);
+  }
+}
+
+Schedule make_schedule(int M, int N, int K, bool gated, int num_pairs) {
+  Schedule s;
+  const int k_blocks = (K + BK - 1) / BK, groups = (k_blocks + 3) / 4;
+  s.tiles_m = (M + 2 * BM - 1) / (2 * BM);
+  s.tiles_n = gated ? N / 256 : (N + BN - 1) / BN;
+  const long long tiles = (long long)s.tiles_m * s.tiles_n;
+  const int rem = int(tiles % num_pairs);
+  s.ksplit = 1;
+  if (rem != 0 && !gated) {
+    // cycles of the last wave: measured 800 per block of K, and for split tiles about 10 us for clearing the
+    // counters and exchanging the sums.  4096 x 4096 x K (34 tiles left over): K = 14336 takes 217 us split in two
+    // and 227 us whole, K = 4096 82 and 79.
+    long long best = 800ll * k_blocks;
+    for (int w = 2; w <= 8 && 2 * w <= groups; ++w) {
+      const long long waves = ((long long)rem * w + num_pairs - 1) / num_pairs;
+      const long long cost = waves * 3200 * ((groups + w - 1) / w) + 16000 + 1000 * w;
+      if (cost < best) {
+        best = cost;
+        s.ksplit = w;
+      }
+    }
+  }
+  s.full_tiles = int(s.ksplit == 1 ? tiles : tiles - rem);
+  s.total_units = s.full_tiles + int(tiles - s.full_tiles) * s.ksplit;
+  return s;
+}
+
+template <bool B_MN, bool GATED, typename T>
+cudaError_t launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, const Schedule& s, void* workspace, int num_pairs, cudaStream_t stream) {
+  auto kern = fp8_gemm_pair_kernel<B_MN, GATED, T>;
+  // function attributes are per device: remember which devices of this process have been set up
+  static bool configured[kMaxDevices] = {};
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
+  if (dev < 0 || dev >= kMaxDevices || !configured[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(SMEM_BYTES));
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < kMaxDevices) configured[dev] = true;
+  }
+  const int rem = s.ksplit > 1 ? (s.total_units - s.full_tiles) / s.ksplit : 0;
+  unsigned int* counters = static_cast<unsigned int*>(workspace);
+  float* parts = rem ? reinterpret_cast<float*>(static_cast<char*>(workspace) + ((size_t(rem) * 2 * sizeof(unsigned int) + 255) & ~size_t(255))) : nullptr;
+  if (rem) {
+    if (cudaError_t e = cudaMemsetAsync(counters, 0, size_t(rem) * 2 * sizeof(unsigned int), stream); e != cudaSuccess) return e;
+  }
+  const int pairs = s.total_units < num_pairs ? s.total_units : num_pairs;
+  kern<<<2 * pairs, NUM_THREADS, SMEM_BYTES, stream>>>(ta, tb, p, s, parts, counters);
+  flush_bounds_record(p.status, stream);
+  return cudaGetLastError();
+}
+
+}  // namespace pair
+
+size_t pair_workspace(int M, int N, int K, bool gated, int num_sms) {
+  const pair::Schedule s = pair::make_schedule(M, N, K, gated, num_sms / 2);
+  if (s.ksplit == 1) return 0;
+  const size_t rem = size_t(s.total_units - s.full_tiles) / s.ksplit;
+  return ((rem * 2 * sizeof(unsigned int) + 255) & ~size_t(255)) + rem * s.ksplit * 2 * pair::PART_FLOATS * sizeof(float);
+}
+
+cudaError_t launch_pair(const Fp8GemmArgs& g, const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int num_sms, cudaStream_t stream) {
+  using namespace pair;
+  const int num_pairs = num_sms / 2;
+  const Schedule s = make_schedule(g.M, g.N, g.K, g.gated, num_pairs);
+  if (g.gated) return launch<false, true, __nv_bfloat16>(ta, tb, p, s, g.workspace, num_pairs, stream);
+  if (g.b.mn_major) {
+    if (g.out == Elem::kBf16) return launch<true, false, __nv_bfloat16>(ta, tb, p, s, g.workspace, num_pairs, stream);
+    if (g.out == Elem::kF16) return launch<true, false, __half>(ta, tb, p, s, g.workspace, num_pairs, stream);
+    return launch<true, false, float>(ta, tb, p, s, g.workspace, num_pairs, stream);
+  }
+  if (g.out == Elem::kBf16) return launch<false, false, __nv_bfloat16>(ta, tb, p, s, g.workspace, num_pairs, stream);
+  if (g.out == Elem::kF16) return launch<false, false, __half>(ta, tb, p, s, g.workspace, num_pairs, stream);
+  return launch<false, false, float>(ta, tb, p, s, g.workspace, num_pairs, stream);
+}
+
+}  // namespace fp8
+}  // namespace elfb

@@ -55,8 +55,10 @@ struct Fp8GemmArgs {
   long long ld_gu = 0;
   uint8_t* gu_scale = nullptr;
   long long ld_gu_scale = 0;
+  void* workspace = nullptr;   // fp8_gemm_workspace() bytes, used by this launch alone
   int* status = nullptr;
 };
+size_t fp8_gemm_workspace(const Fp8GemmArgs& args, int num_sms);
 // Returns nullptr on success, otherwise a description of the failure.
 const char* fp8_gemm(const Fp8GemmArgs& args, int num_sms, cudaStream_t stream);
 

@@ -272,6 +272,19 @@ __device__ __forceinline__ void umma_ss_mxf8(uint32_t tmem_d, uint64_t desc_a, u
       ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
       : "memory");
 }
+// 512 bytes of shared memory (32 rows of 16 bytes, rows consecutive) to 4 TMEM columns: row r to lane r of every
+// 32-lane quarter.  Ordered with the MMAs of the issuing thread.  The pair form copies in both CTAs, each from
+// its own shared memory.
+__device__ __forceinline__ uint64_t make_smem_desc_rows16(uint32_t smem_addr) {
+  // no swizzle; groups of 8 rows are 128 bytes apart
+  return uint64_t((smem_addr & 0x3ffff) >> 4) | (uint64_t(128 >> 4) << 16) | (uint64_t(128 >> 4) << 32) | (uint64_t(1) << 46);
+}
+__device__ __forceinline__ void tmem_cp_32x128b(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void tmem_cp_32x128b_pair(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
 // mbarrier arrives once all tcgen05 ops issued so far by this thread have completed.
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");

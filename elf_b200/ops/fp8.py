@@ -101,6 +101,13 @@ class BlockScaled:
         self.data, self.scale, self.block_rows = data, scale, block_rows
         self.is_model_input = False
 
+    @classmethod
+    def _made(cls, data: torch.Tensor, scale: torch.Tensor, block_rows: int = 1) -> "BlockScaled":
+        """Without the checks: for what this module's own kernels return."""
+        self = object.__new__(cls)
+        self.data, self.scale, self.block_rows, self.is_model_input = data, scale, block_rows, False
+        return self
+
     @property
     def shape(self) -> torch.Size:
         return self.data.shape
@@ -129,8 +136,13 @@ class BlockScaled:
 def _on_kernels(t: torch.Tensor) -> bool:
     if not (t.is_cuda and _gemm._ENABLED):
         return False
-    _ext.require_on_gpu()
+    if _ext._module is None:
+        _ext.require_on_gpu()
     return True
+
+
+def _shift(q: BlockScaled) -> int:
+    return 7 if q.block_rows == BLOCK else 0
 
 
 def _new(shape, block_rows: int, device) -> BlockScaled:
@@ -149,36 +161,14 @@ def _matrix(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
 
 
-def _bytes(t: torch.Tensor) -> torch.Tensor:
-    t = _matrix(t)
-    # a matrix expanded along its rows has pitch 0; the kernels want one place per row
-    return t.contiguous() if t.shape[0] > 1 and t.stride(0) < t.shape[1] else t
-
-
-def _operand(q: BlockScaled) -> Tuple[torch.Tensor, torch.Tensor, int]:
-    """``(data, scale, row_shift)`` as matrices the products take: rows on 16-byte boundaries."""
-    data = _bytes(q.data)
-    if data.data_ptr() % 16 or (data.shape[0] > 1 and data.stride(0) % 16) or data.stride(0) % 16:
-        cols = data.shape[1]
-        padded = torch.empty((data.shape[0], _round_up(cols, 16)), dtype=torch.uint8, device=data.device).view(_E4M3)[:, :cols]
-        data = padded.copy_(data)
-    return data, _bytes(q.scale), 7 if q.block_rows == BLOCK else 0
-
-
-def _need(ok: bool, message: str) -> None:
-    if not ok:
-        raise ValueError(message)
-
-
 def _need_float(t: torch.Tensor, name: str) -> None:
     if t.dtype not in _FLOATS:
         raise TypeError(f"{name} must be bf16, fp16 or fp32, got {t.dtype}")
 
 
-def _same_device(*named) -> None:
-    dev = named[0][1].device
-    for name, t in named[1:]:
-        _need(t is None or t.device == dev, f"{name} is on {t.device if t is not None else None}, {named[0][0]} on {dev}")
+def _same_device(name: str, t, other: str, u) -> None:
+    if u is not None and u.device != t.device:
+        raise ValueError(f"{other} is on {u.device}, {name} on {t.device}")
 
 
 # ------------------------------------------------------------------------------ plain torch forms
@@ -228,45 +218,41 @@ def _rms_ref(h: torch.Tensor, w: torch.Tensor, eps: float):
 
 def _quantize(x: torch.Tensor, block_rows: int) -> BlockScaled:
     _need_float(x, "x")
-    x = x.detach()
     if not _on_kernels(x):
-        return _quantize_ref(x, block_rows)
-    q = _new(x.shape, block_rows, x.device)
-    if x.numel():
-        _ext.get().fp8_quantize(_bytes(x), _matrix(q.data), _matrix(q.scale), block_rows == BLOCK)
-    return q
+        return _quantize_ref(x.detach(), block_rows)
+    return BlockScaled._made(*_ext.get().fp8_quantize(x, block_rows == BLOCK), block_rows)
 
 
 def quantize(x: torch.Tensor) -> BlockScaled:
     """Block-scaled copy of ``x [..., cols]`` (bf16, fp16 or fp32): one scale per row and 128 columns.
     Not differentiable; see ``linear`` and ``gated_ffn``."""
-    _need(x.dim() >= 1, "quantize needs a tensor with at least one dimension")
+    if x.dim() < 1:
+        raise ValueError("quantize needs a tensor with at least one dimension")
     return _quantize(x, 1)
 
 
 def quantize_weight(w: torch.Tensor) -> BlockScaled:
     """Block-scaled copy of a matrix with one scale per tile of 128 x 128, usable in ``linear_forward`` and,
     transposed, in ``linear_input_grad``."""
-    _need(w.dim() == 2, f"quantize_weight needs a matrix, got shape {tuple(w.shape)}")
+    if w.dim() != 2:
+        raise ValueError(f"quantize_weight needs a matrix, got shape {tuple(w.shape)}")
     return _quantize(w, BLOCK)
 
 
 def dequantize(q: BlockScaled, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The values ``q`` stands for: exact in bf16 and fp32; in fp16 rounded, and infinite above 65504.
-    ``out``: matrix (a contiguous last dimension) to write instead of a new tensor."""
+    ``out``: tensor to write instead of a new one; its last dimension contiguous, its rows evenly spaced."""
     if out is None:
         if dtype not in _FLOATS:
             raise TypeError(f"dequantize gives bf16, fp16 or fp32, not {dtype}")
-        out = torch.empty(q.shape, dtype=dtype, device=q.device)
     else:
         _need_float(out, "out")
-        _need(out.shape == q.shape and out.device == q.device and out.stride(-1) == 1, "out does not match the block-scaled tensor")
-    if q.numel() == 0:
-        return out
+        if not (out.shape == q.shape and out.device == q.device):
+            raise ValueError("out does not match the block-scaled tensor")
     if not _on_kernels(q.data):
-        return out.copy_(_values(q).view(q.shape))
-    _ext.get().fp8_dequantize(_bytes(q.data), _bytes(q.scale), 7 if q.block_rows == BLOCK else 0, out if out.dim() == 2 else out.view(-1, out.shape[-1]))
-    return out
+        y = _values(q).view(q.shape)
+        return y.to(dtype) if out is None else out.copy_(y)
+    return _ext.get().fp8_dequantize(q.data, q.scale, _shift(q), dtype, out)
 
 
 # ------------------------------------------------------------------------------ RMSNorm
@@ -274,23 +260,21 @@ def dequantize(q: BlockScaled, dtype: torch.dtype = torch.bfloat16, out: Optiona
 
 def _norm(x, residual, w, eps):
     dim = x.shape[-1]
-    _need(x.dim() >= 1 and w.dim() == 1 and w.numel() == dim, f"the gain must have {dim} elements, got shape {tuple(w.shape)}")
-    _need(residual is None or (residual.shape == x.shape and residual.dtype == x.dtype), "the residual must match x")
-    _same_device(("x", x), ("the gain", w), ("the residual", residual))
+    if not (x.dim() >= 1 and w.dim() == 1 and w.numel() == dim):
+        raise ValueError(f"the gain must have {dim} elements, got shape {tuple(w.shape)}")
+    if not (residual is None or (residual.shape == x.shape and residual.dtype == x.dtype)):
+        raise ValueError("the residual must match x")
+    _same_device("x", x, "the gain", w)
+    _same_device("x", x, "the residual", residual)
     _need_float(x, "x")
-    x, w = x.detach(), w.detach()
-    residual = None if residual is None else residual.detach()
     fits = x.dtype == torch.bfloat16 and w.dtype == torch.bfloat16 and dim % 8 == 0 and 0 < dim <= 8192
-    if not (fits and _on_kernels(x)) or x.numel() == 0:
-        h = x if residual is None else x + residual
+    if not (fits and _on_kernels(x)):
+        x, w = x.detach(), w.detach()
+        h = x if residual is None else x + residual.detach()
         q, rstd = _rms_ref(h, w, eps)
         return q, rstd, h
-    rows = x.numel() // dim
-    q = _new(x.shape, 1, x.device)
-    dense = lambda t: t.contiguous() if t.contiguous().data_ptr() % 16 == 0 else t.contiguous().clone()  # noqa: E731
-    rstd, h = _ext.get().fp8_rmsnorm(dense(x).view(rows, dim), dense(w), eps, None if residual is None else dense(residual).view(rows, dim), _matrix(q.data),
-                                     _matrix(q.scale))
-    return q, rstd.view(x.shape[:-1]), h.view(x.shape)
+    data, scale, rstd, h = _ext.get().fp8_rmsnorm(x, w, eps, residual)
+    return BlockScaled._made(data, scale), rstd, h
 
 
 def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-5) -> Tuple[BlockScaled, torch.Tensor]:
@@ -311,10 +295,13 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, w: torch.Tensor, eps: 
 
 
 def _check_product(a: BlockScaled, b: BlockScaled, reduce_b: int, what: str) -> None:
-    _need(a.block_rows == 1, f"{what}: the activation or gradient must be scaled by rows")
-    _need(b.data.dim() == 2, f"{what}: the weight must be a matrix")
-    _need(a.shape[-1] == b.shape[reduce_b], f"{what}: reduction lengths {a.shape[-1]} and {b.shape[reduce_b]} differ")
-    _same_device(("the activation", a), ("the weight", b))
+    if a.block_rows != 1:
+        raise ValueError(f"{what}: the activation or gradient must be scaled by rows")
+    if b.data.dim() != 2:
+        raise ValueError(f"{what}: the weight must be a matrix")
+    if a.shape[-1] != b.shape[reduce_b]:
+        raise ValueError(f"{what}: reduction lengths {a.shape[-1]} and {b.shape[reduce_b]} differ")
+    _same_device("the activation", a, "the weight", b)
 
 
 def _product(a: BlockScaled, b: BlockScaled, transposed: bool, bias, out_dtype) -> torch.Tensor:
@@ -326,19 +313,16 @@ def _product(a: BlockScaled, b: BlockScaled, transposed: bool, bias, out_dtype) 
         if bias is not None:
             y = y + bias.float()
         return y.to(out_dtype).view(*a.shape[:-1], n)
-    y = torch.empty((*a.shape[:-1], n), dtype=out_dtype, device=a.device)
-    ad, asc, _ = _operand(a)
-    bd, bsc, shift = _operand(b)
     bias = None if bias is None else bias.detach().to(out_dtype).contiguous()
-    _ext.get().fp8_gemm(ad, asc, bd, bsc, shift, transposed, y.view(-1, n), bias, _gemm.status(a.device))
-    return y
+    return _ext.get().fp8_gemm(a.data, a.scale, b.data, b.scale, _shift(b), transposed, out_dtype, bias, _gemm.status(a.device))
 
 
 def linear_forward(x: BlockScaled, w: BlockScaled, bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``x W^T (+ bias)`` for ``x [..., K]`` scaled by rows and ``w [N, K]`` scaled by tiles or rows; accumulated in
     fp32 and rounded once."""
     _check_product(x, w, 1, "linear_forward")
-    _need(bias is None or (bias.shape == (w.shape[0],) and bias.device == w.device), "linear_forward: the bias must be a vector with one element per output")
+    if not (bias is None or (bias.shape == (w.shape[0],) and bias.device == w.device)):
+        raise ValueError("linear_forward: the bias must be a vector with one element per output")
     return _product(x, w, False, bias, out_dtype)
 
 
@@ -346,7 +330,8 @@ def linear_input_grad(dy: BlockScaled, w: BlockScaled, out_dtype: torch.dtype = 
     """``dy W`` for ``dy [..., N]`` scaled by rows and ``w [N, K]`` scaled by tiles.  The weight is read as it
     lies: the tensor core takes it transposed, and a tile's scale serves both directions."""
     _check_product(dy, w, 0, "linear_input_grad")
-    _need(w.block_rows == BLOCK, "linear_input_grad: the weight must be scaled in tiles of 128 x 128 (quantize_weight)")
+    if w.block_rows != BLOCK:
+        raise ValueError("linear_input_grad: the weight must be scaled in tiles of 128 x 128 (quantize_weight)")
     return _product(dy, w, True, None, out_dtype)
 
 
@@ -362,7 +347,7 @@ def _restored(t: Union[BlockScaled, torch.Tensor]) -> torch.Tensor:
     out = torch.empty((rows, _round_up(cols, 8)), dtype=torch.bfloat16, device=t.device)[:, :cols]
     if not isinstance(t, BlockScaled):
         return out.copy_(t)
-    return dequantize(BlockScaled(_bytes(t.data), _bytes(t.scale), t.block_rows), out=out)
+    return _ext.get().fp8_dequantize(t.data if t.data.dim() == 2 else t.data.reshape(rows, cols), t.scale, _shift(t), torch.bfloat16, out)
 
 
 def linear_weight_grad(dy: Union[BlockScaled, torch.Tensor], x: Union[BlockScaled, torch.Tensor], out: Optional[torch.Tensor] = None,
@@ -371,10 +356,11 @@ def linear_weight_grad(dy: Union[BlockScaled, torch.Tensor], x: Union[BlockScale
     tensor path: the reduction runs over tokens, which have scales of their own.  Added to ``out`` when it is
     given (bf16 or fp32); ``push`` as in ``gemm.linear_weight_grad``."""
     n, k = dy.shape[-1], x.shape[-1]
-    _need(dy.shape[:-1].numel() == x.shape[:-1].numel(), "linear_weight_grad: dy and x have different numbers of rows")
-    _same_device(("dy", dy), ("x", x))
-    _need(out is None or (out.shape == (n, k) and out.device == x.device and out.dtype in (torch.bfloat16, torch.float32)),
-          f"linear_weight_grad: out must be a bf16 or fp32 matrix [{n}, {k}]")
+    if dy.shape[:-1].numel() != x.shape[:-1].numel():
+        raise ValueError("linear_weight_grad: dy and x have different numbers of rows")
+    _same_device("dy", dy, "x", x)
+    if not (out is None or (out.shape == (n, k) and out.device == x.device and out.dtype in (torch.bfloat16, torch.float32))):
+        raise ValueError(f"linear_weight_grad: out must be a bf16 or fp32 matrix [{n}, {k}]")
     if out_dtype not in _FLOATS:
         raise TypeError(f"products come in bf16, fp16 or fp32, not {out_dtype}")
     data = x.data if isinstance(x, BlockScaled) else x
@@ -388,7 +374,8 @@ def linear_weight_grad(dy: Union[BlockScaled, torch.Tensor], x: Union[BlockScale
     dw = out if direct else torch.empty((n, _round_up(k, 8)), dtype=dtype, device=x.device)[:, :k]
     args = [_restored(dy), _restored(x), dw, None, True, True, direct, 1.0, _gemm.status(x.device), _gemm._VARIANT, _gemm._SPLIT_TAIL]
     if push:
-        _need(direct, "linear_weight_grad: a push needs a gradient buffer the product can add to in place")
+        if not direct:
+            raise ValueError("linear_weight_grad: a push needs a gradient buffer the product can add to in place")
         args += [push["push_out"], push["push_flags"], push["push_flag_value"], push["push_counter"]]
     _ext.get().gemm(*args)
     if direct:
@@ -407,20 +394,16 @@ def gated_forward(x: BlockScaled, w_gate_up: BlockScaled, keep: bool = True) -> 
     ``gated_backward``.  One kernel: the projections stay in fp32 until the activation is formed."""
     _check_product(x, w_gate_up, 1, "gated_forward")
     f2 = w_gate_up.shape[0]
-    _need(f2 % (2 * BLOCK) == 0, f"gated_forward: the width of gate and of up must be a multiple of {BLOCK}, got {f2} rows in all")
+    if f2 % (2 * BLOCK):
+        raise ValueError(f"gated_forward: the width of gate and of up must be a multiple of {BLOCK}, got {f2} rows in all")
     f = f2 // 2
     if x.numel() == 0 or f == 0 or not _on_kernels(x.data):
         gu = _values(x) @ _values(w_gate_up).T
         act = torch.nn.functional.silu(gu[:, :f]) * gu[:, f:]
         lead = x.shape[:-1]
         return _quantize_ref(act.view(*lead, f), 1), _quantize_ref(gu.view(*lead, f2), 1) if keep else None
-    act = _new((*x.shape[:-1], f), 1, x.device)
-    gu = _new((*x.shape[:-1], f2), 1, x.device) if keep else None
-    xd, xs, _ = _operand(x)
-    wd, ws, shift = _operand(w_gate_up)
-    _ext.get().fp8_gated(xd, xs, wd, ws, shift, _matrix(act.data), _matrix(act.scale), None if gu is None else _matrix(gu.data),
-                         None if gu is None else _matrix(gu.scale), _gemm.status(x.device))
-    return act, gu
+    act, act_scale, gu, gu_scale = _ext.get().fp8_gated(x.data, x.scale, w_gate_up.data, w_gate_up.scale, _shift(w_gate_up), keep, _gemm.status(x.device))
+    return BlockScaled._made(act, act_scale), BlockScaled._made(gu, gu_scale) if keep else None
 
 
 def gated_backward(dy: BlockScaled, w_down: BlockScaled, gate_up: BlockScaled) -> BlockScaled:
@@ -429,10 +412,13 @@ def gated_backward(dy: BlockScaled, w_down: BlockScaled, gate_up: BlockScaled) -
     ``s = sigmoid(gate)``, gate and up restored from their checkpoint."""
     _check_product(dy, w_down, 0, "gated_backward")
     f = w_down.shape[1]
-    _need(w_down.block_rows == BLOCK, "gated_backward: the weight must be scaled in tiles of 128 x 128 (quantize_weight)")
-    _need(f % BLOCK == 0, f"gated_backward: the width of gate and of up must be a multiple of {BLOCK}, got {f}")
-    _need(gate_up.block_rows == 1 and gate_up.shape == (*dy.shape[:-1], 2 * f), f"gated_backward: expected gate_up of shape {(*dy.shape[:-1], 2 * f)}, got {tuple(gate_up.shape)}")
-    _same_device(("dy", dy), ("gate_up", gate_up))
+    if w_down.block_rows != BLOCK:
+        raise ValueError("gated_backward: the weight must be scaled in tiles of 128 x 128 (quantize_weight)")
+    if f % BLOCK:
+        raise ValueError(f"gated_backward: the width of gate and of up must be a multiple of {BLOCK}, got {f}")
+    if not (gate_up.block_rows == 1 and gate_up.shape == (*dy.shape[:-1], 2 * f)):
+        raise ValueError(f"gated_backward: expected gate_up of shape {(*dy.shape[:-1], 2 * f)}, got {tuple(gate_up.shape)}")
+    _same_device("dy", dy, "gate_up", gate_up)
     dact = _product(dy, w_down, True, None, torch.float32).view(-1, f)
     if dact.numel() == 0 or not _on_kernels(dy.data):
         gu = _values(gate_up)
@@ -440,10 +426,7 @@ def gated_backward(dy: BlockScaled, w_down: BlockScaled, gate_up: BlockScaled) -
         s = torch.sigmoid(gate)
         dgu = torch.cat([dact * up * s * (1 + gate * (1 - s)), dact * gate * s], 1)
         return _quantize_ref(dgu.view(gate_up.shape), 1)
-    dgu = _new(gate_up.shape, 1, dy.device)
-    gd, gs, _ = _operand(gate_up)
-    _ext.get().fp8_swiglu_bwd(dact, gd, gs, _matrix(dgu.data), _matrix(dgu.scale))
-    return dgu
+    return BlockScaled._made(*_ext.get().fp8_swiglu_bwd(dact, gate_up.data, gate_up.scale))
 
 
 # ------------------------------------------------------------------------------ differentiable forms
@@ -452,7 +435,8 @@ def gated_backward(dy: BlockScaled, w_down: BlockScaled, gate_up: BlockScaled) -
 def _weight_copy(q: Optional[BlockScaled], w: torch.Tensor, name: str) -> BlockScaled:
     if q is None:
         return quantize_weight(w)
-    _need(q.shape == w.shape and q.block_rows == BLOCK and q.device == w.device, f"{name}: the 8-bit copy does not belong to a weight of shape {tuple(w.shape)} on {w.device}")
+    if not (q.shape == w.shape and q.block_rows == BLOCK and q.device == w.device):
+        raise ValueError(f"{name}: the 8-bit copy does not belong to a weight of shape {tuple(w.shape)} on {w.device}")
     return q
 
 
@@ -476,10 +460,10 @@ class _Linear(torch.autograd.Function):
         dx = dw = db = None
         dyq = quantize(dy) if ctx.needs_input_grad[0] or ctx.needs_input_grad[1] else None
         if ctx.needs_input_grad[0]:
-            wq = BlockScaled(*weight, BLOCK) if ctx.given else quantize_weight(weight[0])
+            wq = BlockScaled._made(*weight, BLOCK) if ctx.given else quantize_weight(weight[0])
             dx = linear_input_grad(dyq, wq, ctx.x_dtype)
         if ctx.needs_input_grad[1]:
-            dw = linear_weight_grad(dyq, BlockScaled(data, scale), out_dtype=ctx.w_dtype)
+            dw = linear_weight_grad(dyq, BlockScaled._made(data, scale), out_dtype=ctx.w_dtype)
         if ctx.needs_input_grad[2]:
             db = _matrix(dy).float().sum(0).to(ctx.bias_dtype)
         return dx, dw, db, None, None
@@ -492,7 +476,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     optimizer step; without it every call makes its own.  The gradients are those of the product with the
     rounded operands, passed through the rounding unchanged."""
     _check_differentiable("linear", x, w, bias)
-    _need(w.dim() == 2 and x.dim() >= 1 and x.shape[-1] == w.shape[1], f"linear: x {tuple(x.shape)} does not match a weight of shape {tuple(w.shape)}")
+    if not (w.dim() == 2 and x.dim() >= 1 and x.shape[-1] == w.shape[1]):
+        raise ValueError(f"linear: x {tuple(x.shape)} does not match a weight of shape {tuple(w.shape)}")
     train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias))
     return _Linear.apply(x, w, bias, w_q, train)
 
@@ -515,12 +500,12 @@ class _GatedFFN(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         *kept, = ctx.saved_tensors
-        xq, act, gu = (BlockScaled(kept[2 * i], kept[2 * i + 1]) for i in range(3))
+        xq, act, gu = (BlockScaled._made(kept[2 * i], kept[2 * i + 1]) for i in range(3))
         rest = kept[6:]
         copies = []
         for given in ctx.given:
             n = 2 if given else 1
-            copies.append(BlockScaled(*rest[:n], BLOCK) if given else quantize_weight(rest[0]))
+            copies.append(BlockScaled._made(*rest[:n], BLOCK) if given else quantize_weight(rest[0]))
             rest = rest[n:]
         gate_up_q, down_q = copies
         x_dtype, gate_up_dtype, down_dtype = ctx.dtypes
@@ -545,9 +530,10 @@ def gated_ffn(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, ga
     ``D + 3F`` bytes a token against ``2 D + 6 F`` in bf16.  ``gate_up_q``, ``down_q``: block-scaled copies of the
     weights, as in ``linear``."""
     _check_differentiable("gated_ffn", x, w_gate_up, w_down)
-    _need(w_gate_up.dim() == 2 and w_down.dim() == 2 and x.dim() >= 1 and x.shape[-1] == w_gate_up.shape[1] and w_gate_up.shape[0] == 2 * w_down.shape[1],
-          f"gated_ffn: shapes x {tuple(x.shape)}, w_gate_up {tuple(w_gate_up.shape)}, w_down {tuple(w_down.shape)} do not match")
-    _need(w_down.shape[1] % BLOCK == 0, f"gated_ffn: the inner width must be a multiple of {BLOCK}, got {w_down.shape[1]}")
+    if not (w_gate_up.dim() == 2 and w_down.dim() == 2 and x.dim() >= 1 and x.shape[-1] == w_gate_up.shape[1] and w_gate_up.shape[0] == 2 * w_down.shape[1]):
+        raise ValueError(f"gated_ffn: shapes x {tuple(x.shape)}, w_gate_up {tuple(w_gate_up.shape)}, w_down {tuple(w_down.shape)} do not match")
+    if w_down.shape[1] % BLOCK:
+        raise ValueError(f"gated_ffn: the inner width must be a multiple of {BLOCK}, got {w_down.shape[1]}")
     train = torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_gate_up, w_down))
     return _GatedFFN.apply(x, w_gate_up, w_down, gate_up_q, down_q, train)
 
@@ -556,4 +542,5 @@ def _check_differentiable(what: str, x: torch.Tensor, *others) -> None:
     for t in (x, *others):
         if t is not None:
             _need_float(t, what)
-            _need(t.device == x.device, f"{what}: all tensors must be on one device, got {t.device} and {x.device}")
+            if t.device != x.device:
+                raise ValueError(f"{what}: all tensors must be on one device, got {t.device} and {x.device}")

@@ -103,11 +103,11 @@ def test_quantize_leaves_neighbours_alone(dev):
 
     x = activations(5, 140, torch.bfloat16, dev)
     data, scale = (torch.full((7, n), 0x5A, dtype=torch.uint8, device=dev) for n in (160, 8))
-    _ext.get().fp8_quantize(x, data[:5, :140], scale[:5, :2], False)
+    _ext.get().fp8_quantize(x, False, data[:5, :140], scale[:5, :2])
     assert bool((data[5:] == 0x5A).all()) and bool((data[:, 140:] == 0x5A).all())
     assert bool((scale[5:] == 0x5A).all()) and bool((scale[:, 2:] == 0x5A).all())
     out = torch.full((7, 160), 7.0, dtype=torch.bfloat16, device=dev)
-    _ext.get().fp8_dequantize(data[:5, :140], scale[:5, :2], 0, out[:5, :140])
+    _ext.get().fp8_dequantize(data[:5, :140], scale[:5, :2], 0, torch.bfloat16, out[:5, :140])
     assert bool((out[5:] == 7).all()) and bool((out[:, 140:] == 7).all())
 
 

@@ -81,6 +81,12 @@ __device__ __forceinline__ float bias_at(const void* bias, int col) {
   else return __bfloat162float(v);
 }
 
+template <typename T>
+__device__ __forceinline__ T rounded(float f) {
+  if constexpr (sizeof(T) == 4) return f;
+  else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(f);
+  else return __float2bfloat16_rn(f);
+}
 // D[row, col .. col+32) = v (+ bias)
 template <typename T>
 __device__ __forceinline__ void store_chunk(const uint32_t (&v)[32], int row, int col, const Params& p) {
@@ -112,12 +118,28 @@ __device__ __forceinline__ void store_chunk(const uint32_t (&v)[32], int row, in
   } else {
 #pragma unroll
     for (int j = 0; j < 32; ++j) {
-      if (col + j < p.N) {
-        if constexpr (sizeof(T) == 4) dst[j] = f[j];
-        else if constexpr (std::is_same<T, __half>::value) dst[j] = __float2half_rn(f[j]);
-        else dst[j] = __float2bfloat16_rn(f[j]);
-      }
+      if (col + j < p.N) dst[j] = rounded<T>(f[j]);
     }
+  }
+}
+
+// D[row, col .. col+4) = s (+ bias); row < M
+template <typename T>
+__device__ __forceinline__ void store_quad(float (&s)[4], int row, int col, const Params& p) {
+  T* dst = static_cast<T*>(p.d) + (long long)row * p.ldd + col;
+  alignas(16) T o[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (p.bias != nullptr && col + j < p.N) s[j] += bias_at<T>(p.bias, col + j);
+    o[j] = rounded<T>(s[j]);
+  }
+  if (p.vec && col + 4 <= p.N) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(o);
+    else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(o);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (col + j < p.N) dst[j] = o[j];
   }
 }
 

@@ -10,101 +10,75 @@
 //   forward     Y  = X . W^T   A = X  [M,K]   B = W [N,K]  K-major   (gated form: B = [gate | up])
 //   input grad  dX = dY . W    A = dY [M,K]   B = W [K,N]  MN-major  (its 128 x 128 tiles scale either way)
 //
-// Structure per CTA (320 threads, one CTA per SM, persistent over 128 x BN tiles):
-//   warp 0      TMA producer: ring of (A 128 x 128, B BN x 128) byte tiles, 128B-swizzled.
-//   warp 1      MMA issuer: 128 x BN x 32 steps into one of two TMEM accumulators.
-//   warps 2..5  epilogue, thread = row.
-//   warps 6..9  scale writers: read the exponent bytes of the next four blocks of K (512 values) from
-//               global memory and store them to one of two TMEM slots, each warp its own quarter of
-//               the lanes.  4 + BN/32 words per lane and 512 values of K: negligible traffic.
+// This file: the kernel for up to 128 rows, and the choice between it and the CTA-pair kernel
+// (fp8_gemm_sm100_2cta.cu).  With few rows the time is that of reading B, so the work is spread over all
+// SMs: one 128 x 128 tile per cluster of up to 8 CTAs that split K among them and add their fp32 sums,
+// in rank order, through distributed shared memory.  16 x 4096 x 14336 (59 MB of weights): see below.
 //
-// TMEM has 512 columns; two 256-column accumulators would leave none for the scales.  The second one
-// therefore starts 32 columns early and shares them with the first; the epilogue reads the shared
-// columns first and the next tile's products start as soon as it has.
+// Roles per CTA (224 threads):
+//   warp 0      TMA producer: ring of (A 128 x 128, B 128 x 128) byte tiles, 128B-swizzled.
+//   warp 1      MMA issuer: 128 x 128 x 32 steps into one TMEM accumulator.
+//   warps 2..5  epilogue, thread = row.
+//   warp 6      scale words: exponent bytes of four blocks of K, from global to shared memory; the MMA thread
+//               copies them to TMEM in order with its MMAs.
 #include "fp8_gemm.cuh"
 
 namespace elfb {
 
 namespace fp8 {
 
-constexpr int STAGES = 4;
-constexpr int NUM_THREADS = 320;
-constexpr int GROUP_M = 8;  // tiles of GROUP_M consecutive M-blocks share B panels in L2
+namespace rows128 {
 
-template <int BN>
-constexpr int kStageBytes = BOX_BYTES * (1 + BN / 128);
-template <int BN>
-constexpr size_t kSmemBytes = size_t(STAGES) * kStageBytes<BN> + 1024 /*align slack*/ + 256 /*barriers*/;
+constexpr int BN = 128;
+constexpr int STAGES = 6;
+constexpr int SLOTS = STAGES / 2;           // two consecutive stages share scale words and are freed together
+constexpr int STAGE_BYTES = 2 * BOX_BYTES;
+constexpr int SF_BYTES = 2 * 512;           // scale words of a slot: 128 rows of A, 128 columns of B
+constexpr int NUM_THREADS = 224;
+constexpr int TMEM_COLUMNS = 256;           // 128 of the accumulator, then two 8-column scale slots
+constexpr int MAX_CLUSTER = 8;
+constexpr size_t SMEM_BYTES = size_t(STAGES) * STAGE_BYTES + SLOTS * SF_BYTES + 1024 /*align slack*/ + 256 /*barriers*/;
+static_assert(STAGES * STAGE_BYTES >= BM * BN * 4, "the sums are exchanged in the ring's memory");
 
-struct Tile {
-  int m0, n0, n1;  // first row of A; first rows of B's two 128-row halves
-};
-
-template <int BN, bool GATED>
-__device__ __forceinline__ Tile tile_at(int t, int tiles_m, int tiles_n, int f) {
-  const int per_group = GROUP_M * tiles_n;
-  const int group = t / per_group;
-  const int first_m = group * GROUP_M;
-  const int rows = min(GROUP_M, tiles_m - first_m);
-  const int in_group = t - group * per_group;
-  Tile r;
-  r.m0 = (first_m + in_group % rows) * BM;
-  if (GATED) {
-    r.n0 = (in_group / rows) * 128;
-    r.n1 = f + r.n0;
-  } else {
-    r.n0 = (in_group / rows) * BN;
-    r.n1 = r.n0 + 128;
-  }
-  return r;
+__device__ __forceinline__ float4 load_cluster_f4(uint32_t cluster_addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr) : "memory");
+  return v;
 }
 
-template <int BN, bool B_MN, bool GATED, typename T>
+template <bool B_MN, typename T>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
-fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ Params p) {
-  constexpr int STAGE = kStageBytes<BN>;
-  constexpr bool OVERLAP = BN == 256;           // the accumulators share 32 columns
-  constexpr int ACC1 = OVERLAP ? 224 : 256;     // first column of the second one
+fp8_gemm_rows128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ Params p, int ksplit) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_aligned = smem_raw + (smem_base - smem_u32(smem_raw));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_aligned + size_t(STAGES) * STAGE);
+  const uint32_t sf_base = smem_base + STAGES * STAGE_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_aligned + size_t(STAGES) * STAGE_BYTES + SLOTS * SF_BYTES);
   const uint32_t bar0 = smem_u32(bars);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
-  auto empty_bar = [&](int s) { return bar0 + 8u * (STAGES + s); };
-  auto acc_full_bar = [&](int a) { return bar0 + 8u * (2 * STAGES + a); };
-  auto acc_empty_bar = [&](int a) { return bar0 + 8u * (2 * STAGES + 2 + a); };  // OVERLAP: only [0], one completion per tile
-  auto sf_full_bar = [&](int s) { return bar0 + 8u * (2 * STAGES + 4 + s); };
-  auto sf_empty_bar = [&](int s) { return bar0 + 8u * (2 * STAGES + 6 + s); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 8);
+  auto empty_bar = [&](int slot) { return bar0 + 8u * (STAGES + slot); };
+  const uint32_t done_bar = bar0 + 8u * (STAGES + SLOTS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + STAGES + SLOTS + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int f = p.N / 2;  // gated: width of the activation
-  const int tiles_m = (p.M + BM - 1) / BM;
-  const int tiles_n = GATED ? f / 128 : (p.N + BN - 1) / BN;
-  const int tiles = tiles_m * tiles_n;
-  const int k_blocks = (p.K + BK - 1) / BK;
+  const int rank = ksplit > 1 ? int(cluster_ctarank()) : 0;
+  const int n0 = int(blockIdx.x) / ksplit * BN;
+  const int k_blocks = (p.K + BK - 1) / BK, groups = (k_blocks + 3) / 4;
+  const int kb0 = 4 * int((long long)groups * rank / ksplit), kb1 = min(k_blocks, 4 * int((long long)groups * (rank + 1) / ksplit));
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(full_bar(s), 1);
-      mbar_init(empty_bar(s), 1);
-    }
-    for (int a = 0; a < 2; ++a) {
-      mbar_init(acc_full_bar(a), 1);
-      mbar_init(acc_empty_bar(a), 4);  // one arrival per epilogue warp
-      mbar_init(sf_full_bar(a), 4);    // one arrival per scale warp
-      mbar_init(sf_empty_bar(a), 1);
-    }
+    for (int s = 0; s < STAGES; ++s) mbar_init(full_bar(s), s & 1 ? 1 : 2);  // a slot's first stage also waits for the scale warp
+    for (int s = 0; s < SLOTS; ++s) mbar_init(empty_bar(s), 1);
+    mbar_init(done_bar, 1);
     fence_barrier_init();
     prefetch_tensormap(&tmap_a);
     prefetch_tensormap(&tmap_b);
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
+    tmem_alloc(smem_u32(tmem_slot), TMEM_COLUMNS);
     tmem_relinquish();
   }
   tc_fence_before_sync();
@@ -115,32 +89,25 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0) {
-      int stage = 0;
+      int slot = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-        const Tile tile = tile_at<BN, GATED>(t, tiles_m, tiles_n, f);
-        for (int kb = 0; kb < k_blocks; ++kb) {
-          if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) {
-            ok = false;
-            break;
-          }
-          const uint32_t sa = smem_base + stage * STAGE, sb = sa + BOX_BYTES, bar = full_bar(stage);
-          mbar_arrive_expect_tx(bar, STAGE);
-          const int k0 = kb * BK;
-          tma_load_2d(sa, &tmap_a, bar, k0, tile.m0);
-          // a box that lies behind B's last row arrives as zeros
-          if (B_MN) {
-            tma_load_2d(sb, &tmap_b, bar, tile.n0, k0);
-            if (BN == 256) tma_load_2d(sb + BOX_BYTES, &tmap_b, bar, tile.n1, k0);
-          } else {
-            tma_load_2d(sb, &tmap_b, bar, k0, tile.n0);
-            if (BN == 256) tma_load_2d(sb + BOX_BYTES, &tmap_b, bar, k0, tile.n1);
-          }
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
+      for (int kb2 = kb0; kb2 < kb1 && ok; kb2 += 2) {
+        if (!mbar_wait(empty_bar(slot), phase ^ 1u, abort_flag)) {
+          ok = false;
+          break;
+        }
+        for (int kb = kb2; kb < min(kb2 + 2, kb1); ++kb) {
+          const int stage = 2 * slot + (kb - kb2);
+          const uint32_t sa = smem_base + stage * STAGE_BYTES, sb = sa + BOX_BYTES, bar = full_bar(stage);
+          mbar_arrive_expect_tx(bar, STAGE_BYTES);
+          tma_load_2d(sa, &tmap_a, bar, kb * BK, 0);
+          if (B_MN) tma_load_2d(sb, &tmap_b, bar, n0, kb * BK);
+          else tma_load_2d(sb, &tmap_b, bar, kb * BK, n0);
+        }
+        if (++slot == SLOTS) {
+          slot = 0;
+          phase ^= 1u;
         }
       }
     }
@@ -150,131 +117,132 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     if (lane == 0) {
       // K-major: rows of 128 bytes, 8-row groups 1024 B apart, a step of 32 values = 32 B.
       // MN-major: 128-wide boxes of 128 k-rows, 8-row groups 1024 B apart, a step of 32 rows = 4096 B.
-      constexpr uint32_t B_LBO = B_MN ? BOX_BYTES : 0;
       constexpr uint32_t B_KSTEP = B_MN ? UMMA_K * 128 : UMMA_K;
-      int stage = 0;
-      uint32_t phase = 0, sf_count = 0;
+      int slot = 0;
+      uint32_t stage_phase = 0, sf_count = 0;
       bool ok = true;
-      int i = 0;  // tiles of this CTA so far
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++i) {
-        const int acc = i & 1;
-        if (OVERLAP) {
-          if (i > 0 && !mbar_wait(acc_empty_bar(0), uint32_t(i - 1) & 1u, abort_flag)) break;
-        } else {
-          if (!mbar_wait(acc_empty_bar(acc), (uint32_t(i >> 1) & 1u) ^ 1u, abort_flag)) break;
-        }
-        tc_fence_after_sync();
-        const uint32_t tmem_d = tmem_base + acc * ACC1;
-        for (int kb = 0; kb < k_blocks; ++kb) {
-          const int slot = sf_count & 1;
-          if ((kb & 3) == 0 && !mbar_wait(sf_full_bar(slot), (sf_count >> 1) & 1u, abort_flag)) {
+      for (int kb2 = kb0; kb2 < kb1 && ok; kb2 += 2) {
+        const uint32_t sfa = tmem_base + BN + (sf_count++ & 1) * 8, sfb = sfa + 4;
+        for (int kb = kb2; kb < min(kb2 + 2, kb1); ++kb) {
+          const int stage = 2 * slot + (kb - kb2);
+          if (!mbar_wait(full_bar(stage), (stage_phase >> stage) & 1u, abort_flag)) {
             ok = false;
             break;
           }
-          if (!mbar_wait(full_bar(stage), phase, abort_flag)) {
-            ok = false;
-            break;
-          }
+          stage_phase ^= 1u << stage;
           tc_fence_after_sync();
-          const uint32_t sa = smem_base + stage * STAGE, sb = sa + BOX_BYTES;
-          const uint32_t sfa = tmem_base + SF_COL + slot * 16, sfb = sfa + 4;
+          const uint32_t sa = smem_base + stage * STAGE_BYTES, sb = sa + BOX_BYTES;
+          if (kb == kb2) {
+            const uint32_t sf = sf_base + slot * SF_BYTES;
+            tmem_cp_32x128b(sfa, make_smem_desc_rows16(sf));
+            tmem_cp_32x128b(sfb, make_smem_desc_rows16(sf + 512));
+          }
           const uint32_t idesc = make_idesc_mxf8(BM, BN, 0u, B_MN ? 1u : 0u, kb & 3);
 #pragma unroll
           for (int k = 0; k < BK / UMMA_K; ++k) {
             const uint64_t da = make_smem_desc_sw128(sa + k * UMMA_K, 0, 1024);
-            const uint64_t db = make_smem_desc_sw128(sb + k * B_KSTEP, B_LBO, 1024);
-            umma_ss_mxf8(tmem_d, da, db, idesc, sfa, sfb, (kb | k) ? 1u : 0u);
-          }
-          umma_commit(empty_bar(stage));
-          if ((kb & 3) == 3 || kb + 1 == k_blocks) {
-            umma_commit(sf_empty_bar(slot));
-            ++sf_count;
-          }
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
+            const uint64_t db = make_smem_desc_sw128(sb + k * B_KSTEP, 0, 1024);
+            umma_ss_mxf8(tmem_base, da, db, idesc, sfa, sfb, (kb > kb0 || k) ? 1u : 0u);
           }
         }
         if (!ok) break;
-        umma_commit(acc_full_bar(acc));
+        umma_commit(empty_bar(slot));
+        if (++slot == SLOTS) slot = 0;
       }
+      if (ok) umma_commit(done_bar);
     }
     __syncwarp();
   } else if (warp < 6) {
-    // ------------------------------------------------------------------ epilogue (warps 2..5)
+    // ------------------------------------------------------------------ accumulator: to D, or to shared memory for the exchange
     const int quarter = warp & 3;  // TMEM lanes [32*quarter, 32*quarter+32) belong to this warp
-    int i = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++i) {
-      const Tile tile = tile_at<BN, GATED>(t, tiles_m, tiles_n, f);
-      const int acc = i & 1;
-      const int row = tile.m0 + quarter * 32 + lane;
-      if (!mbar_wait(acc_full_bar(acc), uint32_t(i >> 1) & 1u, abort_flag)) break;
+    const int row = quarter * 32 + lane;
+    if (mbar_wait(done_bar, 0, abort_flag)) {
       tc_fence_after_sync();
-      const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + acc * ACC1;
-      auto release = [&](int bar) {
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(acc_empty_bar(bar));
-      };
-      if constexpr (GATED) {
-        if (acc == 0) gated_tile<0>(taddr, row, tile.n0, f, p, [&] { release(0); });
-        else gated_tile<1>(taddr, row, tile.n0, f, p, [&] { release(0); });
-      } else {
-        constexpr int CHUNKS = BN / 32;
+      const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16);
+      if (quarter * 32 < p.M) {
 #pragma unroll 1
-        for (int j = 0; j < CHUNKS; ++j) {
-          const int c = OVERLAP && acc == 0 ? CHUNKS - 1 - j : j;  // the shared columns first
+        for (int c = 0; c < BN / 32; ++c) {
+          const int col = n0 + c * 32;
+          if (col >= p.N) break;
           uint32_t v[32];
           tmem_ld_32x32b_x32(taddr + c * 32, v);
           tmem_ld_wait();
-          if (OVERLAP && j == 0) release(0);
-          const int col = tile.n0 + c * 32;
-          if (col < p.N) store_chunk<T>(v, row, col, p);
+          if (ksplit == 1) {
+            store_chunk<T>(v, row, col, p);
+          } else if (row < p.M) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {  // 16-byte pieces of a row, exchanged so that the lanes' stores hit different banks
+              const uint32_t dst = smem_base + uint32_t(row) * (BN * 4) + (uint32_t((c * 8 + q) ^ (row & 31)) << 4);
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v[4 * q]), "r"(v[4 * q + 1]), "r"(v[4 * q + 2]), "r"(v[4 * q + 3]) : "memory");
+            }
+          }
         }
-        if (!OVERLAP) release(acc);
       }
     }
   } else {
-    // ------------------------------------------------------------------ scale writers (warps 6..9)
-    // The words of the next group are fetched before the slot of this one is waited for.
-    const int quarter = warp & 3;
-    int t = blockIdx.x, g = 0;
-    Tile tile = tile_at<BN, GATED>(t, tiles_m, tiles_n, f);
-    RawScales ra, rb0, rb1;
+    // ------------------------------------------------------------------ scale words (warp 6)
+    // A second producer of the ring: the words of a group of four blocks go to both slots of the group.  Those
+    // of the next group are fetched from global memory before a slot is waited for.
+    int g = kb0 / 4, slot = 0;
+    uint32_t phase = 0;
+    RawScales ra, rb;
     auto load = [&] {
-      load_scales(p.sa, tile.m0, p.M, g, k_blocks, lane, ra);
-      load_scales(p.sb, tile.n0, p.N, g, k_blocks, lane, rb0);
-      if (BN == 256) load_scales(p.sb, tile.n1, p.N, g, k_blocks, lane, rb1);
+      load_scales(p.sa, 0, p.M, g, k_blocks, lane, ra);
+      load_scales(p.sb, n0, p.N, g, k_blocks, lane, rb);
     };
-    if (t < tiles) load();
-    for (uint32_t count = 0; t < tiles; ++count) {
-      uint32_t a[4], b0[4], b1[4];
+    if (kb0 < kb1) load();
+    bool ok = true;
+    while (ok && 4 * g < kb1) {
+      uint32_t a[4], b[4];
       combine_scales(p.sa, g, k_blocks, ra, a);
-      combine_scales(p.sb, g, k_blocks, rb0, b0);
-      if (BN == 256) combine_scales(p.sb, g, k_blocks, rb1, b1);
-      if (4 * ++g >= k_blocks) {
-        g = 0;
-        t += gridDim.x;
-        if (t < tiles) tile = tile_at<BN, GATED>(t, tiles_m, tiles_n, f);
+      combine_scales(p.sb, g, k_blocks, rb, b);
+      const int slots = kb1 - 4 * g > 2 ? 2 : 1;
+      ++g;
+      if (4 * g < kb1) load();
+      for (int i = 0; i < slots; ++i) {
+        if (!mbar_wait(empty_bar(slot), phase ^ 1u, abort_flag)) {
+          ok = false;
+          break;
+        }
+        store_scale_words(sf_base + slot * SF_BYTES, lane, a);
+        store_scale_words(sf_base + slot * SF_BYTES + 512, lane, b);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full_bar(2 * slot));
+        if (++slot == SLOTS) {
+          slot = 0;
+          phase ^= 1u;
+        }
       }
-      if (t < tiles) load();
-      const int slot = count & 1;
-      if (!mbar_wait(sf_empty_bar(slot), ((count >> 1) & 1u) ^ 1u, abort_flag)) break;
-      tc_fence_after_sync();
-      const uint32_t dst = tmem_base + (uint32_t(quarter) * 32u << 16) + SF_COL + slot * 16;
-      tmem_st_32x32b_x4(dst, a);
-      tmem_st_32x32b_x4(dst + 4, b0);
-      if (BN == 256) tmem_st_32x32b_x4(dst + 8, b1);
-      tmem_st_wait();
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(sf_full_bar(slot));
     }
   }
 
-  // ------------------------------------------------------------------ common exit
+  // ------------------------------------------------------------------ sums of the cluster
   tc_fence_before_sync();
   __syncthreads();
+  if (ksplit > 1) {
+    cluster_sync_all();
+    // a row's 32 pieces go to 32 consecutive threads; rows are dealt to the CTAs
+    if (!*abort_flag && warp < 4) {
+      const int q = lane;
+      const int col = n0 + 4 * q;
+      for (int row = rank + warp * ksplit; row < p.M; row += 4 * ksplit) {
+        const uint32_t src = smem_base + uint32_t(row) * (BN * 4) + (uint32_t(q ^ (row & 31)) << 4);
+        float4 part[MAX_CLUSTER];
+#pragma unroll
+        for (int r = 0; r < MAX_CLUSTER; ++r)
+          if (r < ksplit) part[r] = load_cluster_f4(map_to_cta(src, r));
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int r = 0; r < MAX_CLUSTER; ++r)
+          if (r < ksplit) s[0] += part[r].x, s[1] += part[r].y, s[2] += part[r].z, s[3] += part[r].w;
+        store_quad<T>(s, row, col, p);
+      }
+    }
+    cluster_sync_all();  // the peers may still be reading this CTA's shared memory
+  }
+
+  // ------------------------------------------------------------------ common exit
   if (*abort_flag) {
     if (threadIdx.x == 0) {
       // let TMA copies that are still in flight land before the CTA's shared memory goes away
@@ -291,51 +259,65 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
   }
   if (warp == 1) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem_base, TMEM_COLS);
+    tmem_dealloc(tmem_base, TMEM_COLUMNS);
   }
 }
 
-template <int BN, bool B_MN, bool GATED, typename T>
+template <bool B_MN, typename T>
 cudaError_t launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int num_sms, cudaStream_t stream) {
-  auto kern = fp8_gemm_kernel<BN, B_MN, GATED, T>;
-  constexpr size_t smem = kSmemBytes<BN>;
+  auto kern = fp8_gemm_rows128_kernel<B_MN, T>;
   // function attributes are per device: remember which devices of this process have been set up
   static bool configured[kMaxDevices] = {};
   int dev = 0;
   if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
   if (dev < 0 || dev >= kMaxDevices || !configured[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(SMEM_BYTES));
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < kMaxDevices) configured[dev] = true;
   }
-  const int tiles = ((p.M + BM - 1) / BM) * (GATED ? p.N / 256 : (p.N + BN - 1) / BN);
-  kern<<<tiles < num_sms ? tiles : num_sms, NUM_THREADS, smem, stream>>>(ta, tb, p);
+  const int tiles = (p.N + BN - 1) / BN, groups = (p.K + 4 * BK - 1) / (4 * BK);
+  int ksplit = 1;  // as many parts as there are SMs for, each at least four blocks of K long
+  while (ksplit < MAX_CLUSTER && 2 * ksplit * tiles <= num_sms && 2 * ksplit <= groups) ksplit *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(tiles) * ksplit);
+  cfg.blockDim = dim3(NUM_THREADS);
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ksplit;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ta, tb, p, ksplit); e != cudaSuccess) return e;
   flush_bounds_record(p.status, stream);
   return cudaGetLastError();
 }
 
-template <int BN>
-cudaError_t dispatch(const Fp8GemmArgs& g, const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int num_sms, cudaStream_t s) {
+}  // namespace rows128
+
+cudaError_t launch_rows128(const Fp8GemmArgs& g, const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int num_sms, cudaStream_t s) {
+  using namespace rows128;
   if (g.b.mn_major) {
-    if (g.out == Elem::kBf16) return launch<BN, true, false, __nv_bfloat16>(ta, tb, p, num_sms, s);
-    if (g.out == Elem::kF16) return launch<BN, true, false, __half>(ta, tb, p, num_sms, s);
-    return launch<BN, true, false, float>(ta, tb, p, num_sms, s);
+    if (g.out == Elem::kBf16) return launch<true, __nv_bfloat16>(ta, tb, p, num_sms, s);
+    if (g.out == Elem::kF16) return launch<true, __half>(ta, tb, p, num_sms, s);
+    return launch<true, float>(ta, tb, p, num_sms, s);
   }
-  if (g.out == Elem::kBf16) return launch<BN, false, false, __nv_bfloat16>(ta, tb, p, num_sms, s);
-  if (g.out == Elem::kF16) return launch<BN, false, false, __half>(ta, tb, p, num_sms, s);
-  return launch<BN, false, false, float>(ta, tb, p, num_sms, s);
+  if (g.out == Elem::kBf16) return launch<false, __nv_bfloat16>(ta, tb, p, num_sms, s);
+  if (g.out == Elem::kF16) return launch<false, __half>(ta, tb, p, num_sms, s);
+  return launch<false, float>(ta, tb, p, num_sms, s);
 }
 
 cudaError_t launch_pair(const Fp8GemmArgs& g, const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int num_sms, cudaStream_t stream);
 size_t pair_workspace(int M, int N, int K, bool gated, int num_sms);
 
-// Few rows leave most of a 256-row tile empty.
-bool use_pair(const Fp8GemmArgs& g, int num_sms) { return num_sms >= 2 && g.M > 128; }
+// The gated form has one kernel; its tile holds a block of gate and one of up.
+bool use_pair(const Fp8GemmArgs& g) { return g.gated || g.M > 128; }
 
 }  // namespace fp8
 
 size_t fp8_gemm_workspace(const Fp8GemmArgs& g, int num_sms) {
-  if (g.M <= 0 || g.N <= 0 || g.K <= 0 || !fp8::use_pair(g, num_sms)) return 0;
+  if (g.M <= 0 || g.N <= 0 || g.K <= 0 || !fp8::use_pair(g)) return 0;
   return fp8::pair_workspace(g.M, g.N, g.K, g.gated, num_sms);
 }
 
@@ -359,13 +341,12 @@ const char* fp8_gemm(const Fp8GemmArgs& g, int num_sms, cudaStream_t stream) {
     if (!aligned(g.act, g.ld_act) || (g.gu && !aligned(g.gu, g.ld_gu))) return "8-bit outputs must be 16-byte aligned with a 16-byte multiple row pitch";
     p.act = g.act, p.act_scale = g.act_scale, p.gu = g.gu, p.gu_scale = g.gu_scale;
     p.ld_act = g.ld_act, p.ld_act_scale = g.ld_act_scale, p.ld_gu = g.ld_gu, p.ld_gu_scale = g.ld_gu_scale;
-    e = use_pair(g, num_sms) ? launch_pair(g, ta, tb, p, num_sms, stream) : launch<256, false, true, __nv_bfloat16>(ta, tb, p, num_sms, stream);
+    e = launch_pair(g, ta, tb, p, num_sms, stream);
   } else {
     const long long esz = g.out == Elem::kF32 ? 4 : 2;
     p.d = g.d, p.ldd = g.ldd, p.bias = g.bias;
     p.vec = ((reinterpret_cast<uintptr_t>(g.d) | uintptr_t(g.ldd * esz)) & 15) == 0;
-    if (use_pair(g, num_sms)) e = launch_pair(g, ta, tb, p, num_sms, stream);
-    else e = g.N > 128 ? dispatch<256>(g, ta, tb, p, num_sms, stream) : dispatch<128>(g, ta, tb, p, num_sms, stream);
+    e = use_pair(g) ? launch_pair(g, ta, tb, p, num_sms, stream) : launch_rows128(g, ta, tb, p, num_sms, stream);
   }
   return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
 }

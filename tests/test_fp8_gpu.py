@@ -350,3 +350,35 @@ def test_gated_backward(dev, m, d, f):
     err_g = err * fg.abs() + (da * fg).abs() * rel + (da.abs() + err) * (u * s).abs() * (g.abs() + 1) * 2.0**-21 * (1 + g.abs())
     err_u = err * fu.abs() + (da * fu).abs() * rel
     check_held(got, torch.cat([da * fg, da * fu], 1), torch.cat([err_g, err_u], 1) + 1e-37)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 4096, 2048), (16, 1000, 5504), (100, 136, 9000), (128, 264, 4100), (77, 20000, 640), (2, 128, 30000)])
+def test_products_of_few_rows(dev, m, n, k):
+    """Up to 128 rows: the reduction is split over the CTAs of a cluster."""
+    from elf_b200.ops import fp8
+
+    x, w = operands(m, n, k, dev, 13)
+    a, b = values(x), values(w).T
+    bias = torch.randn(n, device=dev)
+    y = fp8.linear_forward(x, w, bias, out_dtype=torch.float32)
+    want = a @ b + bias.double()
+    assert ((y.double() - want).abs() <= product_bound(a, b, torch.float32) + (bias.double().abs() + want.abs()) * 2.0**-23).all()
+    assert torch.equal(y, fp8.linear_forward(x, w, bias, out_dtype=torch.float32))  # the order of the sums is fixed
+    dy = fp8.quantize(activations(m, n, torch.bfloat16, dev, 4) * 1e-3)
+    a, b = values(dy), values(w)
+    assert ((fp8.linear_input_grad(dy, w).double() - a @ b).abs() <= product_bound(a, b, torch.bfloat16)).all()
+
+
+def test_split_last_wave(dev):
+    """More tiles than CTA pairs and a long reduction: the last wave's tiles are split along K."""
+    from elf_b200.ops import fp8
+
+    m, n, k = 2304, 2304, 14336 + 200  # 81 tiles: 7 are left over on 74 pairs
+    x, w = operands(m, n, k, dev, 17)
+    a, b = values(x), values(w).T
+    y = fp8.linear_forward(x, w, out_dtype=torch.float32)
+    assert ((y.double() - a @ b).abs() <= product_bound(a, b, torch.float32)).all()
+    # the bound above grows with K; a part of a sum that is lost or added twice is far outside this
+    assert (y.double() - a @ b).norm() / (a @ b).norm() < 1e-4
+    for _ in range(3):
+        assert torch.equal(y, fp8.linear_forward(x, w, out_dtype=torch.float32))

@@ -7,6 +7,7 @@
 #include <utility>
 #include <vector>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include "fp8_ops.h"
@@ -87,8 +88,8 @@ Scaled scaled(const at::Tensor& data, const at::Tensor& scale, int64_t row_shift
 }
 
 // New tensor whose rows are `pitch` elements apart.
-at::Tensor new_rows(at::IntArrayRef lead, int64_t cols, int64_t pitch, const at::TensorOptions& opt) {
-  std::vector<int64_t> sizes(lead.begin(), lead.end()), strides(lead.size() + 1);
+at::Tensor new_rows(at::IntArrayRef lead, int64_t cols, int64_t pitch, at::ScalarType dtype, const at::Device& dev) {
+  c10::SmallVector<int64_t, 6> sizes(lead.begin(), lead.end()), strides(lead.size() + 1);
   sizes.push_back(cols);
   strides.back() = 1;
   int64_t step = pitch;
@@ -96,15 +97,16 @@ at::Tensor new_rows(at::IntArrayRef lead, int64_t cols, int64_t pitch, const at:
     strides[i] = step;
     step *= std::max<int64_t>(sizes[i], 1);
   }
-  return at::empty_strided(sizes, strides, opt);
+  return at::detail::empty_strided_cuda(sizes, strides, dtype, dev);  // past the dispatcher
 }
+
+at::Tensor dense(at::IntArrayRef sizes, at::ScalarType dtype, const at::Device& dev) { return at::detail::empty_cuda(sizes, dtype, dev, c10::nullopt); }
 
 // Block-scaled tensor [*lead, cols] with the row pitches the products want.
 std::pair<at::Tensor, at::Tensor> new_scaled(at::IntArrayRef lead, int64_t cols, bool tiles, const at::Device& dev) {
-  const auto opt = at::TensorOptions().device(dev);
   const int64_t tile_rows[1] = {tiles ? blocks_of(lead[0]) : 0};
-  return {new_rows(lead, cols, round_up(cols, 16), opt.dtype(at::kFloat8_e4m3fn)),
-          new_rows(tiles ? at::IntArrayRef(tile_rows, 1) : lead, blocks_of(cols), round_up(blocks_of(cols), 4), opt.dtype(at::kByte))};
+  return {new_rows(lead, cols, round_up(cols, 16), at::kFloat8_e4m3fn, dev),
+          new_rows(tiles ? at::IntArrayRef(tile_rows, 1) : lead, blocks_of(cols), round_up(blocks_of(cols), 4), at::kByte, dev)};
 }
 
 at::IntArrayRef lead_of(const at::Tensor& t) { return t.sizes().slice(0, t.dim() - 1); }
@@ -131,7 +133,7 @@ at::Tensor dequantize(const at::Tensor& data, const at::Tensor& scale, int64_t r
   const auto dev = data.device();
   const Scaled s = scaled(data, scale, row_shift, "data", dev);
   c10::cuda::CUDAGuard g(dev);
-  at::Tensor y = out.has_value() ? *out : at::empty(data.sizes(), at::TensorOptions().device(dev).dtype(dtype));
+  at::Tensor y = out.has_value() ? *out : dense(data.sizes(), dtype, dev);
   TORCH_CHECK(y.sizes() == data.sizes(), "out must have the shape of data");
   const Mat m = matrix(y, "out", dev, false);
   check(elfb::fp8_dequantize(s.data.bytes(), s.data.pitch, s.scale.bytes(), s.scale.pitch, int(row_shift), y.data_ptr(), elem_of(y, "out"), m.pitch,
@@ -160,10 +162,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> rmsnorm(const at::Ten
   if (residual.has_value()) {
     TORCH_CHECK(residual->sizes() == x.sizes(), "residual must match x");
     res = dense_bf16(*residual, "residual", dev);
-    h = at::empty(x.sizes(), x.options());
+    h = dense(x.sizes(), at::kBFloat16, dev);
   }
   auto q = new_scaled(lead_of(x), dim, false, dev);
-  auto rstd = at::empty(lead_of(x), x.options().dtype(at::kFloat));
+  auto rstd = dense(lead_of(x), at::kFloat, dev);
   const Scaled s = scaled(q.first, q.second, 0, "data", dev, false);
   check(elfb::fp8_rmsnorm(x.data_ptr(), res.defined() ? res.data_ptr() : nullptr, w.data_ptr(), res.defined() ? h.data_ptr() : nullptr, rstd.data_ptr<float>(),
                           s.data.bytes(), s.data.pitch, s.scale.bytes(), s.scale.pitch, rows, int(dim), float(eps), cur()),
@@ -199,7 +201,7 @@ Operand operand(const at::Tensor& data, const at::Tensor& scale, int64_t row_shi
   TORCH_CHECK(r.s.data.rows <= INT_MAX - 1024, name, " has too many rows");
   if (!r.s.data.aligned(16)) {  // TMA wants rows on 16-byte boundaries: a copy with padded rows
     const int64_t lead[1] = {r.s.data.rows};
-    at::Tensor padded = new_rows(at::IntArrayRef(lead, 1), r.s.data.cols, round_up(r.s.data.cols, 16), data.options());
+    at::Tensor padded = new_rows(at::IntArrayRef(lead, 1), r.s.data.cols, round_up(r.s.data.cols, 16), data.scalar_type(), dev);
     padded.copy_(r.s.data.t.dim() == 2 ? r.s.data.t : r.s.data.t.reshape({r.s.data.rows, r.s.data.cols}));
     r.s.data = matrix(padded, name, dev, false);
   }
@@ -244,7 +246,7 @@ at::Tensor gemm(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor
   TORCH_CHECK(g.K == (b_mn_major ? ob.s.data.rows : ob.s.data.cols), "the operands disagree on the reduction length");
   auto sizes = a.sizes().vec();
   sizes.back() = g.N;
-  at::Tensor d = at::empty(sizes, at::TensorOptions().device(dev).dtype(dtype));
+  at::Tensor d = dense(sizes, dtype, dev);
   g.d = d.data_ptr();
   g.ldd = g.N;
   g.out = elem_of(d, "the product");
@@ -257,7 +259,7 @@ at::Tensor gemm(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor
   // from the caching allocator, call by call: two streams or two captured graphs never share it
   at::Tensor workspace;
   if (const size_t bytes = elfb::fp8_gemm_workspace(g, sm_count(dev))) {
-    workspace = at::empty({int64_t(bytes)}, at::TensorOptions().device(dev).dtype(at::kByte));
+    workspace = dense({int64_t(bytes)}, at::kByte, dev);
     g.workspace = workspace.data_ptr();
   }
   const char* err = elfb::fp8_gemm(g, sm_count(dev), cur());
@@ -302,7 +304,7 @@ std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>, c10::optional<at::
   // from the caching allocator, call by call: two streams or two captured graphs never share it
   at::Tensor workspace;
   if (const size_t bytes = elfb::fp8_gemm_workspace(g, sm_count(dev))) {
-    workspace = at::empty({int64_t(bytes)}, at::TensorOptions().device(dev).dtype(at::kByte));
+    workspace = dense({int64_t(bytes)}, at::kByte, dev);
     g.workspace = workspace.data_ptr();
   }
   const char* err = elfb::fp8_gemm(g, sm_count(dev), cur());

@@ -68,7 +68,9 @@ __device__ __forceinline__ void combine_scales(const Scales& s, int g, int block
   const bool word = s.words && 4 * g + 4 <= blocks;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t(&v)[4] = r.v[s.row_shift ? 0 : j];
+    uint32_t v[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) v[b] = s.row_shift ? r.v[0][b] : r.v[j][b];
     w[j] = word ? v[0] : v[0] | v[1] << 8 | v[2] << 16 | v[3] << 24;
   }
 }
@@ -144,87 +146,16 @@ __device__ __forceinline__ void store_quad(float (&s)[4], int row, int col, cons
 }
 
 // 16 values times 2^(127 - byte) to e4m3
-__device__ __forceinline__ void scale_and_store(const uint32_t (&v)[16], float inv, uint8_t* dst) {
+__device__ __forceinline__ void scale_and_store(const float* v, float inv, uint8_t* dst) {
   uint32_t q[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     float s[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float x = __uint_as_float(v[4 * j + k]);
-      s[k] = nan_unless_finite(mul_exact(x, inv), x);
-    }
+    for (int k = 0; k < 4; ++k) s[k] = nan_unless_finite(mul_exact(v[4 * j + k], inv), v[4 * j + k]);
     q[j] = to_e4m3x4(s[0], s[1], s[2], s[3]);
   }
   *reinterpret_cast<uint4*>(dst) = make_uint4(q[0], q[1], q[2], q[3]);
-}
-
-// One tile of the gated form: columns 0..127 of the accumulator are gate, 128..255 up.  One thread per
-// row.  `release` is called once the 32 columns shared with the other accumulator have been read for
-// the last time (ACC 0: the end of up, ACC 1: the beginning of gate).
-//   first sweep (with a checkpoint): the maxima of the row's gate and up blocks
-//   second sweep: gate and up leave in 8 bits, silu(gate) * up collects in 128 registers
-//   then the activation's block is scaled and leaves
-template <int ACC, typename Release>
-__device__ __forceinline__ void gated_tile(uint32_t taddr, int row, int f0, int f, const Params& p, Release&& release) {
-  const bool live = row < p.M;
-  const bool keep = p.gu != nullptr;
-  uint32_t top[2] = {0, 0};
-  uint32_t v[16];
-  if (keep) {
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        tmem_ld_32x32b_x16(taddr + half * 128 + c * 16, v);
-        tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < 16; ++j) top[half] = max(top[half], finite_bits(__uint_as_float(v[j])));
-      }
-    }
-  }
-  const uint32_t byte_g = block_exponent(top[0]), byte_u = block_exponent(top[1]);
-  const float inv_g = inverse_exponent_value(byte_g), inv_u = inverse_exponent_value(byte_u);
-  uint8_t* gate_dst = p.gu + (long long)row * p.ld_gu + f0;
-  float act[128];
-  uint32_t top_act = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    constexpr int kFirst = ACC == 0 ? 7 : 0, kStep = ACC == 0 ? -1 : 1;
-    const int c = kFirst + kStep * i;
-    tmem_ld_32x32b_x16(taddr + c * 16, v);
-    tmem_ld_wait();
-    if (live && keep) scale_and_store(v, inv_g, gate_dst + c * 16);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float g = __uint_as_float(v[j]);
-      act[c * 16 + j] = g * __fdividef(1.f, 1.f + __expf(-g));
-    }
-    tmem_ld_32x32b_x16(taddr + 128 + c * 16, v);
-    tmem_ld_wait();
-    if (i == 1) release();
-    if (live && keep) scale_and_store(v, inv_u, gate_dst + f + c * 16);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      act[c * 16 + j] *= __uint_as_float(v[j]);
-      top_act = max(top_act, finite_bits(act[c * 16 + j]));
-    }
-  }
-  const uint32_t byte = block_exponent(top_act);
-  if (!live) return;
-  uint8_t* dst = p.act + (long long)row * p.ld_act + f0;
-#pragma unroll
-  for (int c = 0; c < 8; ++c) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(act[c * 16 + j]);
-    scale_and_store(v, inverse_exponent_value(byte), dst + c * 16);
-  }
-  p.act_scale[(long long)row * p.ld_act_scale + f0 / 128] = uint8_t(byte);
-  if (keep) {
-    uint8_t* s = p.gu_scale + (long long)row * p.ld_gu_scale;
-    s[f0 / 128] = uint8_t(byte_g);
-    s[(f + f0) / 128] = uint8_t(byte_u);
-  }
 }
 
 // The layout tcgen05.cp wants: 16 bytes per lane, word j for row 32 j + lane.

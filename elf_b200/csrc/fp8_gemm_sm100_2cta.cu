@@ -27,11 +27,14 @@ constexpr int BN = 256;
 constexpr int STAGES = 6;
 constexpr int STAGE_BYTES = 2 * BOX_BYTES;  // per CTA: 128 rows of A, 128 rows of B
 constexpr int SLOTS = STAGES / 2;           // two consecutive stages are freed by one commit
-constexpr int NUM_THREADS = 224;
+constexpr int EPI_WARPS = 8;     // two per quarter of the TMEM lanes, each with one half of the columns
+constexpr int EPI_THREADS = EPI_WARPS * 32;
+constexpr int NUM_THREADS = 96 + EPI_THREADS;
 constexpr int SF_BYTES = 3 * 512;           // scale words of a slot: 128 rows of A, 256 columns of B
 constexpr int GROUP_M = 4;  // tile rows (of 256) that are swept together before moving to the next columns
 constexpr int ACC1 = 224;   // first column of the second accumulator: shares 32 with the first
-constexpr size_t SMEM_BYTES = size_t(STAGES) * STAGE_BYTES + SLOTS * SF_BYTES + 1024 /*align slack*/ + 256 /*barriers*/;
+constexpr int EXCHANGE_BYTES = 3 * 2 * BM * 4;  // block maxima that the two halves of a row tell each other (gated forms)
+constexpr size_t SMEM_BYTES = size_t(STAGES) * STAGE_BYTES + SLOTS * SF_BYTES + EXCHANGE_BYTES + 1024 /*align slack*/ + 256 /*barriers*/;
 constexpr int PART_FLOATS = BM * BN;  // one CTA's half of a tile in the workspace
 
 struct Schedule {
@@ -110,6 +113,64 @@ __device__ __forceinline__ void umma_commit_both(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(uint16_t(3)) : "memory");
 }
 
+// One tile of the gated form: columns 0..127 of the accumulator are gate, 128..255 up.  A thread takes 64 columns
+// of gate and the same of up of one row into registers and gives the accumulator back at once; the maxima of the
+// three blocks (gate, up, activation) are exchanged with the thread that has the row's other half.
+template <typename Release>
+__device__ __forceinline__ void gated_tile(uint32_t taddr, int row, int half, int f0, int f, const Params& p, uint32_t* exchange, Release&& release) {
+  uint32_t raw[4][32];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    tmem_ld_32x32b_x32(taddr + half * 64 + c * 32, raw[c]);
+    tmem_ld_32x32b_x32(taddr + 128 + half * 64 + c * 32, raw[2 + c]);
+  }
+  tmem_ld_wait();
+  release();
+  float g[64], u[64];
+#pragma unroll
+  for (int j = 0; j < 64; ++j) g[j] = __uint_as_float(raw[j / 32][j % 32]), u[j] = __uint_as_float(raw[2 + j / 32][j % 32]);
+  const bool live = row < p.M;
+  const int col = f0 + half * 64;
+  auto block_byte = [&](int which, uint32_t top) {  // exponent byte of the row's block, from both halves
+    exchange[(which * 2 + half) * BM] = top;
+    named_barrier_sync(1, EPI_THREADS);
+    return block_exponent(max(top, exchange[(which * 2 + (half ^ 1)) * BM]));
+  };
+  if (p.gu != nullptr) {
+    uint32_t top_g = 0, top_u = 0;
+#pragma unroll
+    for (int j = 0; j < 64; ++j) top_g = max(top_g, finite_bits(g[j])), top_u = max(top_u, finite_bits(u[j]));
+    exchange[half * BM] = top_g;
+    const uint32_t byte_u = block_byte(1, top_u);
+    const uint32_t byte_g = block_exponent(max(top_g, exchange[(half ^ 1) * BM]));
+    if (live) {
+      uint8_t* dst = p.gu + (long long)row * p.ld_gu + col;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) scale_and_store(g + 16 * c, inverse_exponent_value(byte_g), dst + 16 * c);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) scale_and_store(u + 16 * c, inverse_exponent_value(byte_u), dst + f + 16 * c);
+      if (half == 0) {
+        uint8_t* s = p.gu_scale + (long long)row * p.ld_gu_scale;
+        s[f0 / 128] = uint8_t(byte_g);
+        s[(f + f0) / 128] = uint8_t(byte_u);
+      }
+    }
+  }
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 64; ++j) {
+    g[j] = g[j] * __fdividef(1.f, 1.f + __expf(-g[j])) * u[j];
+    top = max(top, finite_bits(g[j]));
+  }
+  const uint32_t byte = block_byte(2, top);
+  if (live) {
+    uint8_t* dst = p.act + (long long)row * p.ld_act + col;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) scale_and_store(g + 16 * c, inverse_exponent_value(byte), dst + 16 * c);
+    if (half == 0) p.act_scale[(long long)row * p.ld_act_scale + f0 / 128] = uint8_t(byte);
+  }
+}
+
 template <bool B_MN, bool GATED, typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
 fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ Params p,
@@ -118,7 +179,8 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_aligned = smem_raw + (smem_base - smem_u32(smem_raw));
   const uint32_t sf_base = smem_base + STAGES * STAGE_BYTES;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_aligned + size_t(STAGES) * STAGE_BYTES + SLOTS * SF_BYTES);
+  uint32_t* exchange = reinterpret_cast<uint32_t*>(smem_aligned + size_t(STAGES) * STAGE_BYTES + SLOTS * SF_BYTES);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_aligned + size_t(STAGES) * STAGE_BYTES + SLOTS * SF_BYTES + EXCHANGE_BYTES);
   const uint32_t bar0 = smem_u32(bars);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
   auto empty_bar = [&](int slot) { return bar0 + 8u * (STAGES + slot); };
@@ -142,7 +204,7 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     *abort_flag = 0;
     for (int s = 0; s < STAGES; ++s) mbar_init(full_bar(s), s & 1 ? 1 : 3);  // a slot's first stage also waits for both scale warps
     for (int s = 0; s < SLOTS; ++s) mbar_init(empty_bar(s), 1);
-    mbar_init(acc_free_bar, 8);
+    mbar_init(acc_free_bar, 2 * EPI_WARPS);
     for (int a = 0; a < 2; ++a) mbar_init(acc_full_bar(a), 1);
     fence_barrier_init();
     prefetch_tensormap(&tmap_a);
@@ -240,17 +302,18 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       }
     }
     __syncwarp();
-  } else if (warp < 6) {
-    // ------------------------------------------------------------------ epilogue (warps 2..5 of both CTAs)
-    const int quarter = warp & 3;  // TMEM lanes [32*quarter, 32*quarter+32) belong to this warp
+  } else if (warp < 2 + EPI_WARPS) {
+    // ------------------------------------------------------------------ epilogue (warps 2..9 of both CTAs)
+    const int quarter = warp & 3;       // TMEM lanes [32*quarter, 32*quarter+32) belong to this warp
+    const int half = (warp - 2) >> 2;   // plain forms: columns 128 * half onwards; gated: 64 of gate and of up
     const uint32_t free_bar = map_to_cta(acc_free_bar, 0);
     int i = 0;
     for (int u = pair_id; u < sched.total_units; u += num_pairs, ++i) {
       const Unit unit = unit_at(u, sched, k_blocks, width);
       const int acc = i & 1;
       const int row = unit.m0 + int(cta) * BM + quarter * 32 + lane;
-      // all four warps go on or none does: they meet at barriers below
-      if (!named_barrier_all(1, 128, mbar_wait(acc_full_bar(acc), uint32_t(i >> 1) & 1u, abort_flag))) break;
+      // all warps go on or none does: they meet at barriers below
+      if (!named_barrier_all(1, EPI_THREADS, mbar_wait(acc_full_bar(acc), uint32_t(i >> 1) & 1u, abort_flag))) break;
       tc_fence_after_sync();
       const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + acc * ACC1;
       auto release = [&] {
@@ -259,14 +322,13 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         if (lane == 0) mbar_arrive_cluster(free_bar);
       };
       if constexpr (GATED) {
-        if (acc == 0) gated_tile<0>(taddr, row, unit.n0, f, p, release);
-        else gated_tile<1>(taddr, row, unit.n0, f, p, release);
+        gated_tile(taddr, row, half, unit.n0, f, p, exchange + quarter * 32 + lane, release);
       } else {
-        constexpr int CHUNKS = BN / 32;
+        constexpr int CHUNKS = BN / 64;  // of 32 columns, for each half
         if (unit.rest < 0) {
 #pragma unroll 1
           for (int j = 0; j < CHUNKS; ++j) {
-            const int c = acc == 0 ? CHUNKS - 1 - j : j;  // the shared columns first
+            const int c = half * CHUNKS + (acc == 0 ? CHUNKS - 1 - j : j);  // the shared columns first
             uint32_t v[32];
             tmem_ld_32x32b_x32(taddr + c * 32, v);
             tmem_ld_wait();
@@ -282,12 +344,12 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
           float4* tile = reinterpret_cast<float4*>(parts) + ((long long)unit.rest * sched.ksplit * 2 + cta) * (PART_FLOATS / 4) + quarter * 32 + lane;
           constexpr long long PART_STEP = 2 * (PART_FLOATS / 4);
           if (threadIdx.x == 64) *arrived = *reinterpret_cast<volatile unsigned int*>(done);
-          named_barrier_sync(1, 128);
+          named_barrier_sync(1, EPI_THREADS);
           bool last = *arrived == unsigned(others);
           if (!last) {
             float4* mine = tile + unit.part * PART_STEP;
 #pragma unroll 1
-            for (int c = 0; c < CHUNKS; ++c) {
+            for (int c = half * CHUNKS; c < (half + 1) * CHUNKS; ++c) {
               uint32_t v[32];
               tmem_ld_32x32b_x32(taddr + c * 32, v);
               tmem_ld_wait();
@@ -298,15 +360,15 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
               }
             }
             __threadfence();
-            named_barrier_sync(1, 128);  // every thread has also read `arrived`
+            named_barrier_sync(1, EPI_THREADS);  // every thread has also read `arrived`
             if (threadIdx.x == 64) *arrived = atomicAdd(done, 1u);
-            named_barrier_sync(1, 128);
+            named_barrier_sync(1, EPI_THREADS);
             last = *arrived == unsigned(others);
           }
           if (last) {
             __threadfence();
 #pragma unroll 1
-            for (int c = 0; c < CHUNKS; ++c) {
+            for (int c = half * CHUNKS; c < (half + 1) * CHUNKS; ++c) {
               uint32_t v[32];
               tmem_ld_32x32b_x32(taddr + c * 32, v);
               tmem_ld_wait();
@@ -333,13 +395,13 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
               store_chunk<T>(v, row, col, p);
             }
           }
-          named_barrier_sync(1, 128);  // `arrived` may be written again
+          named_barrier_sync(1, EPI_THREADS);  // `arrived` may be written again
           release();
         }
       }
     }
   } else {
-    // ------------------------------------------------------------------ scale words (warp 6 of both CTAs)
+    // ------------------------------------------------------------------ scale words (warp 10 of both CTAs)
     // A second producer of the ring: the words of a group of four blocks go to both slots of the group.  Those
     // of the next group are fetched from global memory before a slot is waited for.
     int u = pair_id, g = 0, slot = 0;

@@ -442,16 +442,14 @@ def _weight_copy(q: Optional[BlockScaled], w: torch.Tensor, name: str) -> BlockS
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, bias, q, train):
+    def forward(ctx, x, w, bias, q):
         xq = quantize(x)
-        y = linear_forward(xq, _weight_copy(q, w, "linear"), bias, x.dtype)
-        if train:
-            # the weight's own tensor is saved when no 8-bit copy was given: the backward makes it
-            # again instead of holding one per call in flight
-            ctx.given = q is not None
-            ctx.w_dtype, ctx.x_dtype, ctx.bias_dtype = w.dtype, x.dtype, None if bias is None else bias.dtype
-            ctx.save_for_backward(xq.data, xq.scale, *((q.data, q.scale) if q is not None else (w,)))
-        return y
+        # the weight's own tensor is saved when no 8-bit copy was given: the backward makes it
+        # again instead of holding one per call in flight
+        ctx.given = q is not None
+        ctx.w_dtype, ctx.x_dtype, ctx.bias_dtype = w.dtype, x.dtype, None if bias is None else bias.dtype
+        ctx.save_for_backward(xq.data, xq.scale, *((q.data, q.scale) if q is not None else (w,)))
+        return linear_forward(xq, _weight_copy(q, w, "linear"), bias, x.dtype)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -466,7 +464,7 @@ class _Linear(torch.autograd.Function):
             dw = linear_weight_grad(dyq, BlockScaled._made(data, scale), out_dtype=ctx.w_dtype)
         if ctx.needs_input_grad[2]:
             db = _matrix(dy).float().sum(0).to(ctx.bias_dtype)
-        return dx, dw, db, None, None
+        return dx, dw, db, None
 
 
 def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, w_q: Optional[BlockScaled] = None) -> torch.Tensor:
@@ -478,23 +476,21 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     _check_differentiable("linear", x, w, bias)
     if not (w.dim() == 2 and x.dim() >= 1 and x.shape[-1] == w.shape[1]):
         raise ValueError(f"linear: x {tuple(x.shape)} does not match a weight of shape {tuple(w.shape)}")
-    train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias))
-    return _Linear.apply(x, w, bias, w_q, train)
+    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias))):
+        return linear_forward(quantize(x), _weight_copy(w_q, w, "linear"), bias, x.dtype)
+    return _Linear.apply(x, w, bias, w_q)
 
 
 class _GatedFFN(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w_gate_up, w_down, gate_up_q, down_q, train):
-        gq, dq = _weight_copy(gate_up_q, w_gate_up, "gated_ffn"), _weight_copy(down_q, w_down, "gated_ffn")
+    def forward(ctx, x, w_gate_up, w_down, gate_up_q, down_q):
         xq = quantize(x)
-        act, gu = gated_forward(xq, gq, keep=train)
-        y = linear_forward(act, dq, None, x.dtype)
-        if train:
-            ctx.given = (gate_up_q is not None, down_q is not None)
-            ctx.dtypes = (x.dtype, w_gate_up.dtype, w_down.dtype)
-            held = [t for q, w in ((gate_up_q, w_gate_up), (down_q, w_down)) for t in ((q.data, q.scale) if q is not None else (w,))]
-            ctx.save_for_backward(xq.data, xq.scale, act.data, act.scale, gu.data, gu.scale, *held)
-        return y
+        act, gu = gated_forward(xq, _weight_copy(gate_up_q, w_gate_up, "gated_ffn"))
+        ctx.given = (gate_up_q is not None, down_q is not None)
+        ctx.dtypes = (x.dtype, w_gate_up.dtype, w_down.dtype)
+        held = [t for q, w in ((gate_up_q, w_gate_up), (down_q, w_down)) for t in ((q.data, q.scale) if q is not None else (w,))]
+        ctx.save_for_backward(xq.data, xq.scale, act.data, act.scale, gu.data, gu.scale, *held)
+        return linear_forward(act, _weight_copy(down_q, w_down, "gated_ffn"), None, x.dtype)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -518,7 +514,7 @@ class _GatedFFN(torch.autograd.Function):
                 dx = linear_input_grad(dgu, gate_up_q, x_dtype)
             if ctx.needs_input_grad[1]:
                 dw_gate_up = linear_weight_grad(dgu, xq, out_dtype=gate_up_dtype)
-        return dx, dw_gate_up, dw_down, None, None, None
+        return dx, dw_gate_up, dw_down, None, None
 
 
 def gated_ffn(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, gate_up_q: Optional[BlockScaled] = None,
@@ -534,8 +530,10 @@ def gated_ffn(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, ga
         raise ValueError(f"gated_ffn: shapes x {tuple(x.shape)}, w_gate_up {tuple(w_gate_up.shape)}, w_down {tuple(w_down.shape)} do not match")
     if w_down.shape[1] % BLOCK:
         raise ValueError(f"gated_ffn: the inner width must be a multiple of {BLOCK}, got {w_down.shape[1]}")
-    train = torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_gate_up, w_down))
-    return _GatedFFN.apply(x, w_gate_up, w_down, gate_up_q, down_q, train)
+    if not (torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_gate_up, w_down))):
+        act, _ = gated_forward(quantize(x), _weight_copy(gate_up_q, w_gate_up, "gated_ffn"), keep=False)
+        return linear_forward(act, _weight_copy(down_q, w_down, "gated_ffn"), None, x.dtype)
+    return _GatedFFN.apply(x, w_gate_up, w_down, gate_up_q, down_q)
 
 
 def _check_differentiable(what: str, x: torch.Tensor, *others) -> None:

@@ -173,23 +173,6 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> rmsnorm(const at::Ten
   return {q.first, q.second, rstd, h};
 }
 
-// d silu(gate) up for dact [..., F] fp32 and gate | up = gu [..., 2F]
-std::pair<at::Tensor, at::Tensor> swiglu_bwd(const at::Tensor& dact, const at::Tensor& gu, const at::Tensor& gu_scale) {
-  const auto dev = dact.device();
-  c10::cuda::CUDAGuard g(dev);
-  const Mat d = matrix(dact, "dact", dev);
-  const Scaled s = scaled(gu, gu_scale, 0, "gate_up", dev);
-  TORCH_CHECK(dact.scalar_type() == at::kFloat && d.cols % 128 == 0, "dact must be fp32, its width a multiple of 128");
-  TORCH_CHECK(s.data.rows == d.rows && s.data.cols == 2 * d.cols, "gate_up does not match dact");
-  TORCH_CHECK(d.aligned(16) && s.data.aligned(16), "rows must be 16-byte aligned");
-  auto q = new_scaled(lead_of(gu), s.data.cols, false, dev);
-  const Scaled o = scaled(q.first, q.second, 0, "d_gate_up", dev, false);
-  check(elfb::fp8_swiglu_backward(static_cast<const float*>(d.t.data_ptr()), d.pitch, s.data.bytes(), s.data.pitch, s.scale.bytes(), s.scale.pitch, o.data.bytes(),
-                                  o.data.pitch, o.scale.bytes(), o.scale.pitch, d.rows, int(d.cols), cur()),
-        "fp8_swiglu_backward");
-  return q;
-}
-
 // An operand of a product and the tensors that keep its memory alive until the launch is queued.
 struct Operand {
   Scaled s;
@@ -231,6 +214,18 @@ int* status_ptr(const at::Tensor& status, const at::Device& dev) {
   return status.data_ptr<int>();
 }
 
+void launch(elfb::Fp8GemmArgs& g, const at::Tensor& status, const at::Device& dev, const char* what) {
+  g.status = status_ptr(status, dev);
+  // from the caching allocator, call by call: two streams or two captured graphs never share it
+  at::Tensor workspace;
+  if (const size_t bytes = elfb::fp8_gemm_workspace(g, sm_count(dev))) {
+    workspace = dense({int64_t(bytes)}, at::kByte, dev);
+    g.workspace = workspace.data_ptr();
+  }
+  const char* err = elfb::fp8_gemm(g, sm_count(dev), cur());
+  TORCH_CHECK(err == nullptr, "elf_b200 ", what, ": ", err);
+}
+
 // a . b^T (b [N, K]), or a . b (b_mn_major, b [K, N]); a [..., K]
 at::Tensor gemm(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& b, const at::Tensor& b_scale, int64_t b_row_shift, bool b_mn_major,
                 at::ScalarType dtype, const c10::optional<at::Tensor>& bias, const at::Tensor& status) {
@@ -255,15 +250,7 @@ at::Tensor gemm(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor
                 "the bias must be a contiguous [N] tensor of the product's dtype");
     g.bias = bias->data_ptr();
   }
-  g.status = status_ptr(status, dev);
-  // from the caching allocator, call by call: two streams or two captured graphs never share it
-  at::Tensor workspace;
-  if (const size_t bytes = elfb::fp8_gemm_workspace(g, sm_count(dev))) {
-    workspace = dense({int64_t(bytes)}, at::kByte, dev);
-    g.workspace = workspace.data_ptr();
-  }
-  const char* err = elfb::fp8_gemm(g, sm_count(dev), cur());
-  TORCH_CHECK(err == nullptr, "elf_b200 fp8_gemm: ", err);
+  launch(g, status, dev, "fp8_gemm");
   return d;
 }
 
@@ -284,7 +271,7 @@ std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>, c10::optional<at::
   TORCH_CHECK(g.N % 256 == 0, "the width of gate and of up must be a multiple of 128");
   auto act = new_scaled(lead_of(a), g.N / 2, false, dev);
   const Scaled sa = scaled(act.first, act.second, 0, "act", dev, false);
-  g.gated = true;
+  g.form = elfb::Fp8Form::kGated;
   g.act = sa.data.bytes();
   g.ld_act = sa.data.pitch;
   g.act_scale = sa.scale.bytes();
@@ -300,16 +287,38 @@ std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>, c10::optional<at::
     gu_data = gu.first;
     gu_scale = gu.second;
   }
-  g.status = status_ptr(status, dev);
-  // from the caching allocator, call by call: two streams or two captured graphs never share it
-  at::Tensor workspace;
-  if (const size_t bytes = elfb::fp8_gemm_workspace(g, sm_count(dev))) {
-    workspace = dense({int64_t(bytes)}, at::kByte, dev);
-    g.workspace = workspace.data_ptr();
-  }
-  const char* err = elfb::fp8_gemm(g, sm_count(dev), cur());
-  TORCH_CHECK(err == nullptr, "elf_b200 fp8_gated: ", err);
+  launch(g, status, dev, "fp8_gated");
   return {act.first, act.second, gu_data, gu_scale};
+}
+
+// gradient [..., 2F] of gate | up for the gradient dy [..., D] of the block's output, w_down [D, F] and gate | up from their checkpoint
+std::pair<at::Tensor, at::Tensor> gated_bwd(const at::Tensor& dy, const at::Tensor& dy_scale, const at::Tensor& w, const at::Tensor& w_scale,
+                                            const at::Tensor& gu, const at::Tensor& gu_scale, const at::Tensor& status) {
+  const auto dev = dy.device();
+  c10::cuda::CUDAGuard guard(dev);
+  const Operand oa = operand(dy, dy_scale, 0, false, "the gradient", dev), ob = operand(w, w_scale, 7, true, "the weight", dev),
+                og = operand(gu, gu_scale, 0, false, "gate_up", dev);
+  elfb::Fp8GemmArgs g;
+  g.form = elfb::Fp8Form::kGatedBackward;
+  g.a = oa.o;
+  g.b = ob.o;
+  g.M = int(oa.s.data.rows);
+  g.K = int(oa.s.data.cols);
+  g.N = int(ob.s.data.cols);
+  TORCH_CHECK(g.K == ob.s.data.rows, "the operands disagree on the reduction length");
+  TORCH_CHECK(g.N % 128 == 0 && og.s.data.rows == g.M && og.s.data.cols == 2 * int64_t(g.N), "gate_up does not match the gradient and the weight");
+  auto dgu = new_scaled(lead_of(gu), 2 * int64_t(g.N), false, dev);
+  const Scaled sd = scaled(dgu.first, dgu.second, 0, "d_gate_up", dev, false);
+  g.act = sd.data.bytes();
+  g.ld_act = sd.data.pitch;
+  g.act_scale = sd.scale.bytes();
+  g.ld_act_scale = sd.scale.pitch;
+  g.gu = og.s.data.bytes();
+  g.ld_gu = og.s.data.pitch;
+  g.gu_scale = og.s.scale.bytes();
+  g.ld_gu_scale = og.s.scale.pitch;
+  launch(g, status, dev, "fp8_gated_bwd");
+  return dgu;
 }
 
 }  // namespace
@@ -318,8 +327,8 @@ void register_fp8(pybind11::module_& m) {
   m.def("fp8_quantize", &quantize, py::arg("x"), py::arg("tiles"), py::arg("data") = c10::nullopt, py::arg("scale") = c10::nullopt);
   m.def("fp8_dequantize", &dequantize, py::arg("data"), py::arg("scale"), py::arg("row_shift"), py::arg("dtype"), py::arg("out") = c10::nullopt);
   m.def("fp8_rmsnorm", &rmsnorm, py::arg("x"), py::arg("w"), py::arg("eps"), py::arg("residual") = c10::nullopt);
-  m.def("fp8_swiglu_bwd", &swiglu_bwd, py::arg("dact"), py::arg("gu"), py::arg("gu_scale"));
   m.def("fp8_gemm", &gemm, py::arg("a"), py::arg("a_scale"), py::arg("b"), py::arg("b_scale"), py::arg("b_row_shift"), py::arg("b_mn_major"), py::arg("dtype"),
         py::arg("bias"), py::arg("status"));
   m.def("fp8_gated", &gated, py::arg("a"), py::arg("a_scale"), py::arg("b"), py::arg("b_scale"), py::arg("b_row_shift"), py::arg("keep"), py::arg("status"));
+  m.def("fp8_gated_bwd", &gated_bwd, py::arg("dy"), py::arg("dy_scale"), py::arg("w"), py::arg("w_scale"), py::arg("gu"), py::arg("gu_scale"), py::arg("status"));
 }

@@ -309,16 +309,16 @@ cudaError_t launch_rows128(const Fp8GemmArgs& g, const CUtensorMap& ta, const CU
 }
 
 cudaError_t launch_pair(const Fp8GemmArgs& g, const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int num_sms, cudaStream_t stream);
-size_t pair_workspace(int M, int N, int K, bool gated, int num_sms);
+size_t pair_workspace(const Fp8GemmArgs& g, int num_sms);
 
-// The gated form has one kernel; its tile holds a block of gate and one of up.
-bool use_pair(const Fp8GemmArgs& g) { return g.gated || g.M > 128; }
+// The gated forms, whose epilogues want whole blocks of 128 columns, have one kernel.
+bool use_pair(const Fp8GemmArgs& g) { return g.form != Fp8Form::kPlain || g.M > 128; }
 
 }  // namespace fp8
 
 size_t fp8_gemm_workspace(const Fp8GemmArgs& g, int num_sms) {
   if (g.M <= 0 || g.N <= 0 || g.K <= 0 || !fp8::use_pair(g)) return 0;
-  return fp8::pair_workspace(g.M, g.N, g.K, g.gated, num_sms);
+  return fp8::pair_workspace(g, num_sms);
 }
 
 const char* make_tmap_bytes(CUtensorMap* out, const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_cols, uint32_t box_rows);
@@ -335,10 +335,11 @@ const char* fp8_gemm(const Fp8GemmArgs& g, int num_sms, cudaStream_t stream) {
   Params p{g.M, g.N, g.K, Scales(g.a), Scales(g.b)};
   p.status = g.status;
   cudaError_t e;
-  if (g.gated) {
+  if (g.form != Fp8Form::kPlain) {
     auto aligned = [](const void* q, long long pitch) { return ((reinterpret_cast<uintptr_t>(q) | uintptr_t(pitch)) & 15) == 0; };
-    if (g.b.mn_major || g.N % 256 != 0) return "the gated product needs K-major weights and a width that is a multiple of 128";
-    if (!aligned(g.act, g.ld_act) || (g.gu && !aligned(g.gu, g.ld_gu))) return "8-bit outputs must be 16-byte aligned with a 16-byte multiple row pitch";
+    const bool backward = g.form == Fp8Form::kGatedBackward;
+    if (g.b.mn_major != backward || g.N % (backward ? 128 : 256) != 0) return "the gated product's width must be a multiple of 128";
+    if (!aligned(g.act, g.ld_act) || (g.gu && !aligned(g.gu, g.ld_gu))) return "8-bit matrices must be 16-byte aligned with a 16-byte multiple row pitch";
     p.act = g.act, p.act_scale = g.act_scale, p.gu = g.gu, p.gu_scale = g.gu_scale;
     p.ld_act = g.ld_act, p.ld_act_scale = g.ld_act_scale, p.ld_gu = g.ld_gu, p.ld_gu_scale = g.ld_gu_scale;
     e = launch_pair(g, ta, tb, p, num_sms, stream);

@@ -171,10 +171,72 @@ __device__ __forceinline__ void gated_tile(uint32_t taddr, int row, int half, in
   }
 }
 
-template <bool B_MN, bool GATED, typename T>
+// One tile of the gated form's backward: the accumulator holds the gradient of the activation, the thread one row
+// of one block of 128 columns.  gate and up come from their checkpoint.
+//   dgate = d up s (1 + gate (1 - s)),  dup = d gate s,  s = sigmoid(gate)
+// are formed twice, once for the maxima of their blocks and once to be scaled: 256 values per row would not stay in
+// registers beside the gradient, and the second exponential hides behind the next tile's products.
+template <typename Release>
+__device__ __forceinline__ void gated_backward_tile(uint32_t taddr, int row, int half, int n0, int f, const Params& p, Release&& release) {
+  uint32_t raw[4][32];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(taddr + half * 128 + c * 32, raw[c]);
+  tmem_ld_wait();
+  release();
+  const int col = n0 + half * 128;
+  if (row >= p.M || col >= f) return;
+  const uint8_t* gate = p.gu + (long long)row * p.ld_gu + col;
+  const uint8_t* scales = p.gu_scale + (long long)row * p.ld_gu_scale + col / 128;
+  const float sg = exponent_value(scales[0]), su = exponent_value(scales[f / 128]);
+  uint8_t* dst = p.act + (long long)row * p.ld_act + col;
+  uint32_t top_g = 0, top_u = 0;
+  float inv_g = 0.f, inv_u = 0.f;
+#pragma unroll
+  for (int pass = 0; pass < 2; ++pass) {
+    uint4 g4 = *reinterpret_cast<const uint4*>(gate), u4 = *reinterpret_cast<const uint4*>(gate + f);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const uint32_t gq[4] = {g4.x, g4.y, g4.z, g4.w}, uq[4] = {u4.x, u4.y, u4.z, u4.w};
+      if (c < 7) {
+        g4 = *reinterpret_cast<const uint4*>(gate + 16 * (c + 1));
+        u4 = *reinterpret_cast<const uint4*>(gate + f + 16 * (c + 1));
+      }
+      float dg[16], du[16];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float2 ge = from_e4m3x2((gq[j / 2] >> (16 * (j & 1))) & 0xffffu), ue = from_e4m3x2((uq[j / 2] >> (16 * (j & 1))) & 0xffffu);
+        const float g[2] = {ge.x * sg, ge.y * sg}, up[2] = {ue.x * su, ue.y * su};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float d = __uint_as_float(raw[c / 2][(c & 1) * 16 + 2 * j + k]);
+          const float sig = __fdividef(1.f, 1.f + __expf(-g[k]));
+          du[2 * j + k] = d * g[k] * sig;
+          dg[2 * j + k] = d * up[k] * sig * (1.f + g[k] * (1.f - sig));
+        }
+      }
+      if (pass == 0) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) top_g = max(top_g, finite_bits(dg[j])), top_u = max(top_u, finite_bits(du[j]));
+      } else {
+        scale_and_store(dg, inv_g, dst + 16 * c);
+        scale_and_store(du, inv_u, dst + f + 16 * c);
+      }
+    }
+    if (pass == 0) {
+      const uint32_t byte_g = block_exponent(top_g), byte_u = block_exponent(top_u);
+      inv_g = inverse_exponent_value(byte_g), inv_u = inverse_exponent_value(byte_u);
+      uint8_t* s = p.act_scale + (long long)row * p.ld_act_scale + col / 128;
+      s[0] = uint8_t(byte_g);
+      s[f / 128] = uint8_t(byte_u);
+    }
+  }
+}
+
+template <bool B_MN, Fp8Form FORM, typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
 fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ Params p,
                      const __grid_constant__ Schedule sched, float* __restrict__ parts, unsigned int* __restrict__ parts_done) {
+  constexpr bool GATED = FORM == Fp8Form::kGated;  // the tile's columns are 128 of gate and the same 128 of up
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_aligned = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -196,7 +258,7 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   const bool leader = cta == 0;
   const int pair_id = blockIdx.x >> 1;
   const int num_pairs = gridDim.x >> 1;
-  const int f = p.N / 2;  // gated: width of the activation
+  const int f = GATED ? p.N / 2 : p.N;  // gated forms: width of the activation
   const int width = GATED ? 128 : BN;
   const int k_blocks = (p.K + BK - 1) / BK;
 
@@ -323,6 +385,8 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       };
       if constexpr (GATED) {
         gated_tile(taddr, row, half, unit.n0, f, p, exchange + quarter * 32 + lane, release);
+      } else if constexpr (FORM == Fp8Form::kGatedBackward) {
+        gated_backward_tile(taddr, row, half, unit.n0, f, p, release);
       } else {
         constexpr int CHUNKS = BN / 64;  // of 32 columns, for each half
         if (unit.rest < 0) {
@@ -476,15 +540,15 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   }
 }
 
-Schedule make_schedule(int M, int N, int K, bool gated, int num_pairs) {
+Schedule make_schedule(int M, int N, int K, Fp8Form form, int num_pairs) {
   Schedule s;
   const int k_blocks = (K + BK - 1) / BK, groups = (k_blocks + 3) / 4;
   s.tiles_m = (M + 2 * BM - 1) / (2 * BM);
-  s.tiles_n = gated ? N / 256 : (N + BN - 1) / BN;
+  s.tiles_n = (N + BN - 1) / BN;  // gated: N is a multiple of 256
   const long long tiles = (long long)s.tiles_m * s.tiles_n;
   const int rem = int(tiles % num_pairs);
   s.ksplit = 1;
-  if (rem != 0 && !gated) {
+  if (rem != 0 && form == Fp8Form::kPlain) {
     // cycles of the last wave: measured 800 per block of K, and for split tiles about 10 us for clearing the
     // counters and exchanging the sums.  4096 x 4096 x K (34 tiles left over): K = 14336 takes 217 us split in two
     // and 227 us whole, K = 4096 82 and 79.
@@ -503,9 +567,9 @@ Schedule make_schedule(int M, int N, int K, bool gated, int num_pairs) {
   return s;
 }
 
-template <bool B_MN, bool GATED, typename T>
+template <bool B_MN, Fp8Form FORM, typename T>
 cudaError_t launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, const Schedule& s, void* workspace, int num_pairs, cudaStream_t stream) {
-  auto kern = fp8_gemm_pair_kernel<B_MN, GATED, T>;
+  auto kern = fp8_gemm_pair_kernel<B_MN, FORM, T>;
   // function attributes are per device: remember which devices of this process have been set up
   static bool configured[kMaxDevices] = {};
   int dev = 0;
@@ -529,8 +593,8 @@ cudaError_t launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p
 
 }  // namespace pair
 
-size_t pair_workspace(int M, int N, int K, bool gated, int num_sms) {
-  const pair::Schedule s = pair::make_schedule(M, N, K, gated, num_sms / 2);
+size_t pair_workspace(const Fp8GemmArgs& g, int num_sms) {
+  const pair::Schedule s = pair::make_schedule(g.M, g.N, g.K, g.form, num_sms / 2);
   if (s.ksplit == 1) return 0;
   const size_t rem = size_t(s.total_units - s.full_tiles) / s.ksplit;
   return ((rem * 2 * sizeof(unsigned int) + 255) & ~size_t(255)) + rem * s.ksplit * 2 * pair::PART_FLOATS * sizeof(float);
@@ -539,16 +603,19 @@ size_t pair_workspace(int M, int N, int K, bool gated, int num_sms) {
 cudaError_t launch_pair(const Fp8GemmArgs& g, const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int num_sms, cudaStream_t stream) {
   using namespace pair;
   const int num_pairs = num_sms / 2;
-  const Schedule s = make_schedule(g.M, g.N, g.K, g.gated, num_pairs);
-  if (g.gated) return launch<false, true, __nv_bfloat16>(ta, tb, p, s, g.workspace, num_pairs, stream);
+  const Schedule s = make_schedule(g.M, g.N, g.K, g.form, num_pairs);
+#define ELFB_LAUNCH(MN, FORM, T) return launch<MN, Fp8Form::FORM, T>(ta, tb, p, s, g.workspace, num_pairs, stream)
+  if (g.form == Fp8Form::kGated) ELFB_LAUNCH(false, kGated, float);
+  if (g.form == Fp8Form::kGatedBackward) ELFB_LAUNCH(true, kGatedBackward, float);
   if (g.b.mn_major) {
-    if (g.out == Elem::kBf16) return launch<true, false, __nv_bfloat16>(ta, tb, p, s, g.workspace, num_pairs, stream);
-    if (g.out == Elem::kF16) return launch<true, false, __half>(ta, tb, p, s, g.workspace, num_pairs, stream);
-    return launch<true, false, float>(ta, tb, p, s, g.workspace, num_pairs, stream);
+    if (g.out == Elem::kBf16) ELFB_LAUNCH(true, kPlain, __nv_bfloat16);
+    if (g.out == Elem::kF16) ELFB_LAUNCH(true, kPlain, __half);
+    ELFB_LAUNCH(true, kPlain, float);
   }
-  if (g.out == Elem::kBf16) return launch<false, false, __nv_bfloat16>(ta, tb, p, s, g.workspace, num_pairs, stream);
-  if (g.out == Elem::kF16) return launch<false, false, __half>(ta, tb, p, s, g.workspace, num_pairs, stream);
-  return launch<false, false, float>(ta, tb, p, s, g.workspace, num_pairs, stream);
+  if (g.out == Elem::kBf16) ELFB_LAUNCH(false, kPlain, __nv_bfloat16);
+  if (g.out == Elem::kF16) ELFB_LAUNCH(false, kPlain, __half);
+  ELFB_LAUNCH(false, kPlain, float);
+#undef ELFB_LAUNCH
 }
 
 }  // namespace fp8

@@ -1,6 +1,6 @@
 // Bandwidth-bound kernels that write or read block-scaled 8-bit tensors: quantise, restore, RMSNorm
-// with an 8-bit output, SwiGLU backward from an 8-bit checkpoint.  Each reads its inputs once and
-// writes its outputs once; all arithmetic is fp32.
+// with an 8-bit output.  Each reads its inputs once and writes its outputs once; all arithmetic is
+// fp32.
 #include "fp8_ops.h"
 
 #include <algorithm>
@@ -269,49 +269,6 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) rmsnorm_fp8_kernel(cons
   }
 }
 
-// ------------------------------------------------------------------------------ SwiGLU backward
-// act = silu(gate) * up with gate and up restored from their checkpoint.  One thread per 16 columns
-// of the activation; the gradients of gate and of up leave in 8 bits.
-__global__ void __launch_bounds__(THREADS) swiglu_bwd_fp8_kernel(const float* __restrict__ dact, long long lda, const uint8_t* __restrict__ gu,
-                                                                 long long ldgu, const uint8_t* __restrict__ gu_scale, long long ldgs,
-                                                                 uint8_t* __restrict__ dgu, long long ldd, uint8_t* __restrict__ dgu_scale,
-                                                                 long long ldds, uint32_t total, uint32_t units_per_row, int f) {
-  const uint32_t u = blockIdx.x * THREADS + threadIdx.x;
-  const bool live = u < total;  // f is a multiple of 128: whole groups of 8 lanes are live or not
-  const long long row = live ? u / units_per_row : 0;
-  const int col = live ? int(u - uint32_t(row) * units_per_row) * UNIT : 0;
-  float dg[UNIT], du[UNIT];
-  {
-    float da[UNIT];
-    load_values<float, UNIT, true>(dact + row * lda + col, UNIT, da);
-    const uint4 g4 = *reinterpret_cast<const uint4*>(gu + row * ldgu + col), u4 = *reinterpret_cast<const uint4*>(gu + row * ldgu + f + col);
-    const uint32_t gq[4] = {g4.x, g4.y, g4.z, g4.w}, uq[4] = {u4.x, u4.y, u4.z, u4.w};
-    const float gs = exponent_value(gu_scale[row * ldgs + col / BLOCK]), us = exponent_value(gu_scale[row * ldgs + (f + col) / BLOCK]);
-#pragma unroll
-    for (int j = 0; j < UNIT / 2; ++j) {
-      const float2 ge = from_e4m3x2((gq[j / 2] >> (16 * (j & 1))) & 0xffffu), ue = from_e4m3x2((uq[j / 2] >> (16 * (j & 1))) & 0xffffu);
-      const float g[2] = {ge.x * gs, ge.y * gs}, up[2] = {ue.x * us, ue.y * us};
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const float sig = __fdividef(1.f, 1.f + __expf(-g[k]));
-        du[2 * j + k] = da[2 * j + k] * g[k] * sig;
-        dg[2 * j + k] = da[2 * j + k] * up[k] * sig * (1.f + g[k] * (1.f - sig));
-      }
-    }
-  }
-  uint32_t q[UNIT / 4];
-  uint32_t byte = quantize_block<UNIT, 8>(dg, q);
-  if (live) {
-    *reinterpret_cast<uint4*>(dgu + row * ldd + col) = make_uint4(q[0], q[1], q[2], q[3]);
-    if ((col & (BLOCK - 1)) == 0) dgu_scale[row * ldds + col / BLOCK] = uint8_t(byte);
-  }
-  byte = quantize_block<UNIT, 8>(du, q);
-  if (live) {
-    *reinterpret_cast<uint4*>(dgu + row * ldd + f + col) = make_uint4(q[0], q[1], q[2], q[3]);
-    if ((col & (BLOCK - 1)) == 0) dgu_scale[row * ldds + (f + col) / BLOCK] = uint8_t(byte);
-  }
-}
-
 bool aligned16(const void* p, long long pitch_bytes) { return ((reinterpret_cast<uintptr_t>(p) | uintptr_t(pitch_bytes)) & 15) == 0; }
 
 // rows per launch, so that a launch's units fit 31 bits
@@ -411,19 +368,6 @@ cudaError_t fp8_rmsnorm(const void* x, const void* residual, const void* w, void
   if (dim <= 4096) ELFB_NORM(128, 4);
   ELFB_NORM(256, 4);
 #undef ELFB_NORM
-}
-
-cudaError_t fp8_swiglu_backward(const float* dact, long long lda, const uint8_t* gu, long long ldgu, const uint8_t* gu_scale, long long ldgs, uint8_t* dgu,
-                                long long ldd, uint8_t* dgu_scale, long long ldds, long long rows, int f, cudaStream_t stream) {
-  if (rows <= 0 || f <= 0) return cudaSuccess;
-  const uint32_t upr = uint32_t(f / UNIT);
-  const long long step = rows_per_launch(upr);
-  for (long long r = 0; r < rows; r += step) {
-    const uint32_t total = uint32_t(std::min(step, rows - r)) * upr;
-    swiglu_bwd_fp8_kernel<<<(total + THREADS - 1) / THREADS, THREADS, 0, stream>>>(dact + r * lda, lda, gu + r * ldgu, ldgu, gu_scale + r * ldgs, ldgs,
-                                                                                   dgu + r * ldd, ldd, dgu_scale + r * ldds, ldds, total, upr, f);
-  }
-  return cudaGetLastError();
 }
 
 }  // namespace elfb

@@ -23,10 +23,6 @@ cudaError_t fp8_dequantize(const uint8_t* data, long long ldq, const uint8_t* sc
 // h = x + residual (bf16, written when residual is given); data/scale = blocks of h * rstd * w
 cudaError_t fp8_rmsnorm(const void* x, const void* residual, const void* w, void* h, float* rstd, uint8_t* data, long long ldq, uint8_t* scale,
                         long long lds, long long rows, int dim, float eps, cudaStream_t stream);
-// dact [rows][f] fp32; gu/dgu [rows][2f] block-scaled (f a multiple of 128): the gradient of silu(gate) * up
-cudaError_t fp8_swiglu_backward(const float* dact, long long lda, const uint8_t* gu, long long ldgu, const uint8_t* gu_scale, long long ldgs, uint8_t* dgu,
-                                long long ldd, uint8_t* dgu_scale, long long ldds, long long rows, int f, cudaStream_t stream);
-
 // One operand of a block-scaled product.  Its scale for (row of the product, block of the
 // reduction) is scale[(row >> row_shift) * row_stride + block * block_stride].
 struct Fp8Operand {
@@ -38,20 +34,25 @@ struct Fp8Operand {
   bool mn_major = false;  // stored [K][MN] instead of [MN][K]
 };
 
+enum class Fp8Form {
+  kPlain,
+  kGated,          // b is [2F][K] (gate rows, up rows): silu(gate) * up and, on request, gate | up leave in 8 bits
+  kGatedBackward,  // b is [K][F] mn_major: the product is the gradient of the activation, that of gate | up leaves in 8 bits
+};
+
 struct Fp8GemmArgs {
+  Fp8Form form = Fp8Form::kPlain;
   Fp8Operand a, b;             // a: [M][K]; b: [N][K], or [K][N] when mn_major
-  void* d = nullptr;           // [M][N], pitch ldd elements
+  void* d = nullptr;           // plain: [M][N], pitch ldd elements
   Elem out = Elem::kBf16;
   long long ldd = 0;
-  const void* bias = nullptr;  // optional [N], type of d
+  const void* bias = nullptr;  // plain, optional: [N], type of d
   int M = 0, N = 0, K = 0;
-  // gated form: b is [2F][K], N = 2F; d is unused, the activation and the two projections leave in 8 bits
-  bool gated = false;
-  uint8_t* act = nullptr;      // [M][F]
+  uint8_t* act = nullptr;      // gated: the activation [M][F]; gated backward: the gradient of gate | up [M][2F]
   long long ld_act = 0;
   uint8_t* act_scale = nullptr;
   long long ld_act_scale = 0;
-  uint8_t* gu = nullptr;       // [M][2F], nullptr when no backward pass follows
+  uint8_t* gu = nullptr;       // gate | up [M][2F]: written by the gated form (nullptr when no backward pass follows), read by its backward
   long long ld_gu = 0;
   uint8_t* gu_scale = nullptr;
   long long ld_gu_scale = 0;

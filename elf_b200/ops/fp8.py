@@ -408,7 +408,7 @@ def gated_forward(x: BlockScaled, w_gate_up: BlockScaled, keep: bool = True) -> 
 
 def gated_backward(dy: BlockScaled, w_down: BlockScaled, gate_up: BlockScaled) -> BlockScaled:
     """Gradient of ``gate_up [..., 2F]`` in 8 bits for the gradient ``dy [..., D]`` of the block's output:
-    ``dact = dy W_down`` in fp32, then ``dgate = dact up s (1 + gate (1 - s))`` and ``dup = dact gate s`` with
+    one kernel, ``dact = dy W_down`` in fp32 and ``dgate = dact up s (1 + gate (1 - s))`` and ``dup = dact gate s`` with
     ``s = sigmoid(gate)``, gate and up restored from their checkpoint."""
     _check_product(dy, w_down, 0, "gated_backward")
     f = w_down.shape[1]
@@ -419,14 +419,14 @@ def gated_backward(dy: BlockScaled, w_down: BlockScaled, gate_up: BlockScaled) -
     if not (gate_up.block_rows == 1 and gate_up.shape == (*dy.shape[:-1], 2 * f)):
         raise ValueError(f"gated_backward: expected gate_up of shape {(*dy.shape[:-1], 2 * f)}, got {tuple(gate_up.shape)}")
     _same_device("dy", dy, "gate_up", gate_up)
-    dact = _product(dy, w_down, True, None, torch.float32).view(-1, f)
-    if dact.numel() == 0 or not _on_kernels(dy.data):
+    if dy.numel() == 0 or f == 0 or not _on_kernels(dy.data):
+        dact = _values(dy) @ _values(w_down)
         gu = _values(gate_up)
         gate, up = gu[:, :f], gu[:, f:]
         s = torch.sigmoid(gate)
         dgu = torch.cat([dact * up * s * (1 + gate * (1 - s)), dact * gate * s], 1)
         return _quantize_ref(dgu.view(gate_up.shape), 1)
-    return BlockScaled._made(*_ext.get().fp8_swiglu_bwd(dact, gate_up.data, gate_up.scale))
+    return BlockScaled._made(*_ext.get().fp8_gated_bwd(dy.data, dy.scale, w_down.data, w_down.scale, gate_up.data, gate_up.scale, _gemm.status(dy.device)))
 
 
 # ------------------------------------------------------------------------------ differentiable forms

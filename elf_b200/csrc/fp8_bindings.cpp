@@ -179,17 +179,17 @@ struct Operand {
   elfb::Fp8Operand o;
 };
 
-Operand operand(const at::Tensor& data, const at::Tensor& scale, int64_t row_shift, bool mn_major, const char* name, const at::Device& dev) {
+Operand operand(const at::Tensor& data, const at::Tensor& scale, int64_t row_shift, bool mn_major, const char* name, const at::Device& dev, int64_t align = 16) {
   Operand r{scaled(data, scale, row_shift, name, dev), {}};
   TORCH_CHECK(r.s.data.rows <= INT_MAX - 1024, name, " has too many rows");
-  if (!r.s.data.aligned(16)) {  // TMA wants rows on 16-byte boundaries: a copy with padded rows
+  if (!r.s.data.aligned(align)) {  // TMA wants rows on 16-byte boundaries: a copy with padded rows
     const int64_t lead[1] = {r.s.data.rows};
-    at::Tensor padded = new_rows(at::IntArrayRef(lead, 1), r.s.data.cols, round_up(r.s.data.cols, 16), data.scalar_type(), dev);
+    at::Tensor padded = new_rows(at::IntArrayRef(lead, 1), r.s.data.cols, round_up(r.s.data.cols, align), data.scalar_type(), dev);
     padded.copy_(r.s.data.t.dim() == 2 ? r.s.data.t : r.s.data.t.reshape({r.s.data.rows, r.s.data.cols}));
     r.s.data = matrix(padded, name, dev, false);
   }
   r.o.data = r.s.data.bytes();
-  r.o.ld = round_up(r.s.data.pitch, 16);  // (a single row may have any pitch)
+  r.o.ld = round_up(r.s.data.pitch, align);  // (a single row may have any pitch)
   r.o.scale = r.s.scale.bytes();
   r.o.mn_major = mn_major;
   if (mn_major) {
@@ -297,7 +297,7 @@ std::pair<at::Tensor, at::Tensor> gated_bwd(const at::Tensor& dy, const at::Tens
   const auto dev = dy.device();
   c10::cuda::CUDAGuard guard(dev);
   const Operand oa = operand(dy, dy_scale, 0, false, "the gradient", dev), ob = operand(w, w_scale, 7, true, "the weight", dev),
-                og = operand(gu, gu_scale, 0, false, "gate_up", dev);
+                og = operand(gu, gu_scale, 0, false, "gate_up", dev, 32);
   elfb::Fp8GemmArgs g;
   g.form = elfb::Fp8Form::kGatedBackward;
   g.a = oa.o;

@@ -145,17 +145,32 @@ __device__ __forceinline__ void store_quad(float (&s)[4], int row, int col, cons
   }
 }
 
-// 16 values times 2^(127 - byte) to e4m3
-__device__ __forceinline__ void scale_and_store(const float* v, float inv, uint8_t* dst) {
-  uint32_t q[4];
+// 32-byte accesses (addresses 32-byte aligned): a lane whose row is its own moves whole sectors.
+__device__ __forceinline__ void load_32_bytes(const uint8_t* p, uint32_t (&v)[8]) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "l"(p));
+}
+__device__ __forceinline__ void store_32_bytes(uint8_t* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+               "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+// N values times 2^(127 - byte) to e4m3
+template <int N>
+__device__ __forceinline__ void to_scaled_e4m3(const float* v, float inv, uint32_t* q) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < N / 4; ++j) {
     float s[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) s[k] = nan_unless_finite(mul_exact(v[4 * j + k], inv), v[4 * j + k]);
     q[j] = to_e4m3x4(s[0], s[1], s[2], s[3]);
   }
-  *reinterpret_cast<uint4*>(dst) = make_uint4(q[0], q[1], q[2], q[3]);
+}
+__device__ __forceinline__ void scale_and_store_32(const float* v, float inv, uint8_t* dst) {
+  uint32_t q[8];
+  to_scaled_e4m3<32>(v, inv, q);
+  store_32_bytes(dst, q);
 }
 
 // The layout tcgen05.cp wants: 16 bytes per lane, word j for row 32 j + lane.

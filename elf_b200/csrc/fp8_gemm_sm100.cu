@@ -336,10 +336,10 @@ const char* fp8_gemm(const Fp8GemmArgs& g, int num_sms, cudaStream_t stream) {
   p.status = g.status;
   cudaError_t e;
   if (g.form != Fp8Form::kPlain) {
-    auto aligned = [](const void* q, long long pitch) { return ((reinterpret_cast<uintptr_t>(q) | uintptr_t(pitch)) & 15) == 0; };
+    auto aligned = [](const void* q, long long pitch) { return ((reinterpret_cast<uintptr_t>(q) | uintptr_t(pitch)) & 31) == 0; };
     const bool backward = g.form == Fp8Form::kGatedBackward;
     if (g.b.mn_major != backward || g.N % (backward ? 128 : 256) != 0) return "the gated product's width must be a multiple of 128";
-    if (!aligned(g.act, g.ld_act) || (g.gu && !aligned(g.gu, g.ld_gu))) return "8-bit matrices must be 16-byte aligned with a 16-byte multiple row pitch";
+    if (!aligned(g.act, g.ld_act) || (g.gu && !aligned(g.gu, g.ld_gu))) return "8-bit matrices of the gated forms must be 32-byte aligned with a 32-byte multiple row pitch";
     p.act = g.act, p.act_scale = g.act_scale, p.gu = g.gu, p.gu_scale = g.gu_scale;
     p.ld_act = g.ld_act, p.ld_act_scale = g.ld_act_scale, p.ld_gu = g.ld_gu, p.ld_gu_scale = g.ld_gu_scale;
     e = launch_pair(g, ta, tb, p, num_sms, stream);

@@ -146,9 +146,9 @@ __device__ __forceinline__ void gated_tile(uint32_t taddr, int row, int half, in
     if (live) {
       uint8_t* dst = p.gu + (long long)row * p.ld_gu + col;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) scale_and_store(g + 16 * c, inverse_exponent_value(byte_g), dst + 16 * c);
+      for (int c = 0; c < 2; ++c) scale_and_store_32(g + 32 * c, inverse_exponent_value(byte_g), dst + 32 * c);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) scale_and_store(u + 16 * c, inverse_exponent_value(byte_u), dst + f + 16 * c);
+      for (int c = 0; c < 2; ++c) scale_and_store_32(u + 32 * c, inverse_exponent_value(byte_u), dst + f + 32 * c);
       if (half == 0) {
         uint8_t* s = p.gu_scale + (long long)row * p.ld_gu_scale;
         s[f0 / 128] = uint8_t(byte_g);
@@ -166,68 +166,107 @@ __device__ __forceinline__ void gated_tile(uint32_t taddr, int row, int half, in
   if (live) {
     uint8_t* dst = p.act + (long long)row * p.ld_act + col;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) scale_and_store(g + 16 * c, inverse_exponent_value(byte), dst + 16 * c);
+    for (int c = 0; c < 2; ++c) scale_and_store_32(g + 32 * c, inverse_exponent_value(byte), dst + 32 * c);
     if (half == 0) p.act_scale[(long long)row * p.ld_act_scale + f0 / 128] = uint8_t(byte);
   }
 }
 
-// One tile of the gated form's backward: the accumulator holds the gradient of the activation, the thread one row
+// One tile of the gated form's backward: the accumulator holds the gradient d of the activation, the thread one row
 // of one block of 128 columns.  gate and up come from their checkpoint.
 //   dgate = d up s (1 + gate (1 - s)),  dup = d gate s,  s = sigmoid(gate)
 // are formed twice, once for the maxima of their blocks and once to be scaled: 256 values per row would not stay in
-// registers beside the gradient, and the second exponential hides behind the next tile's products.
-template <typename Release>
-__device__ __forceinline__ void gated_backward_tile(uint32_t taddr, int row, int half, int n0, int f, const Params& p, Release&& release) {
-  uint32_t raw[4][32];
+// registers.  d stays in TMEM but for the 32 columns shared with the other accumulator, which half of the threads
+// hold.  The checkpoint is read and the result written 32 bytes at a time, whole sectors of a row that is one
+// thread's own: 309 us for 4096 x 14336 x 4096, with 16-byte accesses 350.
+struct GatedGrad {
+  float dg[16], du[16];
+};
+__device__ __forceinline__ void gated_grad(const uint32_t* d, const uint32_t* gq, const uint32_t* uq, float sg, float su, GatedGrad& o) {
 #pragma unroll
-  for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(taddr + half * 128 + c * 32, raw[c]);
-  tmem_ld_wait();
+  for (int j = 0; j < 8; ++j) {
+    const float2 ge = from_e4m3x2((gq[j / 2] >> (16 * (j & 1))) & 0xffffu), ue = from_e4m3x2((uq[j / 2] >> (16 * (j & 1))) & 0xffffu);
+    const float g[2] = {ge.x * sg, ge.y * sg}, up[2] = {ue.x * su, ue.y * su};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float v = __uint_as_float(d[2 * j + k]);
+      const float sig = __fdividef(1.f, 1.f + __expf(-g[k]));
+      o.du[2 * j + k] = v * g[k] * sig;
+      o.dg[2 * j + k] = v * up[k] * sig * (1.f + g[k] * (1.f - sig));
+    }
+  }
+}
+template <typename Release>
+__device__ __forceinline__ void gated_backward_tile(uint32_t taddr, int acc, int row, int half, int n0, int f, const Params& p, Release&& release) {
+  taddr += half * 128;
+  // chunks of 32 columns: of accumulator 0 the last is shared, of accumulator 1 the first
+  const bool shares = half != acc;
+  const int held_chunk = acc == 0 ? 3 : 0, from = shares && acc == 1 ? 1 : 0, to = shares && acc == 0 ? 3 : 4;
+  uint32_t held[32];
+  if (shares) {
+    tmem_ld_32x32b_x32(taddr + held_chunk * 32, held);
+    tmem_ld_wait();
+  }
   release();
   const int col = n0 + half * 128;
-  if (row >= p.M || col >= f) return;
-  const uint8_t* gate = p.gu + (long long)row * p.ld_gu + col;
-  const uint8_t* scales = p.gu_scale + (long long)row * p.ld_gu_scale + col / 128;
+  const bool live = row < p.M && col < f;  // (loads from TMEM are for the whole warp)
+  const long long r = live ? row : 0;
+  const int c0 = live ? col : 0;
+  const uint8_t* gate = p.gu + r * p.ld_gu + c0;
+  const uint8_t* scales = p.gu_scale + r * p.ld_gu_scale + c0 / 128;
   const float sg = exponent_value(scales[0]), su = exponent_value(scales[f / 128]);
-  uint8_t* dst = p.act + (long long)row * p.ld_act + col;
+  uint8_t* dst = p.act + r * p.ld_act + c0;
   uint32_t top_g = 0, top_u = 0;
   float inv_g = 0.f, inv_u = 0.f;
 #pragma unroll
   for (int pass = 0; pass < 2; ++pass) {
-    uint4 g4 = *reinterpret_cast<const uint4*>(gate), u4 = *reinterpret_cast<const uint4*>(gate + f);
+    auto handle = [&](const uint32_t (&d)[32], int c, const uint32_t (&g)[8], const uint32_t (&u)[8]) {
+      uint32_t qg[8], qu[8];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      const uint32_t gq[4] = {g4.x, g4.y, g4.z, g4.w}, uq[4] = {u4.x, u4.y, u4.z, u4.w};
-      if (c < 7) {
-        g4 = *reinterpret_cast<const uint4*>(gate + 16 * (c + 1));
-        u4 = *reinterpret_cast<const uint4*>(gate + f + 16 * (c + 1));
-      }
-      float dg[16], du[16];
+      for (int h = 0; h < 2; ++h) {
+        GatedGrad o;
+        gated_grad(d + 16 * h, g + 4 * h, u + 4 * h, sg, su, o);
+        if (pass == 0) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float2 ge = from_e4m3x2((gq[j / 2] >> (16 * (j & 1))) & 0xffffu), ue = from_e4m3x2((uq[j / 2] >> (16 * (j & 1))) & 0xffffu);
-        const float g[2] = {ge.x * sg, ge.y * sg}, up[2] = {ue.x * su, ue.y * su};
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const float d = __uint_as_float(raw[c / 2][(c & 1) * 16 + 2 * j + k]);
-          const float sig = __fdividef(1.f, 1.f + __expf(-g[k]));
-          du[2 * j + k] = d * g[k] * sig;
-          dg[2 * j + k] = d * up[k] * sig * (1.f + g[k] * (1.f - sig));
+          for (int j = 0; j < 16; ++j) top_g = max(top_g, finite_bits(o.dg[j])), top_u = max(top_u, finite_bits(o.du[j]));
+        } else {
+          to_scaled_e4m3<16>(o.dg, inv_g, qg + 4 * h);
+          to_scaled_e4m3<16>(o.du, inv_u, qu + 4 * h);
         }
       }
-      if (pass == 0) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) top_g = max(top_g, finite_bits(dg[j])), top_u = max(top_u, finite_bits(du[j]));
-      } else {
-        scale_and_store(dg, inv_g, dst + 16 * c);
-        scale_and_store(du, inv_u, dst + f + 16 * c);
+      if (pass == 1 && live) {
+        store_32_bytes(dst + 32 * c, qg);
+        store_32_bytes(dst + f + 32 * c, qu);
       }
+    };
+    uint32_t g[8], u[8], next_g[8], next_u[8];
+    load_32_bytes(gate + 32 * from, next_g);
+    load_32_bytes(gate + f + 32 * from, next_u);
+    if (shares) {
+      load_32_bytes(gate + 32 * held_chunk, g);
+      load_32_bytes(gate + f + 32 * held_chunk, u);
+      handle(held, held_chunk, g, u);
+    }
+#pragma unroll 1
+    for (int c = from; c < to; ++c) {
+      uint32_t d[32];
+      tmem_ld_32x32b_x32(taddr + c * 32, d);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] = next_g[j], u[j] = next_u[j];
+      if (c + 1 < to) {
+        load_32_bytes(gate + 32 * (c + 1), next_g);
+        load_32_bytes(gate + f + 32 * (c + 1), next_u);
+      }
+      tmem_ld_wait();
+      handle(d, c, g, u);
     }
     if (pass == 0) {
       const uint32_t byte_g = block_exponent(top_g), byte_u = block_exponent(top_u);
       inv_g = inverse_exponent_value(byte_g), inv_u = inverse_exponent_value(byte_u);
-      uint8_t* s = p.act_scale + (long long)row * p.ld_act_scale + col / 128;
-      s[0] = uint8_t(byte_g);
-      s[f / 128] = uint8_t(byte_u);
+      if (live) {
+        uint8_t* s = p.act_scale + r * p.ld_act_scale + c0 / 128;
+        s[0] = uint8_t(byte_g);
+        s[f / 128] = uint8_t(byte_u);
+      }
     }
   }
 }
@@ -386,7 +425,7 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       if constexpr (GATED) {
         gated_tile(taddr, row, half, unit.n0, f, p, exchange + quarter * 32 + lane, release);
       } else if constexpr (FORM == Fp8Form::kGatedBackward) {
-        gated_backward_tile(taddr, row, half, unit.n0, f, p, release);
+        gated_backward_tile(taddr, acc, row, half, unit.n0, f, p, release);
       } else {
         constexpr int CHUNKS = BN / 64;  // of 32 columns, for each half
         if (unit.rest < 0) {

@@ -338,9 +338,11 @@ const char* make_tmap_2d(CUtensorMap* out, const void* ptr, int fmt, uint64_t ro
 
 // Row-major [rows][cols] matrix of bytes, pitch `ld`, for the 8-bit products: 128B swizzle, zero fill.
 const char* make_tmap_bytes(CUtensorMap* out, const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_cols, uint32_t box_rows) {
-  static thread_local bool context_ready = false;  // as in make_tmap_2d
+  // a context must be current on the calling thread, as in make_tmap_2d; this call is also legal during a capture
+  static thread_local bool context_ready = false;
   if (!context_ready) {
-    cudaFree(nullptr);
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return "no CUDA device is current";
     context_ready = true;
   }
   EncodeFn enc = get_encode_fn();

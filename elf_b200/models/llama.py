@@ -66,6 +66,7 @@ class LlamaConfig:
     rope_theta: float = 500000.0
     eps: float = 1e-5
     init_std: float = 0.02
+    ffn_fp8: bool = False  # feed-forward products, and what they keep for the backward pass, in 8 bits (split-backward builds)
 
     @property
     def head_dim(self) -> int:
@@ -703,11 +704,14 @@ def build_llama_stages(cfg: LlamaConfig, n_stages: int, only: Optional[Sequence[
     MLP's SwiGLU, where two tensors cross the boundary (pass ``llama_stage_signatures(...)`` to the
     pipeline in that case).  ``cost_model`` (see ``elf_b200.models.llama_costs``) makes the cut for
     measured block times instead of the built-in constants; pass the same one to
-    ``llama_stage_costs`` / ``llama_stage_signatures`` / ``llama_stage_ranges``.  With
+    ``llama_stage_costs`` / ``llama_stage_signatures`` / ``llama_stage_ranges``.  ``cfg.ffn_fp8`` puts the
+    feed-forward layers in 8 bits (``elf_b200.zb_utils.LinearFP8DW``).  With
     ``fused_head_loss`` the last stage ends with the final norm only and the vocabulary projection
     happens inside the loss (``elf_b200.ops.head_loss.ChunkedHeadLoss(stage[-1])`` as loss function)."""
-    from ..zb_utils import replace_layer_with_layer_dw
+    from ..zb_utils import replace_layer_with_layer_dw, replace_linear_with_linear_fp8
 
+    if cfg.ffn_fp8 and not split_backward:
+        raise ValueError("ffn_fp8 needs split_backward=True: the 8-bit layers compute their weight gradients in W passes")
     ranges, parts_per_layer, _ = _stage_ranges(cfg, n_stages, placement, split_layers, cost_model)
     stages: List[Optional[LlamaStage]] = []
     for i, (first, last) in enumerate(ranges):
@@ -726,6 +730,8 @@ def build_llama_stages(cfg: LlamaConfig, n_stages: int, only: Optional[Sequence[
         init_llama_(stage, cfg.init_std, seed + i)
         if split_backward:
             replace_layer_with_layer_dw(stage)
+        if cfg.ffn_fp8:
+            replace_linear_with_linear_fp8(stage, lambda name, _: name.rpartition(".")[2] in ("w_gate_up", "w_down"))
         stages.append(stage)
     return stages
 

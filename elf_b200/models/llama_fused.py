@@ -34,9 +34,10 @@ import torch
 
 from ..ops import _ext
 from ..ops import attention as _attn
+from ..ops import fp8 as _fp8
 from ..ops import fused as _f
 from ..ops import gemm as _gemm
-from ..zb_utils import LayerDW, in_partial_replay
+from ..zb_utils import LayerDW, LinearFP8DW, in_partial_replay
 
 __all__ = ["fused_apply", "attention_half", "mlp_half", "decoder_layer"]
 
@@ -56,6 +57,11 @@ def fused_apply(x: torch.Tensor, *linears) -> bool:
         n, k = lin.weight.shape
         if n % 8 or k % 8:
             return False
+    # layers in 8 bits: the feed-forward pair together, its gate and up blocks whole
+    in_8_bits = [isinstance(lin, LinearFP8DW) for lin in linears]
+    if any(in_8_bits):
+        return in_8_bits[-2:] == [True, True] and not any(in_8_bits[:-2]) and len(linears) in (2, 4) and linears[-1].weight.shape[1] % _fp8.BLOCK == 0 and (
+            linears[-2].weight.shape[0] == 2 * linears[-1].weight.shape[1])
     return True
 
 
@@ -72,8 +78,8 @@ def _norm_grad_target(w: torch.Tensor) -> torch.Tensor:
     return target
 
 
-def _stash_input(linear, t: torch.Tensor) -> None:
-    stash = t.detach()
+def _stash_input(linear, t) -> None:
+    stash = t if isinstance(t, _fp8.BlockScaled) else t.detach()
     stash.is_model_input = False  # produced inside the node: a checkpointed re-run regenerates it
     linear.last_input = stash
 
@@ -167,24 +173,52 @@ def _attn_backward_body(blk, x, mode, saved, dy: torch.Tensor) -> torch.Tensor:
     return ext.rmsnorm_bwd(d_h1.view(b, s, d), x, blk.norm1.weight, rstd1, _norm_grad_target(blk.norm1.weight), True, dy, None)
 
 
-def _mlp_forward_body(blk, h2: torch.Tensor, x2: torch.Tensor):
-    """``y = x2 + w_down(swiglu(w_gate_up(h2)))`` for the normalised ``h2`` of ``x2``."""
+def _mlp_in_8_bits(blk) -> bool:
+    return isinstance(blk.w_gate_up, LinearFP8DW)
+
+
+def _second_norm(blk, x: torch.Tensor, residual=None):
+    """``(h2, rstd2, x2)``: ``x2 = x + residual`` and its norm, block-scaled for feed-forward layers in 8 bits."""
+    if not _mlp_in_8_bits(blk):
+        return _ext.get().rmsnorm_fwd(x, blk.norm2.weight, blk.norm2.eps, residual)
+    if residual is None:
+        h2, rstd2 = _fp8.rms_norm(x, blk.norm2.weight, blk.norm2.eps)
+        return h2, rstd2.view(-1), x
+    h2, rstd2, x2 = _fp8.add_rms_norm(x, residual, blk.norm2.weight, blk.norm2.eps)
+    return h2, rstd2.view(-1), x2
+
+
+def _mlp_forward_body(blk, h2, x2: torch.Tensor):
+    """``y = x2 + w_down(swiglu(w_gate_up(h2)))`` for the normalised ``h2`` of ``x2``, and the tensors the backward
+    needs: the gate and up projections, or their 8-bit copy (values, scales)."""
     ext = _ext.get()
     _stash_input(blk.w_gate_up, h2)
+    if _mlp_in_8_bits(blk):
+        act, gu = _fp8.gated_forward(h2, blk.w_gate_up.weight_q())
+        _stash_input(blk.w_down, act)
+        dn = _fp8.linear_forward(act, blk.w_down.weight_q())
+        return ext.residual_add(dn, x2), (gu.data, gu.scale)
     gu = _gemm.linear_forward(h2, blk.w_gate_up.weight)
     act = ext.swiglu_fwd(gu)
     _stash_input(blk.w_down, act)
     dn = _gemm.linear_forward(act, blk.w_down.weight)
-    return ext.residual_add(dn, x2), gu  # dn += x2, in place
+    return ext.residual_add(dn, x2), (gu,)  # dn += x2, in place
 
 
 def _mlp_backward_body(blk, x2, rstd2, gu, dy: torch.Tensor) -> torch.Tensor:
     ext = _ext.get()
-    blk.w_down._accumulate_grad_output(dy)
-    d_act = _gemm.linear_input_grad(dy, blk.w_down.weight)
-    d_gu = ext.swiglu_bwd(d_act, gu)
-    blk.w_gate_up._accumulate_grad_output(d_gu)
-    d_h2 = _gemm.linear_input_grad(d_gu, blk.w_gate_up.weight)
+    if len(gu) == 2:
+        dyq = _fp8.quantize(dy)
+        blk.w_down._accumulate_grad_output(dyq)
+        d_gu = _fp8.gated_backward(dyq, blk.w_down.weight_q(), _fp8.BlockScaled._made(*gu))
+        blk.w_gate_up._accumulate_grad_output(d_gu)
+        d_h2 = _fp8.linear_input_grad(d_gu, blk.w_gate_up.weight_q())
+    else:
+        blk.w_down._accumulate_grad_output(dy)
+        d_act = _gemm.linear_input_grad(dy, blk.w_down.weight)
+        d_gu = ext.swiglu_bwd(d_act, gu[0])
+        blk.w_gate_up._accumulate_grad_output(d_gu)
+        d_h2 = _gemm.linear_input_grad(d_gu, blk.w_gate_up.weight)
     return ext.rmsnorm_bwd(d_h2, x2, blk.norm2.weight, rstd2, _norm_grad_target(blk.norm2.weight), True, dy, None)
 
 
@@ -214,15 +248,15 @@ class _MLPHalf(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, blk, *weights):
         x = x.contiguous()
-        h2, rstd2, _ = _ext.get().rmsnorm_fwd(x, blk.norm2.weight, blk.norm2.eps, None)
+        h2, rstd2, _ = _second_norm(blk, x)
         y, gu = _mlp_forward_body(blk, h2, x)
         ctx.blk = blk
-        ctx.save_for_backward(x, rstd2, gu)
+        ctx.save_for_backward(x, rstd2, *gu)
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x, rstd2, gu = ctx.saved_tensors
+        x, rstd2, *gu = ctx.saved_tensors
         dx = _mlp_backward_body(ctx.blk, x, rstd2, gu, dy.contiguous())
         return (dx, None) + (None,) * 3
 
@@ -232,15 +266,16 @@ class _DecoderLayer(torch.autograd.Function):
     def forward(ctx, x, blk, *weights):
         x = x.contiguous()
         o, mode, saved = _attn_forward_body(blk, x)
-        h2, rstd2, x2 = _ext.get().rmsnorm_fwd(o, blk.norm2.weight, blk.norm2.eps, x)  # x2 = o + x, h2 = rmsnorm(x2)
+        h2, rstd2, x2 = _second_norm(blk, o, x)  # x2 = o + x, h2 = rmsnorm(x2)
         y, gu = _mlp_forward_body(blk, h2, x2)
-        ctx.blk, ctx.mode = blk, mode
-        ctx.save_for_backward(x, x2, rstd2, gu, *saved)
+        ctx.blk, ctx.mode, ctx.n_gu = blk, mode, len(gu)
+        ctx.save_for_backward(x, x2, rstd2, *gu, *saved)
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x, x2, rstd2, gu, *saved = ctx.saved_tensors
+        x, x2, rstd2, *rest = ctx.saved_tensors
+        gu, saved = rest[: ctx.n_gu], rest[ctx.n_gu :]
         dx2 = _mlp_backward_body(ctx.blk, x2, rstd2, gu, dy.contiguous())
         dx = _attn_backward_body(ctx.blk, x, ctx.mode, saved, dx2)
         return (dx, None) + (None,) * 6

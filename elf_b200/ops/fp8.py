@@ -124,7 +124,9 @@ class BlockScaled:
         return self.data.numel()
 
     def to(self, device, non_blocking: bool = False) -> "BlockScaled":
-        return BlockScaled(self.data.to(device, non_blocking=non_blocking), self.scale.to(device, non_blocking=non_blocking), self.block_rows)
+        moved = BlockScaled._made(self.data.to(device, non_blocking=non_blocking), self.scale.to(device, non_blocking=non_blocking), self.block_rows)
+        moved.is_model_input = self.is_model_input
+        return moved
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         return dequantize(self, dtype)

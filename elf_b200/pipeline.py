@@ -45,6 +45,7 @@ from .scheduling import add_comms, check_schedule_validity, schedule_to_str
 from .scheduling.scheduling import OperationType
 from .utils.placement import Placement
 from .utils.shipping import broadcast_models, recv_models, send_models, transport_device
+from .zb_utils import LinearFP8DW
 
 logger = logging.getLogger("pipeline")
 
@@ -305,6 +306,8 @@ class Pipeline:
         for block in self.blocks:
             for layer in block.dw_layers():
                 layer.clear()
+                if isinstance(layer, LinearFP8DW):
+                    layer.begin_step()
         if self.grad_sync is not None and any(op.op is OperationType.ALL_REDUCE_PARAM_GRADS for op in self.schedule):
             # only a step that exchanges gradients opens a new exchange epoch (and flips the inbox
             # parity): an inference step in between must not let the next training step write

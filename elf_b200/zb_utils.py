@@ -24,17 +24,21 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .ops import fp8 as _fp8
 from .ops import gemm as _gemm
 
 __all__ = [
     "LayerDW",
     "LinearDX",
     "LinearDW",
+    "LinearFP8DX",
+    "LinearFP8DW",
     "Conv1dDX",
     "Conv1dDW",
     "MappingDW",
     "replace_layer_with_layer_dw",
     "replace_linear_with_linear_dw",
+    "replace_linear_with_linear_fp8",
     "LayerDWTracer",
     "partial_dx_recomputation",
     "in_partial_replay",
@@ -218,6 +222,111 @@ LinearDW.register_dx_function(LinearDX)
 
 
 # ---------------------------------------------------------------------------------------
+# Linear in 8 bits
+# ---------------------------------------------------------------------------------------
+
+
+class LinearFP8DX(torch.autograd.Function):
+    """``y = x Wᵀ + b`` with both products of the B pass in 8 bits; the backward returns only ``dx``."""
+
+    @staticmethod
+    def forward(ctx, input, weight, bias, linear):
+        # weight/bias are arguments so the output requires grad even if ``input`` does not
+        ctx.linear, ctx.dtype = linear, input.dtype
+        xq = _fp8.quantize(input)
+        linear._store_input_q(xq, input.grad_fn is None)
+        # saved (although unused here) so that torch.utils.checkpoint recomputes it
+        ctx.save_for_backward(xq.data, xq.scale)
+        return _fp8.linear_forward(xq, linear.weight_q(), bias, input.dtype)
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        linear = ctx.linear
+        dyq = _fp8.quantize(grad_output)
+        linear._accumulate_grad_output(dyq)
+        if not ctx.needs_input_grad[0]:
+            return None, None, None, None
+        return _fp8.linear_input_grad(dyq, linear.weight_q(), ctx.dtype), None, None, None
+
+
+class LinearFP8DW(LinearDW):
+    """``LinearDW`` in 8 bits (``elf_b200.ops.fp8``): the forward and the input gradient are products of block-scaled
+    operands, and what waits for the W pass — the layer's input and its output's gradient — is kept in 8 bits,
+    half the bytes of the 16-bit stash.  The weight gradient itself is a 16-bit product of the restored
+    values, accumulated (and pushed to the other replicas) like ``LinearDW``'s.
+
+    The weight's 8-bit copy is made once per pipeline step (``begin_step``) and dropped at its end; outside a
+    step, where nothing says when the weight changes, every pass makes its own."""
+
+    def __init__(self, linear: nn.Linear, *args, **kwargs):
+        super().__init__(linear, *args, **kwargs)
+        self._hold_weight_q = False
+        self._weight_q: Optional[_fp8.BlockScaled] = None
+
+    def weight_q(self) -> _fp8.BlockScaled:
+        if self._weight_q is not None:
+            return self._weight_q
+        q = _fp8.quantize_weight(self.weight)
+        if self._hold_weight_q:
+            self._weight_q = q
+        return q
+
+    def begin_step(self) -> None:
+        """The weight stays as it is until ``clear``: one 8-bit copy serves all micro-batches."""
+        self._hold_weight_q, self._weight_q = True, None
+
+    def clear(self) -> None:
+        super().clear()
+        self._hold_weight_q, self._weight_q = False, None
+
+    def _store_input_q(self, xq: _fp8.BlockScaled, is_model_input: bool) -> None:
+        xq.is_model_input = is_model_input  # see LayerDW._store_input
+        self.last_input = xq
+
+    def _accumulate_grad_output(self, grad_output) -> None:
+        prev = getattr(self, "last_grad_output", None)
+        if prev is not None:  # applied several times in one forward: the sum is kept in 16 bits
+            restored = lambda t: t.dequantize(torch.float32) if isinstance(t, _fp8.BlockScaled) else t.float()
+            grad_output = (restored(prev) + restored(grad_output)).to(torch.bfloat16)
+        self.last_grad_output = grad_output
+
+    def forward(self, x, *args, **kwargs):
+        return LinearFP8DX.apply(x, self.weight, self.bias, self)
+
+    def backward(self, mb_id: int) -> None:
+        x, g = self._take(mb_id)
+        dev = self.weight.device
+        if x.device != dev:
+            x = x.to(dev, non_blocking=True)
+        if g.device != dev:
+            g = g.to(dev, non_blocking=True)
+        with torch.no_grad():
+            grad = self.weight.grad
+            if grad is not None and grad.dtype in (torch.bfloat16, torch.float32) and grad.is_contiguous():
+                push = None
+                plan = getattr(self, "_push", None)
+                if plan is not None and getattr(self, "_final_pass", False) and grad.dtype == self.weight.dtype and _gemm.usable(grad, self.weight):
+                    push = plan.target()
+                self.weight.grad = _fp8.linear_weight_grad(g, x, out=grad, push=push)
+            else:
+                dw = _fp8.linear_weight_grad(g, x, out_dtype=self.weight.dtype)
+                if grad is None:
+                    self.weight.grad = dw
+                else:
+                    grad.add_(dw)
+            if self.bias is not None:
+                g2 = g.dequantize(torch.float32) if isinstance(g, _fp8.BlockScaled) else g.float()
+                db = _flat2d(g2).sum(0)
+                if self.bias.grad is None:
+                    self.bias.grad = db.to(self.bias.dtype)
+                else:
+                    self.bias.grad.add_(db)
+
+
+LinearFP8DW.register_dx_function(LinearFP8DX)
+
+
+# ---------------------------------------------------------------------------------------
 # Conv1d (torch/cuDNN ops; no sm_100a kernel: not on any benchmarked path)
 # ---------------------------------------------------------------------------------------
 
@@ -353,6 +462,21 @@ def replace_linear_with_linear_dw(model: nn.Module, device=None) -> nn.Module:
     def make(m):
         if isinstance(m, nn.Linear) and not isinstance(m, LayerDW):
             return LinearDW(m)
+        return None
+
+    _swap_children(model, make)
+    return model
+
+
+def replace_linear_with_linear_fp8(model: nn.Module, select=None) -> nn.Module:
+    """In place: swap ``nn.Linear`` and ``LinearDW`` layers for ``LinearFP8DW``, all of them or those for which
+    ``select(name, module)`` is true.  Layers already in 8 bits stay."""
+
+    names = {id(m): name for name, m in model.named_modules()}
+
+    def make(m):
+        if type(m) in (nn.Linear, LinearDW) and (select is None or select(names[id(m)], m)):
+            return LinearFP8DW(m)
         return None
 
     _swap_children(model, make)

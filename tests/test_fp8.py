@@ -1,0 +1,286 @@
+"""8-bit operators on the CPU: their plain forms against the definition, gradients, refusals, the split-backward
+layer and the Llama option."""
+
+import copy
+
+import pytest
+import torch
+
+from elf_b200 import Pipeline
+from elf_b200.models.llama import LlamaConfig, LlamaMLPBlock, build_llama_stages, llama_loss_fn
+from elf_b200.ops import fp8
+from elf_b200.ops.fp8 import BlockScaled
+from elf_b200.zb_utils import LinearDW, LinearFP8DW, replace_layer_with_layer_dw, replace_linear_with_linear_fp8
+
+from .fp8_oracle import held, product_bound, values
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def rand(*shape, dtype=torch.float32, seed=0):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 130), (130, 256), (5, 1000)])
+def test_plain_quantize_is_exact(rows, cols, dtype):
+    x = rand(rows, cols, dtype=dtype, seed=rows) * 30
+    x[0, 0] = float("inf")
+    if cols > 1:
+        x[-1, 1] = float("nan")
+        x[:, 2::3] *= 1e-3
+    for make, block_rows in ((fp8.quantize, 1), (fp8.quantize_weight, 128)):
+        q = make(x)
+        want, exps = held(x, block_rows)
+        assert torch.equal(q.scale, exps)
+        assert torch.equal(values(q).isnan(), want.isnan()) and torch.equal(values(q).nan_to_num(0.0), want.nan_to_num(0.0))
+        assert torch.equal(q.dequantize(torch.float32).double().nan_to_num(0.0), want.nan_to_num(0.0))
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (7, 130, 140), (40, 64, 300)])
+def test_plain_products(m, n, k):
+    x, dy, w = fp8.quantize(rand(m, k)), fp8.quantize(rand(m, n, seed=1)), fp8.quantize_weight(rand(n, k, seed=2))
+    for got, a, b in ((fp8.linear_forward(x, w), values(x), values(w).T), (fp8.linear_input_grad(dy, w), values(dy), values(w)),
+                      (fp8.linear_weight_grad(dy, x), values(dy).T, values(x))):
+        assert got.dtype == torch.bfloat16 and ((got.double() - a @ b).abs() <= product_bound(a, b, torch.bfloat16)).all()
+
+
+def test_gate_gradient_formula_against_differences():
+    """d silu(g) u as the operators form it, against central differences in 64 bits."""
+    g, u, d = (rand(64, seed=s).double() * 4 for s in (0, 1, 2))
+    f = lambda g, u: (torch.nn.functional.silu(g) * u * d).sum()
+    s = torch.sigmoid(g)
+    for i in range(64):
+        e = torch.zeros(64, dtype=torch.float64)
+        e[i] = 1e-5
+        # the second differences' error: h^2/6 of a third derivative below 1, plus rounding 2^-52 / h
+        assert abs((f(g + e, u) - f(g - e, u)) / 2e-5 - d[i] * u[i] * s[i] * (1 + g[i] * (1 - s[i]))) < 1e-8
+        assert abs((f(g, u + e) - f(g, u - e)) / 2e-5 - d[i] * g[i] * s[i]) < 1e-8
+
+
+def test_linear_gradients_are_those_of_the_rounded_operands():
+    x, w, b = rand(2, 9, 200).requires_grad_(), rand(72, 200, seed=1).requires_grad_(), rand(72, seed=2).requires_grad_()
+    dy = rand(2, 9, 72, seed=3)
+    y = fp8.linear(x, w, b)
+    y.backward(dy)
+    xq, wq, dyq = (held(t.detach().reshape(-1, t.shape[-1]), r)[0] for t, r in ((x, 1), (w, 128), (dy, 1)))
+    for got, a, m in ((x.grad, dyq, wq), (w.grad, dyq.T, xq)):
+        assert ((got.reshape(-1, got.shape[-1]).double() - a @ m).abs() <= product_bound(a, m, torch.float32)).all()
+    assert ((y.detach().view(18, 72).double() - (xq @ wq.T + b.detach().double())).abs() <= product_bound(xq, wq.T, torch.float32) + 1e-6).all()
+    # 18 fp32 additions
+    assert ((b.grad.double() - dy.double().sum((0, 1))).abs() <= 18 * 2.0**-24 * dy.double().abs().sum((0, 1))).all()
+    # with the copy the program keeps: the same
+    x2, w2 = x.detach().clone().requires_grad_(), w.detach().clone().requires_grad_()
+    y2 = fp8.linear(x2, w2, b.detach(), fp8.quantize_weight(w.detach()))
+    y2.backward(dy)
+    assert torch.equal(y2, y) and torch.equal(x2.grad, x.grad) and torch.equal(w2.grad, w.grad)
+
+
+def test_gated_ffn_matches_its_parts_and_saves_8_bits():
+    x, wg, wd = rand(12, 144, seed=4).requires_grad_(), (rand(512, 144, seed=5) * 0.1).requires_grad_(), (rand(80, 256, seed=6) * 0.1).requires_grad_()
+    dy = rand(12, 80, seed=7)
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (kept.append(t), t)[1], lambda t: t):
+        y = fp8.gated_ffn(x, wg, wd)
+    y.backward(dy)
+    weights = {wg.data_ptr(), wd.data_ptr()}
+    activations = [t for t in kept if t.data_ptr() not in weights]
+    assert all(t.element_size() == 1 for t in activations)
+    assert sum(t.numel() for t in activations if t.dtype != torch.uint8) == 12 * (144 + 3 * 256)
+    gq, dq = fp8.quantize_weight(wg.detach()), fp8.quantize_weight(wd.detach())
+    xq = fp8.quantize(x.detach())
+    act, gu = fp8.gated_forward(xq, gq)
+    assert torch.equal(y, fp8.linear_forward(act, dq, out_dtype=torch.float32))
+    dgu = fp8.gated_backward(fp8.quantize(dy), dq, gu)
+    assert torch.equal(x.grad, fp8.linear_input_grad(dgu, gq, torch.float32))
+    assert torch.equal(wg.grad, fp8.linear_weight_grad(dgu, xq, out_dtype=torch.float32))
+    assert torch.equal(wd.grad, fp8.linear_weight_grad(dy, act, out_dtype=torch.float32))
+    with torch.no_grad():
+        assert torch.equal(fp8.gated_ffn(x, wg, wd), y)
+
+
+def test_only_requested_gradients():
+    x, w = rand(4, 64), rand(8, 64).requires_grad_()
+    fp8.linear(x, w).sum().backward()
+    assert w.grad is not None and x.grad is None
+    x, wg, wd = rand(4, 64).requires_grad_(), rand(256, 64), rand(8, 128)
+    fp8.gated_ffn(x, wg, wd).sum().backward()
+    assert x.grad is not None
+    wd.requires_grad_()
+    fp8.gated_ffn(x.detach(), wg, wd).sum().backward()
+    assert wd.grad is not None
+
+
+def test_refusals():
+    data, scale = torch.zeros(4, 200).to(torch.float8_e4m3fn), torch.zeros(4, 2, dtype=torch.uint8)
+    q, w = BlockScaled(data, scale), fp8.quantize_weight(rand(256, 200))
+    with pytest.raises(TypeError, match="float8_e4m3fn"):
+        BlockScaled(torch.zeros(4, 200), scale)
+    with pytest.raises(ValueError, match="block_rows"):
+        BlockScaled(data, scale, 64)
+    with pytest.raises(ValueError, match="expected exponents"):
+        BlockScaled(data, scale[:, :1])
+    with pytest.raises(ValueError, match="expected exponents"):
+        BlockScaled(data, scale, 128)
+    with pytest.raises(TypeError, match="bf16, fp16 or fp32"):
+        fp8.quantize(torch.zeros(4, 4, dtype=torch.int32))
+    with pytest.raises(TypeError, match="bf16, fp16 or fp32"):
+        fp8.quantize(torch.zeros(4, 4, dtype=torch.float64))
+    with pytest.raises(ValueError, match="at least one dimension"):
+        fp8.quantize(torch.tensor(1.0))
+    with pytest.raises(ValueError, match="matrix"):
+        fp8.quantize_weight(torch.zeros(2, 3, 4))
+    with pytest.raises(TypeError, match="not torch.float64"):
+        fp8.dequantize(q, torch.float64)
+    with pytest.raises(ValueError, match="out does not match"):
+        fp8.dequantize(q, out=torch.empty(4, 100))
+    with pytest.raises(ValueError, match="reduction lengths"):
+        fp8.linear_forward(fp8.quantize(rand(4, 199)), w)
+    with pytest.raises(ValueError, match="scaled by rows"):
+        fp8.linear_forward(w, w)
+    with pytest.raises(ValueError, match="bias"):
+        fp8.linear_forward(q, w, torch.zeros(3))
+    with pytest.raises(TypeError, match="products come in"):
+        fp8.linear_forward(q, w, out_dtype=torch.float64)
+    with pytest.raises(ValueError, match="tiles of 128 x 128"):
+        fp8.linear_input_grad(fp8.quantize(rand(4, 256)), fp8.quantize(rand(256, 200)))
+    with pytest.raises(ValueError, match="numbers of rows"):
+        fp8.linear_weight_grad(q, fp8.quantize(rand(5, 8)))
+    with pytest.raises(ValueError, match="out must be"):
+        fp8.linear_weight_grad(q, q, out=torch.zeros(200, 199))
+    with pytest.raises(ValueError, match="multiple of 128"):
+        fp8.gated_forward(q, fp8.quantize_weight(rand(200, 200)))
+    with pytest.raises(ValueError, match="multiple of 128"):
+        fp8.gated_ffn(rand(4, 16), rand(200, 16), rand(16, 100))
+    with pytest.raises(ValueError, match="do not match"):
+        fp8.gated_ffn(rand(4, 16), rand(256, 16), rand(16, 256))
+    with pytest.raises(ValueError, match="expected gate_up"):
+        fp8.gated_backward(fp8.quantize(rand(4, 16)), fp8.quantize_weight(rand(16, 128)), q)
+    with pytest.raises(ValueError, match="does not match a weight"):
+        fp8.linear(rand(4, 16), rand(8, 17))
+    with pytest.raises(ValueError, match="8-bit copy"):
+        fp8.linear(rand(4, 200), rand(8, 200), w_q=w)
+    with pytest.raises(ValueError, match="gain"):
+        fp8.rms_norm(rand(4, 16), torch.ones(8))
+    with pytest.raises(ValueError, match="residual"):
+        fp8.add_rms_norm(rand(4, 16), rand(4, 8), torch.ones(16))
+    with pytest.raises(ValueError, match="on one device"):
+        fp8.linear(rand(4, 16), torch.empty(8, 16, device="meta"))
+
+
+# ------------------------------------------------------------------------------ split-backward layer
+
+
+def test_split_backward_layer():
+    lin = torch.nn.Linear(200, 72)
+    layer = LinearFP8DW(copy.deepcopy(lin))
+    x = rand(2, 9, 200).requires_grad_()
+    dy = rand(2, 9, 72, seed=1)
+    h = x * 1.0
+    y = layer(h)
+    y.backward(dy)
+    assert layer.weight.grad is None  # B pass leaves parameters alone
+    assert isinstance(layer.last_input, BlockScaled) and isinstance(layer.last_grad_output, BlockScaled)
+    assert not layer.last_input.is_model_input
+    layer.move_last_computed("input", 3)
+    layer.move_last_computed("grad_output", 3)
+    layer.offload_last(3, "cpu")
+    layer.backward(3)
+    x2 = x.detach().clone().requires_grad_()
+    ref = fp8.linear(x2, lin.weight, lin.bias)
+    ref.backward(dy)
+    assert torch.equal(y, ref) and torch.equal(x.grad, x2.grad)
+    assert torch.equal(layer.weight.grad, lin.weight.grad)
+    # the bias gradient sums the 8-bit stash: each value is off by 2^-4 of itself or 2^-10 of its block's scale
+    assert ((layer.bias.grad - lin.bias.grad).abs() <= (dy.abs() * 2.0**-4 + dy.abs().amax() * 2.0**-16).sum((0, 1)) + 1e-5).all()
+    with pytest.raises(ValueError, match="incomplete"):
+        layer.backward(3)
+    first = layer.weight.grad.clone()
+    layer(x.detach())  # accumulates, and a stage input stays
+    assert layer.last_input.is_model_input
+    layer.last_grad_output = fp8.quantize(dy)
+    layer.move_last_computed("input", 0)
+    layer.move_last_computed("grad_output", 0)
+    layer.backward(0)
+    assert torch.allclose(layer.weight.grad, 2 * first, rtol=1e-5, atol=1e-5)
+
+
+def test_weight_copy_is_held_for_a_step_only():
+    layer = LinearFP8DW(torch.nn.Linear(64, 32, bias=False))
+    x = rand(4, 64)
+    before = layer(x)
+    with torch.no_grad():
+        layer.weight.mul_(2)
+    assert torch.equal(layer(x), 2 * before)  # outside a step: always the weight as it is
+    layer.begin_step()
+    q = layer.weight_q()
+    assert layer.weight_q() is q
+    layer.clear()
+    with torch.no_grad():
+        layer.weight.mul_(2)
+    assert torch.equal(layer(x), 4 * before)
+
+
+def test_layer_applied_twice_sums_its_output_gradients():
+    layer = LinearFP8DW(torch.nn.Linear(64, 64, bias=False))
+    x = rand(4, 64).requires_grad_()
+    layer(layer(x)).sum().backward()
+    assert isinstance(layer.last_grad_output, torch.Tensor) and layer.last_grad_output.dtype == torch.bfloat16
+
+
+def test_replacement_selects_layers():
+    model = torch.nn.Sequential(torch.nn.Linear(8, 8), torch.nn.ReLU(), torch.nn.Linear(8, 8))
+    replace_layer_with_layer_dw(model)
+    replace_linear_with_linear_fp8(model, lambda name, m: name == "2")
+    assert type(model[0]) is LinearDW and type(model[2]) is LinearFP8DW
+    inner = model[2]
+    replace_linear_with_linear_fp8(model)
+    assert type(model[0]) is LinearFP8DW and model[2] is inner
+
+
+# ------------------------------------------------------------------------------ Llama
+
+CFG = LlamaConfig(n_layers=2, d_model=128, n_heads=4, n_kv_heads=2, ffn=256, vocab=512, seq_len=32, rope_theta=10000.0)
+
+
+def test_llama_option_builds_8_bit_layers():
+    cfg = LlamaConfig(**{**CFG.__dict__, "ffn_fp8": True})
+    (stage,) = build_llama_stages(cfg, 1, dtype=torch.float32)
+    kinds = {name.rpartition(".")[2]: type(m) for name, m in stage.named_modules() if isinstance(m, LinearDW)}
+    assert kinds == {"wqkv": LinearDW, "wo": LinearDW, "w_gate_up": LinearFP8DW, "w_down": LinearFP8DW, "out": LinearDW}
+    assert [n for n, _ in stage.named_parameters()] == [n for n, _ in build_llama_stages(CFG, 1, dtype=torch.float32)[0].named_parameters()]
+    with pytest.raises(ValueError, match="split_backward"):
+        build_llama_stages(cfg, 1, split_backward=False)
+
+
+@pytest.mark.parametrize("scheduler", ["zbv", "afab", "full_remat"])
+def test_llama_pipeline_steps_in_8_bits(scheduler):
+    """Whole steps through the pipeline: the loss and the gradients stay near those of the 16-bit feed-forward
+    layers.  Rounding an operand to e4m3 moves it by at most 2^-4 of itself, 2^-4 / sqrt(3) = 3.6 % in the mean
+    square; a feed-forward gradient passes five such roundings, 3.6 % sqrt(5) = 8 %, and 16 % allows for their meeting
+    in the second layer."""
+    tok = torch.randint(0, CFG.vocab, (4, CFG.seq_len + 1), generator=torch.Generator().manual_seed(0))
+    grads, losses = [], []
+    for ffn_fp8 in (False, True):
+        cfg = LlamaConfig(**{**CFG.__dict__, "ffn_fp8": ffn_fp8})
+        placement = [0, 0]
+        stages = build_llama_stages(cfg, 2, dtype=torch.float32, seed=3)
+        pipe = Pipeline(stages, None, partitioner=False, scheduler=scheduler, placement=placement, outputs="none")
+        for _ in range(2):
+            pipe.zero_grad()
+            _, loss = pipe(tok[:, :-1].contiguous(), tok[:, 1:].contiguous(), llama_loss_fn, split_size=1)
+        losses.append(float(loss))
+        grads.append({n: p.grad.clone() for n, p in pipe.named_parameters()})
+        assert all(m._weight_q is None and m.is_empty("input") for b in pipe.blocks for m in b.dw_layers() if isinstance(m, LinearFP8DW))
+    assert abs(losses[0] - losses[1]) < 0.02 * losses[0]
+    for name, g in grads[0].items():
+        assert (grads[1][name] - g).norm() <= 0.16 * g.norm(), name
+
+
+def test_mlp_block_composes_on_cpu():
+    torch.manual_seed(0)
+    blk = LlamaMLPBlock(CFG)
+    replace_linear_with_linear_fp8(blk)
+    x = rand(2, 8, CFG.d_model).requires_grad_()
+    blk(x).sum().backward()
+    assert x.grad is not None and isinstance(blk.w_down.last_input, BlockScaled)

@@ -25,6 +25,12 @@ elfb::Elem elem_of(const at::Tensor& t, const char* name) {
   return elfb::Elem::kF32;
 }
 
+int sm_count(const at::Device& dev) { return at::cuda::getDeviceProperties(dev.index())->multiProcessorCount; }
+int* status_ptr(const at::Tensor& status, const at::Device& dev) {
+  TORCH_CHECK(status.is_cuda() && status.device() == dev && status.scalar_type() == at::kInt && status.numel() >= 4, "status must be an int32[4] tensor on ", dev);
+  return status.data_ptr<int>();
+}
+
 int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
 int64_t round_up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
@@ -168,7 +174,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> rmsnorm(const at::Ten
   auto rstd = dense(lead_of(x), at::kFloat, dev);
   const Scaled s = scaled(q.first, q.second, 0, "data", dev, false);
   check(elfb::fp8_rmsnorm(x.data_ptr(), res.defined() ? res.data_ptr() : nullptr, w.data_ptr(), res.defined() ? h.data_ptr() : nullptr, rstd.data_ptr<float>(),
-                          s.data.bytes(), s.data.pitch, s.scale.bytes(), s.scale.pitch, rows, int(dim), float(eps), cur()),
+                          s.data.bytes(), s.data.pitch, s.scale.bytes(), s.scale.pitch, rows, int(dim), float(eps), sm_count(dev), cur()),
         "fp8_rmsnorm");
   return {q.first, q.second, rstd, h};
 }
@@ -207,12 +213,7 @@ Operand operand(const at::Tensor& data, const at::Tensor& scale, int64_t row_shi
   return r;
 }
 
-int sm_count(const at::Device& dev) { return at::cuda::getDeviceProperties(dev.index())->multiProcessorCount; }
 
-int* status_ptr(const at::Tensor& status, const at::Device& dev) {
-  TORCH_CHECK(status.is_cuda() && status.device() == dev && status.scalar_type() == at::kInt && status.numel() >= 4, "status must be an int32[4] tensor on ", dev);
-  return status.data_ptr<int>();
-}
 
 void launch(elfb::Fp8GemmArgs& g, const at::Tensor& status, const at::Device& dev, const char* what) {
   g.status = status_ptr(status, dev);
@@ -326,7 +327,7 @@ std::pair<at::Tensor, at::Tensor> gated_bwd(const at::Tensor& dy, const at::Tens
 void register_fp8(pybind11::module_& m) {
   m.def("fp8_quantize", &quantize, py::arg("x"), py::arg("tiles"), py::arg("data") = c10::nullopt, py::arg("scale") = c10::nullopt);
   m.def("fp8_dequantize", &dequantize, py::arg("data"), py::arg("scale"), py::arg("row_shift"), py::arg("dtype"), py::arg("out") = c10::nullopt);
-  m.def("fp8_rmsnorm", &rmsnorm, py::arg("x"), py::arg("w"), py::arg("eps"), py::arg("residual") = c10::nullopt);
+  m.def("fp8_rmsnorm", &rmsnorm, py::arg("x"), py::arg("w"), py::arg("eps"), py::arg("residual"));
   m.def("fp8_gemm", &gemm, py::arg("a"), py::arg("a_scale"), py::arg("b"), py::arg("b_scale"), py::arg("b_row_shift"), py::arg("b_mn_major"), py::arg("dtype"),
         py::arg("bias"), py::arg("status"));
   m.def("fp8_gated", &gated, py::arg("a"), py::arg("a_scale"), py::arg("b"), py::arg("b_scale"), py::arg("b_row_shift"), py::arg("keep"), py::arg("status"));

@@ -6,6 +6,7 @@
 #include <algorithm>
 
 #include "fp8_block.cuh"
+#include "sm100_ptx.cuh"
 
 namespace elfb {
 
@@ -14,6 +15,8 @@ namespace {
 constexpr int BLOCK = 128;  // columns that share a scale
 constexpr int UNIT = 16;    // consecutive values a thread holds: 8 lanes make up a block
 constexpr int THREADS = 256;
+constexpr int NORM_THREADS = 256;
+constexpr int UNITS = 2;    // groups of 16 values per thread of the streaming kernels
 
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __uint_as_float(uint32_t(__bfloat16_as_ushort(v)) << 16); }
@@ -27,39 +30,63 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { re
 template <>
 __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-// N consecutive values as fp32.  VEC: the address is a multiple of 16 bytes and all N exist.
-template <typename T, int N, bool VEC>
-__device__ __forceinline__ void load_values(const T* p, int have, float (&v)[N]) {
-  if constexpr (VEC) {
-    constexpr int PER = 16 / sizeof(T);
+// How a thread's 16 values are moved: one by one, or in pieces of 16 or 32 bytes that the address is a multiple of.
+enum class Access { kRagged, kPieces16, kPieces32 };
+
+__device__ __forceinline__ void load_piece(const void* p, uint4& a) { a = *static_cast<const uint4*>(p); }
+__device__ __forceinline__ void load_piece(const void* p, uint4& a, uint4& b) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+               : "l"(p));
+}
+__device__ __forceinline__ void store_piece(void* p, uint4 a, uint4 b) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
+}
+
+// UNIT consecutive values as they lie in memory.
+template <typename T>
+struct Raw {
+  uint4 q[UNIT * sizeof(T) / 16];
+};
+template <typename T, Access A>
+__device__ __forceinline__ void load_raw(const T* p, int have, Raw<T>& r) {
+  constexpr int N = UNIT * sizeof(T) / 16;
+  if constexpr (A == Access::kPieces32) {
 #pragma unroll
-    for (int i = 0; i < N / PER; ++i) {
-      const uint4 q = reinterpret_cast<const uint4*>(p)[i];
-      const T* e = reinterpret_cast<const T*>(&q);
+    for (int i = 0; i < N; i += 2) load_piece(reinterpret_cast<const uint4*>(p) + i, r.q[i], r.q[i + 1]);
+  } else if constexpr (A == Access::kPieces16) {
 #pragma unroll
-      for (int j = 0; j < PER; ++j) v[i * PER + j] = to_float(e[j]);
-    }
+    for (int i = 0; i < N; ++i) load_piece(reinterpret_cast<const uint4*>(p) + i, r.q[i]);
   } else {
+    T* e = reinterpret_cast<T*>(r.q);
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = j < have ? to_float(p[j]) : 0.f;
+    for (int j = 0; j < UNIT; ++j) e[j] = j < have ? p[j] : from_float<T>(0.f);
   }
 }
-template <typename T, int N, bool VEC>
-__device__ __forceinline__ void store_values(T* p, int have, const float (&v)[N]) {
-  if constexpr (VEC) {
-    constexpr int PER = 16 / sizeof(T);
+template <typename T>
+__device__ __forceinline__ void unpack(const Raw<T>& r, float (&v)[UNIT]) {
+  const T* e = reinterpret_cast<const T*>(r.q);
 #pragma unroll
-    for (int i = 0; i < N / PER; ++i) {
-      uint4 q;
-      T* e = reinterpret_cast<T*>(&q);
+  for (int j = 0; j < UNIT; ++j) v[j] = to_float(e[j]);
+}
+template <typename T, Access A>
+__device__ __forceinline__ void store_values(T* p, int have, const float (&v)[UNIT]) {
+  constexpr int N = UNIT * sizeof(T) / 16;
+  Raw<T> r;
+  T* e = reinterpret_cast<T*>(r.q);
 #pragma unroll
-      for (int j = 0; j < PER; ++j) e[j] = from_float<T>(v[i * PER + j]);
-      reinterpret_cast<uint4*>(p)[i] = q;
-    }
+  for (int j = 0; j < UNIT; ++j) e[j] = from_float<T>(v[j]);
+  if constexpr (A == Access::kPieces32) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) store_piece(reinterpret_cast<uint4*>(p) + i, r.q[i], r.q[i + 1]);
+  } else if constexpr (A == Access::kPieces16) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) reinterpret_cast<uint4*>(p)[i] = r.q[i];
   } else {
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (j < have) p[j] = from_float<T>(v[j]);
+    for (int j = 0; j < UNIT; ++j)
+      if (j < have) p[j] = e[j];
   }
 }
 __device__ __forceinline__ void store_bytes_ragged(uint8_t* p, int have, const uint32_t (&q)[UNIT / 4]) {
@@ -69,37 +96,48 @@ __device__ __forceinline__ void store_bytes_ragged(uint8_t* p, int have, const u
 }
 
 // ------------------------------------------------------------------------------ quantise
-// One thread per 16 values; the 8 lanes of a block find its maximum with three shuffles.
-template <typename T, bool VEC>
+// A thread takes two groups of 16 values, 256 groups apart, and loads both before it looks at either; the 8 lanes
+// of a block find its maximum with three shuffles.
+template <typename T, Access A>
 __global__ void __launch_bounds__(THREADS) quantize_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ data, long long ldq,
                                                                 uint8_t* __restrict__ scale, long long lds, uint32_t total, uint32_t units_per_row,
                                                                 int cols) {
-  const uint32_t u = blockIdx.x * THREADS + threadIdx.x;
-  const uint32_t row = u / units_per_row;
-  const int col = int(u - row * units_per_row) * UNIT;
-  const int have = u < total ? min(cols - col, UNIT) : 0;  // 0 or less: padding of a row's last block
-  float v[UNIT];
-  if (have > 0) {
-    load_values<T, UNIT, VEC>(x + (long long)row * ldx + col, have, v);
-  } else {
+  Raw<T> raw[UNITS];
+  uint32_t row[UNITS];
+  int col[UNITS], have[UNITS];
 #pragma unroll
-    for (int j = 0; j < UNIT; ++j) v[j] = 0.f;
+  for (int i = 0; i < UNITS; ++i) {
+    const uint32_t u = (blockIdx.x * UNITS + i) * THREADS + threadIdx.x;
+    row[i] = u / units_per_row;
+    col[i] = int(u - row[i] * units_per_row) * UNIT;
+    have[i] = u < total ? min(cols - col[i], UNIT) : 0;  // 0 or less: padding of a row's last block
+    if (have[i] > 0) {
+      load_raw<T, A>(x + (long long)row[i] * ldx + col[i], have[i], raw[i]);
+    } else {
+#pragma unroll
+      for (uint4& q : raw[i].q) q = make_uint4(0, 0, 0, 0);
+    }
   }
-  uint32_t q[UNIT / 4];
-  const uint32_t byte = quantize_block<UNIT, 8>(v, q);
-  if (have > 0) {
-    uint8_t* dst = data + (long long)row * ldq + col;
-    if constexpr (VEC)
-      *reinterpret_cast<uint4*>(dst) = make_uint4(q[0], q[1], q[2], q[3]);
-    else
-      store_bytes_ragged(dst, have, q);
-    if ((col & (BLOCK - 1)) == 0) scale[(long long)row * lds + col / BLOCK] = uint8_t(byte);
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) {
+    float v[UNIT];
+    unpack<T>(raw[i], v);
+    uint32_t q[UNIT / 4];
+    const uint32_t byte = quantize_block<UNIT, 8>(v, q);
+    if (have[i] > 0) {
+      uint8_t* dst = data + (long long)row[i] * ldq + col[i];
+      if constexpr (A != Access::kRagged)
+        *reinterpret_cast<uint4*>(dst) = make_uint4(q[0], q[1], q[2], q[3]);
+      else
+        store_bytes_ragged(dst, have[i], q);
+      if ((col[i] & (BLOCK - 1)) == 0) scale[(long long)row[i] * lds + col[i] / BLOCK] = uint8_t(byte);
+    }
   }
 }
 
 // One block of threads per 128 x 128 tile: every thread holds four groups of 16 values (rows 32
 // apart), so the tile is read once.
-template <typename T, bool VEC>
+template <typename T, Access A>
 __global__ void __launch_bounds__(THREADS) quantize_tiles_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ data, long long ldq,
                                                                  uint8_t* __restrict__ scale, long long lds, long long rows, int cols) {
   __shared__ uint32_t warp_max[2][THREADS / 32];
@@ -112,7 +150,9 @@ __global__ void __launch_bounds__(THREADS) quantize_tiles_kernel(const T* __rest
   for (int i = 0; i < 4; ++i) {
     const long long row = row0 + 32 * i;
     if (have_cols > 0 && row < rows) {
-      load_values<T, UNIT, VEC>(x + row * ldx + col, have_cols, v[i]);
+      Raw<T> raw;
+      load_raw<T, A>(x + row * ldx + col, have_cols, raw);
+      unpack<T>(raw, v[i]);
     } else {
 #pragma unroll
       for (int j = 0; j < UNIT; ++j) v[i][j] = 0.f;
@@ -152,7 +192,7 @@ __global__ void __launch_bounds__(THREADS) quantize_tiles_kernel(const T* __rest
 #pragma unroll
     for (int j = 0; j < UNIT / 4; ++j) q[j] = to_e4m3x4(s[4 * j], s[4 * j + 1], s[4 * j + 2], s[4 * j + 3]);
     uint8_t* dst = data + row * ldq + col;
-    if constexpr (VEC)
+    if constexpr (A != Access::kRagged)
       *reinterpret_cast<uint4*>(dst) = make_uint4(q[0], q[1], q[2], q[3]);
     else
       store_bytes_ragged(dst, have_cols, q);
@@ -161,74 +201,110 @@ __global__ void __launch_bounds__(THREADS) quantize_tiles_kernel(const T* __rest
 }
 
 // ------------------------------------------------------------------------------ restore
-template <typename T, bool VEC>
+template <typename T, Access A>
 __global__ void __launch_bounds__(THREADS) dequantize_kernel(const uint8_t* __restrict__ data, long long ldq, const uint8_t* __restrict__ scale,
                                                              long long lds, int row_shift, T* __restrict__ y, long long ldy, uint32_t total,
                                                              uint32_t units_per_row, long long first_row, int cols) {
-  const uint32_t u = blockIdx.x * THREADS + threadIdx.x;
-  if (u >= total) return;
-  const uint32_t r = u / units_per_row;
-  const int col = int(u - r * units_per_row) * UNIT;
-  const long long row = first_row + r;
-  const int have = min(cols - col, UNIT);
-  const uint8_t* src = data + row * ldq + col;
-  uint32_t q[UNIT / 4];
-  if constexpr (VEC) {
-    const uint4 t = *reinterpret_cast<const uint4*>(src);
-    q[0] = t.x, q[1] = t.y, q[2] = t.z, q[3] = t.w;
-  } else {
+  uint32_t q[UNITS][UNIT / 4], byte[UNITS];
+  long long row[UNITS];
+  int col[UNITS], have[UNITS];
 #pragma unroll
-    for (int j = 0; j < UNIT / 4; ++j) q[j] = 0;
+  for (int i = 0; i < UNITS; ++i) {
+    const uint32_t u = (blockIdx.x * UNITS + i) * THREADS + threadIdx.x;
+    const uint32_t r = u / units_per_row;
+    row[i] = first_row + r;
+    col[i] = int(u - r * units_per_row) * UNIT;
+    have[i] = u < total ? min(cols - col[i], UNIT) : 0;
+    if (have[i] <= 0) continue;
+    const uint8_t* src = data + row[i] * ldq + col[i];
+    if constexpr (A != Access::kRagged) {
+      const uint4 t = *reinterpret_cast<const uint4*>(src);
+      q[i][0] = t.x, q[i][1] = t.y, q[i][2] = t.z, q[i][3] = t.w;
+    } else {
 #pragma unroll
-    for (int j = 0; j < UNIT; ++j)
-      if (j < have) q[j / 4] |= uint32_t(src[j]) << (8 * (j % 4));
+      for (int j = 0; j < UNIT / 4; ++j) q[i][j] = 0;
+#pragma unroll
+      for (int j = 0; j < UNIT; ++j)
+        if (j < have[i]) q[i][j / 4] |= uint32_t(src[j]) << (8 * (j % 4));
+    }
+    byte[i] = scale[(row[i] >> row_shift) * lds + col[i] / BLOCK];
   }
-  const float s = exponent_value(scale[(row >> row_shift) * lds + col / BLOCK]);
-  float v[UNIT];
 #pragma unroll
-  for (int j = 0; j < UNIT / 4; ++j) {
-    const float2 lo = from_e4m3x2(q[j] & 0xffffu), hi = from_e4m3x2(q[j] >> 16);
-    v[4 * j] = mul_exact(lo.x, s);
-    v[4 * j + 1] = mul_exact(lo.y, s);
-    v[4 * j + 2] = mul_exact(hi.x, s);
-    v[4 * j + 3] = mul_exact(hi.y, s);
+  for (int i = 0; i < UNITS; ++i) {
+    if (have[i] <= 0) continue;
+    const float s = exponent_value(byte[i]);
+    float v[UNIT];
+#pragma unroll
+    for (int j = 0; j < UNIT / 4; ++j) {
+      const float2 lo = from_e4m3x2(q[i][j] & 0xffffu), hi = from_e4m3x2(q[i][j] >> 16);
+      v[4 * j] = mul_exact(lo.x, s);
+      v[4 * j + 1] = mul_exact(lo.y, s);
+      v[4 * j + 2] = mul_exact(hi.x, s);
+      v[4 * j + 3] = mul_exact(hi.y, s);
+    }
+    store_values<T, A>(y + row[i] * ldy + col[i], have[i], v);
   }
-  store_values<T, UNIT, VEC>(y + row * ldy + col, have, v);
 }
 
 // ------------------------------------------------------------------------------ RMSNorm
 // h = x + residual (rounded to bf16, as the next residual addition reads it), y = h * rstd * w, y in
-// 8 bits.  TPR threads per row hold it in registers, 8 values (16 bytes) per thread and step; the 16
-// lanes whose values make up a block scale it with four shuffles.
-template <int TPR, int VPT, bool RESIDUAL>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) rmsnorm_fp8_kernel(const uint4* __restrict__ x, const uint4* __restrict__ res,
-                                                                            const uint4* __restrict__ w, uint4* __restrict__ h, float* __restrict__ rstd,
-                                                                            uint8_t* __restrict__ data, long long ldq, uint8_t* __restrict__ scale,
-                                                                            long long lds, long long rows, int dim8, float inv_dim, float eps) {
-  constexpr int ROWS = TPR < 128 ? 128 / TPR : 1;  // rows per block
-  __shared__ float red[TPR / 32 + 1];
-  const int t = threadIdx.x % TPR;
-  const long long row = (long long)blockIdx.x * ROWS + threadIdx.x / TPR;
-  const bool live = row < rows;
+// 8 bits.  Each thread holds 8 values (16 bytes) of a row per step; the 16 lanes whose values make up a
+// block scale it with four shuffles.
+__device__ __forceinline__ void unpack8(uint4 q, float (&v)[8]) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+}
+// v = x + r rounded to bf16; returns it packed
+__device__ __forceinline__ uint4 add_rounded(uint4 x, uint4 r, float (&v)[8]) {
+  float a[8], b[8];
+  unpack8(x, a);
+  unpack8(r, b);
+  const uint4 h = make_uint4(pack_bf16x2(a[0] + b[0], a[1] + b[1]), pack_bf16x2(a[2] + b[2], a[3] + b[3]), pack_bf16x2(a[4] + b[4], a[5] + b[5]),
+                             pack_bf16x2(a[6] + b[6], a[7] + b[7]));
+  unpack8(h, v);
+  return h;
+}
+
+struct NormArgs {
+  const uint4 *x, *res, *w;
+  uint4* h;
+  float* rstd;
+  uint8_t *data, *scale;
+  long long ldq, lds, rows;
+  int dim8;
+  float inv_dim, eps;
+};
+
+// 8 normalised values of column group c to 8 bits; all 32 lanes of the warp call this
+__device__ __forceinline__ void store_normalised(const NormArgs& p, long long row, int c, bool live, const float (&v)[8], uint4 gain, float rs) {
+  float g[8], y[8];
+  unpack8(gain, g);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) y[j] = c < p.dim8 ? v[j] * rs * g[j] : 0.f;
+  uint32_t q[2];
+  const uint32_t byte = quantize_block<8, 16>(y, q);
+  if (live && c < p.dim8) {
+    *reinterpret_cast<uint2*>(p.data + row * p.ldq + c * 8) = make_uint2(q[0], q[1]);
+    if ((c & 15) == 0) p.scale[row * p.lds + c / 16] = uint8_t(byte);
+  }
+}
+
+// Rows of up to 1024 values: a warp per row.
+template <int VPT, bool RESIDUAL>
+__global__ void __launch_bounds__(256) rmsnorm_fp8_warp_kernel(const __grid_constant__ NormArgs p) {
+  const int lane = threadIdx.x & 31;
+  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= p.rows) return;
   float v[VPT][8];
   float ss = 0.f;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int c = t + i * TPR;
-    if (live && c < dim8) {
-      load_values<__nv_bfloat16, 8, true>(reinterpret_cast<const __nv_bfloat16*>(x + row * dim8 + c), 8, v[i]);
-      if (RESIDUAL) {
-        float r[8];
-        load_values<__nv_bfloat16, 8, true>(reinterpret_cast<const __nv_bfloat16*>(res + row * dim8 + c), 8, r);
-        uint4 packed;
-        __nv_bfloat16* e = reinterpret_cast<__nv_bfloat16*>(&packed);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          e[j] = __float2bfloat16_rn(v[i][j] + r[j]);
-          v[i][j] = to_float(e[j]);
-        }
-        h[row * dim8 + c] = packed;
-      }
+    const int c = lane + i * 32;
+    if (c < p.dim8) {
+      const long long at = row * p.dim8 + c;
+      if (RESIDUAL) p.h[at] = add_rounded(p.x[at], p.res[at], v[i]);
+      else unpack8(p.x[at], v[i]);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
@@ -238,38 +314,82 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) rmsnorm_fp8_kernel(cons
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if (TPR > 32) {
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
+  const float rs = rsqrtf(ss * p.inv_dim + p.eps);
+  if (lane == 0) p.rstd[row] = rs;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int c = lane + i * 32;
+    if (i * 32 >= p.dim8) break;
+    store_normalised(p, row, c, true, v[i], c < p.dim8 ? p.w[c] : make_uint4(0, 0, 0, 0), rs);
+  }
+}
+
+// Wider rows: a block per row, four blocks per SM that walk the rows; the next row's loads are issued before the
+// current one is reduced.  4096 x 4096 with residual (117 MB): 24 us, 75 % of the copy bandwidth; one block per row
+// without the walk 29.6 us; 128 or 512 threads per row 27 us; a ring of rows in shared memory filled by bulk copies
+// 27 us (the time goes into the two dependent sweeps of a row, not into too few bytes in flight).
+template <int VPT, bool RESIDUAL>
+__global__ void __launch_bounds__(NORM_THREADS, VPT == 4 ? 2 : 1) rmsnorm_fp8_block_kernel(const __grid_constant__ NormArgs p) {
+  __shared__ float red[2][NORM_THREADS / 32];
+  const int t = threadIdx.x;
+  uint4 nx[VPT], nr[VPT], gain[VPT];
+  auto fetch = [&](long long row) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = t + i * NORM_THREADS;
+      if (row < p.rows && c < p.dim8) {
+        nx[i] = p.x[row * p.dim8 + c];
+        if (RESIDUAL) nr[i] = p.res[row * p.dim8 + c];
+      }
+    }
+  };
+  fetch(blockIdx.x);
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) gain[i] = t + i * NORM_THREADS < p.dim8 ? p.w[t + i * NORM_THREADS] : make_uint4(0, 0, 0, 0);
+  int turn = 0;
+  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+    float v[VPT][8];
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = t + i * NORM_THREADS;
+      if (c < p.dim8) {
+        if (RESIDUAL) p.h[row * p.dim8 + c] = add_rounded(nx[i], nr[i], v[i]);
+        else unpack8(nx[i], v[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
+    }
+    fetch(row + gridDim.x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if ((t & 31) == 0) red[turn][t >> 5] = ss;  // the other half may still be read by warps of the last round
     __syncthreads();
     ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < TPR / 32; ++i) ss += red[i];
-  }
-  const float rs = rsqrtf(ss * inv_dim + eps);
-  if (live && t == 0) rstd[row] = rs;
+    for (int i = 0; i < NORM_THREADS / 32; ++i) ss += red[turn][i];
+    const float rs = rsqrtf(ss * p.inv_dim + p.eps);
+    if (t == 0) p.rstd[row] = rs;
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int c = t + i * TPR;
-    if ((c & ~31) >= dim8) break;  // the whole warp is past the row
-    float g[8], y[8];
-    if (c < dim8) {
-      load_values<__nv_bfloat16, 8, true>(reinterpret_cast<const __nv_bfloat16*>(w + c), 8, g);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) g[j] = 0.f;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = c < dim8 ? v[i][j] * rs * g[j] : 0.f;
-    uint32_t q[2];
-    const uint32_t byte = quantize_block<8, 16>(y, q);
-    if (live && c < dim8) {
-      *reinterpret_cast<uint2*>(data + row * ldq + c * 8) = make_uint2(q[0], q[1]);
-      if ((c & 15) == 0) scale[row * lds + c / 16] = uint8_t(byte);
+    for (int i = 0; i < VPT; ++i) {
+      const int c = t + i * NORM_THREADS;
+      if ((c & ~31) >= p.dim8) break;  // the whole warp is past the row
+      store_normalised(p, row, c, true, v[i], gain[i], rs);
     }
   }
 }
 
-bool aligned16(const void* p, long long pitch_bytes) { return ((reinterpret_cast<uintptr_t>(p) | uintptr_t(pitch_bytes)) & 15) == 0; }
+bool aligned(const void* p, long long pitch_bytes, int to) { return (reinterpret_cast<uintptr_t>(p) | uintptr_t(pitch_bytes)) % to == 0; }
+// wide: the 16- or 32-bit matrix; bytes: the 8-bit one
+Access access_for(const void* wide, long long wide_pitch, const void* bytes, long long bytes_pitch, int cols) {
+  if (cols % UNIT != 0 || !aligned(wide, wide_pitch, 16) || !aligned(bytes, bytes_pitch, 16)) return Access::kRagged;
+  return aligned(wide, wide_pitch, 32) ? Access::kPieces32 : Access::kPieces16;
+}
+#define ELFB_ACCESS(KERNEL, T, A) \
+  (A == Access::kPieces32 ? KERNEL<T, Access::kPieces32> : A == Access::kPieces16 ? KERNEL<T, Access::kPieces16> : KERNEL<T, Access::kRagged>)
 
 // rows per launch, so that a launch's units fit 31 bits
 long long rows_per_launch(uint32_t units_per_row) { return std::max(1ll, (1ll << 30) / units_per_row); }
@@ -277,13 +397,13 @@ long long rows_per_launch(uint32_t units_per_row) { return std::max(1ll, (1ll <<
 template <typename T>
 cudaError_t quantize_rows_as(const void* x, long long ldx, uint8_t* data, long long ldq, uint8_t* scale, long long lds, long long rows, int cols,
                              cudaStream_t stream) {
-  const bool vec = cols % UNIT == 0 && aligned16(x, ldx * sizeof(T)) && aligned16(data, ldq);
+  const Access how = access_for(x, ldx * sizeof(T), data, ldq, cols);
   const uint32_t upr = uint32_t((cols + BLOCK - 1) / BLOCK) * (BLOCK / UNIT);
   const long long step = rows_per_launch(upr);
   for (long long r = 0; r < rows; r += step) {
     const uint32_t total = uint32_t(std::min(step, rows - r)) * upr;
-    auto* kern = vec ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>;
-    kern<<<(total + THREADS - 1) / THREADS, THREADS, 0, stream>>>(static_cast<const T*>(x) + r * ldx, ldx, data + r * ldq, ldq, scale + r * lds, lds, total,
+    auto* kern = ELFB_ACCESS(quantize_rows_kernel, T, how);
+    kern<<<(total + UNITS * THREADS - 1) / (UNITS * THREADS), THREADS, 0, stream>>>(static_cast<const T*>(x) + r * ldx, ldx, data + r * ldq, ldq, scale + r * lds, lds, total,
                                                                   upr, cols);
   }
   return cudaGetLastError();
@@ -292,13 +412,13 @@ cudaError_t quantize_rows_as(const void* x, long long ldx, uint8_t* data, long l
 template <typename T>
 cudaError_t quantize_tiles_as(const void* x, long long ldx, uint8_t* data, long long ldq, uint8_t* scale, long long lds, long long rows, int cols,
                               cudaStream_t stream) {
-  const bool vec = cols % UNIT == 0 && aligned16(x, ldx * sizeof(T)) && aligned16(data, ldq);
+  const Access how = access_for(x, ldx * sizeof(T), data, ldq, cols);
   constexpr long long kGridY = 65535;
   const long long tiles = (rows + BLOCK - 1) / BLOCK;
   for (long long t = 0; t < tiles; t += kGridY) {
     const long long r = t * BLOCK;
     const dim3 grid((cols + BLOCK - 1) / BLOCK, unsigned(std::min(kGridY, tiles - t)));
-    auto* kern = vec ? quantize_tiles_kernel<T, true> : quantize_tiles_kernel<T, false>;
+    auto* kern = ELFB_ACCESS(quantize_tiles_kernel, T, how);
     kern<<<grid, THREADS, 0, stream>>>(static_cast<const T*>(x) + r * ldx, ldx, data + r * ldq, ldq, scale + t * lds, lds, rows - r, cols);
   }
   return cudaGetLastError();
@@ -307,25 +427,35 @@ cudaError_t quantize_tiles_as(const void* x, long long ldx, uint8_t* data, long 
 template <typename T>
 cudaError_t dequantize_as(const uint8_t* data, long long ldq, const uint8_t* scale, long long lds, int row_shift, void* y, long long ldy, long long rows,
                           int cols, cudaStream_t stream) {
-  const bool vec = cols % UNIT == 0 && aligned16(y, ldy * sizeof(T)) && aligned16(data, ldq);
+  const Access how = access_for(y, ldy * sizeof(T), data, ldq, cols);
   const uint32_t upr = uint32_t((cols + UNIT - 1) / UNIT);
   const long long step = rows_per_launch(upr);
   for (long long r = 0; r < rows; r += step) {
     const uint32_t total = uint32_t(std::min(step, rows - r)) * upr;
-    auto* kern = vec ? dequantize_kernel<T, true> : dequantize_kernel<T, false>;
-    kern<<<(total + THREADS - 1) / THREADS, THREADS, 0, stream>>>(data, ldq, scale, lds, row_shift, static_cast<T*>(y), ldy, total, upr, r, cols);
+    auto* kern = ELFB_ACCESS(dequantize_kernel, T, how);
+    kern<<<(total + UNITS * THREADS - 1) / (UNITS * THREADS), THREADS, 0, stream>>>(data, ldq, scale, lds, row_shift, static_cast<T*>(y), ldy, total, upr, r, cols);
   }
   return cudaGetLastError();
 }
 
-template <int TPR, int VPT>
-cudaError_t rmsnorm_as(const void* x, const void* residual, const void* w, void* h, float* rstd, uint8_t* data, long long ldq, uint8_t* scale, long long lds,
-                       long long rows, int dim, float eps, cudaStream_t stream) {
-  constexpr int threads = TPR < 128 ? 128 : TPR;
-  const long long blocks = (rows + threads / TPR - 1) / (threads / TPR);
-  auto* kern = residual ? rmsnorm_fp8_kernel<TPR, VPT, true> : rmsnorm_fp8_kernel<TPR, VPT, false>;
-  kern<<<unsigned(blocks), threads, 0, stream>>>(static_cast<const uint4*>(x), static_cast<const uint4*>(residual), static_cast<const uint4*>(w),
-                                                 static_cast<uint4*>(h), rstd, data, ldq, scale, lds, rows, dim / 8, 1.f / float(dim), eps);
+template <int VPT>
+cudaError_t rmsnorm_warps(const NormArgs& p, cudaStream_t stream) {
+  auto* kern = p.res ? rmsnorm_fp8_warp_kernel<VPT, true> : rmsnorm_fp8_warp_kernel<VPT, false>;
+  constexpr long long kRows = 1ll << 33;  // of one launch: its blocks fit the grid
+  for (long long r = 0; r < p.rows; r += kRows) {
+    NormArgs q = p;
+    q.rows = std::min(kRows, p.rows - r);
+    q.x += r * p.dim8, q.rstd += r, q.data += r * p.ldq, q.scale += r * p.lds;
+    if (p.res) q.res += r * p.dim8, q.h += r * p.dim8;
+    kern<<<unsigned((q.rows + 7) / 8), 256, 0, stream>>>(q);
+  }
+  return cudaGetLastError();
+}
+
+template <int VPT>
+cudaError_t rmsnorm_blocks(const NormArgs& p, int num_sms, cudaStream_t stream) {
+  auto* kern = p.res ? rmsnorm_fp8_block_kernel<VPT, true> : rmsnorm_fp8_block_kernel<VPT, false>;
+  kern<<<unsigned(std::min(p.rows, 4ll * num_sms)), NORM_THREADS, 0, stream>>>(p);
   return cudaGetLastError();
 }
 
@@ -356,18 +486,17 @@ cudaError_t fp8_dequantize(const uint8_t* data, long long ldq, const uint8_t* sc
 }
 
 cudaError_t fp8_rmsnorm(const void* x, const void* residual, const void* w, void* h, float* rstd, uint8_t* data, long long ldq, uint8_t* scale,
-                        long long lds, long long rows, int dim, float eps, cudaStream_t stream) {
+                        long long lds, long long rows, int dim, float eps, int num_sms, cudaStream_t stream) {
   if (rows <= 0) return cudaSuccess;
-  if (dim <= 0 || dim % 8 || dim > 8192 || rows > (1ll << 31) - 1) return cudaErrorInvalidValue;
-  // the fewest threads per row that still hold it in at most four 16-byte steps each
-#define ELFB_NORM(TPR, VPT) return rmsnorm_as<TPR, VPT>(x, residual, w, h, rstd, data, ldq, scale, lds, rows, dim, eps, stream)
-  if (dim <= 256) ELFB_NORM(32, 1);
-  if (dim <= 512) ELFB_NORM(32, 2);
-  if (dim <= 1024) ELFB_NORM(32, 4);
-  if (dim <= 2048) ELFB_NORM(128, 2);
-  if (dim <= 4096) ELFB_NORM(128, 4);
-  ELFB_NORM(256, 4);
-#undef ELFB_NORM
+  if (dim <= 0 || dim % 8 || dim > 8192) return cudaErrorInvalidValue;
+  const NormArgs p{static_cast<const uint4*>(x), static_cast<const uint4*>(residual), static_cast<const uint4*>(w), static_cast<uint4*>(h), rstd, data, scale,
+                   ldq, lds, rows, dim / 8, 1.f / float(dim), eps};
+  if (dim <= 256) return rmsnorm_warps<1>(p, stream);
+  if (dim <= 512) return rmsnorm_warps<2>(p, stream);
+  if (dim <= 1024) return rmsnorm_warps<4>(p, stream);
+  if (dim <= 2048) return rmsnorm_blocks<1>(p, num_sms, stream);
+  if (dim <= 4096) return rmsnorm_blocks<2>(p, num_sms, stream);
+  return rmsnorm_blocks<4>(p, num_sms, stream);
 }
 
 }  // namespace elfb

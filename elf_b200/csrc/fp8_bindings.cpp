@@ -322,6 +322,17 @@ std::pair<at::Tensor, at::Tensor> gated_bwd(const at::Tensor& dy, const at::Tens
   return dgu;
 }
 
+// The gated feed-forward block: x to 8 bits, act = silu(gate) * up, y = act . w_down^T, one call for its three kernels.
+// With `keep` also what its backward pass works from: (y, x, act, gate_up), each block-scaled tensor as values and scales.
+std::vector<c10::optional<at::Tensor>> ffn(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wg_scale, const at::Tensor& wd, const at::Tensor& wd_scale,
+                                           bool keep, const at::Tensor& status) {
+  const auto xq = quantize(x, false, c10::nullopt, c10::nullopt);
+  auto [act, act_scale, gu, gu_scale] = gated(xq.first, xq.second, wg, wg_scale, 7, keep, status);
+  at::Tensor y = gemm(act, act_scale, wd, wd_scale, 7, false, x.scalar_type(), c10::nullopt, status);
+  if (!keep) return {y};
+  return {y, xq.first, xq.second, act, act_scale, gu, gu_scale};
+}
+
 }  // namespace
 
 void register_fp8(pybind11::module_& m) {
@@ -331,5 +342,6 @@ void register_fp8(pybind11::module_& m) {
   m.def("fp8_gemm", &gemm, py::arg("a"), py::arg("a_scale"), py::arg("b"), py::arg("b_scale"), py::arg("b_row_shift"), py::arg("b_mn_major"), py::arg("dtype"),
         py::arg("bias"), py::arg("status"));
   m.def("fp8_gated", &gated, py::arg("a"), py::arg("a_scale"), py::arg("b"), py::arg("b_scale"), py::arg("b_row_shift"), py::arg("keep"), py::arg("status"));
+  m.def("fp8_ffn", &ffn, py::arg("x"), py::arg("wg"), py::arg("wg_scale"), py::arg("wd"), py::arg("wd_scale"), py::arg("keep"), py::arg("status"));
   m.def("fp8_gated_bwd", &gated_bwd, py::arg("dy"), py::arg("dy_scale"), py::arg("w"), py::arg("w_scale"), py::arg("gu"), py::arg("gu_scale"), py::arg("status"));
 }

@@ -437,7 +437,7 @@ def gated_backward(dy: BlockScaled, w_down: BlockScaled, gate_up: BlockScaled) -
 def _weight_copy(q: Optional[BlockScaled], w: torch.Tensor, name: str) -> BlockScaled:
     if q is None:
         return quantize_weight(w)
-    if not (q.shape == w.shape and q.block_rows == BLOCK and q.device == w.device):
+    if q.data.shape != w.shape or q.block_rows != BLOCK or q.data.device != w.device:
         raise ValueError(f"{name}: the 8-bit copy does not belong to a weight of shape {tuple(w.shape)} on {w.device}")
     return q
 
@@ -483,16 +483,26 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     return _Linear.apply(x, w, bias, w_q)
 
 
+def _ffn_forward(x: torch.Tensor, gate_up_q: BlockScaled, down_q: BlockScaled, keep: bool):
+    """``(y, [x, act, gate_up])``: the output and, with ``keep``, values and scales of what the backward needs."""
+    if x.numel() and _on_kernels(x):
+        y, *kept = _ext.get().fp8_ffn(x, gate_up_q.data, gate_up_q.scale, down_q.data, down_q.scale, keep, _gemm.status(x.device))
+        return y, kept
+    xq = quantize(x)
+    act, gu = gated_forward(xq, gate_up_q, keep)
+    y = linear_forward(act, down_q, None, x.dtype)
+    return y, [t for q in (xq, act, gu) for t in (q.data, q.scale)] if keep else []
+
+
 class _GatedFFN(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate_up, w_down, gate_up_q, down_q):
-        xq = quantize(x)
-        act, gu = gated_forward(xq, _weight_copy(gate_up_q, w_gate_up, "gated_ffn"))
+        y, kept = _ffn_forward(x, _weight_copy(gate_up_q, w_gate_up, "gated_ffn"), _weight_copy(down_q, w_down, "gated_ffn"), True)
         ctx.given = (gate_up_q is not None, down_q is not None)
         ctx.dtypes = (x.dtype, w_gate_up.dtype, w_down.dtype)
         held = [t for q, w in ((gate_up_q, w_gate_up), (down_q, w_down)) for t in ((q.data, q.scale) if q is not None else (w,))]
-        ctx.save_for_backward(xq.data, xq.scale, act.data, act.scale, gu.data, gu.scale, *held)
-        return linear_forward(act, _weight_copy(down_q, w_down, "gated_ffn"), None, x.dtype)
+        ctx.save_for_backward(*kept, *held)
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -533,8 +543,7 @@ def gated_ffn(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, ga
     if w_down.shape[1] % BLOCK:
         raise ValueError(f"gated_ffn: the inner width must be a multiple of {BLOCK}, got {w_down.shape[1]}")
     if not (torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_gate_up, w_down))):
-        act, _ = gated_forward(quantize(x), _weight_copy(gate_up_q, w_gate_up, "gated_ffn"), keep=False)
-        return linear_forward(act, _weight_copy(down_q, w_down, "gated_ffn"), None, x.dtype)
+        return _ffn_forward(x, _weight_copy(gate_up_q, w_gate_up, "gated_ffn"), _weight_copy(down_q, w_down, "gated_ffn"), False)[0]
     return _GatedFFN.apply(x, w_gate_up, w_down, gate_up_q, down_q)
 
 

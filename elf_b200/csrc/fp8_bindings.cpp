@@ -174,7 +174,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> rmsnorm(const at::Ten
   auto rstd = dense(lead_of(x), at::kFloat, dev);
   const Scaled s = scaled(q.first, q.second, 0, "data", dev, false);
   check(elfb::fp8_rmsnorm(x.data_ptr(), res.defined() ? res.data_ptr() : nullptr, w.data_ptr(), res.defined() ? h.data_ptr() : nullptr, rstd.data_ptr<float>(),
-                          s.data.bytes(), s.data.pitch, s.scale.bytes(), s.scale.pitch, rows, int(dim), float(eps), sm_count(dev), cur()),
+                          s.data.bytes(), s.data.pitch, s.scale.bytes(), s.scale.pitch, rows, int(dim), eps, sm_count(dev), cur()),
         "fp8_rmsnorm");
   return {q.first, q.second, rstd, h};
 }

@@ -26,7 +26,7 @@ namespace pair {
 constexpr int BN = 256;
 constexpr int STAGES = 6;
 constexpr int STAGE_BYTES = 2 * BOX_BYTES;  // per CTA: 128 rows of A, 128 rows of B
-constexpr int SLOTS = STAGES / 2;           // two consecutive stages are freed by one commit
+constexpr int SLOTS = STAGES / 2;           // two consecutive stages are filled, waited for and freed together
 constexpr int EPI_WARPS = 8;     // two per quarter of the TMEM lanes, each with one half of the columns
 constexpr int EPI_THREADS = EPI_WARPS * 32;
 constexpr int NUM_THREADS = 96 + EPI_THREADS;
@@ -107,6 +107,34 @@ __device__ __forceinline__ void umma_ss_mxf8_pair(uint32_t tmem_d, uint64_t desc
 // announces are shared memory of this CTA, made visible to the tensor core's copy by the proxy fence before it.
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// Four accumulating MMAs, a block of K apart by A_STEP and B_STEP in the descriptors' address units; returns whether the
+// barrier's phase had completed when the test, issued before them, came up.
+template <int A_STEP, int B_STEP>
+__device__ __forceinline__ bool umma_x4_then_ready(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t sfa, uint32_t bar, uint32_t parity) {
+  uint32_t ready;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, t;\n\t"
+      ".reg .b64 a, b;\n\t"
+      "setp.eq.b32 p, 0, 0;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 t, [%7], %8;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%1], %2, %3, %4, [%5], [%6], p;\n\t"
+      "add.s64 a, %2, %9;\n\t"
+      "add.s64 b, %3, %10;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%1], a, b, %4, [%5], [%6], p;\n\t"
+      "add.s64 a, a, %9;\n\t"
+      "add.s64 b, b, %10;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%1], a, b, %4, [%5], [%6], p;\n\t"
+      "add.s64 a, a, %9;\n\t"
+      "add.s64 b, b, %10;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%1], a, b, %4, [%5], [%6], p;\n\t"
+      "selp.u32 %0, 1, 0, t;\n\t"
+      "}\n"
+      : "=r"(ready)
+      : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(sfa), "r"(sfa + 4), "r"(bar), "r"(parity), "n"(A_STEP), "n"(B_STEP)
+      : "memory");
+  return ready != 0;
 }
 // arrive on the barrier at this offset in both CTAs once all MMAs issued so far have completed
 __device__ __forceinline__ void umma_commit_both(uint32_t bar) {
@@ -283,11 +311,11 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   uint32_t* exchange = reinterpret_cast<uint32_t*>(smem_aligned + size_t(STAGES) * STAGE_BYTES + SLOTS * SF_BYTES);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem_aligned + size_t(STAGES) * STAGE_BYTES + SLOTS * SF_BYTES + EXCHANGE_BYTES);
   const uint32_t bar0 = smem_u32(bars);
-  auto full_bar = [&](int s) { return bar0 + 8u * s; };
-  auto empty_bar = [&](int slot) { return bar0 + 8u * (STAGES + slot); };
-  auto acc_full_bar = [&](int a) { return bar0 + 8u * (2 * STAGES + a); };
-  const uint32_t acc_free_bar = bar0 + 8u * (2 * STAGES + 2);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 3);
+  auto full_bar = [&](int slot) { return bar0 + 8u * slot; };
+  auto empty_bar = [&](int slot) { return bar0 + 8u * (SLOTS + slot); };
+  auto acc_full_bar = [&](int a) { return bar0 + 8u * (2 * SLOTS + a); };
+  const uint32_t acc_free_bar = bar0 + 8u * (2 * SLOTS + 2);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * SLOTS + 3);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile unsigned int* arrived = tmem_slot + 2;
 
@@ -303,8 +331,10 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
-    for (int s = 0; s < STAGES; ++s) mbar_init(full_bar(s), s & 1 ? 1 : 3);  // a slot's first stage also waits for both scale warps
-    for (int s = 0; s < SLOTS; ++s) mbar_init(empty_bar(s), 1);
+    for (int s = 0; s < SLOTS; ++s) {
+      mbar_init(full_bar(s), 3);  // the leader's arrive.expect_tx and both scale warps
+      mbar_init(empty_bar(s), 1);
+    }
     mbar_init(acc_free_bar, 2 * EPI_WARPS);
     for (int a = 0; a < 2; ++a) mbar_init(acc_full_bar(a), 1);
     fence_barrier_init();
@@ -337,12 +367,12 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
             ok = false;
             break;
           }
-          for (int kb = kb2; kb < min(kb2 + 2, unit.kb1); ++kb) {
-            const int stage = 2 * slot + (kb - kb2);
-            const uint32_t sa = smem_base + stage * STAGE_BYTES, sb = sa + BOX_BYTES;
-            const uint32_t bar = map_to_cta(full_bar(stage), 0);
-            if (leader) mbar_arrive_expect_tx(full_bar(stage), 2 * STAGE_BYTES);
-            const int k0 = kb * BK;
+          const int blocks = min(2, unit.kb1 - kb2);
+          const uint32_t bar = map_to_cta(full_bar(slot), 0);
+          if (leader) mbar_arrive_expect_tx(full_bar(slot), blocks * 2 * STAGE_BYTES);
+          for (int b = 0; b < blocks; ++b) {
+            const uint32_t sa = smem_base + (2 * slot + b) * STAGE_BYTES, sb = sa + BOX_BYTES;
+            const int k0 = (kb2 + b) * BK;
             tma_load_2d_pair(sa, &tmap_a, bar, k0, m0);
             if (B_MN) tma_load_2d_pair(sb, &tmap_b, bar, n0, k0);
             else tma_load_2d_pair(sb, &tmap_b, bar, k0, n0);
@@ -358,45 +388,48 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer (leader only)
     if (leader && lane == 0) {
+      // A barrier test queues up behind the MMAs issued before it and its answer is late by then: one test per four MMAs
+      // made the loop 730 cycles per block of K where the MMAs alone take 523 (512 at best).  So there is one test per
+      // slot of eight, it is issued before the slot's last four and its answer read after them (`umma_x4_then_ready`);
+      // descriptors are one addition each.
       constexpr uint32_t B_KSTEP = B_MN ? UMMA_K * 128 : UMMA_K;  // see fp8_gemm_sm100.cu; one 128-wide box per CTA
+      constexpr uint32_t IDESC = make_idesc_mxf8(2 * BM, BN, 0u, B_MN ? 1u : 0u, 0), IDESC_STEP = (1u << 4) | (1u << 29);
+      const uint64_t desc_a0 = make_smem_desc_sw128(smem_base, 0, 1024), desc_b0 = make_smem_desc_sw128(smem_base + BOX_BYTES, 0, 1024);
+      const uint64_t desc_sf0 = make_smem_desc_rows16(sf_base);
       int slot = 0;
-      uint32_t sf_count = 0;
+      uint32_t phase = 0, sf_count = 0;
       bool ok = true;
       int i = 0;  // units of this pair so far
-      uint32_t stage_phase = 0;  // bit s: parity of stage s (a unit with an odd number of blocks leaves half a slot unused)
       for (int u = pair_id; u < sched.total_units && ok; u += num_pairs, ++i) {
         const Unit unit = unit_at(u, sched, k_blocks, width);
         const int acc = i & 1;
         if (i > 0 && !mbar_wait(acc_free_bar, uint32_t(i - 1) & 1u, abort_flag)) break;
         tc_fence_after_sync();
         const uint32_t tmem_d = tmem_base + acc * ACC1;
-        for (int kb2 = unit.kb0; kb2 < unit.kb1 && ok; kb2 += 2) {
-          const uint32_t sfa = tmem_base + SF_COL + (sf_count++ & 1) * 16, sfb = sfa + 4;
-          for (int kb = kb2; kb < min(kb2 + 2, unit.kb1); ++kb) {
-            const int stage = 2 * slot + (kb - kb2);
-            if (!mbar_wait(full_bar(stage), (stage_phase >> stage) & 1u, abort_flag)) {
-              ok = false;
-              break;
-            }
-            stage_phase ^= 1u << stage;
-            tc_fence_after_sync();
-            const uint32_t sa = smem_base + stage * STAGE_BYTES, sb = sa + BOX_BYTES;
-            if (kb == kb2) {
-              const uint32_t sf = sf_base + slot * SF_BYTES;
-#pragma unroll
-              for (int j = 0; j < 3; ++j) tmem_cp_32x128b_pair(sfa + 4 * j, make_smem_desc_rows16(sf + 512 * j));
-            }
-            const uint32_t idesc = make_idesc_mxf8(2 * BM, BN, 0u, B_MN ? 1u : 0u, kb & 3);
-#pragma unroll
-            for (int k = 0; k < BK / UMMA_K; ++k) {
-              const uint64_t da = make_smem_desc_sw128(sa + k * UMMA_K, 0, 1024);
-              const uint64_t db = make_smem_desc_sw128(sb + k * B_KSTEP, 0, 1024);
-              umma_ss_mxf8_pair(tmem_d, da, db, idesc, sfa, sfb, (kb > unit.kb0 || k) ? 1u : 0u);
-            }
+        bool ready = false;
+        for (int kb = unit.kb0; kb < unit.kb1; kb += 2) {
+          if (!ready && !mbar_wait(full_bar(slot), phase, abort_flag)) {
+            ok = false;
+            break;
           }
-          if (!ok) break;
+          const int next = slot + 1 == SLOTS ? 0 : slot + 1;
+          const uint32_t next_phase = phase ^ (next == 0 ? 1u : 0u);
+          const uint32_t sfa = tmem_base + SF_COL + (sf_count++ & 1) * 16;
+          const uint64_t sf = desc_sf0 + uint32_t(slot * (SF_BYTES >> 4));
+#pragma unroll
+          for (int j = 0; j < 3; ++j) tmem_cp_32x128b_pair(sfa + 4 * j, sf + 32 * j);
+          const uint64_t da = desc_a0 + uint32_t(slot * (2 * STAGE_BYTES >> 4)), db = desc_b0 + uint32_t(slot * (2 * STAGE_BYTES >> 4));
+          const uint32_t idesc = IDESC + (kb & 3) * IDESC_STEP;
+#pragma unroll
+          for (int k = 0; k < BK / UMMA_K; ++k)
+            umma_ss_mxf8_pair(tmem_d, da + ((k * UMMA_K) >> 4), db + ((k * B_KSTEP) >> 4), idesc, sfa, sfa + 4, (kb > unit.kb0 || k) ? 1u : 0u);
+          ready = false;
+          if (kb + 1 < unit.kb1)
+            ready = umma_x4_then_ready<(UMMA_K >> 4), (B_KSTEP >> 4)>(tmem_d, da + (STAGE_BYTES >> 4), db + (STAGE_BYTES >> 4), idesc + IDESC_STEP, sfa,
+                                                                      full_bar(next), next_phase) && kb + 2 < unit.kb1;
           umma_commit_both(empty_bar(slot));
-          if (++slot == SLOTS) slot = 0;
+          slot = next;
+          phase = next_phase;
         }
         if (!ok) break;
         umma_commit_both(acc_full_bar(acc));
@@ -545,7 +578,7 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         store_scale_words(sf_base + slot * SF_BYTES + 1024, lane, b1);
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(full_bar(2 * slot), 0));
+        if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(full_bar(slot), 0));
         if (++slot == SLOTS) {
           slot = 0;
           phase ^= 1u;

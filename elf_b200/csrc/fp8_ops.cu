@@ -273,15 +273,61 @@ struct NormArgs {
   uint8_t *data, *scale;
   long long ldq, lds, rows;
   int dim8;
-  float inv_dim, eps;
+  double inv_dim, eps;
 };
 
-// 8 normalised values of column group c to 8 bits; all 32 lanes of the warp call this
-__device__ __forceinline__ void store_normalised(const NormArgs& p, long long row, int c, bool live, const float (&v)[8], uint4 gain, float rs) {
+// A value next to the middle between two e4m3 values goes to the wrong one when its fp32 error is larger than its
+// distance, and is off by a whole step then.  So the sum of squares is compensated, the statistic (ss / dim + eps)^-1/2
+// carried as two floats (one Newton step in 64 bits from the fp32 root), and the product rounded to odd: the last bit
+// says that something was cut off, and the rounding to e4m3 is that of the exact product.
+template <int N>
+__device__ __forceinline__ double square_sum(const float (&v)[N][8]) {
+  float sum = 0.f, lost = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float y = fmaf(v[i][j], v[i][j], -lost), t = sum + y;  // the square is exact: v has 8 significant bits
+      lost = (t - sum) - y;
+      sum = t;
+    }
+  if (isfinite(sum)) return double(sum) - double(lost);
+  sum = 0.f;  // the compensation turns an infinity into NaN
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum = fmaf(v[i][j], v[i][j], sum);
+  return double(sum);
+}
+struct InverseRms {
+  float hi, lo;
+};
+__device__ __forceinline__ InverseRms inverse_rms(double ss, const NormArgs& p) {
+  const double m = fma(ss, p.inv_dim, p.eps);
+  const double r0 = double(rsqrtf(float(m)));
+  const double r = fma(0.5 * r0, fma(-m * r0, r0, 1.0), r0);
+  // rows whose statistic fp32 cannot hold take the fp32 root: 0 for infinity, NaN for NaN
+  const float hi = isfinite(r) ? float(r) : float(r0);
+  return {hi, isfinite(r) ? float(r - double(hi)) : 0.f};
+}
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// 8 normalised values of column group c (zeros past the row) to 8 bits; all 32 lanes of the warp call this
+__device__ __forceinline__ void store_normalised(const NormArgs& p, long long row, int c, bool live, const float (&v)[8], uint4 gain, InverseRms rs) {
   float g[8], y[8];
   unpack8(gain, g);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) y[j] = c < p.dim8 ? v[j] * rs * g[j] : 0.f;
+  for (int j = 0; j < 8; ++j) {
+    const float t = v[j] * g[j];  // exact: both have 8 significant bits
+    const float tail = t * rs.lo;
+    float q = __fmaf_rz(t, rs.hi, tail);
+    if (fmaf(t, rs.hi, -q) + tail != 0.f) q = __uint_as_float(__float_as_uint(q) | 1u);
+    y[j] = q;
+  }
   uint32_t q[2];
   const uint32_t byte = quantize_block<8, 16>(y, q);
   if (live && c < p.dim8) {
@@ -297,7 +343,6 @@ __global__ void __launch_bounds__(256) rmsnorm_fp8_warp_kernel(const __grid_cons
   const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (row >= p.rows) return;
   float v[VPT][8];
-  float ss = 0.f;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int c = lane + i * 32;
@@ -309,13 +354,9 @@ __global__ void __launch_bounds__(256) rmsnorm_fp8_warp_kernel(const __grid_cons
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  const float rs = rsqrtf(ss * p.inv_dim + p.eps);
-  if (lane == 0) p.rstd[row] = rs;
+  const InverseRms rs = inverse_rms(warp_sum(square_sum(v)), p);
+  if (lane == 0) p.rstd[row] = rs.hi;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int c = lane + i * 32;
@@ -330,7 +371,7 @@ __global__ void __launch_bounds__(256) rmsnorm_fp8_warp_kernel(const __grid_cons
 // 27 us (the time goes into the two dependent sweeps of a row, not into too few bytes in flight).
 template <int VPT, bool RESIDUAL>
 __global__ void __launch_bounds__(NORM_THREADS, VPT == 4 ? 2 : 1) rmsnorm_fp8_block_kernel(const __grid_constant__ NormArgs p) {
-  __shared__ float red[2][NORM_THREADS / 32];
+  __shared__ double red[2][NORM_THREADS / 32];
   const int t = threadIdx.x;
   uint4 nx[VPT], nr[VPT], gain[VPT];
   auto fetch = [&](long long row) {
@@ -349,8 +390,7 @@ __global__ void __launch_bounds__(NORM_THREADS, VPT == 4 ? 2 : 1) rmsnorm_fp8_bl
   int turn = 0;
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
     float v[VPT][8];
-    float ss = 0.f;
-#pragma unroll
+  #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = t + i * NORM_THREADS;
       if (c < p.dim8) {
@@ -360,19 +400,16 @@ __global__ void __launch_bounds__(NORM_THREADS, VPT == 4 ? 2 : 1) rmsnorm_fp8_bl
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
       }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
     }
     fetch(row + gridDim.x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if ((t & 31) == 0) red[turn][t >> 5] = ss;  // the other half may still be read by warps of the last round
+    double sum = warp_sum(square_sum(v));
+    if ((t & 31) == 0) red[turn][t >> 5] = sum;  // the other half may still be read by warps of the last round
     __syncthreads();
-    ss = 0.f;
+    sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < NORM_THREADS / 32; ++i) ss += red[turn][i];
-    const float rs = rsqrtf(ss * p.inv_dim + p.eps);
-    if (t == 0) p.rstd[row] = rs;
+    for (int i = 0; i < NORM_THREADS / 32; ++i) sum += red[turn][i];
+    const InverseRms rs = inverse_rms(sum, p);
+    if (t == 0) p.rstd[row] = rs.hi;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = t + i * NORM_THREADS;
@@ -486,11 +523,11 @@ cudaError_t fp8_dequantize(const uint8_t* data, long long ldq, const uint8_t* sc
 }
 
 cudaError_t fp8_rmsnorm(const void* x, const void* residual, const void* w, void* h, float* rstd, uint8_t* data, long long ldq, uint8_t* scale,
-                        long long lds, long long rows, int dim, float eps, int num_sms, cudaStream_t stream) {
+                        long long lds, long long rows, int dim, double eps, int num_sms, cudaStream_t stream) {
   if (rows <= 0) return cudaSuccess;
   if (dim <= 0 || dim % 8 || dim > 8192) return cudaErrorInvalidValue;
   const NormArgs p{static_cast<const uint4*>(x), static_cast<const uint4*>(residual), static_cast<const uint4*>(w), static_cast<uint4*>(h), rstd, data, scale,
-                   ldq, lds, rows, dim / 8, 1.f / float(dim), eps};
+                   ldq, lds, rows, dim / 8, 1.0 / double(dim), eps};
   if (dim <= 256) return rmsnorm_warps<1>(p, stream);
   if (dim <= 512) return rmsnorm_warps<2>(p, stream);
   if (dim <= 1024) return rmsnorm_warps<4>(p, stream);

@@ -22,7 +22,7 @@ cudaError_t fp8_dequantize(const uint8_t* data, long long ldq, const uint8_t* sc
                            long long rows, int cols, cudaStream_t stream);
 // h = x + residual (bf16, written when residual is given); data/scale = blocks of h * rstd * w
 cudaError_t fp8_rmsnorm(const void* x, const void* residual, const void* w, void* h, float* rstd, uint8_t* data, long long ldq, uint8_t* scale,
-                        long long lds, long long rows, int dim, float eps, int num_sms, cudaStream_t stream);
+                        long long lds, long long rows, int dim, double eps, int num_sms, cudaStream_t stream);
 // One operand of a block-scaled product.  Its scale for (row of the product, block of the
 // reduction) is scale[(row >> row_shift) * row_stride + block * block_stride].
 struct Fp8Operand {

@@ -11,6 +11,7 @@
 #include <c10/cuda/CUDAGuard.h>
 
 #include "fp8_ops.h"
+#include "gemm_sm100.h"
 
 namespace {
 
@@ -333,6 +334,80 @@ std::vector<c10::optional<at::Tensor>> ffn(const at::Tensor& x, const at::Tensor
   return {y, xq.first, xq.second, act, act_scale, gu, gu_scale};
 }
 
+// bf16 matrix for the 16-bit product, its rows on 16-byte boundaries: the values of a block-scaled tensor, or a plain tensor
+Mat restored(const at::Tensor& t, const c10::optional<at::Tensor>& scale, const char* name, const at::Device& dev) {
+  Mat m = matrix(scale.has_value() ? t : t.to(at::kBFloat16), name, dev);
+  if (!scale.has_value() && m.aligned(16)) return m;
+  const int64_t lead[1] = {m.rows};
+  at::Tensor out = new_rows(at::IntArrayRef(lead, 1), m.cols, round_up(m.cols, 8), at::kBFloat16, dev);
+  if (scale.has_value()) {
+    const Scaled s = scaled(t, *scale, 0, name, dev);
+    check(elfb::fp8_dequantize(s.data.bytes(), s.data.pitch, s.scale.bytes(), s.scale.pitch, 0, out.data_ptr(), elfb::Elem::kBf16, round_up(m.cols, 8), m.rows,
+                               int(m.cols), cur()),
+          "fp8_dequantize");
+  } else {
+    out.copy_(m.t.dim() == 2 ? m.t : m.t.reshape({m.rows, m.cols}));
+  }
+  Mat r{out, m.rows, m.cols, round_up(m.cols, 8)};
+  return r;
+}
+
+// dy^T x over all leading dimensions, on the 16-bit tensor path; added to `out` when it is given.  Either operand block-scaled
+// (with its scales) or plain.
+at::Tensor weight_grad(const at::Tensor& dy, const c10::optional<at::Tensor>& dy_scale, const at::Tensor& x, const c10::optional<at::Tensor>& x_scale,
+                       const c10::optional<at::Tensor>& out, at::ScalarType dtype, const at::Tensor& status, int64_t variant, bool split_tail) {
+  const auto dev = x.device();
+  c10::cuda::CUDAGuard guard(dev);
+  const Mat a = restored(dy, dy_scale, "dy", dev), b = restored(x, x_scale, "x", dev);
+  TORCH_CHECK(a.rows == b.rows && a.rows <= INT_MAX, "dy and x must have the same number of rows");
+  // fp16 results, and widths whose rows are not on 16-byte boundaries, go through a buffer
+  const bool direct = out.has_value() && b.cols % 8 == 0 && out->is_contiguous() && reinterpret_cast<uintptr_t>(out->data_ptr()) % 16 == 0;
+  const int64_t lead[1] = {a.cols};
+  const at::ScalarType held = !out.has_value() && dtype == at::kBFloat16 ? at::kBFloat16 : at::kFloat;
+  at::Tensor dw = direct ? *out : new_rows(at::IntArrayRef(lead, 1), b.cols, round_up(b.cols, 8), held, dev);
+  elfb::GemmArgs g;
+  g.fmt = 1;
+  g.M = int(a.cols);
+  g.N = int(b.cols);
+  g.K = int(a.rows);
+  g.a = a.t.data_ptr();
+  g.b = b.t.data_ptr();
+  g.d = dw.data_ptr();
+  g.lda = a.pitch;
+  g.ldb = b.pitch;
+  g.ldd = direct ? b.cols : round_up(b.cols, 8);
+  g.a_mn_major = g.b_mn_major = true;
+  g.out_f32 = dw.scalar_type() == at::kFloat;
+  g.accumulate = direct;
+  g.variant = int(variant);
+  g.split_tail = split_tail;
+  g.status = status_ptr(status, dev);
+  const char* err = elfb::gemm_tcgen05(g, sm_count(dev), cur());
+  TORCH_CHECK(err == nullptr, "elf_b200 fp8_weight_grad: ", err);
+  if (direct) return dw;
+  if (out.has_value()) {
+    at::Tensor sum = *out;
+    return sum.add_(dw);
+  }
+  return dw.scalar_type() == dtype ? dw.contiguous() : dw.to(dtype).contiguous();
+}
+
+// Backward of `ffn` from what it kept: (dx, dw_gate_up, dw_down), each only on request.
+std::vector<c10::optional<at::Tensor>> ffn_bwd(const at::Tensor& dy, const std::vector<at::Tensor>& kept, const at::Tensor& wg, const at::Tensor& wg_scale,
+                                               const at::Tensor& wd, const at::Tensor& wd_scale, const std::vector<bool>& need,
+                                               const std::vector<at::ScalarType>& dtypes, const at::Tensor& status, int64_t variant, bool split_tail) {
+  TORCH_CHECK(kept.size() == 6 && need.size() == 3 && dtypes.size() == 3, "fp8_ffn_bwd: bad arguments");
+  std::vector<c10::optional<at::Tensor>> grads(3);
+  if (need[2]) grads[2] = weight_grad(dy, c10::nullopt, kept[2], kept[3], c10::nullopt, dtypes[2], status, variant, split_tail);
+  if (need[0] || need[1]) {
+    const auto dyq = quantize(dy, false, c10::nullopt, c10::nullopt);
+    const auto dgu = gated_bwd(dyq.first, dyq.second, wd, wd_scale, kept[4], kept[5], status);
+    if (need[0]) grads[0] = gemm(dgu.first, dgu.second, wg, wg_scale, 7, true, dtypes[0], c10::nullopt, status);
+    if (need[1]) grads[1] = weight_grad(dgu.first, dgu.second, kept[0], kept[1], c10::nullopt, dtypes[1], status, variant, split_tail);
+  }
+  return grads;
+}
+
 }  // namespace
 
 void register_fp8(pybind11::module_& m) {
@@ -343,5 +418,9 @@ void register_fp8(pybind11::module_& m) {
         py::arg("bias"), py::arg("status"));
   m.def("fp8_gated", &gated, py::arg("a"), py::arg("a_scale"), py::arg("b"), py::arg("b_scale"), py::arg("b_row_shift"), py::arg("keep"), py::arg("status"));
   m.def("fp8_ffn", &ffn, py::arg("x"), py::arg("wg"), py::arg("wg_scale"), py::arg("wd"), py::arg("wd_scale"), py::arg("keep"), py::arg("status"));
+  m.def("fp8_weight_grad", &weight_grad, py::arg("dy"), py::arg("dy_scale"), py::arg("x"), py::arg("x_scale"), py::arg("out"), py::arg("dtype"), py::arg("status"),
+        py::arg("variant"), py::arg("split_tail"));
+  m.def("fp8_ffn_bwd", &ffn_bwd, py::arg("dy"), py::arg("kept"), py::arg("wg"), py::arg("wg_scale"), py::arg("wd"), py::arg("wd_scale"), py::arg("need"),
+        py::arg("dtypes"), py::arg("status"), py::arg("variant"), py::arg("split_tail"));
   m.def("fp8_gated_bwd", &gated_bwd, py::arg("dy"), py::arg("dy_scale"), py::arg("w"), py::arg("w_scale"), py::arg("gu"), py::arg("gu_scale"), py::arg("status"));
 }

@@ -338,18 +338,8 @@ def linear_input_grad(dy: BlockScaled, w: BlockScaled, out_dtype: torch.dtype = 
 
 
 def _restored(t: Union[BlockScaled, torch.Tensor]) -> torch.Tensor:
-    """bf16 matrix for the 16-bit weight-gradient product, its rows on 16-byte boundaries.  Exact for a
-    block-scaled tensor."""
-    cols = t.shape[-1]
-    rows = t.numel() // cols
-    if not isinstance(t, BlockScaled):
-        t = _matrix(t.detach().to(torch.bfloat16))
-        if t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 and t.stride(0) >= cols:
-            return t
-    out = torch.empty((rows, _round_up(cols, 8)), dtype=torch.bfloat16, device=t.device)[:, :cols]
-    if not isinstance(t, BlockScaled):
-        return out.copy_(t)
-    return _ext.get().fp8_dequantize(t.data if t.data.dim() == 2 else t.data.reshape(rows, cols), t.scale, _shift(t), torch.bfloat16, out)
+    """bf16 matrix for the 16-bit weight-gradient product.  Exact for a block-scaled tensor."""
+    return _matrix(t.dequantize() if isinstance(t, BlockScaled) else t.detach().to(torch.bfloat16))
 
 
 def linear_weight_grad(dy: Union[BlockScaled, torch.Tensor], x: Union[BlockScaled, torch.Tensor], out: Optional[torch.Tensor] = None,
@@ -370,21 +360,12 @@ def linear_weight_grad(dy: Union[BlockScaled, torch.Tensor], x: Union[BlockScale
         plain = lambda t: _values(t) if isinstance(t, BlockScaled) else _matrix(t.detach()).float()  # noqa: E731
         dw = plain(dy).T @ plain(x)
         return dw.to(out_dtype) if out is None else out.add_(dw)
-    # fp16 results, and widths whose rows are not on 16-byte boundaries, go through a buffer
-    direct = out is not None and k % 8 == 0 and out.is_contiguous() and out.data_ptr() % 16 == 0
-    dtype = torch.bfloat16 if out is None and out_dtype == torch.bfloat16 else torch.float32
-    dw = out if direct else torch.empty((n, _round_up(k, 8)), dtype=dtype, device=x.device)[:, :k]
-    args = [_restored(dy), _restored(x), dw, None, True, True, direct, 1.0, _gemm.status(x.device), _gemm._VARIANT, _gemm._SPLIT_TAIL]
-    if push:
-        if not direct:
-            raise ValueError("linear_weight_grad: a push needs a gradient buffer the product can add to in place")
-        args += [push["push_out"], push["push_flags"], push["push_flag_value"], push["push_counter"]]
-    _ext.get().gemm(*args)
-    if direct:
-        return out
-    if out is not None:
-        return out.add_(dw)
-    return dw.to(out_dtype) if dtype != out_dtype else dw.contiguous()
+    if not push:
+        pair = lambda t: (t.data, t.scale) if isinstance(t, BlockScaled) else (t.detach(), None)  # noqa: E731
+        return _ext.get().fp8_weight_grad(*pair(dy), *pair(x), out, out_dtype, _gemm.status(data.device), _gemm._VARIANT, _gemm._SPLIT_TAIL)
+    if out is None or k % 8 or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError("linear_weight_grad: a push needs a gradient buffer the product can add to in place")
+    return _gemm.linear_weight_grad(_restored(dy), _restored(x), out=out, push=push)
 
 
 # ------------------------------------------------------------------------------ gated feed-forward block
@@ -507,24 +488,29 @@ class _GatedFFN(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        *kept, = ctx.saved_tensors
-        xq, act, gu = (BlockScaled._made(kept[2 * i], kept[2 * i + 1]) for i in range(3))
-        rest = kept[6:]
+        tensors = ctx.saved_tensors
+        kept, rest = tensors[:6], tensors[6:]
         copies = []
         for given in ctx.given:
             n = 2 if given else 1
             copies.append(BlockScaled._made(*rest[:n], BLOCK) if given else quantize_weight(rest[0]))
             rest = rest[n:]
         gate_up_q, down_q = copies
+        need = list(ctx.needs_input_grad[:3])
+        if dy.numel() and down_q.numel() and _on_kernels(dy):
+            grads = _ext.get().fp8_ffn_bwd(dy, list(kept), gate_up_q.data, gate_up_q.scale, down_q.data, down_q.scale, need, list(ctx.dtypes),
+                                           _gemm.status(dy.device), _gemm._VARIANT, _gemm._SPLIT_TAIL)
+            return (*grads, None, None)
+        xq, act, gu = (BlockScaled._made(kept[2 * i], kept[2 * i + 1]) for i in range(3))
         x_dtype, gate_up_dtype, down_dtype = ctx.dtypes
         dx = dw_gate_up = dw_down = None
-        if ctx.needs_input_grad[2]:
+        if need[2]:
             dw_down = linear_weight_grad(dy, act, out_dtype=down_dtype)
-        if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
+        if need[0] or need[1]:
             dgu = gated_backward(quantize(dy), down_q, gu)
-            if ctx.needs_input_grad[0]:
+            if need[0]:
                 dx = linear_input_grad(dgu, gate_up_q, x_dtype)
-            if ctx.needs_input_grad[1]:
+            if need[1]:
                 dw_gate_up = linear_weight_grad(dgu, xq, out_dtype=gate_up_dtype)
         return dx, dw_gate_up, dw_down, None, None
 

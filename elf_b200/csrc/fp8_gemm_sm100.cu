@@ -13,7 +13,7 @@
 // This file: the kernel for up to 128 rows, and the choice between it and the CTA-pair kernel
 // (fp8_gemm_sm100_2cta.cu).  With few rows the time is that of reading B, so the work is spread over all
 // SMs: one 128 x 128 tile per cluster of up to 8 CTAs that split K among them and add their fp32 sums,
-// in rank order, through distributed shared memory.  16 x 4096 x 14336 (59 MB of weights): see below.
+// in rank order, through distributed shared memory.
 //
 // Roles per CTA (224 threads):
 //   warp 0      TMA producer: ring of (A 128 x 128, B 128 x 128) byte tiles, 128B-swizzled.
@@ -30,15 +30,28 @@ namespace fp8 {
 namespace rows128 {
 
 constexpr int BN = 128;
-constexpr int STAGES = 6;
-constexpr int SLOTS = STAGES / 2;           // two consecutive stages share scale words and are freed together
-constexpr int STAGE_BYTES = 2 * BOX_BYTES;
+// A's box holds ROWS (32 or 128) rows.  The MMA always reads 128; behind a box of 32 lies B's, whose bytes end in
+// accumulator rows that nobody looks at.  Up to 32 rows leave room for two CTAs per SM, one of which starts or ends
+// while the other streams.  16 x 4096 x 14336: 15.9 us, of which 5.5 stream the weights, 3.5 wait for the launch and the
+// first bytes and 3.3 add the parts; one CTA per SM 16.0, without the split 45.5.
+template <int ROWS>
+constexpr int CTAS_PER_SM = ROWS == 32 ? 2 : 1;
+template <int ROWS>
+constexpr int STAGES = ROWS == 32 ? 4 : 6;
+template <int ROWS>
+constexpr int SLOTS = STAGES<ROWS> / 2;     // two consecutive stages share scale words and are freed together
+template <int ROWS>
+constexpr int A_BYTES = ROWS * BK;
+template <int ROWS>
+constexpr int STAGE_BYTES = A_BYTES<ROWS> + BOX_BYTES;
 constexpr int SF_BYTES = 2 * 512;           // scale words of a slot: 128 rows of A, 128 columns of B
 constexpr int NUM_THREADS = 224;
 constexpr int TMEM_COLUMNS = 256;           // 128 of the accumulator, then two 8-column scale slots
 constexpr int MAX_CLUSTER = 8;
-constexpr size_t SMEM_BYTES = size_t(STAGES) * STAGE_BYTES + SLOTS * SF_BYTES + 1024 /*align slack*/ + 256 /*barriers*/;
-static_assert(STAGES * STAGE_BYTES >= BM * BN * 4, "the sums are exchanged in the ring's memory");
+template <int ROWS>
+constexpr size_t SMEM_BYTES = size_t(STAGES<ROWS>) * STAGE_BYTES<ROWS> + SLOTS<ROWS> * SF_BYTES + 1024 /*align slack*/ + 256 /*barriers*/;
+static_assert(STAGES<32> * STAGE_BYTES<32> >= 32 * BN * 4 && STAGES<128> * STAGE_BYTES<128> >= BM * BN * 4, "the sums are exchanged in the ring's memory");
+static_assert(STAGE_BYTES<32> >= BM * BK, "an MMA reads 128 rows from where A begins: they end inside the stage");
 
 __device__ __forceinline__ float4 load_cluster_f4(uint32_t cluster_addr) {
   float4 v;
@@ -46,19 +59,19 @@ __device__ __forceinline__ float4 load_cluster_f4(uint32_t cluster_addr) {
   return v;
 }
 
-template <bool B_MN, typename T>
-__global__ void __launch_bounds__(NUM_THREADS, 1)
+template <int ROWS, bool B_MN, typename T>
+__global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM<ROWS>)
 fp8_gemm_rows128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ Params p, int ksplit) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_aligned = smem_raw + (smem_base - smem_u32(smem_raw));
-  const uint32_t sf_base = smem_base + STAGES * STAGE_BYTES;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_aligned + size_t(STAGES) * STAGE_BYTES + SLOTS * SF_BYTES);
+  const uint32_t sf_base = smem_base + STAGES<ROWS> * STAGE_BYTES<ROWS>;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_aligned + size_t(STAGES<ROWS>) * STAGE_BYTES<ROWS> + SLOTS<ROWS> * SF_BYTES);
   const uint32_t bar0 = smem_u32(bars);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
-  auto empty_bar = [&](int slot) { return bar0 + 8u * (STAGES + slot); };
-  const uint32_t done_bar = bar0 + 8u * (STAGES + SLOTS);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + STAGES + SLOTS + 1);
+  auto empty_bar = [&](int slot) { return bar0 + 8u * (STAGES<ROWS> + slot); };
+  const uint32_t done_bar = bar0 + 8u * (STAGES<ROWS> + SLOTS<ROWS>);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + STAGES<ROWS> + SLOTS<ROWS> + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
@@ -70,8 +83,8 @@ fp8_gemm_rows128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
-    for (int s = 0; s < STAGES; ++s) mbar_init(full_bar(s), s & 1 ? 1 : 2);  // a slot's first stage also waits for the scale warp
-    for (int s = 0; s < SLOTS; ++s) mbar_init(empty_bar(s), 1);
+    for (int s = 0; s < STAGES<ROWS>; ++s) mbar_init(full_bar(s), s & 1 ? 1 : 2);  // a slot's first stage also waits for the scale warp
+    for (int s = 0; s < SLOTS<ROWS>; ++s) mbar_init(empty_bar(s), 1);
     mbar_init(done_bar, 1);
     fence_barrier_init();
     prefetch_tensormap(&tmap_a);
@@ -99,13 +112,13 @@ fp8_gemm_rows128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
         }
         for (int kb = kb2; kb < min(kb2 + 2, kb1); ++kb) {
           const int stage = 2 * slot + (kb - kb2);
-          const uint32_t sa = smem_base + stage * STAGE_BYTES, sb = sa + BOX_BYTES, bar = full_bar(stage);
-          mbar_arrive_expect_tx(bar, STAGE_BYTES);
+          const uint32_t sa = smem_base + stage * STAGE_BYTES<ROWS>, sb = sa + A_BYTES<ROWS>, bar = full_bar(stage);
+          mbar_arrive_expect_tx(bar, STAGE_BYTES<ROWS>);
           tma_load_2d(sa, &tmap_a, bar, kb * BK, 0);
           if (B_MN) tma_load_2d(sb, &tmap_b, bar, n0, kb * BK);
           else tma_load_2d(sb, &tmap_b, bar, kb * BK, n0);
         }
-        if (++slot == SLOTS) {
+        if (++slot == SLOTS<ROWS>) {
           slot = 0;
           phase ^= 1u;
         }
@@ -131,7 +144,7 @@ fp8_gemm_rows128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
           }
           stage_phase ^= 1u << stage;
           tc_fence_after_sync();
-          const uint32_t sa = smem_base + stage * STAGE_BYTES, sb = sa + BOX_BYTES;
+          const uint32_t sa = smem_base + stage * STAGE_BYTES<ROWS>, sb = sa + A_BYTES<ROWS>;
           if (kb == kb2) {
             const uint32_t sf = sf_base + slot * SF_BYTES;
             tmem_cp_32x128b(sfa, make_smem_desc_rows16(sf));
@@ -147,7 +160,7 @@ fp8_gemm_rows128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
         }
         if (!ok) break;
         umma_commit(empty_bar(slot));
-        if (++slot == SLOTS) slot = 0;
+        if (++slot == SLOTS<ROWS>) slot = 0;
       }
       if (ok) umma_commit(done_bar);
     }
@@ -209,7 +222,7 @@ fp8_gemm_rows128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(full_bar(2 * slot));
-        if (++slot == SLOTS) {
+        if (++slot == SLOTS<ROWS>) {
           slot = 0;
           phase ^= 1u;
         }
@@ -263,25 +276,25 @@ fp8_gemm_rows128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
   }
 }
 
-template <bool B_MN, typename T>
+template <int ROWS, bool B_MN, typename T>
 cudaError_t launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int num_sms, cudaStream_t stream) {
-  auto kern = fp8_gemm_rows128_kernel<B_MN, T>;
+  auto kern = fp8_gemm_rows128_kernel<ROWS, B_MN, T>;
   // function attributes are per device: remember which devices of this process have been set up
   static bool configured[kMaxDevices] = {};
   int dev = 0;
   if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
   if (dev < 0 || dev >= kMaxDevices || !configured[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(SMEM_BYTES));
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(SMEM_BYTES<ROWS>));
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < kMaxDevices) configured[dev] = true;
   }
   const int tiles = (p.N + BN - 1) / BN, groups = (p.K + 4 * BK - 1) / (4 * BK);
   int ksplit = 1;  // as many parts as there are SMs for, each at least four blocks of K long
-  while (ksplit < MAX_CLUSTER && 2 * ksplit * tiles <= num_sms && 2 * ksplit <= groups) ksplit *= 2;
+  while (ksplit < MAX_CLUSTER && 2 * ksplit * tiles <= num_sms * CTAS_PER_SM<ROWS> && 2 * ksplit <= groups) ksplit *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(tiles) * ksplit);
   cfg.blockDim = dim3(NUM_THREADS);
-  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.dynamicSmemBytes = SMEM_BYTES<ROWS>;
   cfg.stream = stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -298,14 +311,16 @@ cudaError_t launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p
 
 cudaError_t launch_rows128(const Fp8GemmArgs& g, const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int num_sms, cudaStream_t s) {
   using namespace rows128;
+#define ELFB_LAUNCH(MN, T) return g.M <= 32 ? launch<32, MN, T>(ta, tb, p, num_sms, s) : launch<128, MN, T>(ta, tb, p, num_sms, s)
   if (g.b.mn_major) {
-    if (g.out == Elem::kBf16) return launch<true, __nv_bfloat16>(ta, tb, p, num_sms, s);
-    if (g.out == Elem::kF16) return launch<true, __half>(ta, tb, p, num_sms, s);
-    return launch<true, float>(ta, tb, p, num_sms, s);
+    if (g.out == Elem::kBf16) ELFB_LAUNCH(true, __nv_bfloat16);
+    if (g.out == Elem::kF16) ELFB_LAUNCH(true, __half);
+    ELFB_LAUNCH(true, float);
   }
-  if (g.out == Elem::kBf16) return launch<false, __nv_bfloat16>(ta, tb, p, num_sms, s);
-  if (g.out == Elem::kF16) return launch<false, __half>(ta, tb, p, num_sms, s);
-  return launch<false, float>(ta, tb, p, num_sms, s);
+  if (g.out == Elem::kBf16) ELFB_LAUNCH(false, __nv_bfloat16);
+  if (g.out == Elem::kF16) ELFB_LAUNCH(false, __half);
+  ELFB_LAUNCH(false, float);
+#undef ELFB_LAUNCH
 }
 
 cudaError_t launch_pair(const Fp8GemmArgs& g, const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int num_sms, cudaStream_t stream);
@@ -327,7 +342,7 @@ const char* fp8_gemm(const Fp8GemmArgs& g, int num_sms, cudaStream_t stream) {
   using namespace fp8;
   if (g.M <= 0 || g.N <= 0 || g.K <= 0) return nullptr;
   CUtensorMap ta, tb;
-  const char* err = make_tmap_bytes(&ta, g.a.data, uint64_t(g.M), uint64_t(g.K), uint64_t(g.a.ld), BK, BM);
+  const char* err = make_tmap_bytes(&ta, g.a.data, uint64_t(g.M), uint64_t(g.K), uint64_t(g.a.ld), BK, use_pair(g) || g.M > 32 ? BM : 32);
   if (err) return err;
   if (g.b.mn_major) err = make_tmap_bytes(&tb, g.b.data, uint64_t(g.K), uint64_t(g.N), uint64_t(g.b.ld), 128, BK);
   else              err = make_tmap_bytes(&tb, g.b.data, uint64_t(g.N), uint64_t(g.K), uint64_t(g.b.ld), BK, 128);

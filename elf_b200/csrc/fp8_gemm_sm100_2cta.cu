@@ -136,11 +136,6 @@ __device__ __forceinline__ bool umma_x4_then_ready(uint32_t tmem_d, uint64_t des
       : "memory");
   return ready != 0;
 }
-// arrive on the barrier at this offset in both CTAs once all MMAs issued so far have completed
-__device__ __forceinline__ void umma_commit_both(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(uint16_t(3)) : "memory");
-}
-
 // One tile of the gated form: columns 0..127 of the accumulator are gate, 128..255 up.  A thread takes 64 columns
 // of gate and the same of up of one row into registers and gives the accumulator back at once; the maxima of the
 // three blocks (gate, up, activation) are exchanged with the thread that has the row's other half.

@@ -8,11 +8,11 @@
 // what lets the tensor pipe run closer to its peak under the power cap.
 //
 // Synchronisation (every wait bounded, see sm100_ptx.cuh):
-//   full[s]      lives in the EVEN CTA (the leader).  The leader's producer arms it with the
+//   full[s]      (one per slot of two stages) lives in the EVEN CTA (the leader).  The leader's producer arms it with the
 //                byte count of both CTAs' loads; both CTAs' TMA copies complete on it
 //                (the odd CTA addresses it through the cluster window; no multicast).
 //   empty[s]     one per CTA; the leader's MMA thread commits to both after the MMAs that
-//                read stage s.
+//                read the two stages of slot s.
 //   acc_full[a]  one per CTA; committed by the leader after the last MMA of a tile.
 //   acc_empty[a] in the leader; the epilogue warps of both CTAs arrive on it (8 arrivals).
 // Only the leader's MMA thread issues MMAs.  TMEM is allocated and freed with the
@@ -34,6 +34,7 @@ constexpr int BM = 128;          // rows per CTA (256 per pair)
 constexpr int BN = 256;          // columns per pair tile
 constexpr int BK = 64;
 constexpr int STAGES = 6;
+constexpr int SLOTS = STAGES / 2;  // two consecutive stages are filled, waited for and freed together
 constexpr int UMMA_K = 16;
 constexpr int A_BYTES = BM * BK * 2;        // 16 KiB
 constexpr int B_BYTES = (BN / 2) * BK * 2;  // 16 KiB: this CTA's half of the B slab
@@ -123,6 +124,35 @@ __device__ __forceinline__ WorkUnit work_unit(int unit, const Schedule& s, int k
   return wu;
 }
 
+// Four accumulating MMAs, k-steps of A_STEP and B_STEP descriptor address units; returns whether the barrier's phase had
+// completed when the test, issued before them, came up.
+template <int A_STEP, int B_STEP>
+__device__ __forceinline__ bool umma_x4_then_ready(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t bar, uint32_t parity) {
+  uint32_t ready;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, t;\n\t"
+      ".reg .b64 a, b;\n\t"
+      "setp.eq.b32 p, 0, 0;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 t, [%5], %6;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%1], %2, %3, %4, p;\n\t"
+      "add.s64 a, %2, %7;\n\t"
+      "add.s64 b, %3, %8;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%1], a, b, %4, p;\n\t"
+      "add.s64 a, a, %7;\n\t"
+      "add.s64 b, b, %8;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%1], a, b, %4, p;\n\t"
+      "add.s64 a, a, %7;\n\t"
+      "add.s64 b, b, %8;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%1], a, b, %4, p;\n\t"
+      "selp.u32 %0, 1, 0, t;\n\t"
+      "}\n"
+      : "=r"(ready)
+      : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(bar), "r"(parity), "n"(A_STEP), "n"(B_STEP)
+      : "memory");
+  return ready != 0;
+}
+
 template <bool A_MN, bool B_MN, bool OUT_F32, bool ACCUM, bool BIAS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
 gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
@@ -135,11 +165,11 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
   const uint32_t staging_base = smem_base + STAGES * STAGE_BYTES;  // 1024-byte aligned
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem_aligned + size_t(STAGES) * STAGE_BYTES + STAGING_BYTES);
   const uint32_t bar0 = smem_u32(bars);
-  auto full_bar = [&](int s) { return bar0 + 8u * s; };
-  auto empty_bar = [&](int s) { return bar0 + 8u * (STAGES + s); };
-  auto acc_full_bar = [&](int a) { return bar0 + 8u * (2 * STAGES + a); };
-  auto acc_empty_bar = [&](int a) { return bar0 + 8u * (2 * STAGES + 2 + a); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 4);
+  auto full_bar = [&](int slot) { return bar0 + 8u * slot; };
+  auto empty_bar = [&](int slot) { return bar0 + 8u * (SLOTS + slot); };
+  auto acc_full_bar = [&](int a) { return bar0 + 8u * (2 * SLOTS + a); };
+  auto acc_empty_bar = [&](int a) { return bar0 + 8u * (2 * SLOTS + 2 + a); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * SLOTS + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
@@ -154,7 +184,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
-    for (int s = 0; s < STAGES; ++s) {
+    for (int s = 0; s < SLOTS; ++s) {
       mbar_init(full_bar(s), 1);   // used in the leader only: its producer's arrive.expect_tx
       mbar_init(empty_bar(s), 1);  // one commit per use
     }
@@ -179,7 +209,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (both CTAs)
     if (lane == 0) {
-      int stage = 0;
+      int slot = 0;
       uint32_t phase = 0;
       bool ok = true;
       for (int unit = pair_id; unit < num_units && ok; unit += num_pairs) {
@@ -187,31 +217,33 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
         const int m0 = wu.m * (2 * BM) + int(cta) * BM;  // this CTA's 128 rows
         constexpr int half = BN / 2;
         const int n0 = wu.n0 + int(cta) * half;          // this CTA's half of the B rows
-        constexpr uint32_t pair_tx = 2u * (A_BYTES + B_BYTES);
-        for (int kb = wu.kb0; kb < wu.kb1; ++kb) {
-          if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) {
+        for (int kb2 = wu.kb0; kb2 < wu.kb1; kb2 += 2) {
+          if (!mbar_wait(empty_bar(slot), phase ^ 1u, abort_flag)) {
             ok = false;
             break;
           }
-          const uint32_t sa = smem_base + stage * STAGE_BYTES;
-          const uint32_t sb = sa + A_BYTES;
-          const uint32_t bar = map_to_cta(full_bar(stage), 0);  // the leader's barrier
-          if (leader) mbar_arrive_expect_tx(full_bar(stage), pair_tx);
-          const int k0 = kb * BK;
-          if (A_MN) {
+          const int blocks = min(2, wu.kb1 - kb2);
+          const uint32_t bar = map_to_cta(full_bar(slot), 0);  // the leader's barrier
+          if (leader) mbar_arrive_expect_tx(full_bar(slot), uint32_t(blocks) * 2u * STAGE_BYTES);
+          for (int i = 0; i < blocks; ++i) {
+            const uint32_t sa = smem_base + (2 * slot + i) * STAGE_BYTES;
+            const uint32_t sb = sa + A_BYTES;
+            const int k0 = (kb2 + i) * BK;
+            if (A_MN) {
 #pragma unroll
-            for (int j = 0; j < BM / 64; ++j) tma_load_2d_pair(sa + j * (BK * 128), &tmap_a, bar, m0 + 64 * j, k0);
-          } else {
-            tma_load_2d_pair(sa, &tmap_a, bar, k0, m0);
-          }
-          if (B_MN) {
+              for (int j = 0; j < BM / 64; ++j) tma_load_2d_pair(sa + j * (BK * 128), &tmap_a, bar, m0 + 64 * j, k0);
+            } else {
+              tma_load_2d_pair(sa, &tmap_a, bar, k0, m0);
+            }
+            if (B_MN) {
 #pragma unroll
-            for (int j = 0; j < half / 64; ++j) tma_load_2d_pair(sb + j * (BK * 128), &tmap_b, bar, n0 + 64 * j, k0);
-          } else {
-            tma_load_2d_pair(sb, &tmap_b, bar, k0, n0);
+              for (int j = 0; j < half / 64; ++j) tma_load_2d_pair(sb + j * (BK * 128), &tmap_b, bar, n0 + 64 * j, k0);
+            } else {
+              tma_load_2d_pair(sb, &tmap_b, bar, k0, n0);
+            }
           }
-          if (++stage == STAGES) {
-            stage = 0;
+          if (++slot == SLOTS) {
+            slot = 0;
             phase ^= 1u;
           }
         }
@@ -223,41 +255,42 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
     if (leader && lane == 0) {
       constexpr uint32_t A_LBO = A_MN ? BK * 128 : 0, B_LBO = B_MN ? BK * 128 : 0;
       constexpr uint32_t A_KSTEP = A_MN ? UMMA_K * 128 : UMMA_K * 2, B_KSTEP = B_MN ? UMMA_K * 128 : UMMA_K * 2;
-      int stage = 0;
+      // A barrier test queues up behind the MMAs issued before it, so its answer comes when the tensor pipe has nearly
+      // run dry.  There is one test per slot of eight MMAs, issued before the slot's last four and read after them.
+      int slot = 0;
       uint32_t phase = 0;
       int acc = 0;
       uint32_t acc_phase = 0;
       bool ok = true;
       const uint32_t idesc = make_idesc_f16(fmt, 2 * BM, BN, A_MN ? 1u : 0u, B_MN ? 1u : 0u);
+      const uint64_t desc_a0 = make_smem_desc_sw128(smem_base, A_LBO, 1024), desc_b0 = make_smem_desc_sw128(smem_base + A_BYTES, B_LBO, 1024);
       for (int unit = pair_id; unit < num_units && ok; unit += num_pairs) {
         const WorkUnit wu = work_unit(unit, sched, k_blocks);
         if (!mbar_wait(acc_empty_bar(acc), acc_phase ^ 1u, abort_flag)) break;
         tc_fence_after_sync();
         const uint32_t tmem_d = tmem_base + acc * BN;
-        for (int kb = wu.kb0; kb < wu.kb1; ++kb) {
-          if (!mbar_wait(full_bar(stage), phase, abort_flag)) {
+        bool ready = false;
+        for (int kb = wu.kb0; kb < wu.kb1; kb += 2) {
+          if (!ready && !mbar_wait(full_bar(slot), phase, abort_flag)) {
             ok = false;
             break;
           }
-          tc_fence_after_sync();
-          const uint32_t sa = smem_base + stage * STAGE_BYTES;
-          const uint32_t sb = sa + A_BYTES;
+          const int next = slot + 1 == SLOTS ? 0 : slot + 1;
+          const uint32_t next_phase = phase ^ (next == 0 ? 1u : 0u);
+          const uint64_t da = desc_a0 + uint32_t(slot * (2 * STAGE_BYTES >> 4)), db = desc_b0 + uint32_t(slot * (2 * STAGE_BYTES >> 4));
 #pragma unroll
-          for (int k = 0; k < BK / UMMA_K; ++k) {
-            const uint64_t da = make_smem_desc_sw128(sa + k * A_KSTEP, A_LBO, 1024);
-            const uint64_t db = make_smem_desc_sw128(sb + k * B_KSTEP, B_LBO, 1024);
-            umma_ss_pair(tmem_d, da, db, idesc, (kb > wu.kb0 || k) ? 1u : 0u);
-          }
-          umma_commit_pair(map_to_cta(empty_bar(stage), 0));
-          umma_commit_pair(map_to_cta(empty_bar(stage), 1));
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
+          for (int k = 0; k < BK / UMMA_K; ++k)
+            umma_ss_pair(tmem_d, da + ((k * A_KSTEP) >> 4), db + ((k * B_KSTEP) >> 4), idesc, (kb > wu.kb0 || k) ? 1u : 0u);
+          ready = false;
+          if (kb + 1 < wu.kb1)
+            ready = umma_x4_then_ready<int(A_KSTEP >> 4), int(B_KSTEP >> 4)>(tmem_d, da + (STAGE_BYTES >> 4), db + (STAGE_BYTES >> 4), idesc, full_bar(next), next_phase) &&
+                    kb + 2 < wu.kb1;
+          umma_commit_both(empty_bar(slot));
+          slot = next;
+          phase = next_phase;
         }
         if (!ok) break;
-        umma_commit_pair(map_to_cta(acc_full_bar(acc), 0));
-        umma_commit_pair(map_to_cta(acc_full_bar(acc), 1));
+        umma_commit_both(acc_full_bar(acc));
         if (++acc == 2) {
           acc = 0;
           acc_phase ^= 1u;

@@ -404,6 +404,11 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t bar_cluster_addr) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_cluster_addr) : "memory");
 }
 
+// arrive on the barrier at this shared-memory offset in BOTH CTAs of the pair when all MMAs issued so far have completed
+__device__ __forceinline__ void umma_commit_both(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(uint16_t(3)) : "memory");
+}
+
 // ----------------------------------------------------------------------------------------
 // Descriptors
 // ----------------------------------------------------------------------------------------

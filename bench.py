@@ -48,6 +48,7 @@ def parse_args():
     ap.add_argument("--split-thirds", action="store_true", help="also allow a stage boundary after the MLP's SwiGLU (two tensors cross it); finer balance for deep pipelines")
     ap.add_argument("--timeline", default=None, help="write every rank's per-operation device timeline of one extra step (JSON) to this file")
     ap.add_argument("--chunked-head", action="store_true", help="LM head + cross entropy with the vocabulary in chunks: the logits (1 GB per micro-batch) are never materialised, at the price of one more pass over the head's matrix")
+    ap.add_argument("--ffn-fp8", action="store_true", help="feed-forward products, and what they keep for the backward pass, in 8 bits (another numerical recipe: the result is not the headline number)")
     ap.add_argument("--grad-sync", choices=["auto", "nccl", "symm"], default="auto", help="with --dp > 1: peer-memory gradient exchange fused into the weight-gradient GEMM, or NCCL all-reduce")
     ap.add_argument("--p2p", choices=["auto", "nccl", "copy"], default="auto", help="stage-to-stage transport: NCCL send/recv kernels, or copy-engine writes into the consumer's ring buffer")
     ap.add_argument("--no-calibrate", action="store_true", help="cut the stages and lay the schedule out for the built-in cost constants instead of times measured at start-up (for comparison)")
@@ -73,6 +74,8 @@ def run_ours(args):
         cfg = replace(cfg, seq_len=args.seq_len)
     if args.layers:
         cfg = replace(cfg, n_layers=args.layers)
+    if args.ffn_fp8:
+        cfg = replace(cfg, ffn_fp8=True)
     dp = args.dp
     pp = world // dp
     placement = Placement.default(args.scheduler, pp)
@@ -266,7 +269,7 @@ def run_ours(args):
         "higher_is_better": True,
         "scaling": "strong",
         "vs_baseline": (value / BASELINE_TOKENS_PER_S) if BASELINE_TOKENS_PER_S else None,
-        "dtype": "bf16",
+        "dtype": "bf16, feed-forward products fp8 (e4m3, block-scaled)" if args.ffn_fp8 else "bf16",
         "data": "synthetic uniform token ids, N(0,0.02) random-init weights",
         "config": {
             "model": f"{args.model} ({cfg.n_layers} layers, d={cfg.d_model}, {cfg.n_heads}q/{cfg.n_kv_heads}kv heads, ffn={cfg.ffn}, vocab={cfg.vocab})",

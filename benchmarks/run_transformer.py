@@ -22,6 +22,7 @@ import logging
 import os
 import sys
 import time
+from dataclasses import replace as _replace
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 if ROOT not in sys.path:
@@ -69,6 +70,7 @@ def parse_args():
     ap.add_argument("--memory-budget", type=int, help="MB per GPU; enables ILP rematerialisation")
     ap.add_argument("--tracer", default="default", choices=TRACERS.available() if len(TRACERS) else ["default"])
     ap.add_argument("--grad-sync", default="auto", choices=["auto", "nccl", "symm"])
+    ap.add_argument("--ffn-fp8", action="store_true", help="Llama models: feed-forward products, and what they keep for the backward pass, in 8 bits")
     ap.add_argument("--check", action="store_true", help="before timing, compare one pipeline step (outputs, loss, every gradient) with the same model run in a single process")
     ap.add_argument("--p2p", default="auto", choices=["auto", "nccl", "copy"], help="stage-to-stage transport")
     ap.add_argument("--offload-ilp", action="store_true", help="with --memory-budget: let the ILP also offload activations to pinned host memory")
@@ -130,10 +132,8 @@ def main():
         # graph front end on the Llama model: the worker rank builds the whole decoder as one flat
         # nn.Sequential of fused blocks, traces it, times every node on its GPU, cuts it with the
         # chosen partitioner and ships the stages; the other ranks only pass the sample
-        cfg = LLAMA_CONFIGS[args.model]
+        cfg = _replace(LLAMA_CONFIGS[args.model], ffn_fp8=args.ffn_fp8)
         if args.seq_len:
-            from dataclasses import replace as _replace
-
             cfg = _replace(cfg, seq_len=args.seq_len)
         model = build_llama(cfg, device=device, dtype=dtype, seed=1234, split_backward=True) if rank == 0 else None
         parts, signatures, partitioner = model, None, args.partitioner
@@ -141,7 +141,7 @@ def main():
         sample = torch.randint(0, vocab, (args.mb_size, seq), device=device)
         n_params = cfg.n_params()
     elif args.architecture == "llama":
-        cfg = LLAMA_CONFIGS[args.model]
+        cfg = _replace(LLAMA_CONFIGS[args.model], ffn_fp8=args.ffn_fp8)
         mine = placement.get_ids(pp_rank)
         stages = build_llama_stages(cfg, len(placement), only=mine, device=device, dtype=dtype, seed=1234, placement=list(placement), split_layers=args.split_layers)
         if args.scheduler == "zbv" and pp > 1 and not args.checkpointing and not args.offloading and args.memory_budget is None:

@@ -279,6 +279,13 @@ class LinearFP8DW(LinearDW):
         super().clear()
         self._hold_weight_q, self._weight_q = False, None
 
+    def __getstate__(self):
+        """Copies and shipped layers start without pending micro-batches: a profiling pass leaves its last input behind,
+        and 8-bit tensors do not go through plain pickle."""
+        state = self.__dict__.copy()
+        state.update(ctx={"input": [], "grad_output": []}, last_input=None, last_grad_output=None, _hold_weight_q=False, _weight_q=None)
+        return state
+
     def _store_input_q(self, xq: _fp8.BlockScaled, is_model_input: bool) -> None:
         xq.is_model_input = is_model_input  # see LayerDW._store_input
         self.last_input = xq

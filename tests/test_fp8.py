@@ -228,6 +228,19 @@ def test_layer_applied_twice_sums_its_output_gradients():
     assert isinstance(layer.last_grad_output, torch.Tensor) and layer.last_grad_output.dtype == torch.bfloat16
 
 
+def test_layer_ships_without_its_stash():
+    import pickle
+
+    layer = LinearFP8DW(torch.nn.Linear(64, 32))
+    layer(rand(4, 64))
+    layer.move_last_computed("input", 1)
+    layer(rand(4, 64))
+    for twin in (pickle.loads(pickle.dumps(layer)), copy.deepcopy(layer)):
+        assert twin.last_input is None and twin.is_empty("input") and twin._weight_q is None
+        assert torch.equal(twin(rand(4, 64)), layer(rand(4, 64)))
+    assert isinstance(layer.ctx["input"][1], BlockScaled)
+
+
 def test_replacement_selects_layers():
     model = torch.nn.Sequential(torch.nn.Linear(8, 8), torch.nn.ReLU(), torch.nn.Linear(8, 8))
     replace_layer_with_layer_dw(model)
@@ -284,3 +297,21 @@ def test_mlp_block_composes_on_cpu():
     x = rand(2, 8, CFG.d_model).requires_grad_()
     blk(x).sum().backward()
     assert x.grad is not None and isinstance(blk.w_down.last_input, BlockScaled)
+
+
+@pytest.mark.parametrize("partitioner", ["handcrafted", "naive"])
+def test_command_runs_in_8_bits(partitioner):
+    """``run_transformer.py --ffn-fp8``: hand-made stages, and a traced, cut and shipped model."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    cmd = [sys.executable, "-m", "torch.distributed.run", "--nnodes=1", "--nproc-per-node=2", "--master-addr", "127.0.0.1", "--master-port", "29797",
+           os.path.join(root, "benchmarks", "run_transformer.py"), "--architecture", "llama", "--name", "llama-tiny", "--partitioner", partitioner, "--ffn-fp8",
+           "--scheduler", "zbh1", "--nmb", "4", "--mb-size", "1", "--niters", "1", "--warmup", "1", "--backend", "gloo"]
+    if partitioner != "handcrafted":
+        cmd.append("--check")  # one step against the same model in a single process
+    out = subprocess.run(cmd, cwd=root, capture_output=True, text=True, timeout=300, env=dict(os.environ, CUDA_VISIBLE_DEVICES=""))
+    assert out.returncode == 0, out.stdout[-1500:] + out.stderr[-3000:]
+    assert "tokens_per_s" in out.stdout

@@ -156,21 +156,34 @@ __device__ __forceinline__ void store_32_bytes(uint8_t* p, const uint32_t (&v)[8
                "r"(v[6]), "r"(v[7])
                : "memory");
 }
-// N values times 2^(127 - byte) to e4m3
-template <int N>
+// N values times 2^(127 - byte) to e4m3.  ODD: some may not be finite and become NaN; without it that costs nothing.
+template <int N, bool ODD>
 __device__ __forceinline__ void to_scaled_e4m3(const float* v, float inv, uint32_t* q) {
 #pragma unroll
   for (int j = 0; j < N / 4; ++j) {
     float s[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) s[k] = nan_unless_finite(mul_exact(v[4 * j + k], inv), v[4 * j + k]);
+    for (int k = 0; k < 4; ++k) {
+      s[k] = mul_exact(v[4 * j + k], inv);
+      if (ODD) s[k] = nan_unless_finite(s[k], v[4 * j + k]);
+    }
     q[j] = to_e4m3x4(s[0], s[1], s[2], s[3]);
   }
 }
-__device__ __forceinline__ void scale_and_store_32(const float* v, float inv, uint8_t* dst) {
-  uint32_t q[8];
-  to_scaled_e4m3<32>(v, inv, q);
-  store_32_bytes(dst, q);
+template <int N, bool ODD>
+__device__ __forceinline__ void scale_and_store(const float* v, float inv, uint8_t* dst) {
+#pragma unroll
+  for (int c = 0; c < N / 32; ++c) {
+    uint32_t q[8];
+    to_scaled_e4m3<32, ODD>(v + 32 * c, inv, q);
+    store_32_bytes(dst + 32 * c, q);
+  }
+}
+template <int N, bool ODD>
+__device__ __forceinline__ uint32_t magnitude(const float* v, uint32_t top = 0) {  // of those that are finite
+#pragma unroll
+  for (int j = 0; j < N; ++j) top = max(top, ODD ? finite_bits(v[j]) : abs_bits(v[j]));
+  return top;
 }
 
 // The layout tcgen05.cp wants: 16 bytes per lane, word j for row 32 j + lane.

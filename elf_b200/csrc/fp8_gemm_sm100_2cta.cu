@@ -159,19 +159,25 @@ __device__ __forceinline__ void gated_tile(uint32_t taddr, int row, int half, in
     named_barrier_sync(1, EPI_THREADS);
     return block_exponent(max(top, exchange[(which * 2 + (half ^ 1)) * BM]));
   };
+  // blocks without infinities and NaN, practically all, take the branches that do not look for them
+  auto any = [](bool odd) { return __any_sync(0xffffffffu, odd) != 0; };
   if (p.gu != nullptr) {
-    uint32_t top_g = 0, top_u = 0;
-#pragma unroll
-    for (int j = 0; j < 64; ++j) top_g = max(top_g, finite_bits(g[j])), top_u = max(top_u, finite_bits(u[j]));
+    uint32_t top_g = magnitude<64, false>(g), top_u = magnitude<64, false>(u);
+    const bool odd = any(top_g >= kInfBits || top_u >= kInfBits);
+    if (odd) top_g = magnitude<64, true>(g), top_u = magnitude<64, true>(u);
     exchange[half * BM] = top_g;
     const uint32_t byte_u = block_byte(1, top_u);
     const uint32_t byte_g = block_exponent(max(top_g, exchange[(half ^ 1) * BM]));
     if (live) {
       uint8_t* dst = p.gu + (long long)row * p.ld_gu + col;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) scale_and_store_32(g + 32 * c, inverse_exponent_value(byte_g), dst + 32 * c);
-#pragma unroll
-      for (int c = 0; c < 2; ++c) scale_and_store_32(u + 32 * c, inverse_exponent_value(byte_u), dst + f + 32 * c);
+      const float inv_g = inverse_exponent_value(byte_g), inv_u = inverse_exponent_value(byte_u);
+      if (odd) {
+        scale_and_store<64, true>(g, inv_g, dst);
+        scale_and_store<64, true>(u, inv_u, dst + f);
+      } else {
+        scale_and_store<64, false>(g, inv_g, dst);
+        scale_and_store<64, false>(u, inv_u, dst + f);
+      }
       if (half == 0) {
         uint8_t* s = p.gu_scale + (long long)row * p.ld_gu_scale;
         s[f0 / 128] = uint8_t(byte_g);
@@ -179,17 +185,16 @@ __device__ __forceinline__ void gated_tile(uint32_t taddr, int row, int half, in
       }
     }
   }
-  uint32_t top = 0;
 #pragma unroll
-  for (int j = 0; j < 64; ++j) {
-    g[j] = g[j] * __fdividef(1.f, 1.f + __expf(-g[j])) * u[j];
-    top = max(top, finite_bits(g[j]));
-  }
+  for (int j = 0; j < 64; ++j) g[j] = g[j] * __fdividef(1.f, 1.f + __expf(-g[j])) * u[j];
+  uint32_t top = magnitude<64, false>(g);
+  const bool odd = any(top >= kInfBits);
+  if (odd) top = magnitude<64, true>(g);
   const uint32_t byte = block_byte(2, top);
   if (live) {
     uint8_t* dst = p.act + (long long)row * p.ld_act + col;
-#pragma unroll
-    for (int c = 0; c < 2; ++c) scale_and_store_32(g + 32 * c, inverse_exponent_value(byte), dst + 32 * c);
+    if (odd) scale_and_store<64, true>(g, inverse_exponent_value(byte), dst);
+    else scale_and_store<64, false>(g, inverse_exponent_value(byte), dst);
     if (half == 0) p.act_scale[(long long)row * p.ld_act_scale + f0 / 128] = uint8_t(byte);
   }
 }
@@ -201,20 +206,25 @@ __device__ __forceinline__ void gated_tile(uint32_t taddr, int row, int half, in
 // registers.  d stays in TMEM but for the 32 columns shared with the other accumulator, which half of the threads
 // hold.  The checkpoint is read and the result written 32 bytes at a time, whole sectors of a row that is one
 // thread's own: 309 us for 4096 x 14336 x 4096, with 16-byte accesses 350.
-struct GatedGrad {
-  float dg[16], du[16];
+//
+// With t = d s and the scales sg, su of gate and up taken out of the sums (powers of two: exact),
+//   dup = sg (t gate_q),  dgate = su (up_q (t + t gate_q sg (1 - s))).
+struct GateScales {
+  float sg;       // gate = gate_q * sg
+  float log2e;    // -log2(e) * sg
 };
-__device__ __forceinline__ void gated_grad(const uint32_t* d, const uint32_t* gq, const uint32_t* uq, float sg, float su, GatedGrad& o) {
+// dup / sg and dgate / su for 16 columns
+__device__ __forceinline__ void gated_grad(const uint32_t* d, const uint32_t* gq, const uint32_t* uq, GateScales c, float (&dg)[16], float (&du)[16]) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float2 ge = from_e4m3x2((gq[j / 2] >> (16 * (j & 1))) & 0xffffu), ue = from_e4m3x2((uq[j / 2] >> (16 * (j & 1))) & 0xffffu);
-    const float g[2] = {ge.x * sg, ge.y * sg}, up[2] = {ue.x * su, ue.y * su};
+    const float2 g2 = from_e4m3x2((gq[j / 2] >> (16 * (j & 1))) & 0xffffu), u2 = from_e4m3x2((uq[j / 2] >> (16 * (j & 1))) & 0xffffu);
+    const float g[2] = {g2.x, g2.y}, up[2] = {u2.x, u2.y};
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const float v = __uint_as_float(d[2 * j + k]);
-      const float sig = __fdividef(1.f, 1.f + __expf(-g[k]));
-      o.du[2 * j + k] = v * g[k] * sig;
-      o.dg[2 * j + k] = v * up[k] * sig * (1.f + g[k] * (1.f - sig));
+      const float sig = __fdividef(1.f, 1.f + exp2f(g[k] * c.log2e));
+      const float t = __uint_as_float(d[2 * j + k]) * sig;
+      du[2 * j + k] = t * g[k];
+      dg[2 * j + k] = up[k] * fmaf(t * g[k], fmaf(-sig, c.sg, c.sg), t);
     }
   }
 }
@@ -237,37 +247,17 @@ __device__ __forceinline__ void gated_backward_tile(uint32_t taddr, int acc, int
   const uint8_t* gate = p.gu + r * p.ld_gu + c0;
   const uint8_t* scales = p.gu_scale + r * p.ld_gu_scale + c0 / 128;
   const float sg = exponent_value(scales[0]), su = exponent_value(scales[f / 128]);
+  const GateScales gs{sg, -1.4426950408889634f * sg};
   uint8_t* dst = p.act + r * p.ld_act + c0;
-  uint32_t top_g = 0, top_u = 0;
-  float inv_g = 0.f, inv_u = 0.f;
-#pragma unroll
-  for (int pass = 0; pass < 2; ++pass) {
-    auto handle = [&](const uint32_t (&d)[32], int c, const uint32_t (&g)[8], const uint32_t (&u)[8]) {
-      uint32_t qg[8], qu[8];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        GatedGrad o;
-        gated_grad(d + 16 * h, g + 4 * h, u + 4 * h, sg, su, o);
-        if (pass == 0) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) top_g = max(top_g, finite_bits(o.dg[j])), top_u = max(top_u, finite_bits(o.du[j]));
-        } else {
-          to_scaled_e4m3<16>(o.dg, inv_g, qg + 4 * h);
-          to_scaled_e4m3<16>(o.du, inv_u, qu + 4 * h);
-        }
-      }
-      if (pass == 1 && live) {
-        store_32_bytes(dst + 32 * c, qg);
-        store_32_bytes(dst + f + 32 * c, qu);
-      }
-    };
+  // calls handle(d, gate_q, up_q, chunk) for the row's four chunks, the checkpoint of the next one on its way
+  auto sweep = [&](auto&& handle) {
     uint32_t g[8], u[8], next_g[8], next_u[8];
     load_32_bytes(gate + 32 * from, next_g);
     load_32_bytes(gate + f + 32 * from, next_u);
     if (shares) {
       load_32_bytes(gate + 32 * held_chunk, g);
       load_32_bytes(gate + f + 32 * held_chunk, u);
-      handle(held, held_chunk, g, u);
+      handle(held, g, u, held_chunk);
     }
 #pragma unroll 1
     for (int c = from; c < to; ++c) {
@@ -280,17 +270,65 @@ __device__ __forceinline__ void gated_backward_tile(uint32_t taddr, int acc, int
         load_32_bytes(gate + f + 32 * (c + 1), next_u);
       }
       tmem_ld_wait();
-      handle(d, c, g, u);
+      handle(d, g, u, c);
     }
-    if (pass == 0) {
-      const uint32_t byte_g = block_exponent(top_g), byte_u = block_exponent(top_u);
-      inv_g = inverse_exponent_value(byte_g), inv_u = inverse_exponent_value(byte_u);
-      if (live) {
-        uint8_t* s = p.act_scale + r * p.ld_act_scale + c0 / 128;
-        s[0] = uint8_t(byte_g);
-        s[f / 128] = uint8_t(byte_u);
+  };
+  // Maxima of gradient / scale; multiplying by the scale keeps their order.  Infinite or NaN gradients, practically
+  // never there, make the sweep run once more looking at finite ones only.
+  uint32_t top_g = 0, top_u = 0;
+  sweep([&](const uint32_t (&d)[32], const uint32_t (&g)[8], const uint32_t (&u)[8], int) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float dg[16], du[16];
+      gated_grad(d + 16 * h, g + 4 * h, u + 4 * h, gs, dg, du);
+      top_g = magnitude<16, false>(dg, top_g);
+      top_u = magnitude<16, false>(du, top_u);
+    }
+  });
+  auto odd_at = [&](uint32_t top, float scale) { return abs_bits(mul_exact(__uint_as_float(top), scale)) >= kInfBits; };
+  const bool odd = __any_sync(0xffffffffu, odd_at(top_g, su) || odd_at(top_u, sg));
+  if (odd) {
+    top_g = top_u = 0;
+    sweep([&](const uint32_t (&d)[32], const uint32_t (&g)[8], const uint32_t (&u)[8], int) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float dg[16], du[16];
+        gated_grad(d + 16 * h, g + 4 * h, u + 4 * h, gs, dg, du);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          top_g = max(top_g, odd_at(__float_as_uint(dg[j]), su) ? 0u : abs_bits(dg[j]));
+          top_u = max(top_u, odd_at(__float_as_uint(du[j]), sg) ? 0u : abs_bits(du[j]));
+        }
       }
-    }
+    });
+  }
+  const uint32_t byte_g = block_exponent(abs_bits(mul_exact(__uint_as_float(top_g), su))), byte_u = block_exponent(abs_bits(mul_exact(__uint_as_float(top_u), sg)));
+  const float inv_g = inverse_exponent_value(byte_g), inv_u = inverse_exponent_value(byte_u);
+  auto emit = [&](auto odd_tag) {
+    constexpr bool ODD = decltype(odd_tag)::value;
+    sweep([&](const uint32_t (&d)[32], const uint32_t (&g)[8], const uint32_t (&u)[8], int c) {
+      uint32_t qg[8], qu[8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float dg[16], du[16];
+        gated_grad(d + 16 * h, g + 4 * h, u + 4 * h, gs, dg, du);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) dg[j] = mul_exact(dg[j], su), du[j] = mul_exact(du[j], sg);
+        to_scaled_e4m3<16, ODD>(dg, inv_g, qg + 4 * h);
+        to_scaled_e4m3<16, ODD>(du, inv_u, qu + 4 * h);
+      }
+      if (live) {
+        store_32_bytes(dst + 32 * c, qg);
+        store_32_bytes(dst + f + 32 * c, qu);
+      }
+    });
+  };
+  if (odd) emit(std::true_type());
+  else emit(std::false_type());
+  if (live) {
+    uint8_t* s = p.act_scale + r * p.ld_act_scale + c0 / 128;
+    s[0] = uint8_t(byte_g);
+    s[f / 128] = uint8_t(byte_u);
   }
 }
 

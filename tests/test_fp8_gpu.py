@@ -176,6 +176,22 @@ def test_rms_norm(dev, rows, dim, residual):
     assert (top <= 448 * scale * slack).all() and (top * slack >= 224 * scale).all()
 
 
+@pytest.mark.parametrize("rows,dim", [(4000, 1024), (4096, 4096)])
+def test_rms_norm_rounds_once(dev, rows, dim):
+    """The 8-bit values are the roundings of the exact ones: an error of 1e-9 in a row's statistic moves one value in 10^8."""
+    from elf_b200.ops import fp8
+
+    for seed in range(24):
+        x = activations(rows, dim, torch.bfloat16, dev, seed)
+        w = (1 + 0.1 * torch.randn(dim, device=dev)).to(torch.bfloat16)
+        xd = x.double()
+        y = xd / (xd.square().sum(1, keepdim=True) / dim + 1e-5).sqrt() * w.double()
+        q = fp8.rms_norm(x, w, 1e-5)[0]
+        unit = torch.exp2(q.scale.double() - 127).repeat_interleave(128, 1)
+        step = unit * torch.exp2(torch.floor(torch.log2((y / unit).abs().clamp_min(2.0**-6))) - 3)
+        assert torch.equal(values(q), torch.round(y / step) * step)
+
+
 def test_rms_norm_rows_without_finite_values(dev):
     from elf_b200.ops import fp8
 

@@ -41,8 +41,8 @@ struct Params {
 };
 
 // Exponent bytes of blocks 4g .. 4g+3 for rows row0 + lane, + 32, + 64, + 96 of an operand, as they come from
-// memory: nothing here looks at a loaded value, so a warp issues the loads of all operands and goes on
-// (combining them at once cost the products 10 to 30 % of their time, waiting for this warp).
+// memory: nothing here looks at a loaded value, so a warp issues the loads of all operands and goes on; they are
+// combined one group of blocks later, when they have long arrived.
 struct RawScales {
   uint32_t v[4][4];  // [row][byte]; aligned words: [row][0]; one scale for all 128 rows: [0]
 };

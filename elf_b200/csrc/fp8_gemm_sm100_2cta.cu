@@ -3,13 +3,16 @@
 //
 // Why pairs: a 128 x 256 tile on one CTA fetches 48 KiB for 512 cycles of 8-bit MMA, 25 TB/s over the chip,
 // which is more than L2 delivers; the pair fetches 32 KiB per CTA in the same time (each its own 128 rows
-// of A and half of B).  4096 x 4096 x 14336: 249 us with single CTAs.
+// of A and half of B).  4096 x 4096 x 14336: 176 us; a kernel of single CTAs with 128 x 256 tiles took 249.
+// What bounds it: the tensor pipe, 79 % busy at 180 us there and 84 % in the gradient's form (4096 x 4096 x 28672,
+// 344 us); under a lasting load the chip's power, which takes the clock from 1.9 to 1.1 - 1.4 GHz.
 //
-// Roles per CTA as in fp8_gemm_sm100.cu.  The even CTA's MMA thread issues for both.  Barriers:
-//   full[s]      even CTA: armed with both CTAs' bytes, both CTAs' copies complete on it; for the first of two
-//                stages both CTAs' scale warps arrive too, when their words lie in shared memory
-//   empty[s/2]   one per CTA, committed to both once for two stages: a commit costs about as much as a step
-//                of MMA (two single commits per stage instead: 218 us against 200 in the loop alone)
+// Roles per CTA as in fp8_gemm_sm100.cu.  The even CTA's MMA thread issues for both.  Barriers, each of a slot of two
+// stages:
+//   full[s]      even CTA: armed with both CTAs' bytes, both CTAs' copies complete on it, and both CTAs' scale warps
+//                arrive when their words lie in shared memory
+//   empty[s]     one per CTA, committed to both at once: a commit costs about as much as a step of MMA (two single
+//                commits per stage instead: 218 us against 200 in the loop alone)
 //   acc_full[a]  one per CTA, committed to both
 //   acc_free     even CTA: the epilogue warps of both arrive once the columns the two accumulators share
 //                have been read (8 arrivals per unit)
@@ -205,7 +208,11 @@ __device__ __forceinline__ void gated_tile(uint32_t taddr, int row, int half, in
 // are formed twice, once for the maxima of their blocks and once to be scaled: 256 values per row would not stay in
 // registers.  d stays in TMEM but for the 32 columns shared with the other accumulator, which half of the threads
 // hold.  The checkpoint is read and the result written 32 bytes at a time, whole sectors of a row that is one
-// thread's own: 309 us for 4096 x 14336 x 4096, with 16-byte accesses 350.
+// thread's own: 16-byte accesses cost 40 us more.
+//
+// 4096 x 14336 x 4096: 283 us (180 without this epilogue, 142 at the 8-bit peak); the epilogue of a tile outlasts the
+// next tile's MMAs.  Its arithmetic alone beside the MMAs takes 243, loads and stores with next to no arithmetic
+// 273, one sweep 250.  Neither 16 epilogue warps (289) nor fetching the next tile's checkpoint into L2 (291) helped.
 //
 // With t = d s and the scales sg, su of gate and up taken out of the sums (powers of two: exact),
 //   dup = sg (t gate_q),  dgate = su (up_q (t + t gate_q sg (1 - s))).
@@ -653,14 +660,17 @@ Schedule make_schedule(int M, int N, int K, Fp8Form form, int num_pairs) {
   const long long tiles = (long long)s.tiles_m * s.tiles_n;
   const int rem = int(tiles % num_pairs);
   s.ksplit = 1;
-  if (rem != 0 && form == Fp8Form::kPlain) {
-    // cycles of the last wave: measured 800 per block of K, and for split tiles about 10 us for clearing the
-    // counters and exchanging the sums.  4096 x 4096 x K (34 tiles left over): K = 14336 takes 217 us split in two
-    // and 227 us whole, K = 4096 82 and 79.
-    long long best = 800ll * k_blocks;
+  if (rem != 0 && form == Fp8Form::kPlain && k_blocks >= 48) {
+    // Cycles of the last wave, fitted to rem = 16, 32, 34, 54, 64 tiles, K = 1024 .. 14336, split 1 to 8 ways: 600 per
+    // block of K, and for split tiles 6000 to clear the counters and 200 for each part that is written and read back.
+    // N = 4096, whole against split in two (us):  256 rows, K = 4096: 20.5 and 23.2; K = 14336: 45.1 and 35.5 (in four
+    // 31.7); 2048 rows (54 of 128 tiles left over), K = 14336: 97 and 110; 4096 rows (34 left over): 188 and 184.
+    // Shorter reductions, where a split would gain 3 us for a tile or two at best, stay whole: a row's result does not
+    // depend on the number of rows then.
+    long long best = 600ll * k_blocks;
     for (int w = 2; w <= 8 && 2 * w <= groups; ++w) {
       const long long waves = ((long long)rem * w + num_pairs - 1) / num_pairs;
-      const long long cost = waves * 3200 * ((groups + w - 1) / w) + 16000 + 1000 * w;
+      const long long cost = waves * 2400 * ((groups + w - 1) / w) + 6000 + 200ll * rem * w;
       if (cost < best) {
         best = cost;
         s.ksplit = w;

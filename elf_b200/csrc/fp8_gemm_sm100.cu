@@ -32,8 +32,9 @@ namespace rows128 {
 constexpr int BN = 128;
 // A's box holds ROWS (32 or 128) rows.  The MMA always reads 128; behind a box of 32 lies B's, whose bytes end in
 // accumulator rows that nobody looks at.  Up to 32 rows leave room for two CTAs per SM, one of which starts or ends
-// while the other streams.  16 x 4096 x 14336: 15.9 us, of which 5.5 stream the weights, 3.5 wait for the launch and the
-// first bytes and 3.3 add the parts; one CTA per SM 16.0, without the split 45.5.
+// while the other streams.  16 x 4096 x 14336, one launch after the other: 15.9 us (59 MB: 9.0 at the copy rate); a launch
+// by itself spends 5.5 on the weights (in L2), 3.5 until the first bytes, most of it hidden behind the launch before, and
+// 3.3 on adding the parts.  Without the split 45.5.
 template <int ROWS>
 constexpr int CTAS_PER_SM = ROWS == 32 ? 2 : 1;
 template <int ROWS>
@@ -98,6 +99,7 @@ fp8_gemm_rows128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
+  await_previous();
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
@@ -291,18 +293,8 @@ cudaError_t launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p
   const int tiles = (p.N + BN - 1) / BN, groups = (p.K + 4 * BK - 1) / (4 * BK);
   int ksplit = 1;  // as many parts as there are SMs for, each at least four blocks of K long
   while (ksplit < MAX_CLUSTER && 2 * ksplit * tiles <= num_sms * CTAS_PER_SM<ROWS> && 2 * ksplit <= groups) ksplit *= 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(tiles) * ksplit);
-  cfg.blockDim = dim3(NUM_THREADS);
-  cfg.dynamicSmemBytes = SMEM_BYTES<ROWS>;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = ksplit;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  if (cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ta, tb, p, ksplit); e != cudaSuccess) return e;
+  if (cudaError_t e = launch_overlapped(kern, unsigned(tiles) * ksplit, NUM_THREADS, SMEM_BYTES<ROWS>, unsigned(ksplit), stream, ta, tb, p, ksplit); e != cudaSuccess)
+    return e;
   flush_bounds_record(p.status, stream);
   return cudaGetLastError();
 }

@@ -390,6 +390,7 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   cluster_sync_all();  // both CTAs' barriers are initialised before anyone touches the peer's
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
+  await_previous();
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (both CTAs)
@@ -701,7 +702,7 @@ cudaError_t launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p
     if (cudaError_t e = cudaMemsetAsync(counters, 0, size_t(rem) * 2 * sizeof(unsigned int), stream); e != cudaSuccess) return e;
   }
   const int pairs = s.total_units < num_pairs ? s.total_units : num_pairs;
-  kern<<<2 * pairs, NUM_THREADS, SMEM_BYTES, stream>>>(ta, tb, p, s, parts, counters);
+  if (cudaError_t e = launch_overlapped(kern, unsigned(2 * pairs), NUM_THREADS, SMEM_BYTES, 0, stream, ta, tb, p, s, parts, counters); e != cudaSuccess) return e;
   flush_bounds_record(p.status, stream);
   return cudaGetLastError();
 }

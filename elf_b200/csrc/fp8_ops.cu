@@ -103,6 +103,7 @@ template <typename T, Access A>
 __global__ void __launch_bounds__(THREADS) quantize_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ data, long long ldq,
                                                                 uint8_t* __restrict__ scale, long long lds, uint32_t total, uint32_t units_per_row,
                                                                 int cols) {
+  await_previous();
   Raw<T> raw[UNITS];
   uint32_t row[UNITS];
   int col[UNITS], have[UNITS];
@@ -142,6 +143,7 @@ template <typename T, Access A>
 __global__ void __launch_bounds__(THREADS) quantize_tiles_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ data, long long ldq,
                                                                  uint8_t* __restrict__ scale, long long lds, long long rows, int cols) {
   __shared__ uint32_t warp_max[2][THREADS / 32];
+  await_previous();
   const int col = blockIdx.x * BLOCK + (threadIdx.x & 7) * UNIT;
   const long long row0 = (long long)blockIdx.y * BLOCK + (threadIdx.x >> 3);
   const int have_cols = min(cols - col, UNIT);
@@ -208,6 +210,7 @@ template <typename T, Access A>
 __global__ void __launch_bounds__(THREADS) dequantize_kernel(const uint8_t* __restrict__ data, long long ldq, const uint8_t* __restrict__ scale,
                                                              long long lds, int row_shift, T* __restrict__ y, long long ldy, uint32_t total,
                                                              uint32_t units_per_row, long long first_row, int cols) {
+  await_previous();
   uint32_t q[UNITS][UNIT / 4], byte[UNITS];
   long long row[UNITS];
   int col[UNITS], have[UNITS];
@@ -340,6 +343,7 @@ __device__ __forceinline__ void store_normalised(const NormArgs& p, long long ro
 // Rows of up to 1024 values: a warp per row.
 template <int VPT, bool RESIDUAL>
 __global__ void __launch_bounds__(256) rmsnorm_fp8_warp_kernel(const __grid_constant__ NormArgs p) {
+  await_previous();
   const int lane = threadIdx.x & 31;
   const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (row >= p.rows) return;
@@ -373,6 +377,7 @@ __global__ void __launch_bounds__(256) rmsnorm_fp8_warp_kernel(const __grid_cons
 template <int VPT, bool RESIDUAL>
 __global__ void __launch_bounds__(NORM_THREADS, VPT == 4 ? 2 : 1) rmsnorm_fp8_block_kernel(const __grid_constant__ NormArgs p) {
   __shared__ double red[2][NORM_THREADS / 32];
+  await_previous();
   const int t = threadIdx.x;
   uint4 nx[VPT], nr[VPT], gain[VPT];
   auto fetch = [&](long long row) {
@@ -441,10 +446,12 @@ cudaError_t quantize_rows_as(const void* x, long long ldx, uint8_t* data, long l
   for (long long r = 0; r < rows; r += step) {
     const uint32_t total = uint32_t(std::min(step, rows - r)) * upr;
     auto* kern = ELFB_ACCESS(quantize_rows_kernel, T, how);
-    kern<<<(total + UNITS * THREADS - 1) / (UNITS * THREADS), THREADS, 0, stream>>>(static_cast<const T*>(x) + r * ldx, ldx, data + r * ldq, ldq, scale + r * lds, lds, total,
-                                                                  upr, cols);
+    if (cudaError_t e = launch_overlapped(kern, (total + UNITS * THREADS - 1) / (UNITS * THREADS), THREADS, 0, 0, stream, static_cast<const T*>(x) + r * ldx, ldx,
+                                          data + r * ldq, ldq, scale + r * lds, lds, total, upr, cols);
+        e != cudaSuccess)
+      return e;
   }
-  return cudaGetLastError();
+  return cudaSuccess;
 }
 
 template <typename T>
@@ -457,9 +464,12 @@ cudaError_t quantize_tiles_as(const void* x, long long ldx, uint8_t* data, long 
     const long long r = t * BLOCK;
     const dim3 grid((cols + BLOCK - 1) / BLOCK, unsigned(std::min(kGridY, tiles - t)));
     auto* kern = ELFB_ACCESS(quantize_tiles_kernel, T, how);
-    kern<<<grid, THREADS, 0, stream>>>(static_cast<const T*>(x) + r * ldx, ldx, data + r * ldq, ldq, scale + t * lds, lds, rows - r, cols);
+    if (cudaError_t e = launch_overlapped(kern, grid, THREADS, 0, 0, stream, static_cast<const T*>(x) + r * ldx, ldx, data + r * ldq, ldq, scale + t * lds, lds,
+                                          rows - r, cols);
+        e != cudaSuccess)
+      return e;
   }
-  return cudaGetLastError();
+  return cudaSuccess;
 }
 
 template <typename T>
@@ -471,9 +481,12 @@ cudaError_t dequantize_as(const uint8_t* data, long long ldq, const uint8_t* sca
   for (long long r = 0; r < rows; r += step) {
     const uint32_t total = uint32_t(std::min(step, rows - r)) * upr;
     auto* kern = ELFB_ACCESS(dequantize_kernel, T, how);
-    kern<<<(total + UNITS * THREADS - 1) / (UNITS * THREADS), THREADS, 0, stream>>>(data, ldq, scale, lds, row_shift, static_cast<T*>(y), ldy, total, upr, r, cols);
+    if (cudaError_t e = launch_overlapped(kern, (total + UNITS * THREADS - 1) / (UNITS * THREADS), THREADS, 0, 0, stream, data, ldq, scale, lds, row_shift,
+                                          static_cast<T*>(y), ldy, total, upr, r, cols);
+        e != cudaSuccess)
+      return e;
   }
-  return cudaGetLastError();
+  return cudaSuccess;
 }
 
 template <int VPT>
@@ -485,16 +498,15 @@ cudaError_t rmsnorm_warps(const NormArgs& p, cudaStream_t stream) {
     q.rows = std::min(kRows, p.rows - r);
     q.x += r * p.dim8, q.rstd += r, q.data += r * p.ldq, q.scale += r * p.lds;
     if (p.res) q.res += r * p.dim8, q.h += r * p.dim8;
-    kern<<<unsigned((q.rows + 7) / 8), 256, 0, stream>>>(q);
+    if (cudaError_t e = launch_overlapped(kern, unsigned((q.rows + 7) / 8), 256, 0, 0, stream, q); e != cudaSuccess) return e;
   }
-  return cudaGetLastError();
+  return cudaSuccess;
 }
 
 template <int VPT>
 cudaError_t rmsnorm_blocks(const NormArgs& p, int num_sms, cudaStream_t stream) {
   auto* kern = p.res ? rmsnorm_fp8_block_kernel<VPT, true> : rmsnorm_fp8_block_kernel<VPT, false>;
-  kern<<<unsigned(std::min(p.rows, 4ll * num_sms)), NORM_THREADS, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_overlapped(kern, unsigned(std::min(p.rows, 4ll * num_sms)), NORM_THREADS, 0, 0, stream, p);
 }
 
 }  // namespace

@@ -4,6 +4,7 @@
     python benchmarks/kernels.py gemm        # tcgen05 GEMMs vs cuBLAS on the Llama-3-8B layer shapes
     python benchmarks/kernels.py attention   # tcgen05 flash attention forward vs the library SDPA
     python benchmarks/kernels.py fused       # bandwidth of the fused elementwise / norm / loss / optimizer kernels
+    python benchmarks/kernels.py fp8         # 8-bit products, gated block and bandwidth-bound kernels next to the bf16 ones
     python benchmarks/kernels.py one-gemm [fwd|dx|dw] [M N K]   # a few launches of one GEMM (small case for a profiler)
     python benchmarks/kernels.py one-attention [B S Hq Hkv]     # a few launches of the attention forward and backward
     python benchmarks/kernels.py one-fused                      # a few launches of every fused bandwidth-bound kernel
@@ -186,6 +187,53 @@ def bench_fused(args):
     G.check_status(dev)
 
 
+def bench_fp8(args):
+    from elf_b200.ops import fp8
+
+    hbm, burst, _, src = measured_peaks()
+    dev = torch.device("cuda")
+    T, D, FF = 4096, 4096, 14336
+
+    def randn(*shape):
+        return torch.randn(*shape, device=dev, dtype=torch.bfloat16)
+
+    print(f"# 8-bit operators on Llama-3-8B shapes (T={T} tokens), median of {args.rounds} interleaved rounds x {args.iters} launches; 8-bit peak taken as twice the cuBLAS bf16 burst ({2 * burst:.0f} TFLOP/s, {src})")
+    print("| product | 8-bit us | TFLOP/s | fraction of peak | bf16 us | bf16 / 8-bit |")
+    print("|---|---|---|---|---|---|")
+    x, wgu, wd = randn(T, D), randn(2 * FF, D) * 0.02, randn(D, FF) * 0.02
+    xq, wguq, wdq = fp8.quantize(x), fp8.quantize_weight(wgu), fp8.quantize_weight(wd)
+    act, dgu = randn(T, FF), randn(T, 2 * FF) * 1e-3
+    actq, dguq, dyq = fp8.quantize(act), fp8.quantize(dgu), fp8.quantize(x)
+    _, kept = fp8.gated_forward(xq, wguq)[:2]
+    gu = randn(T, 2 * FF)
+    few = fp8.quantize(act[:16])
+    products = {
+        "forward 16x4096x14336": (lambda: fp8.linear_forward(few, wdq), lambda: G.linear_forward(act[:16], wd), 16 * D * FF),
+        "forward 4096x4096x14336": (lambda: fp8.linear_forward(actq, wdq), lambda: G.linear_forward(act, wd), T * D * FF),
+        "gated forward 4096x28672x4096": (lambda: fp8.gated_forward(xq, wguq), lambda: fused.swiglu(G.linear_forward(x, wgu)), 2 * T * D * FF),
+        "gated backward 4096x14336x4096": (lambda: fp8.gated_backward(dyq, wdq, kept), lambda: G.linear_input_grad(x, wd), T * D * FF),
+        "input grad 4096x4096x28672": (lambda: fp8.linear_input_grad(dguq, wguq), lambda: G.linear_input_grad(dgu, wgu), 2 * T * D * FF),
+        "weight grad 28672x4096x4096": (lambda: fp8.linear_weight_grad(dguq, xq), lambda: G.linear_weight_grad(dgu, x), 2 * T * D * FF),
+    }
+    for name, (ours, bf16, mnk) in products.items():
+        t = interleaved({"ours": ours, "bf16": bf16}, args.iters, args.rounds)
+        tf = 2 * mnk / t["ours"] / 1e9
+        print(f"| {name} | {t['ours'] * 1e3:.1f} | {tf:.0f} | {tf / (2 * burst):.2f} | {t['bf16'] * 1e3:.1f} | {t['bf16'] / t['ours']:.2f} |", flush=True)
+    print(f"\n| kernel | bytes per launch | us | GB/s | fraction of {hbm:.0f} GB/s |")
+    print("|---|---|---|---|---|")
+    wn, res = torch.ones(D, device=dev, dtype=torch.bfloat16), randn(T, D)
+    streams = {
+        "quantize 4096x28672": (lambda: fp8.quantize(gu), T * 2 * FF * 3),
+        "quantize weight 28672x4096": (lambda: fp8.quantize_weight(wgu), T * 2 * FF * 3),
+        "dequantize 4096x28672": (lambda: fp8.dequantize(dguq), T * 2 * FF * 3),
+        "add + rms_norm 4096x4096": (lambda: fp8.add_rms_norm(x, res, wn, 1e-5), T * D * 7),
+    }
+    for name, (fn, nbytes) in streams.items():
+        t = interleaved({"k": fn}, args.iters, args.rounds)["k"]
+        print(f"| {name} | {nbytes / 1e6:.0f} MB | {t * 1e3:.1f} | {nbytes / t / 1e6:.0f} | {nbytes / t / 1e6 / hbm:.2f} |", flush=True)
+    G.check_status(dev)
+
+
 def one_gemm(args):
     dev = torch.device("cuda")
     mode = args.rest[0] if args.rest else "fwd"
@@ -255,13 +303,13 @@ def one_fused(args):
 
 def main():
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
-    ap.add_argument("what", choices=["gemm", "attention", "fused", "one-gemm", "one-attention", "one-fused"])
+    ap.add_argument("what", choices=["gemm", "attention", "fused", "fp8", "one-gemm", "one-attention", "one-fused"])
     ap.add_argument("rest", nargs="*")
     ap.add_argument("--iters", type=int, default=10)
     ap.add_argument("--rounds", type=int, default=5)
     args = ap.parse_args()
     _ext.require_on_gpu()
-    {"gemm": bench_gemm, "attention": bench_attention, "fused": bench_fused, "one-gemm": one_gemm, "one-attention": one_attention, "one-fused": one_fused}[args.what](args)
+    {"gemm": bench_gemm, "attention": bench_attention, "fused": bench_fused, "fp8": bench_fp8, "one-gemm": one_gemm, "one-attention": one_attention, "one-fused": one_fused}[args.what](args)
 
 
 if __name__ == "__main__":

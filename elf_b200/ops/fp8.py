@@ -242,7 +242,7 @@ def quantize_weight(w: torch.Tensor) -> BlockScaled:
 
 
 def dequantize(q: BlockScaled, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """The values ``q`` stands for: exact in bf16 and fp32; in fp16 rounded, and infinite above 65504.
+    """The values ``q`` stands for: exact in fp32 and, from 2^-133 up, in bf16; in fp16 rounded, and infinite above 65504.
     ``out``: tensor to write instead of a new one; its last dimension contiguous, its rows evenly spaced."""
     if out is None:
         if dtype not in _FLOATS:
@@ -321,7 +321,8 @@ def _product(a: BlockScaled, b: BlockScaled, transposed: bool, bias, out_dtype) 
 
 def linear_forward(x: BlockScaled, w: BlockScaled, bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``x W^T (+ bias)`` for ``x [..., K]`` scaled by rows and ``w [N, K]`` scaled by tiles or rows; accumulated in
-    fp32 and rounded once."""
+    fp32 and rounded once.  On the GPU a bias of another type is taken in ``out_dtype``, the type a layer of that type holds
+    it in."""
     _check_product(x, w, 1, "linear_forward")
     if not (bias is None or (bias.shape == (w.shape[0],) and bias.device == w.device)):
         raise ValueError("linear_forward: the bias must be a vector with one element per output")
@@ -350,6 +351,8 @@ def linear_weight_grad(dy: Union[BlockScaled, torch.Tensor], x: Union[BlockScale
     n, k = dy.shape[-1], x.shape[-1]
     if dy.shape[:-1].numel() != x.shape[:-1].numel():
         raise ValueError("linear_weight_grad: dy and x have different numbers of rows")
+    if any(isinstance(t, BlockScaled) and t.block_rows != 1 for t in (dy, x)):
+        raise ValueError("linear_weight_grad: activations and gradients must be scaled by rows")
     _same_device("dy", dy, "x", x)
     if not (out is None or (out.shape == (n, k) and out.device == x.device and out.dtype in (torch.bfloat16, torch.float32))):
         raise ValueError(f"linear_weight_grad: out must be a bf16 or fp32 matrix [{n}, {k}]")
@@ -466,7 +469,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
 
 def _ffn_forward(x: torch.Tensor, gate_up_q: BlockScaled, down_q: BlockScaled, keep: bool):
     """``(y, [x, act, gate_up])``: the output and, with ``keep``, values and scales of what the backward needs."""
-    if x.numel() and _on_kernels(x):
+    if x.numel() and down_q.numel() and _on_kernels(x):
         y, *kept = _ext.get().fp8_ffn(x, gate_up_q.data, gate_up_q.scale, down_q.data, down_q.scale, keep, _gemm.status(x.device))
         return y, kept
     xq = quantize(x)
@@ -497,7 +500,7 @@ class _GatedFFN(torch.autograd.Function):
             rest = rest[n:]
         gate_up_q, down_q = copies
         need = list(ctx.needs_input_grad[:3])
-        if dy.numel() and down_q.numel() and _on_kernels(dy):
+        if dy.numel() and gate_up_q.numel() and down_q.numel() and _on_kernels(dy):
             grads = _ext.get().fp8_ffn_bwd(dy, list(kept), gate_up_q.data, gate_up_q.scale, down_q.data, down_q.scale, need, list(ctx.dtypes),
                                            _gemm.status(dy.device), _gemm._VARIANT, _gemm._SPLIT_TAIL)
             return (*grads, None, None)

@@ -146,6 +146,8 @@ def test_refusals():
         fp8.linear_input_grad(fp8.quantize(rand(4, 256)), fp8.quantize(rand(256, 200)))
     with pytest.raises(ValueError, match="numbers of rows"):
         fp8.linear_weight_grad(q, fp8.quantize(rand(5, 8)))
+    with pytest.raises(ValueError, match="scaled by rows"):
+        fp8.linear_weight_grad(w, fp8.quantize(rand(256, 8)))
     with pytest.raises(ValueError, match="out must be"):
         fp8.linear_weight_grad(q, q, out=torch.zeros(200, 199))
     with pytest.raises(ValueError, match="multiple of 128"):
@@ -166,6 +168,15 @@ def test_refusals():
         fp8.add_rms_norm(rand(4, 16), rand(4, 8), torch.ones(16))
     with pytest.raises(ValueError, match="on one device"):
         fp8.linear(rand(4, 16), torch.empty(8, 16, device="meta"))
+
+
+@pytest.mark.parametrize("m,d,f,out", [(0, 16, 128, 8), (3, 0, 128, 8), (3, 16, 0, 8), (3, 16, 128, 0)])
+def test_gated_ffn_without_elements(m, d, f, out):
+    x, wg, wd = (torch.randn(*s, requires_grad=True) for s in ((m, d), (2 * f, d), (out, f)))
+    y = fp8.gated_ffn(x, wg, wd)
+    assert y.shape == (m, out) and (not y.any() or (d and f))
+    for g, t in zip(torch.autograd.grad(y.sum(), (x, wg, wd)), (x, wg, wd)):
+        assert g.shape == t.shape and not g.isnan().any()
 
 
 # ------------------------------------------------------------------------------ split-backward layer

@@ -185,6 +185,54 @@ def test_two_streams_at_once(dev):
         assert all(torch.equal(t, w) for t in g)
 
 
+def test_captured_with_a_fork(dev):
+    """One captured stream forks into two and joins; kernels at the fork and behind the join."""
+    from elf_b200.ops import fp8
+
+    x, w = operands(2304, 2304, 14336, dev, 3)
+    small = activations(300, 640, torch.bfloat16, dev)
+
+    def work(fork):
+        a = fp8.quantize(small)
+        main = torch.cuda.current_stream(dev)
+        if fork:
+            side.wait_stream(main)
+        with torch.cuda.stream(side if fork else main):
+            b = fp8.linear_forward(x, w)
+            b = fp8.quantize(b)
+        c = fp8.dequantize(a)
+        if fork:
+            main.wait_stream(side)
+        return fp8.dequantize(b), fp8.dequantize(fp8.quantize(c))
+
+    side = torch.cuda.Stream(dev)
+    want = work(False)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work(True)
+    for _ in range(3):
+        for t in got:
+            t.fill_(7)
+        graph.replay()
+        assert all(torch.equal(g, w_) for g, w_ in zip(got, want))
+
+
+@pytest.mark.parametrize("m,d,f,out", [(0, 16, 128, 8), (3, 0, 128, 8), (3, 16, 0, 8), (3, 16, 128, 0)])
+def test_gated_ffn_without_elements(dev, m, d, f, out):
+    from elf_b200.ops import fp8
+
+    spoilt = torch.full((64,), float("nan"), device=dev)  # what a result that nobody writes would be made of
+    del spoilt
+    x, wg, wd = (torch.randn(*s, device=dev, dtype=torch.bfloat16, requires_grad=True) for s in ((m, d), (2 * f, d), (out, f)))
+    y = fp8.gated_ffn(x, wg, wd)
+    assert y.shape == (m, out) and not y.isnan().any() and (not y.any() or (d and f))
+    with torch.no_grad():
+        assert torch.equal(fp8.gated_ffn(x, wg, wd), y)
+    for g, t in zip(torch.autograd.grad(y.sum(), (x, wg, wd)), (x, wg, wd)):
+        assert g.shape == t.shape and not g.isnan().any()
+
+
 def test_captured_and_replayed(dev):
     """Forward and backward of the block in one graph, a split product in another, replayed in turn with new inputs."""
     from elf_b200.ops import fp8

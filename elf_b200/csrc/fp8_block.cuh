@@ -46,6 +46,39 @@ __device__ __forceinline__ float mul_exact(float a, float b) {
   return r;
 }
 
+// Two fp32 operations in one instruction, on a pair in a 64-bit register; subnormal numbers survive.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 halves(uint64_t p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2_towards_zero(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rz.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// larger magnitude of the two (the sign is arbitrary), NaN if either is
+__device__ __forceinline__ float larger_magnitude(float a, float b) {
+  float r;
+  asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 constexpr uint32_t kInfBits = 0x7f800000u;
 
 // Exponent byte of a block whose largest finite magnitude has the bits `amax` (an fp32 pattern):
@@ -93,35 +126,41 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v) {
   return v;
 }
 
-// Scales and converts the N values a lane holds of a 128-column block shared by W consecutive lanes
-// (all 32 lanes of the warp call this).  Returns the block's exponent byte.  Blocks without
-// infinities and NaN, practically all, take the branch without per-value tests.
-template <int N, int W>
-__device__ __forceinline__ uint32_t quantize_block(const float (&v)[N], uint32_t (&out)[N / 4]) {
-  uint32_t m = 0;
+template <int N>
+__device__ __forceinline__ void scaled_to_e4m3(const float (&v)[N], float inv, uint32_t (&out)[N / 4]) {
+  const uint64_t inv2 = pair_of(inv, inv);
 #pragma unroll
-  for (int j = 0; j < N; ++j) m = max(m, abs_bits(v[j]));
-  m = group_max<W>(m);
-  const bool odd = m >= kInfBits;
-  if (__any_sync(0xffffffffu, odd)) {
+  for (int j = 0; j < N / 4; ++j) {
+    const float2 a = halves(mul2(pair_of(v[4 * j], v[4 * j + 1]), inv2)), b = halves(mul2(pair_of(v[4 * j + 2], v[4 * j + 3]), inv2));
+    out[j] = to_e4m3x4(a.x, a.y, b.x, b.y);
+  }
+}
+template <int N>
+__device__ __forceinline__ void scaled_to_e4m3_odd(const float (&v)[N], float inv, uint32_t (&out)[N / 4]) {  // with infinities or NaN
+#pragma unroll
+  for (int j = 0; j < N / 4; ++j) {
+    float s[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s[k] = nan_unless_finite(mul_exact(v[4 * j + k], inv), v[4 * j + k]);
+    out[j] = to_e4m3x4(s[0], s[1], s[2], s[3]);
+  }
+}
+// Scales and converts the N values a lane holds of a 128-column block shared by W consecutive lanes (all 32 lanes of
+// the warp call this); `top` is the largest magnitude among the lane's values.  Returns the block's exponent byte.
+// Blocks without infinities and NaN, practically all, take the branch without per-value tests.
+template <int N, int W>
+__device__ __forceinline__ uint32_t quantize_block(const float (&v)[N], uint32_t top, uint32_t (&out)[N / 4]) {
+  top = group_max<W>(top);
+  if (__any_sync(0xffffffffu, top >= kInfBits)) {
     uint32_t f = 0;
 #pragma unroll
     for (int j = 0; j < N; ++j) f = max(f, finite_bits(v[j]));
-    f = group_max<W>(f);
-    const uint32_t byte = block_exponent(f);
-    const float inv = inverse_exponent_value(byte);
-    float s[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) s[j] = nan_unless_finite(mul_exact(v[j], inv), v[j]);
-#pragma unroll
-    for (int j = 0; j < N / 4; ++j) out[j] = to_e4m3x4(s[4 * j], s[4 * j + 1], s[4 * j + 2], s[4 * j + 3]);
+    const uint32_t byte = block_exponent(group_max<W>(f));
+    scaled_to_e4m3_odd(v, inverse_exponent_value(byte), out);
     return byte;
   }
-  const uint32_t byte = block_exponent(m);
-  const float inv = inverse_exponent_value(byte);
-#pragma unroll
-  for (int j = 0; j < N / 4; ++j)
-    out[j] = to_e4m3x4(mul_exact(v[4 * j], inv), mul_exact(v[4 * j + 1], inv), mul_exact(v[4 * j + 2], inv), mul_exact(v[4 * j + 3], inv));
+  const uint32_t byte = block_exponent(top);
+  scaled_to_e4m3(v, inverse_exponent_value(byte), out);
   return byte;
 }
 

@@ -4,6 +4,7 @@
 #include "fp8_ops.h"
 
 #include <algorithm>
+#include <type_traits>
 
 #include "fp8_block.cuh"
 #include "sm100_ptx.cuh"
@@ -16,6 +17,7 @@ constexpr int BLOCK = 128;  // columns that share a scale
 constexpr int UNIT = 16;    // consecutive values a thread holds: 8 lanes make up a block
 constexpr int THREADS = 256;
 constexpr int NORM_THREADS = 256;
+constexpr int TILE_THREADS = 512;
 constexpr int UNITS = 2;    // groups of 16 values per thread of the streaming kernels
 
 __device__ __forceinline__ float to_float(float v) { return v; }
@@ -70,6 +72,25 @@ __device__ __forceinline__ void unpack(const Raw<T>& r, float (&v)[UNIT]) {
 #pragma unroll
   for (int j = 0; j < UNIT; ++j) v[j] = to_float(e[j]);
 }
+// Largest magnitude as the bits of an fp32 number, those of infinity or more if a value is not finite.  16-bit values are
+// compared two at a time, as integers.
+template <typename T>
+__device__ __forceinline__ uint32_t largest(const Raw<T>& r) {
+  uint32_t top = 0;
+#pragma unroll
+  for (const uint4& q : r.q) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (sizeof(T) == 4) top = max(top, w[j] & 0x7fffffffu);
+      else top = __vmaxu2(top, w[j] & 0x7fff7fffu);
+    }
+  }
+  if constexpr (sizeof(T) == 4) return top;
+  const uint32_t m = max(top >> 16, top & 0xffffu);
+  if constexpr (std::is_same<T, __half>::value) return m >= 0x7c00u ? kInfBits : __float_as_uint(__half2float(__ushort_as_half(uint16_t(m))));
+  else return m << 16;
+}
 template <typename T, Access A>
 __device__ __forceinline__ void store_values(T* p, int have, const float (&v)[UNIT]) {
   constexpr int N = UNIT * sizeof(T) / 16;
@@ -98,7 +119,7 @@ __device__ __forceinline__ void store_bytes_ragged(uint8_t* p, int have, const u
 // ------------------------------------------------------------------------------ quantise
 // A thread takes two groups of 16 values, 256 groups apart, and loads both before it looks at either; the 8 lanes
 // of a block find its maximum with three shuffles.  Bound by memory: 4096 x 28672 bf16 (353 MB read and written)
-// 57 us, 6.2 TB/s.
+// 51 us, 6.9 TB/s.
 template <typename T, Access A>
 __global__ void __launch_bounds__(THREADS) quantize_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ data, long long ldq,
                                                                 uint8_t* __restrict__ scale, long long lds, uint32_t total, uint32_t units_per_row,
@@ -125,7 +146,7 @@ __global__ void __launch_bounds__(THREADS) quantize_rows_kernel(const T* __restr
     float v[UNIT];
     unpack<T>(raw[i], v);
     uint32_t q[UNIT / 4];
-    const uint32_t byte = quantize_block<UNIT, 8>(v, q);
+    const uint32_t byte = quantize_block<UNIT, 8>(v, largest(raw[i]), q);
     if (have[i] > 0) {
       uint8_t* dst = data + (long long)row[i] * ldq + col[i];
       if constexpr (A != Access::kRagged)
@@ -137,63 +158,65 @@ __global__ void __launch_bounds__(THREADS) quantize_rows_kernel(const T* __restr
   }
 }
 
-// One block of threads per 128 x 128 tile: every thread holds four groups of 16 values (rows 32
-// apart), so the tile is read once.
+// One block of threads per 128 x 128 tile: every thread holds two groups of 16 values (64 rows apart), so the tile is
+// read once.  Bound by memory: 28672 x 4096 bf16 (353 MB) 65 us, 5.4 TB/s; with 256 threads of four groups, one block to an
+// SM, 129.
 template <typename T, Access A>
-__global__ void __launch_bounds__(THREADS) quantize_tiles_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ data, long long ldq,
+__global__ void __launch_bounds__(TILE_THREADS, 2) quantize_tiles_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ data, long long ldq,
                                                                  uint8_t* __restrict__ scale, long long lds, long long rows, int cols) {
-  __shared__ uint32_t warp_max[2][THREADS / 32];
+  __shared__ uint32_t warp_max[TILE_THREADS / 32];
   await_previous();
   const int col = blockIdx.x * BLOCK + (threadIdx.x & 7) * UNIT;
   const long long row0 = (long long)blockIdx.y * BLOCK + (threadIdx.x >> 3);
   const int have_cols = min(cols - col, UNIT);
-  float v[4][UNIT];
-  uint32_t any = 0, finite = 0;
+  constexpr int GROUPS = BLOCK * BLOCK / UNIT / TILE_THREADS, STEP = BLOCK / GROUPS;
+  Raw<T> raw[GROUPS];  // all loads are issued before the first is looked at
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const long long row = row0 + 32 * i;
+  for (int i = 0; i < GROUPS; ++i) {
+    const long long row = row0 + STEP * i;
     if (have_cols > 0 && row < rows) {
-      Raw<T> raw;
-      load_raw<T, A>(x + row * ldx + col, have_cols, raw);
-      unpack<T>(raw, v[i]);
+      load_raw<T, A>(x + row * ldx + col, have_cols, raw[i]);
     } else {
 #pragma unroll
-      for (int j = 0; j < UNIT; ++j) v[i][j] = 0.f;
-    }
-#pragma unroll
-    for (int j = 0; j < UNIT; ++j) {
-      any = max(any, abs_bits(v[i][j]));
-      finite = max(finite, finite_bits(v[i][j]));
+      for (uint4& q : raw[i].q) q = make_uint4(0, 0, 0, 0);
     }
   }
-  any = group_max<32>(any);
-  finite = group_max<32>(finite);
-  if ((threadIdx.x & 31) == 0) {
-    warp_max[0][threadIdx.x >> 5] = any;
-    warp_max[1][threadIdx.x >> 5] = finite;
-  }
-  __syncthreads();
-  any = finite = 0;
+  uint32_t top = 0;
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) {
-    any = max(any, warp_max[0][w]);
-    finite = max(finite, warp_max[1][w]);
+  for (int i = 0; i < GROUPS; ++i) top = max(top, largest(raw[i]));
+  auto tile_max = [&](uint32_t m) {
+    m = group_max<32>(m);
+    if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < TILE_THREADS / 32; ++w) m = max(m, warp_max[w]);
+    return m;
+  };
+  top = tile_max(top);
+  const bool odd = top >= kInfBits;
+  if (odd) {  // the largest of the finite values counts
+    top = 0;
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) {
+      float v[UNIT];
+      unpack<T>(raw[i], v);
+#pragma unroll
+      for (int j = 0; j < UNIT; ++j) top = max(top, finite_bits(v[j]));
+    }
+    __syncthreads();
+    top = tile_max(top);
   }
-  const uint32_t byte = block_exponent(finite);
+  const uint32_t byte = block_exponent(top);
   const float inv = inverse_exponent_value(byte);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const long long row = row0 + 32 * i;
+  for (int i = 0; i < GROUPS; ++i) {
+    const long long row = row0 + STEP * i;
     if (have_cols <= 0 || row >= rows) continue;
-    float s[UNIT];
-#pragma unroll
-    for (int j = 0; j < UNIT; ++j) {
-      s[j] = mul_exact(v[i][j], inv);
-      if (any >= kInfBits) s[j] = nan_unless_finite(s[j], v[i][j]);
-    }
+    float v[UNIT];
+    unpack<T>(raw[i], v);
     uint32_t q[UNIT / 4];
-#pragma unroll
-    for (int j = 0; j < UNIT / 4; ++j) q[j] = to_e4m3x4(s[4 * j], s[4 * j + 1], s[4 * j + 2], s[4 * j + 3]);
+    if (odd) scaled_to_e4m3_odd(v, inv, q);
+    else scaled_to_e4m3(v, inv, q);
     uint8_t* dst = data + row * ldq + col;
     if constexpr (A != Access::kRagged)
       *reinterpret_cast<uint4*>(dst) = make_uint4(q[0], q[1], q[2], q[3]);
@@ -205,7 +228,7 @@ __global__ void __launch_bounds__(THREADS) quantize_tiles_kernel(const T* __rest
 
 // ------------------------------------------------------------------------------ restore
 // value = data 2^(byte - 127), exact in fp32, one rounding where the output has fewer bits.  Units as above.  Bound by
-// memory: 4096 x 28672 to bf16 (353 MB) 50 us, 7.0 TB/s of which L2 keeps a part.
+// memory: 4096 x 28672 to bf16 (353 MB) 53 us, 6.6 TB/s.
 template <typename T, Access A>
 __global__ void __launch_bounds__(THREADS) dequantize_kernel(const uint8_t* __restrict__ data, long long ldq, const uint8_t* __restrict__ scale,
                                                              long long lds, int row_shift, T* __restrict__ y, long long ldy, uint32_t total,
@@ -287,21 +310,41 @@ struct NormArgs {
 // carried as two floats (one Newton step in 64 bits from the fp32 root), and the product rounded to odd: the last bit
 // says that something was cut off, and the rounding to e4m3 is that of the exact product.
 //
-// What each addition to the sum cuts off is computed exactly and added up beside it: Kahan's shorter chain, which
-// rounds the next square together with the correction, left errors of 1e-9, enough for one value in 10^8.
+// The sum starts from a power of two B above all it will hold, so it stays in [B, 2B) and what an addition cuts off its
+// square is exact: square - (new sum - old sum).  Those rests add up beside it.  (Kahan's sum rounds the next square
+// together with the correction: errors of 1e-9, enough to move one value in 10^8.)
 template <int N>
 __device__ __forceinline__ double square_sum(const float (&v)[N][8]) {
-  float sum = 0.f, cut = 0.f;
+  float top = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float sq = v[i][j] * v[i][j];  // exact: v has 8 significant bits
-      const float t = sum + sq, added = t - sum;
-      cut += (sum - (t - added)) + (sq - added);
+    for (int j = 0; j < 8; ++j) top = larger_magnitude(top, v[i][j]);
+  // |v| < 2^(e + 1), the N * 8 <= 32 squares of a thread < 2^(2 e + 7)
+  const int e = int(abs_bits(top) >> 23) - 127;
+  if (e < -50 || e > 58) {  // far from everyday values: in 64 bits
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum = fma(double(v[i][j]), double(v[i][j]), sum);
+    return sum;
+  }
+  const float base = __uint_as_float(uint32_t(2 * e + 7 + 127) << 23);
+  uint64_t sum = pair_of(base, base), rest = pair_of(0.f, 0.f);  // of even and of odd columns
+  const uint64_t minus_one = pair_of(-1.f, -1.f);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      const uint64_t x = pair_of(v[i][j], v[i][j + 1]);
+      const uint64_t t = fma2(x, x, sum);
+      const uint64_t cut = fma2(x, x, fma2(t, minus_one, sum));
+      rest = fma2(cut, pair_of(1.f, 1.f), rest);
       sum = t;
     }
-  return isfinite(sum) ? double(sum) + double(cut) : double(sum);
+  const float2 s = halves(sum), r = halves(rest);
+  return (double(s.x - base) + double(s.y - base)) + double(r.x + r.y);
 }
 struct InverseRms {
   float hi, lo;
@@ -324,16 +367,28 @@ __device__ __forceinline__ double warp_sum(double v) {
 __device__ __forceinline__ void store_normalised(const NormArgs& p, long long row, int c, bool live, const float (&v)[8], uint4 gain, InverseRms rs) {
   float g[8], y[8];
   unpack8(gain, g);
+  const uint64_t hi = pair_of(rs.hi, rs.hi), lo = pair_of(rs.lo, rs.lo);
+  float top = 0.f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float t = v[j] * g[j];  // exact: both have 8 significant bits
-    const float tail = t * rs.lo;
-    float q = __fmaf_rz(t, rs.hi, tail);
-    if (fmaf(t, rs.hi, -q) + tail != 0.f) q = __uint_as_float(__float_as_uint(q) | 1u);
-    y[j] = q;
+  for (int j = 0; j < 8; j += 2) {
+    const uint64_t t = mul2(pair_of(v[j], v[j + 1]), pair_of(g[j], g[j + 1]));  // exact: both have 8 significant bits
+    float2 q;
+    if (rs.lo != 0.f) {  // hi + lo has more than 24 bits, its product with any t but 0 as well
+      q = halves(fma2_towards_zero(t, hi, mul2(t, lo)));
+      q.x = __uint_as_float(__float_as_uint(q.x) | 1u);
+      q.y = __uint_as_float(__float_as_uint(q.y) | 1u);
+    } else {
+      const float2 s = halves(t);
+      q.x = __fmul_rz(s.x, rs.hi);
+      q.y = __fmul_rz(s.y, rs.hi);
+      if (fmaf(s.x, rs.hi, -q.x) != 0.f) q.x = __uint_as_float(__float_as_uint(q.x) | 1u);
+      if (fmaf(s.y, rs.hi, -q.y) != 0.f) q.y = __uint_as_float(__float_as_uint(q.y) | 1u);
+    }
+    y[j] = q.x, y[j + 1] = q.y;
+    top = larger_magnitude(top, larger_magnitude(q.x, q.y));
   }
   uint32_t q[2];
-  const uint32_t byte = quantize_block<8, 16>(y, q);
+  const uint32_t byte = quantize_block<8, 16>(y, abs_bits(top), q);
   if (live && c < p.dim8) {
     *reinterpret_cast<uint2*>(p.data + row * p.ldq + c * 8) = make_uint2(q[0], q[1]);
     if ((c & 15) == 0) p.scale[row * p.lds + c / 16] = uint8_t(byte);
@@ -370,12 +425,15 @@ __global__ void __launch_bounds__(256) rmsnorm_fp8_warp_kernel(const __grid_cons
   }
 }
 
-// Wider rows: a block per row, four blocks per SM that walk the rows; the next row's loads are issued before the
-// current one is reduced.  4096 x 4096 with residual (117 MB): 24 us, 75 % of the copy bandwidth; one block per row
-// without the walk 29.6 us; 128 or 512 threads per row 27 us; a ring of rows in shared memory filled by bulk copies
-// 27 us (the time goes into the two dependent sweeps of a row, not into too few bytes in flight).
+// Wider rows: a block per row, as many blocks as fit an SM, which walk the rows; the next row's loads are issued before
+// the current one is reduced.  4096 x 4096 with residual (117 MB): 23 us, 78 % of the copy bandwidth, and 18 without (84 MB,
+// 72 %).  What bounds it is instructions as much as bytes: one fp32 operation at a time instead of pairs 26 us; two or
+// four blocks per SM (four spill registers) 24 and 29; 128 or 512 threads per row, or a ring of rows in shared memory
+// filled by bulk copies, 3 us more when that was 24.
+template <int VPT>
+constexpr int NORM_BLOCKS = VPT == 1 ? 4 : VPT == 2 ? 3 : 2;  // per SM
 template <int VPT, bool RESIDUAL>
-__global__ void __launch_bounds__(NORM_THREADS, VPT == 4 ? 2 : 1) rmsnorm_fp8_block_kernel(const __grid_constant__ NormArgs p) {
+__global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS<VPT>) rmsnorm_fp8_block_kernel(const __grid_constant__ NormArgs p) {
   __shared__ double red[2][NORM_THREADS / 32];
   await_previous();
   const int t = threadIdx.x;
@@ -464,7 +522,7 @@ cudaError_t quantize_tiles_as(const void* x, long long ldx, uint8_t* data, long 
     const long long r = t * BLOCK;
     const dim3 grid((cols + BLOCK - 1) / BLOCK, unsigned(std::min(kGridY, tiles - t)));
     auto* kern = ELFB_ACCESS(quantize_tiles_kernel, T, how);
-    if (cudaError_t e = launch_overlapped(kern, grid, THREADS, 0, 0, stream, static_cast<const T*>(x) + r * ldx, ldx, data + r * ldq, ldq, scale + t * lds, lds,
+    if (cudaError_t e = launch_overlapped(kern, grid, TILE_THREADS, 0, 0, stream, static_cast<const T*>(x) + r * ldx, ldx, data + r * ldq, ldq, scale + t * lds, lds,
                                           rows - r, cols);
         e != cudaSuccess)
       return e;
@@ -506,7 +564,7 @@ cudaError_t rmsnorm_warps(const NormArgs& p, cudaStream_t stream) {
 template <int VPT>
 cudaError_t rmsnorm_blocks(const NormArgs& p, int num_sms, cudaStream_t stream) {
   auto* kern = p.res ? rmsnorm_fp8_block_kernel<VPT, true> : rmsnorm_fp8_block_kernel<VPT, false>;
-  return launch_overlapped(kern, unsigned(std::min(p.rows, 4ll * num_sms)), NORM_THREADS, 0, 0, stream, p);
+  return launch_overlapped(kern, unsigned(std::min(p.rows, (long long)NORM_BLOCKS<VPT> * num_sms)), NORM_THREADS, 0, 0, stream, p);
 }
 
 }  // namespace

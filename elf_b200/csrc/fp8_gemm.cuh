@@ -159,15 +159,15 @@ __device__ __forceinline__ void store_32_bytes(uint8_t* p, const uint32_t (&v)[8
 // N values times 2^(127 - byte) to e4m3.  ODD: some may not be finite and become NaN; without it that costs nothing.
 template <int N, bool ODD>
 __device__ __forceinline__ void to_scaled_e4m3(const float* v, float inv, uint32_t* q) {
+  const uint64_t inv2 = pair_of(inv, inv);
 #pragma unroll
   for (int j = 0; j < N / 4; ++j) {
-    float s[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      s[k] = mul_exact(v[4 * j + k], inv);
-      if (ODD) s[k] = nan_unless_finite(s[k], v[4 * j + k]);
+    float2 a = halves(mul2(pair_of(v[4 * j], v[4 * j + 1]), inv2)), b = halves(mul2(pair_of(v[4 * j + 2], v[4 * j + 3]), inv2));
+    if (ODD) {
+      a = make_float2(nan_unless_finite(a.x, v[4 * j]), nan_unless_finite(a.y, v[4 * j + 1]));
+      b = make_float2(nan_unless_finite(b.x, v[4 * j + 2]), nan_unless_finite(b.y, v[4 * j + 3]));
     }
-    q[j] = to_e4m3x4(s[0], s[1], s[2], s[3]);
+    q[j] = to_e4m3x4(a.x, a.y, b.x, b.y);
   }
 }
 template <int N, bool ODD>
@@ -179,11 +179,19 @@ __device__ __forceinline__ void scale_and_store(const float* v, float inv, uint8
     store_32_bytes(dst + 32 * c, q);
   }
 }
+// largest magnitude as fp32 bits; ODD: of the values that are finite, otherwise infinity or more if one is not
 template <int N, bool ODD>
-__device__ __forceinline__ uint32_t magnitude(const float* v, uint32_t top = 0) {  // of those that are finite
+__device__ __forceinline__ uint32_t magnitude(const float* v, uint32_t top = 0) {
+  if constexpr (ODD) {
 #pragma unroll
-  for (int j = 0; j < N; ++j) top = max(top, ODD ? finite_bits(v[j]) : abs_bits(v[j]));
-  return top;
+    for (int j = 0; j < N; ++j) top = max(top, finite_bits(v[j]));
+    return top;
+  } else {
+    float m[4] = {__uint_as_float(top), 0.f, 0.f, 0.f};  // four short chains
+#pragma unroll
+    for (int j = 0; j < N; ++j) m[j % 4] = larger_magnitude(m[j % 4], v[j]);
+    return abs_bits(larger_magnitude(larger_magnitude(m[0], m[1]), larger_magnitude(m[2], m[3])));
+  }
 }
 
 // The layout tcgen05.cp wants: 16 bytes per lane, word j for row 32 j + lane.

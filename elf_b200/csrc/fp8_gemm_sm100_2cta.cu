@@ -139,6 +139,13 @@ __device__ __forceinline__ bool umma_x4_then_ready(uint32_t tmem_d, uint64_t des
       : "memory");
   return ready != 0;
 }
+constexpr float kLog2e = 1.4426950408889634f;
+// sigmoid of two values given times -log2(e)
+__device__ __forceinline__ uint64_t sigmoid2(uint64_t x) {
+  const float2 a = halves(x);
+  const float2 b = halves(fma2(pair_of(exp2f(a.x), exp2f(a.y)), pair_of(1.f, 1.f), pair_of(1.f, 1.f)));
+  return pair_of(__fdividef(1.f, b.x), __fdividef(1.f, b.y));
+}
 // One tile of the gated form: columns 0..127 of the accumulator are gate, 128..255 up.  A thread takes 64 columns
 // of gate and the same of up of one row into registers and gives the accumulator back at once; the maxima of the
 // three blocks (gate, up, activation) are exchanged with the thread that has the row's other half.
@@ -189,7 +196,11 @@ __device__ __forceinline__ void gated_tile(uint32_t taddr, int row, int half, in
     }
   }
 #pragma unroll
-  for (int j = 0; j < 64; ++j) g[j] = g[j] * __fdividef(1.f, 1.f + __expf(-g[j])) * u[j];
+  for (int j = 0; j < 64; j += 2) {
+    const uint64_t g2 = pair_of(g[j], g[j + 1]);
+    const float2 a = halves(mul2(mul2(g2, sigmoid2(mul2(g2, pair_of(-kLog2e, -kLog2e)))), pair_of(u[j], u[j + 1])));
+    g[j] = a.x, g[j + 1] = a.y;
+  }
   uint32_t top = magnitude<64, false>(g);
   const bool odd = any(top >= kInfBits);
   if (odd) top = magnitude<64, true>(g);
@@ -210,9 +221,10 @@ __device__ __forceinline__ void gated_tile(uint32_t taddr, int row, int half, in
 // hold.  The checkpoint is read and the result written 32 bytes at a time, whole sectors of a row that is one
 // thread's own: 16-byte accesses cost 40 us more.
 //
-// 4096 x 14336 x 4096: 283 us (180 without this epilogue, 142 at the 8-bit peak); the epilogue of a tile outlasts the
-// next tile's MMAs.  Its arithmetic alone beside the MMAs takes 243, loads and stores with next to no arithmetic
-// 273, one sweep 250.  Neither 16 epilogue warps (289) nor fetching the next tile's checkpoint into L2 (291) helped.
+// 4096 x 14336 x 4096: 264 us (180 without this epilogue, 142 at the 8-bit peak); the epilogue of a tile outlasts the
+// next tile's MMAs.  Before its arithmetic went by pairs it took 283: arithmetic alone beside the MMAs 243, loads and
+// stores with next to no arithmetic 273, one sweep 250.  Neither 16 epilogue warps (289) nor fetching the next tile's
+// checkpoint into L2 (291) helped.
 //
 // With t = d s and the scales sg, su of gate and up taken out of the sums (powers of two: exact),
 //   dup = sg (t gate_q),  dgate = su (up_q (t + t gate_q sg (1 - s))).
@@ -222,17 +234,15 @@ struct GateScales {
 };
 // dup / sg and dgate / su for 16 columns
 __device__ __forceinline__ void gated_grad(const uint32_t* d, const uint32_t* gq, const uint32_t* uq, GateScales c, float (&dg)[16], float (&du)[16]) {
+  const uint64_t sg = pair_of(c.sg, c.sg), minus_sg = pair_of(-c.sg, -c.sg), log2e = pair_of(c.log2e, c.log2e);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float2 g2 = from_e4m3x2((gq[j / 2] >> (16 * (j & 1))) & 0xffffu), u2 = from_e4m3x2((uq[j / 2] >> (16 * (j & 1))) & 0xffffu);
-    const float g[2] = {g2.x, g2.y}, up[2] = {u2.x, u2.y};
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const float sig = __fdividef(1.f, 1.f + exp2f(g[k] * c.log2e));
-      const float t = __uint_as_float(d[2 * j + k]) * sig;
-      du[2 * j + k] = t * g[k];
-      dg[2 * j + k] = up[k] * fmaf(t * g[k], fmaf(-sig, c.sg, c.sg), t);
-    }
+    const uint64_t g = pair_of(g2.x, g2.y), sig = sigmoid2(mul2(g, log2e));
+    const uint64_t t = mul2(pair_of(__uint_as_float(d[2 * j]), __uint_as_float(d[2 * j + 1])), sig), tg = mul2(t, g);
+    const float2 a = halves(mul2(pair_of(u2.x, u2.y), fma2(tg, fma2(sig, minus_sg, sg), t))), b = halves(tg);
+    dg[2 * j] = a.x, dg[2 * j + 1] = a.y;
+    du[2 * j] = b.x, du[2 * j + 1] = b.y;
   }
 }
 template <typename Release>
@@ -254,7 +264,7 @@ __device__ __forceinline__ void gated_backward_tile(uint32_t taddr, int acc, int
   const uint8_t* gate = p.gu + r * p.ld_gu + c0;
   const uint8_t* scales = p.gu_scale + r * p.ld_gu_scale + c0 / 128;
   const float sg = exponent_value(scales[0]), su = exponent_value(scales[f / 128]);
-  const GateScales gs{sg, -1.4426950408889634f * sg};
+  const GateScales gs{sg, -kLog2e * sg};
   uint8_t* dst = p.act + r * p.ld_act + c0;
   // calls handle(d, gate_q, up_q, chunk) for the row's four chunks, the checkpoint of the next one on its way
   auto sweep = [&](auto&& handle) {
@@ -320,7 +330,11 @@ __device__ __forceinline__ void gated_backward_tile(uint32_t taddr, int acc, int
         float dg[16], du[16];
         gated_grad(d + 16 * h, g + 4 * h, u + 4 * h, gs, dg, du);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) dg[j] = mul_exact(dg[j], su), du[j] = mul_exact(du[j], sg);
+        for (int j = 0; j < 16; j += 2) {
+          const float2 a = halves(mul2(pair_of(dg[j], dg[j + 1]), pair_of(su, su))), b = halves(mul2(pair_of(du[j], du[j + 1]), pair_of(sg, sg)));
+          dg[j] = a.x, dg[j + 1] = a.y;
+          du[j] = b.x, du[j + 1] = b.y;
+        }
         to_scaled_e4m3<16, ODD>(dg, inv_g, qg + 4 * h);
         to_scaled_e4m3<16, ODD>(du, inv_u, qu + 4 * h);
       }

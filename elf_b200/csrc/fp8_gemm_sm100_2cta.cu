@@ -564,7 +564,7 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
               tmem_ld_32x32b_x32(taddr + c * 32, v);
               tmem_ld_wait();
               const int col = unit.n0 + c * 32;
-              if (col >= p.N || row >= p.M) continue;
+              if (col >= p.N) continue;
               float s[32];
 #pragma unroll
               for (int j = 0; j < 32; ++j) s[j] = 0.f;
@@ -576,7 +576,7 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                 } else {
                   float4 t[8];
 #pragma unroll
-                  for (int q = 0; q < 8; ++q) t[q] = __ldcg(tile + part * PART_STEP + (c * 8 + q) * BM);
+                  for (int q = 0; q < 8; ++q) t[q] = row < p.M ? __ldcg(tile + part * PART_STEP + (c * 8 + q) * BM) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                   for (int q = 0; q < 8; ++q) s[4 * q] += t[q].x, s[4 * q + 1] += t[q].y, s[4 * q + 2] += t[q].z, s[4 * q + 3] += t[q].w;
                 }

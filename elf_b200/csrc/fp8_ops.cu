@@ -32,8 +32,9 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { re
 template <>
 __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-// How a thread's 16 values are moved: one by one, or in pieces of 16 or 32 bytes that the address is a multiple of.
-enum class Access { kRagged, kPieces16, kPieces32 };
+// How a thread's 16 values are moved: in pieces of 16 or 32 bytes where rows start on such addresses, otherwise in
+// 16-byte pieces shifted into place.  Units that a row's end cuts off go one value at a time.
+enum class Access { kShifted, kPieces16, kPieces32 };
 
 __device__ __forceinline__ void load_piece(const void* p, uint4& a) { a = *static_cast<const uint4*>(p); }
 __device__ __forceinline__ void load_piece(const void* p, uint4& a, uint4& b) {
@@ -51,19 +52,45 @@ template <typename T>
 struct Raw {
   uint4 q[UNIT * sizeof(T) / 16];
 };
+// N words of the stream w, from its byte `shift` (0 to 15) on
+template <int N>
+__device__ __forceinline__ void shifted(uint32_t (&w)[N + 4], uint32_t shift, uint32_t (&out)[N]) {
+  if (shift & 8)
+#pragma unroll
+    for (int j = 0; j < N + 2; ++j) w[j] = w[j + 2];
+  if (shift & 4)
+#pragma unroll
+    for (int j = 0; j < N + 1; ++j) w[j] = w[j + 1];
+#pragma unroll
+  for (int j = 0; j < N; ++j) out[j] = __funnelshift_r(w[j], w[j + 1], (shift & 3) * 8);
+}
+struct Span {  // of a matrix in memory: what may be read around a row
+  uintptr_t begin, end;
+};
 template <typename T, Access A>
-__device__ __forceinline__ void load_raw(const T* p, int have, Raw<T>& r) {
+__device__ __forceinline__ void load_raw(const T* p, int have, Span span, Raw<T>& r) {
   constexpr int N = UNIT * sizeof(T) / 16;
-  if constexpr (A == Access::kPieces32) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p), base = at & ~uintptr_t(15);
+  if (have < UNIT || (A == Access::kShifted && !(base >= span.begin && base + 16 * (N + 1) <= span.end))) {
+    T* e = reinterpret_cast<T*>(r.q);
+#pragma unroll
+    for (int j = 0; j < UNIT; ++j) e[j] = j < have ? p[j] : from_float<T>(0.f);
+  } else if constexpr (A == Access::kPieces32) {
 #pragma unroll
     for (int i = 0; i < N; i += 2) load_piece(reinterpret_cast<const uint4*>(p) + i, r.q[i], r.q[i + 1]);
   } else if constexpr (A == Access::kPieces16) {
 #pragma unroll
     for (int i = 0; i < N; ++i) load_piece(reinterpret_cast<const uint4*>(p) + i, r.q[i]);
   } else {
-    T* e = reinterpret_cast<T*>(r.q);
+    uint32_t w[4 * N + 4], out[4 * N];
 #pragma unroll
-    for (int j = 0; j < UNIT; ++j) e[j] = j < have ? p[j] : from_float<T>(0.f);
+    for (int i = 0; i <= N; ++i) {
+      const uint4 t = reinterpret_cast<const uint4*>(base)[i];
+      w[4 * i] = t.x, w[4 * i + 1] = t.y, w[4 * i + 2] = t.z, w[4 * i + 3] = t.w;
+    }
+    shifted<4 * N>(w, uint32_t(at & 15), out);
+#pragma unroll
+    for (int i = 0; i < N; ++i) r.q[i] = make_uint4(out[4 * i], out[4 * i + 1], out[4 * i + 2], out[4 * i + 3]);
   }
 }
 template <typename T>
@@ -91,24 +118,56 @@ __device__ __forceinline__ uint32_t largest(const Raw<T>& r) {
   if constexpr (std::is_same<T, __half>::value) return m >= 0x7c00u ? kInfBits : __float_as_uint(__half2float(__ushort_as_half(uint16_t(m))));
   else return m << 16;
 }
+// Stores a lane's unit of a row; all 32 lanes of the warp call this, lanes with consecutive units.  kShifted: 16-byte
+// pieces lie across two lanes' units; a lane stores those that begin in its own, with the start of the next lane's.
 template <typename T, Access A>
-__device__ __forceinline__ void store_values(T* p, int have, const float (&v)[UNIT]) {
+__device__ __forceinline__ void store_values(T* p, int col, int have, const float (&v)[UNIT]) {
   constexpr int N = UNIT * sizeof(T) / 16;
   Raw<T> r;
   T* e = reinterpret_cast<T*>(r.q);
 #pragma unroll
   for (int j = 0; j < UNIT; ++j) e[j] = from_float<T>(v[j]);
+  int last = have;  // elements stored one by one
   if constexpr (A == Access::kPieces32) {
+    if (have >= UNIT) {
+      last = 0;
 #pragma unroll
-    for (int i = 0; i < N; i += 2) store_piece(reinterpret_cast<uint4*>(p) + i, r.q[i], r.q[i + 1]);
+      for (int i = 0; i < N; i += 2) store_piece(reinterpret_cast<uint4*>(p) + i, r.q[i], r.q[i + 1]);
+    }
   } else if constexpr (A == Access::kPieces16) {
+    if (have >= UNIT) {
+      last = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) reinterpret_cast<uint4*>(p)[i] = r.q[i];
+      for (int i = 0; i < N; ++i) reinterpret_cast<uint4*>(p)[i] = r.q[i];
+    }
   } else {
+    const int lane = threadIdx.x & 31;
+    const int next_col = __shfl_down_sync(0xffffffffu, col, 1), next_have = __shfl_down_sync(0xffffffffu, have, 1);
+    uint32_t w[4 * N + 4], out[4 * N];
 #pragma unroll
-    for (int j = 0; j < UNIT; ++j)
-      if (j < have) p[j] = e[j];
+    for (int i = 0; i < N; ++i) w[4 * i] = r.q[i].x, w[4 * i + 1] = r.q[i].y, w[4 * i + 2] = r.q[i].z, w[4 * i + 3] = r.q[i].w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[4 * N + j] = __shfl_down_sync(0xffffffffu, w[j], 1);
+    if (have >= UNIT) {
+      const uint32_t head = (16 - uint32_t(reinterpret_cast<uintptr_t>(p) & 15)) & 15;  // bytes before the first piece
+      const bool joined = lane < 31 && next_col == col + UNIT && next_have >= UNIT;     // the next lane's start is at hand
+      const bool taken = lane > 0 && col > 0;                                           // the lane before stores this one's start
+      uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(p) + head);
+      shifted<4 * N>(w, head, out);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i + 1 < N || head == 0 || joined) dst[i] = make_uint4(out[4 * i], out[4 * i + 1], out[4 * i + 2], out[4 * i + 3]);
+      // what is left: a start that nobody takes, an end that nobody joins
+      const int before = int(head / sizeof(T)), after = head == 0 ? UNIT : before + (N - 1) * int(16 / sizeof(T));
+#pragma unroll
+      for (int j = 0; j < UNIT; ++j)
+        if ((j < before && !taken) || (j >= after && !joined)) p[j] = e[j];
+      return;
+    }
   }
+#pragma unroll
+  for (int j = 0; j < UNIT; ++j)
+    if (j < last) p[j] = e[j];
 }
 __device__ __forceinline__ void store_bytes_ragged(uint8_t* p, int have, const uint32_t (&q)[UNIT / 4]) {
 #pragma unroll
@@ -123,7 +182,7 @@ __device__ __forceinline__ void store_bytes_ragged(uint8_t* p, int have, const u
 template <typename T, Access A>
 __global__ void __launch_bounds__(THREADS) quantize_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ data, long long ldq,
                                                                 uint8_t* __restrict__ scale, long long lds, uint32_t total, uint32_t units_per_row,
-                                                                int cols) {
+                                                                int cols, Span span, bool packed) {
   await_previous();
   Raw<T> raw[UNITS];
   uint32_t row[UNITS];
@@ -135,7 +194,7 @@ __global__ void __launch_bounds__(THREADS) quantize_rows_kernel(const T* __restr
     col[i] = int(u - row[i] * units_per_row) * UNIT;
     have[i] = u < total ? min(cols - col[i], UNIT) : 0;  // 0 or less: padding of a row's last block
     if (have[i] > 0) {
-      load_raw<T, A>(x + (long long)row[i] * ldx + col[i], have[i], raw[i]);
+      load_raw<T, A>(x + (long long)row[i] * ldx + col[i], have[i], span, raw[i]);
     } else {
 #pragma unroll
       for (uint4& q : raw[i].q) q = make_uint4(0, 0, 0, 0);
@@ -149,10 +208,8 @@ __global__ void __launch_bounds__(THREADS) quantize_rows_kernel(const T* __restr
     const uint32_t byte = quantize_block<UNIT, 8>(v, largest(raw[i]), q);
     if (have[i] > 0) {
       uint8_t* dst = data + (long long)row[i] * ldq + col[i];
-      if constexpr (A != Access::kRagged)
-        *reinterpret_cast<uint4*>(dst) = make_uint4(q[0], q[1], q[2], q[3]);
-      else
-        store_bytes_ragged(dst, have[i], q);
+      if (packed && have[i] == UNIT) *reinterpret_cast<uint4*>(dst) = make_uint4(q[0], q[1], q[2], q[3]);
+      else store_bytes_ragged(dst, have[i], q);
       if ((col[i] & (BLOCK - 1)) == 0) scale[(long long)row[i] * lds + col[i] / BLOCK] = uint8_t(byte);
     }
   }
@@ -163,7 +220,7 @@ __global__ void __launch_bounds__(THREADS) quantize_rows_kernel(const T* __restr
 // SM, 129.
 template <typename T, Access A>
 __global__ void __launch_bounds__(TILE_THREADS, 2) quantize_tiles_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ data, long long ldq,
-                                                                 uint8_t* __restrict__ scale, long long lds, long long rows, int cols) {
+                                                                 uint8_t* __restrict__ scale, long long lds, long long rows, int cols, Span span, bool packed) {
   __shared__ uint32_t warp_max[TILE_THREADS / 32];
   await_previous();
   const int col = blockIdx.x * BLOCK + (threadIdx.x & 7) * UNIT;
@@ -175,7 +232,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 2) quantize_tiles_kernel(const T
   for (int i = 0; i < GROUPS; ++i) {
     const long long row = row0 + STEP * i;
     if (have_cols > 0 && row < rows) {
-      load_raw<T, A>(x + row * ldx + col, have_cols, raw[i]);
+      load_raw<T, A>(x + row * ldx + col, have_cols, span, raw[i]);
     } else {
 #pragma unroll
       for (uint4& q : raw[i].q) q = make_uint4(0, 0, 0, 0);
@@ -218,10 +275,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 2) quantize_tiles_kernel(const T
     if (odd) scaled_to_e4m3_odd(v, inv, q);
     else scaled_to_e4m3(v, inv, q);
     uint8_t* dst = data + row * ldq + col;
-    if constexpr (A != Access::kRagged)
-      *reinterpret_cast<uint4*>(dst) = make_uint4(q[0], q[1], q[2], q[3]);
-    else
-      store_bytes_ragged(dst, have_cols, q);
+    if (packed && have_cols == UNIT) *reinterpret_cast<uint4*>(dst) = make_uint4(q[0], q[1], q[2], q[3]);
+    else store_bytes_ragged(dst, have_cols, q);
   }
   if (threadIdx.x == 0) scale[(long long)blockIdx.y * lds + blockIdx.x] = uint8_t(byte);
 }
@@ -232,7 +287,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 2) quantize_tiles_kernel(const T
 template <typename T, Access A>
 __global__ void __launch_bounds__(THREADS) dequantize_kernel(const uint8_t* __restrict__ data, long long ldq, const uint8_t* __restrict__ scale,
                                                              long long lds, int row_shift, T* __restrict__ y, long long ldy, uint32_t total,
-                                                             uint32_t units_per_row, long long first_row, int cols) {
+                                                             uint32_t units_per_row, long long first_row, int cols, bool packed) {
   await_previous();
   uint32_t q[UNITS][UNIT / 4], byte[UNITS];
   long long row[UNITS];
@@ -244,9 +299,10 @@ __global__ void __launch_bounds__(THREADS) dequantize_kernel(const uint8_t* __re
     row[i] = first_row + r;
     col[i] = int(u - r * units_per_row) * UNIT;
     have[i] = u < total ? min(cols - col[i], UNIT) : 0;
+    q[i][0] = q[i][1] = q[i][2] = q[i][3] = byte[i] = 0;
     if (have[i] <= 0) continue;
     const uint8_t* src = data + row[i] * ldq + col[i];
-    if constexpr (A != Access::kRagged) {
+    if (packed && have[i] == UNIT) {
       const uint4 t = *reinterpret_cast<const uint4*>(src);
       q[i][0] = t.x, q[i][1] = t.y, q[i][2] = t.z, q[i][3] = t.w;
     } else {
@@ -260,7 +316,6 @@ __global__ void __launch_bounds__(THREADS) dequantize_kernel(const uint8_t* __re
   }
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) {
-    if (have[i] <= 0) continue;
     const float s = exponent_value(byte[i]);
     float v[UNIT];
 #pragma unroll
@@ -271,7 +326,7 @@ __global__ void __launch_bounds__(THREADS) dequantize_kernel(const uint8_t* __re
       v[4 * j + 2] = mul_exact(hi.x, s);
       v[4 * j + 3] = mul_exact(hi.y, s);
     }
-    store_values<T, A>(y + row[i] * ldy + col[i], have[i], v);
+    store_values<T, A>(y + row[i] * ldy + col[i], col[i], have[i], v);
   }
 }
 
@@ -484,13 +539,16 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS<VPT>) rmsnorm_fp8_bl
 }
 
 bool aligned(const void* p, long long pitch_bytes, int to) { return (reinterpret_cast<uintptr_t>(p) | uintptr_t(pitch_bytes)) % to == 0; }
-// wide: the 16- or 32-bit matrix; bytes: the 8-bit one
-Access access_for(const void* wide, long long wide_pitch, const void* bytes, long long bytes_pitch, int cols) {
-  if (cols % UNIT != 0 || !aligned(wide, wide_pitch, 16) || !aligned(bytes, bytes_pitch, 16)) return Access::kRagged;
-  return aligned(wide, wide_pitch, 32) ? Access::kPieces32 : Access::kPieces16;
+Access access_for(const void* p, long long pitch_bytes) {
+  return aligned(p, pitch_bytes, 32) ? Access::kPieces32 : aligned(p, pitch_bytes, 16) ? Access::kPieces16 : Access::kShifted;
 }
 #define ELFB_ACCESS(KERNEL, T, A) \
-  (A == Access::kPieces32 ? KERNEL<T, Access::kPieces32> : A == Access::kPieces16 ? KERNEL<T, Access::kPieces16> : KERNEL<T, Access::kRagged>)
+  (A == Access::kPieces32 ? KERNEL<T, Access::kPieces32> : A == Access::kPieces16 ? KERNEL<T, Access::kPieces16> : KERNEL<T, Access::kShifted>)
+template <typename T>
+Span span_of(const void* x, long long ldx, long long rows, int cols) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(x);
+  return {at, at + uintptr_t((rows - 1) * ldx + cols) * sizeof(T)};
+}
 
 // rows per launch, so that a launch's units fit 31 bits
 long long rows_per_launch(uint32_t units_per_row) { return std::max(1ll, (1ll << 30) / units_per_row); }
@@ -498,14 +556,16 @@ long long rows_per_launch(uint32_t units_per_row) { return std::max(1ll, (1ll <<
 template <typename T>
 cudaError_t quantize_rows_as(const void* x, long long ldx, uint8_t* data, long long ldq, uint8_t* scale, long long lds, long long rows, int cols,
                              cudaStream_t stream) {
-  const Access how = access_for(x, ldx * sizeof(T), data, ldq, cols);
+  const Access how = access_for(x, ldx * sizeof(T));
+  const Span span = span_of<T>(x, ldx, rows, cols);
+  const bool packed = aligned(data, ldq, 16);
   const uint32_t upr = uint32_t((cols + BLOCK - 1) / BLOCK) * (BLOCK / UNIT);
   const long long step = rows_per_launch(upr);
   for (long long r = 0; r < rows; r += step) {
     const uint32_t total = uint32_t(std::min(step, rows - r)) * upr;
     auto* kern = ELFB_ACCESS(quantize_rows_kernel, T, how);
     if (cudaError_t e = launch_overlapped(kern, (total + UNITS * THREADS - 1) / (UNITS * THREADS), THREADS, 0, 0, stream, static_cast<const T*>(x) + r * ldx, ldx,
-                                          data + r * ldq, ldq, scale + r * lds, lds, total, upr, cols);
+                                          data + r * ldq, ldq, scale + r * lds, lds, total, upr, cols, span, packed);
         e != cudaSuccess)
       return e;
   }
@@ -515,7 +575,9 @@ cudaError_t quantize_rows_as(const void* x, long long ldx, uint8_t* data, long l
 template <typename T>
 cudaError_t quantize_tiles_as(const void* x, long long ldx, uint8_t* data, long long ldq, uint8_t* scale, long long lds, long long rows, int cols,
                               cudaStream_t stream) {
-  const Access how = access_for(x, ldx * sizeof(T), data, ldq, cols);
+  const Access how = access_for(x, ldx * sizeof(T));
+  const Span span = span_of<T>(x, ldx, rows, cols);
+  const bool packed = aligned(data, ldq, 16);
   constexpr long long kGridY = 65535;
   const long long tiles = (rows + BLOCK - 1) / BLOCK;
   for (long long t = 0; t < tiles; t += kGridY) {
@@ -523,7 +585,7 @@ cudaError_t quantize_tiles_as(const void* x, long long ldx, uint8_t* data, long 
     const dim3 grid((cols + BLOCK - 1) / BLOCK, unsigned(std::min(kGridY, tiles - t)));
     auto* kern = ELFB_ACCESS(quantize_tiles_kernel, T, how);
     if (cudaError_t e = launch_overlapped(kern, grid, TILE_THREADS, 0, 0, stream, static_cast<const T*>(x) + r * ldx, ldx, data + r * ldq, ldq, scale + t * lds, lds,
-                                          rows - r, cols);
+                                          rows - r, cols, span, packed);
         e != cudaSuccess)
       return e;
   }
@@ -533,14 +595,15 @@ cudaError_t quantize_tiles_as(const void* x, long long ldx, uint8_t* data, long 
 template <typename T>
 cudaError_t dequantize_as(const uint8_t* data, long long ldq, const uint8_t* scale, long long lds, int row_shift, void* y, long long ldy, long long rows,
                           int cols, cudaStream_t stream) {
-  const Access how = access_for(y, ldy * sizeof(T), data, ldq, cols);
+  const Access how = access_for(y, ldy * sizeof(T));
+  const bool packed = aligned(data, ldq, 16);
   const uint32_t upr = uint32_t((cols + UNIT - 1) / UNIT);
   const long long step = rows_per_launch(upr);
   for (long long r = 0; r < rows; r += step) {
     const uint32_t total = uint32_t(std::min(step, rows - r)) * upr;
     auto* kern = ELFB_ACCESS(dequantize_kernel, T, how);
     if (cudaError_t e = launch_overlapped(kern, (total + UNITS * THREADS - 1) / (UNITS * THREADS), THREADS, 0, 0, stream, data, ldq, scale, lds, row_shift,
-                                          static_cast<T*>(y), ldy, total, upr, r, cols);
+                                          static_cast<T*>(y), ldy, total, upr, r, cols, packed);
         e != cudaSuccess)
       return e;
   }

@@ -180,6 +180,15 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> rmsnorm(const at::Ten
   return {q.first, q.second, rstd, h};
 }
 
+// the rows of `m` in new memory, `pitch` elements apart
+at::Tensor repacked(const Mat& m, int64_t pitch, const at::Device& dev) {
+  const int64_t lead[1] = {m.rows}, size = m.t.element_size();
+  TORCH_CHECK(m.cols * size <= INT_MAX - 1024, "rows are too wide to be copied");
+  at::Tensor out = new_rows(at::IntArrayRef(lead, 1), m.cols, pitch, m.t.scalar_type(), dev);
+  check(elfb::fp8_repack(m.t.data_ptr(), m.pitch * size, out.data_ptr(), pitch * size, m.rows, int(m.cols * size), cur()), "fp8_repack");
+  return out;
+}
+
 // An operand of a product and the tensors that keep its memory alive until the launch is queued.
 struct Operand {
   Scaled s;
@@ -190,9 +199,7 @@ Operand operand(const at::Tensor& data, const at::Tensor& scale, int64_t row_shi
   Operand r{scaled(data, scale, row_shift, name, dev), {}};
   TORCH_CHECK(r.s.data.rows <= INT_MAX - 1024, name, " has too many rows");
   if (!r.s.data.aligned(align)) {  // TMA wants rows on 16-byte boundaries: a copy with padded rows
-    const int64_t lead[1] = {r.s.data.rows};
-    at::Tensor padded = new_rows(at::IntArrayRef(lead, 1), r.s.data.cols, round_up(r.s.data.cols, align), data.scalar_type(), dev);
-    padded.copy_(r.s.data.t.dim() == 2 ? r.s.data.t : r.s.data.t.reshape({r.s.data.rows, r.s.data.cols}));
+    const at::Tensor padded = repacked(r.s.data, round_up(r.s.data.cols, align), dev);
     r.s.data = matrix(padded, name, dev, false);
   }
   r.o.data = r.s.data.bytes();
@@ -213,8 +220,6 @@ Operand operand(const at::Tensor& data, const at::Tensor& scale, int64_t row_shi
   }
   return r;
 }
-
-
 
 void launch(elfb::Fp8GemmArgs& g, const at::Tensor& status, const at::Device& dev, const char* what) {
   g.status = status_ptr(status, dev);
@@ -338,15 +343,16 @@ std::vector<c10::optional<at::Tensor>> ffn(const at::Tensor& x, const at::Tensor
 Mat restored(const at::Tensor& t, const c10::optional<at::Tensor>& scale, const char* name, const at::Device& dev) {
   Mat m = matrix(scale.has_value() ? t : t.to(at::kBFloat16), name, dev);
   if (!scale.has_value() && m.aligned(16)) return m;
-  const int64_t lead[1] = {m.rows};
-  at::Tensor out = new_rows(at::IntArrayRef(lead, 1), m.cols, round_up(m.cols, 8), at::kBFloat16, dev);
+  at::Tensor out;
   if (scale.has_value()) {
+    const int64_t lead[1] = {m.rows};
+    out = new_rows(at::IntArrayRef(lead, 1), m.cols, round_up(m.cols, 8), at::kBFloat16, dev);
     const Scaled s = scaled(t, *scale, 0, name, dev);
     check(elfb::fp8_dequantize(s.data.bytes(), s.data.pitch, s.scale.bytes(), s.scale.pitch, 0, out.data_ptr(), elfb::Elem::kBf16, round_up(m.cols, 8), m.rows,
                                int(m.cols), cur()),
           "fp8_dequantize");
   } else {
-    out.copy_(m.t.dim() == 2 ? m.t : m.t.reshape({m.rows, m.cols}));
+    out = repacked(m, round_up(m.cols, 8), dev);
   }
   Mat r{out, m.rows, m.cols, round_up(m.cols, 8)};
   return r;
@@ -389,7 +395,8 @@ at::Tensor weight_grad(const at::Tensor& dy, const c10::optional<at::Tensor>& dy
     at::Tensor sum = *out;
     return sum.add_(dw);
   }
-  return dw.scalar_type() == dtype ? dw.contiguous() : dw.to(dtype).contiguous();
+  if (dw.scalar_type() != dtype) return dw.to(dtype).contiguous();
+  return dw.is_contiguous() ? dw : repacked(matrix(dw, "the gradient", dev, false), b.cols, dev);
 }
 
 // Backward of `ffn` from what it kept: (dx, dw_gate_up, dw_down), each only on request.

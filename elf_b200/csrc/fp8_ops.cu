@@ -74,7 +74,7 @@ __device__ __forceinline__ void load_raw(const T* p, int have, Span span, Raw<T>
   if (have < UNIT || (A == Access::kShifted && !(base >= span.begin && base + 16 * (N + 1) <= span.end))) {
     T* e = reinterpret_cast<T*>(r.q);
 #pragma unroll
-    for (int j = 0; j < UNIT; ++j) e[j] = j < have ? p[j] : from_float<T>(0.f);
+    for (int j = 0; j < UNIT; ++j) e[j] = j < have ? p[j] : T{};
   } else if constexpr (A == Access::kPieces32) {
 #pragma unroll
     for (int i = 0; i < N; i += 2) load_piece(reinterpret_cast<const uint4*>(p) + i, r.q[i], r.q[i + 1]);
@@ -121,12 +121,9 @@ __device__ __forceinline__ uint32_t largest(const Raw<T>& r) {
 // Stores a lane's unit of a row; all 32 lanes of the warp call this, lanes with consecutive units.  kShifted: 16-byte
 // pieces lie across two lanes' units; a lane stores those that begin in its own, with the start of the next lane's.
 template <typename T, Access A>
-__device__ __forceinline__ void store_values(T* p, int col, int have, const float (&v)[UNIT]) {
+__device__ __forceinline__ void store_raw(T* p, int col, int have, const Raw<T>& r) {
   constexpr int N = UNIT * sizeof(T) / 16;
-  Raw<T> r;
-  T* e = reinterpret_cast<T*>(r.q);
-#pragma unroll
-  for (int j = 0; j < UNIT; ++j) e[j] = from_float<T>(v[j]);
+  const T* e = reinterpret_cast<const T*>(r.q);
   int last = have;  // elements stored one by one
   if constexpr (A == Access::kPieces32) {
     if (have >= UNIT) {
@@ -168,6 +165,14 @@ __device__ __forceinline__ void store_values(T* p, int col, int have, const floa
 #pragma unroll
   for (int j = 0; j < UNIT; ++j)
     if (j < last) p[j] = e[j];
+}
+template <typename T, Access A>
+__device__ __forceinline__ void store_values(T* p, int col, int have, const float (&v)[UNIT]) {
+  Raw<T> r;
+  T* e = reinterpret_cast<T*>(r.q);
+#pragma unroll
+  for (int j = 0; j < UNIT; ++j) e[j] = from_float<T>(v[j]);
+  store_raw<T, A>(p, col, have, r);
 }
 __device__ __forceinline__ void store_bytes_ragged(uint8_t* p, int have, const uint32_t (&q)[UNIT / 4]) {
 #pragma unroll
@@ -328,6 +333,27 @@ __global__ void __launch_bounds__(THREADS) dequantize_kernel(const uint8_t* __re
     }
     store_values<T, A>(y + row[i] * ldy + col[i], col[i], have[i], v);
   }
+}
+
+// ------------------------------------------------------------------------------ rows moved to another pitch
+template <Access FROM, Access TO>
+__global__ void __launch_bounds__(THREADS) repack_kernel(const uint8_t* __restrict__ src, long long ld_src, uint8_t* __restrict__ dst, long long ld_dst,
+                                                         uint32_t total, uint32_t units_per_row, int row_bytes, Span span) {
+  await_previous();
+  Raw<uint8_t> raw[2 * UNITS];
+  uint32_t row[2 * UNITS];
+  int col[2 * UNITS], have[2 * UNITS];
+#pragma unroll
+  for (int i = 0; i < 2 * UNITS; ++i) {
+    const uint32_t u = (blockIdx.x * 2 * UNITS + i) * THREADS + threadIdx.x;
+    row[i] = u / units_per_row;
+    col[i] = int(u - row[i] * units_per_row) * UNIT;
+    have[i] = u < total ? min(row_bytes - col[i], UNIT) : 0;
+    if (have[i] > 0) load_raw<uint8_t, FROM>(src + (long long)row[i] * ld_src + col[i], have[i], span, raw[i]);
+    else raw[i].q[0] = make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < 2 * UNITS; ++i) store_raw<uint8_t, TO>(dst + (long long)row[i] * ld_dst + col[i], col[i], have[i], raw[i]);
 }
 
 // ------------------------------------------------------------------------------ RMSNorm
@@ -654,6 +680,26 @@ cudaError_t fp8_dequantize(const uint8_t* data, long long ldq, const uint8_t* sc
   if (type == Elem::kBf16) return dequantize_as<__nv_bfloat16>(data, ldq, scale, lds, row_shift, y, ldy, rows, cols, stream);
   if (type == Elem::kF16) return dequantize_as<__half>(data, ldq, scale, lds, row_shift, y, ldy, rows, cols, stream);
   return dequantize_as<float>(data, ldq, scale, lds, row_shift, y, ldy, rows, cols, stream);
+}
+
+cudaError_t fp8_repack(const void* src, long long ld_src, void* dst, long long ld_dst, long long rows, int row_bytes, cudaStream_t stream) {
+  if (rows <= 0 || row_bytes <= 0) return cudaSuccess;
+  const uint8_t* from = static_cast<const uint8_t*>(src);
+  uint8_t* to = static_cast<uint8_t*>(dst);
+  const Span span = span_of<uint8_t>(src, ld_src, rows, row_bytes);
+  const uint32_t upr = uint32_t((row_bytes + UNIT - 1) / UNIT);
+  const long long step = rows_per_launch(upr);
+  constexpr Access P = Access::kPieces16, S = Access::kShifted;
+  const bool from_pieces = aligned(src, ld_src, 16), to_pieces = aligned(dst, ld_dst, 16);
+  auto* kern = from_pieces ? (to_pieces ? repack_kernel<P, P> : repack_kernel<P, S>) : to_pieces ? repack_kernel<S, P> : repack_kernel<S, S>;
+  for (long long r = 0; r < rows; r += step) {
+    const uint32_t total = uint32_t(std::min(step, rows - r)) * upr;
+    if (cudaError_t e = launch_overlapped(kern, (total + 2 * UNITS * THREADS - 1) / (2 * UNITS * THREADS), THREADS, 0, 0, stream, from + r * ld_src, ld_src,
+                                          to + r * ld_dst, ld_dst, total, upr, row_bytes, span);
+        e != cudaSuccess)
+      return e;
+  }
+  return cudaSuccess;
 }
 
 cudaError_t fp8_rmsnorm(const void* x, const void* residual, const void* w, void* h, float* rstd, uint8_t* data, long long ldq, uint8_t* scale,

@@ -20,6 +20,8 @@ cudaError_t fp8_quantize_tiles(const void* x, Elem type, long long ldx, uint8_t*
 // scale row of matrix row r is r >> row_shift (0 or 7)
 cudaError_t fp8_dequantize(const uint8_t* data, long long ldq, const uint8_t* scale, long long lds, int row_shift, void* y, Elem type, long long ldy,
                            long long rows, int cols, cudaStream_t stream);
+// copies rows of bytes to another pitch (pitches in bytes)
+cudaError_t fp8_repack(const void* src, long long ld_src, void* dst, long long ld_dst, long long rows, int row_bytes, cudaStream_t stream);
 // h = x + residual (bf16, written when residual is given); data/scale = blocks of h * rstd * w
 cudaError_t fp8_rmsnorm(const void* x, const void* residual, const void* w, void* h, float* rstd, uint8_t* data, long long ldq, uint8_t* scale,
                         long long lds, long long rows, int dim, double eps, int num_sms, cudaStream_t stream);

@@ -111,6 +111,49 @@ def test_quantize_leaves_neighbours_alone(dev):
     assert bool((out[5:] == 7).all()) and bool((out[:, 140:] == 7).all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [1, 15, 16, 17, 40, 127, 129, 515, 1040])
+def test_rows_that_start_anywhere(dev, dtype, cols):
+    """Views at every offset to 16 bytes, with rows that touch: neighbours are neither read into a block nor written."""
+    from elf_b200.ops import fp8
+
+    rows = 37
+    want_x = activations(rows, cols, dtype, dev, cols)
+    aligned = torch.zeros(rows, -(-cols // 16) * 16, dtype=dtype, device=dev)[:, :cols]
+    aligned.copy_(want_x)
+    want, want_w = fp8.quantize(aligned), fp8.quantize_weight(aligned)
+    restored = fp8.dequantize(want, dtype, out=torch.zeros_like(aligned))
+    for offset in range(0, 32 // dtype.itemsize + 1):
+        for pitch in (cols, cols + 1, cols + 3):
+            buffer = torch.full((offset + rows * pitch + 40,), 3e4, dtype=dtype, device=dev)
+            view = buffer[offset : offset + rows * pitch].view(rows, pitch)[:, :cols]
+            view.copy_(want_x)
+            for got, ref in ((fp8.quantize(view), want), (fp8.quantize_weight(view), want_w)):
+                assert torch.equal(got.scale, ref.scale) and torch.equal(got.data.view(torch.uint8), ref.data.view(torch.uint8))
+            buffer.fill_(5)
+            fp8.dequantize(want, out=view)
+            assert torch.equal(view, restored)
+            view.fill_(5)
+            assert (buffer == 5).all()
+
+
+@pytest.mark.parametrize("n,k", [(1, 1), (7, 33), (40, 129), (33, 1043), (129, 7)])
+def test_weight_grad_of_odd_widths(dev, n, k):
+    """Rows of the result start anywhere; operands from 8 bits and as they are."""
+    from elf_b200.ops import fp8
+
+    dy, x = activations(300, n, torch.bfloat16, dev, n), activations(300, k, torch.bfloat16, dev, k)
+    dyq, xq = fp8.quantize(dy), fp8.quantize(x)
+    for a, b, av, bv in ((dyq, xq, values(dyq), values(xq)), (dy, xq, dy.double(), values(xq)), (dy, x, dy.double(), x.double())):
+        for out in DTYPES:
+            got = fp8.linear_weight_grad(a, b, out_dtype=out)
+            assert got.shape == (n, k) and got.is_contiguous()
+            # an fp32 sum of 300 products, rounded once (through fp32 to fp16)
+            mag = av.abs().T @ bv.abs()
+            want = av.T @ bv
+            assert ((got.double() - want).abs() <= mag * 300 * 2.0**-23 + want.abs() * torch.finfo(out).eps + 2.0**-24).all()
+
+
 def test_empty_tensors(dev):
     from elf_b200.ops import fp8
 

@@ -476,7 +476,8 @@ __device__ __forceinline__ void store_normalised(const NormArgs& p, long long ro
   }
 }
 
-// Rows of up to 1024 values: a warp per row.
+// Rows of up to 1536 values: a warp per row.  15465 x 1304: 23 us, a block per row 33; 8192 x 2048 with residual 32 and 27,
+// so wider rows take a block.
 template <int VPT, bool RESIDUAL>
 __global__ void __launch_bounds__(256) rmsnorm_fp8_warp_kernel(const __grid_constant__ NormArgs p) {
   await_previous();
@@ -512,17 +513,17 @@ __global__ void __launch_bounds__(256) rmsnorm_fp8_warp_kernel(const __grid_cons
 // four blocks per SM (four spill registers) 24 and 29; 128 or 512 threads per row, or a ring of rows in shared memory
 // filled by bulk copies, 3 us more when that was 24.
 template <int VPT>
-constexpr int NORM_BLOCKS = VPT == 1 ? 4 : VPT == 2 ? 3 : 2;  // per SM
+constexpr int NORM_BLOCKS = VPT == 1 ? 4 : VPT == 2 ? 3 : 2;  // of NORM_THREADS, per SM
 template <int VPT, bool RESIDUAL>
 __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS<VPT>) rmsnorm_fp8_block_kernel(const __grid_constant__ NormArgs p) {
   __shared__ double red[2][NORM_THREADS / 32];
   await_previous();
-  const int t = threadIdx.x;
+  const int t = threadIdx.x, threads = blockDim.x;
   uint4 nx[VPT], nr[VPT], gain[VPT];
   auto fetch = [&](long long row) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int c = t + i * NORM_THREADS;
+      const int c = t + i * threads;
       if (row < p.rows && c < p.dim8) {
         nx[i] = p.x[row * p.dim8 + c];
         if (RESIDUAL) nr[i] = p.res[row * p.dim8 + c];
@@ -531,13 +532,13 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS<VPT>) rmsnorm_fp8_bl
   };
   fetch(blockIdx.x);
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) gain[i] = t + i * NORM_THREADS < p.dim8 ? p.w[t + i * NORM_THREADS] : make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < VPT; ++i) gain[i] = t + i * threads < p.dim8 ? p.w[t + i * threads] : make_uint4(0, 0, 0, 0);
   int turn = 0;
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
     float v[VPT][8];
   #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int c = t + i * NORM_THREADS;
+      const int c = t + i * threads;
       if (c < p.dim8) {
         if (RESIDUAL) p.h[row * p.dim8 + c] = add_rounded(nx[i], nr[i], v[i]);
         else unpack8(nx[i], v[i]);
@@ -552,12 +553,13 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS<VPT>) rmsnorm_fp8_bl
     __syncthreads();
     sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < NORM_THREADS / 32; ++i) sum += red[turn][i];
+    for (int i = 0; i < NORM_THREADS / 32; ++i)
+      if (i < threads / 32) sum += red[turn][i];
     const InverseRms rs = inverse_rms(sum, p);
     if (t == 0) p.rstd[row] = rs.hi;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int c = t + i * NORM_THREADS;
+      const int c = t + i * threads;
       if ((c & ~31) >= p.dim8) break;  // the whole warp is past the row
       store_normalised(p, row, c, true, v[i], gain[i], rs);
     }
@@ -653,7 +655,9 @@ cudaError_t rmsnorm_warps(const NormArgs& p, cudaStream_t stream) {
 template <int VPT>
 cudaError_t rmsnorm_blocks(const NormArgs& p, int num_sms, cudaStream_t stream) {
   auto* kern = p.res ? rmsnorm_fp8_block_kernel<VPT, true> : rmsnorm_fp8_block_kernel<VPT, false>;
-  return launch_overlapped(kern, unsigned(std::min(p.rows, (long long)NORM_BLOCKS<VPT> * num_sms)), NORM_THREADS, 0, 0, stream, p);
+  // whole warps, as many as the row fills: 1000 x 5120 on 160 threads instead of 256
+  const int threads = ((p.dim8 + VPT - 1) / VPT + 31) / 32 * 32, per_sm = NORM_BLOCKS<VPT> * NORM_THREADS / threads;
+  return launch_overlapped(kern, unsigned(std::min(p.rows, (long long)per_sm * num_sms)), unsigned(threads), 0, 0, stream, p);
 }
 
 }  // namespace
@@ -711,6 +715,7 @@ cudaError_t fp8_rmsnorm(const void* x, const void* residual, const void* w, void
   if (dim <= 256) return rmsnorm_warps<1>(p, stream);
   if (dim <= 512) return rmsnorm_warps<2>(p, stream);
   if (dim <= 1024) return rmsnorm_warps<4>(p, stream);
+  if (dim <= 1536) return rmsnorm_warps<6>(p, stream);
   if (dim <= 2048) return rmsnorm_blocks<1>(p, num_sms, stream);
   if (dim <= 4096) return rmsnorm_blocks<2>(p, num_sms, stream);
   return rmsnorm_blocks<4>(p, num_sms, stream);

@@ -514,11 +514,11 @@ __global__ void __launch_bounds__(256) rmsnorm_fp8_warp_kernel(const __grid_cons
 // filled by bulk copies, 3 us more when that was 24.
 template <int VPT>
 constexpr int NORM_BLOCKS = VPT == 1 ? 4 : VPT == 2 ? 3 : 2;  // of NORM_THREADS, per SM
-template <int VPT, bool RESIDUAL>
+template <int VPT, bool RESIDUAL, bool FULL>  // FULL: NORM_THREADS threads, otherwise fewer
 __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS<VPT>) rmsnorm_fp8_block_kernel(const __grid_constant__ NormArgs p) {
   __shared__ double red[2][NORM_THREADS / 32];
   await_previous();
-  const int t = threadIdx.x, threads = blockDim.x;
+  const int t = threadIdx.x, threads = FULL ? NORM_THREADS : int(blockDim.x);
   uint4 nx[VPT], nr[VPT], gain[VPT];
   auto fetch = [&](long long row) {
 #pragma unroll
@@ -654,9 +654,10 @@ cudaError_t rmsnorm_warps(const NormArgs& p, cudaStream_t stream) {
 
 template <int VPT>
 cudaError_t rmsnorm_blocks(const NormArgs& p, int num_sms, cudaStream_t stream) {
-  auto* kern = p.res ? rmsnorm_fp8_block_kernel<VPT, true> : rmsnorm_fp8_block_kernel<VPT, false>;
   // whole warps, as many as the row fills: 1000 x 5120 on 160 threads instead of 256
   const int threads = ((p.dim8 + VPT - 1) / VPT + 31) / 32 * 32, per_sm = NORM_BLOCKS<VPT> * NORM_THREADS / threads;
+  auto* kern = threads == NORM_THREADS ? (p.res ? rmsnorm_fp8_block_kernel<VPT, true, true> : rmsnorm_fp8_block_kernel<VPT, false, true>)
+                                       : (p.res ? rmsnorm_fp8_block_kernel<VPT, true, false> : rmsnorm_fp8_block_kernel<VPT, false, false>);
   return launch_overlapped(kern, unsigned(std::min(p.rows, (long long)per_sm * num_sms)), unsigned(threads), 0, 0, stream, p);
 }
 

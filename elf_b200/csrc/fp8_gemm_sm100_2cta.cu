@@ -149,6 +149,8 @@ __device__ __forceinline__ uint64_t sigmoid2(uint64_t x) {
 // One tile of the gated form: columns 0..127 of the accumulator are gate, 128..255 up.  A thread takes 64 columns
 // of gate and the same of up of one row into registers and gives the accumulator back at once; the maxima of the
 // three blocks (gate, up, activation) are exchanged with the thread that has the row's other half.
+// 4096 x 28672 x 4096: 379 us of 285 at the 8-bit peak (393 before its arithmetic went by fp32 pairs), tensor pipe 71 %
+// busy: 32 blocks of K are about as long as this epilogue, and the last of 25 waves is a quarter full.
 template <typename Release>
 __device__ __forceinline__ void gated_tile(uint32_t taddr, int row, int half, int f0, int f, const Params& p, uint32_t* exchange, Release&& release) {
   uint32_t raw[4][32];

@@ -336,6 +336,7 @@ __global__ void __launch_bounds__(THREADS) dequantize_kernel(const uint8_t* __re
 }
 
 // ------------------------------------------------------------------------------ rows moved to another pitch
+// TMA wants rows on 16-byte boundaries, a caller's tensor or a dense result may have them anywhere: one pass over the bytes.
 template <Access FROM, Access TO>
 __global__ void __launch_bounds__(THREADS) repack_kernel(const uint8_t* __restrict__ src, long long ld_src, uint8_t* __restrict__ dst, long long ld_dst,
                                                          uint32_t total, uint32_t units_per_row, int row_bytes, Span span) {

@@ -388,6 +388,12 @@ at::Tensor weight_grad(const at::Tensor& dy, const c10::optional<at::Tensor>& dy
   g.variant = int(variant);
   g.split_tail = split_tail;
   g.status = status_ptr(status, dev);
+  // tiles that are split along the tokens: parts in fp32, one order of sums
+  at::Tensor workspace;
+  if (const size_t bytes = elfb::gemm_pair_workspace(g, sm_count(dev))) {
+    workspace = dense({int64_t(bytes)}, at::kByte, dev);
+    g.workspace = workspace.data_ptr();
+  }
   const char* err = elfb::gemm_tcgen05(g, sm_count(dev), cur());
   TORCH_CHECK(err == nullptr, "elf_b200 fp8_weight_grad: ", err);
   if (direct) return dw;

@@ -1,5 +1,6 @@
 // Host entry point of the tcgen05 GEMM family (gemm_sm100.cu).
 #pragma once
+#include <cstddef>
 #include <cuda_runtime.h>
 
 #include "dp_reduce.h"
@@ -21,11 +22,16 @@ struct GemmArgs {
   int* status = nullptr;       // optional device int[4] error record
   int variant = 0;             // 0 = single-CTA kernel, 1 = CTA-pair kernel (cta_group::2)
   bool split_tail = true;      // cut the tiles of the last, partial wave into column strips
+  void* workspace = nullptr;   // optional: gemm_pair_workspace() bytes, used by this launch alone (see there)
   PushTarget push;             // optional: also store D into peer GPUs' inboxes and flag them (16-bit D only)
 };
 
 // Returns nullptr on success, otherwise a static description of the failure.
 const char* gemm_tcgen05(const GemmArgs& args, int num_sms, cudaStream_t stream);
+
+// Bytes with which the CTA-pair kernel keeps the parts of its K-split tiles in fp32, added in one order and rounded once;
+// without a workspace the parts are added to D in L2, in D's type and in the order they finish.  0: no tile is split.
+size_t gemm_pair_workspace(const GemmArgs& args, int num_sms);
 
 // Same contract, CTA-pair kernel (gemm_sm100_2cta.cu).
 const char* gemm_tcgen05_pair(const GemmArgs& args, int num_sms, cudaStream_t stream);

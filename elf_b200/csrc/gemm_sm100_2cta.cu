@@ -18,6 +18,7 @@
 // Only the leader's MMA thread issues MMAs.  TMEM is allocated and freed with the
 // cta_group::2 forms by warp 1 of both CTAs.
 
+#include <algorithm>
 #include <cstdio>
 #include <cstdlib>
 
@@ -42,6 +43,7 @@ constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
 constexpr int NUM_THREADS = 192;
 constexpr int TMEM_COLS = 512;
 constexpr int DEFAULT_GROUP_M = 4;  // tile rows (of 256) that are swept together before moving to the next columns
+constexpr int PART_FLOATS = BM * BN;  // one CTA's half of a tile in the workspace
 constexpr int STAGING_BYTES = 2 * 16384;  // two 128-row x 128-byte chunks for the TMA-store epilogue
 constexpr size_t SMEM_BYTES = size_t(STAGES) * STAGE_BYTES + STAGING_BYTES + 1024 + 256;
 
@@ -60,7 +62,9 @@ struct WorkUnit {
 // Tiles are dealt round-robin to the CTA pairs.  When the tile count is not a multiple of
 // the pair count the last, partly filled wave would cost a whole tile time with most SMs
 // idle; instead each tile of that wave is split along K into `ksplit` units that run on
-// different pairs and add their partial sums to D (TMA add-reduce in L2).  Unlike a split
+// different pairs and add their partial sums to D (TMA add-reduce in L2), or leave them in fp32 in a
+// workspace for the last one to add in their order (2048 x 5504 from 2047 tokens, with the operands'
+// restores: 51 and 55 us).  Unlike a split
 // along N this keeps the 256x256 tile's ratio of MMA work to bytes loaded.
 struct Schedule {
   int tiles_m, tiles_n, full_tiles, ksplit, total_units, group_m;
@@ -158,7 +162,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
 gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                          const __grid_constant__ CUtensorMap tmap_d, void* __restrict__ d_ptr, const void* __restrict__ bias_ptr, int M, int N, int K, long long ldd,
                          uint32_t fmt, float alpha, int max_split, int group_m, int* __restrict__ status, const __grid_constant__ PushTarget push,
-                         const __grid_constant__ PeerMaps peer_maps) {
+                         const __grid_constant__ PeerMaps peer_maps, float* __restrict__ parts, unsigned int* __restrict__ parts_done) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_aligned = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -171,6 +175,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
   auto acc_empty_bar = [&](int a) { return bar0 + 8u * (2 * SLOTS + 2 + a); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * SLOTS + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile unsigned int* arrived = tmem_slot + 2;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -319,12 +324,48 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
       const WorkUnit wu = work_unit(unit, sched, k_blocks);
       const int row0 = wu.m * (2 * BM) + int(cta) * BM;
       const int row = row0 + quarter * 32 + lane;
-      const bool add_bias = BIAS && wu.part == 0;
+      const bool joined = wu.partial && parts != nullptr;  // fp32 parts in the workspace, added by the last to finish
+      const bool add_bias = BIAS && (wu.part == 0 || joined);
       const int n0 = wu.n0;
       if (!mbar_wait(acc_full_bar(acc), acc_phase, abort_flag)) break;
       tc_fence_after_sync();
       const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + acc * BN;
-      {
+      bool finish = true;  // this unit's sums are D's
+      const float4* tile = nullptr;
+      constexpr long long PART_STEP = 2 * (PART_FLOATS / 4);
+      if (joined) {
+        // Workspace layout [tile][part][CTA][4 columns][row]: a warp's access covers 512 consecutive bytes.
+        const int rest = (unit - sched.full_tiles) % ((sched.total_units - sched.full_tiles) / sched.ksplit);
+        const unsigned others = unsigned(sched.ksplit - 1);
+        unsigned int* done = parts_done + rest * 2 + cta;
+        float4* first = reinterpret_cast<float4*>(parts) + ((long long)rest * sched.ksplit * 2 + cta) * (PART_FLOATS / 4) + quarter * 32 + lane;
+        tile = first;
+        if (ep_tid == 0) *arrived = *reinterpret_cast<volatile unsigned int*>(done);
+        named_barrier_sync(1, 128);
+        finish = *arrived == others;
+        if (!finish) {
+          float4* mine = first + wu.part * PART_STEP;
+#pragma unroll 1
+          for (int c = 0; c < BN / 32; ++c) {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(taddr + c * 32, v);
+            tmem_ld_wait();
+            if (n0 + c * 32 < N && row < M) {
+#pragma unroll
+              for (int q = 0; q < 8; ++q)
+                mine[(c * 8 + q) * BM] = make_float4(__uint_as_float(v[4 * q]), __uint_as_float(v[4 * q + 1]), __uint_as_float(v[4 * q + 2]), __uint_as_float(v[4 * q + 3]));
+            }
+          }
+          __threadfence();
+          named_barrier_sync(1, 128);  // every thread has also read `arrived`
+          if (ep_tid == 0) *arrived = atomicAdd(done, 1u);
+          named_barrier_sync(1, 128);
+          finish = *arrived == others;
+        }
+        __threadfence();
+        named_barrier_sync(1, 128);  // `arrived` may be written again
+      }
+      if (finish) {
         const int r_local = quarter * 32 + lane;          // row inside this CTA's 128-row slab
         const uint32_t swz = uint32_t(r_local & 7);
 #pragma unroll 1
@@ -341,6 +382,26 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
             uint32_t v[32];
             tmem_ld_32x32b_x32(taddr + c * CHUNK_COLS + h * 32, v);
             tmem_ld_wait();
+            if (joined && row < M && col + h * 32 < N) {  // the parts in their order, whoever is last
+              float s[32];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) s[j] = 0.f;
+#pragma unroll 1
+              for (int part = 0; part < sched.ksplit; ++part) {
+                if (part == wu.part) {
+#pragma unroll
+                  for (int j = 0; j < 32; ++j) s[j] += __uint_as_float(v[j]);
+                } else {
+                  float4 t[8];
+#pragma unroll
+                  for (int q = 0; q < 8; ++q) t[q] = __ldcg(tile + part * PART_STEP + ((c * (CHUNK_COLS / 32) + h) * 8 + q) * BM);
+#pragma unroll
+                  for (int q = 0; q < 8; ++q) s[4 * q] += t[q].x, s[4 * q + 1] += t[q].y, s[4 * q + 2] += t[q].z, s[4 * q + 3] += t[q].w;
+                }
+              }
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(s[j]);
+            }
             float f[32];
 #pragma unroll
             for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]) * alpha;
@@ -419,7 +480,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
           fence_proxy_async_smem();
           named_barrier_sync(1, 128);
           if (ep_tid == 0) {
-            if ((ACCUM && !pushing) || wu.partial) tma_reduce_add_2d(&tmap_d, buf, col, row0);
+            if ((ACCUM && !pushing) || (wu.partial && !joined)) tma_reduce_add_2d(&tmap_d, buf, col, row0);
             else tma_store_2d(&tmap_d, buf, col, row0);
             for (int p = 0; p < push.n_peers; ++p) tma_store_2d(&peer_maps.m[p], buf, col, row0);
             tma_store_commit();
@@ -469,6 +530,21 @@ const char* make_tmap_2d(CUtensorMap* out, const void* ptr, int fmt, uint64_t ro
 const char* make_tmap_out(CUtensorMap* out, const void* ptr, int fmt, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_cols,
                           uint32_t box_rows);
 
+// the workspace begins with two arrival counters per split tile
+static size_t parts_offset(int split_tiles) { return (size_t(split_tiles) * 2 * sizeof(unsigned int) + 255) & ~size_t(255); }
+static int split_limit(const GemmArgs& g) {  // a pushing launch stores finished sums; partial sums of a K-split tile cannot be pushed
+  return !g.split_tail || g.push.n_peers > 0 ? 1 : 4;
+}
+size_t gemm_pair_workspace(const GemmArgs& g, int num_sms) {
+  using namespace pair;
+  if (g.variant != 1 || num_sms < 2 || g.M <= 0 || g.N <= 0 || g.K <= 0) return 0;
+  const int tiles = ((g.M + 2 * BM - 1) / (2 * BM)) * ((g.N + BN - 1) / BN);
+  const Schedule s = make_schedule(g.M, g.N, (g.K + BK - 1) / BK, std::min(tiles, num_sms / 2), split_limit(g), DEFAULT_GROUP_M);
+  if (s.ksplit == 1) return 0;
+  const int rem = (s.total_units - s.full_tiles) / s.ksplit;
+  return parts_offset(rem) + size_t(rem) * s.ksplit * 2 * PART_FLOATS * sizeof(float);
+}
+
 template <bool A_MN, bool B_MN, bool OUT_F32, bool ACCUM, bool BIAS>
 static cudaError_t launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td, const GemmArgs& g, int num_sms, cudaStream_t stream) {
   using namespace pair;
@@ -485,15 +561,19 @@ static cudaError_t launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, con
   const int tiles = ((g.M + 2 * BM - 1) / (2 * BM)) * ((g.N + BN - 1) / BN);
   int pairs = num_sms / 2;
   if (tiles < pairs) pairs = tiles;
-  // a pushing launch stores finished sums; partial sums of a K-split tile cannot be pushed
-  const int max_split = (!g.split_tail || g.push.n_peers > 0) ? 1 : 4;
+  const int max_split = split_limit(g);
   static const int group_m = [] {
     const char* e = getenv("ELF_B200_GEMM_GROUP_M");
     const int v = e ? atoi(e) : DEFAULT_GROUP_M;
     return v >= 1 && v <= 64 ? v : DEFAULT_GROUP_M;
   }();
   const Schedule sched = make_schedule(g.M, g.N, (g.K + BK - 1) / BK, pairs, max_split, group_m);
-  if (sched.ksplit > 1 && !g.accumulate) {
+  float* parts = nullptr;
+  if (sched.ksplit > 1 && g.workspace != nullptr) {
+    const size_t counters = parts_offset((sched.total_units - sched.full_tiles) / sched.ksplit);
+    parts = reinterpret_cast<float*>(static_cast<char*>(g.workspace) + counters);
+    if (cudaError_t e = cudaMemsetAsync(g.workspace, 0, counters, stream); e != cudaSuccess) return e;
+  } else if (sched.ksplit > 1 && !g.accumulate) {
     // K-split tiles add their partial sums to D, so D must start at zero there.  The split
     // tiles are the last ones of the tile order, all inside the row band that starts at the
     // first row of the group holding the first of them: one memset clears that band (the
@@ -514,7 +594,7 @@ static cudaError_t launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, con
     if (make_tmap_out(&peers.m[p], g.push.peer_out[p], g.out_f32 ? 2 : g.fmt, (uint64_t)g.M, (uint64_t)g.N, (uint64_t)g.ldd, g.out_f32 ? 32 : 64, BM) != nullptr)
       return cudaErrorInvalidValue;
   }
-  kern<<<2 * pairs, NUM_THREADS, SMEM_BYTES, stream>>>(ta, tb, td, g.d, g.bias, g.M, g.N, g.K, g.ldd, (uint32_t)g.fmt, g.alpha, max_split, group_m, g.status, g.push, peers);
+  kern<<<2 * pairs, NUM_THREADS, SMEM_BYTES, stream>>>(ta, tb, td, g.d, g.bias, g.M, g.N, g.K, g.ldd, (uint32_t)g.fmt, g.alpha, max_split, group_m, g.status, g.push, peers, parts, static_cast<unsigned int*>(g.workspace));
   flush_bounds_record(g.status, stream);
   return cudaGetLastError();
 }

@@ -346,7 +346,8 @@ def _restored(t: Union[BlockScaled, torch.Tensor]) -> torch.Tensor:
 def linear_weight_grad(dy: Union[BlockScaled, torch.Tensor], x: Union[BlockScaled, torch.Tensor], out: Optional[torch.Tensor] = None,
                        out_dtype: torch.dtype = torch.bfloat16, push: Optional[dict] = None) -> torch.Tensor:
     """``dy^T x`` summed over all leading dimensions, from 8-bit checkpoints or 16-bit tensors, on the bf16
-    tensor path: the reduction runs over tokens, which have scales of their own.  Added to ``out`` when it is
+    tensor path: the reduction runs over tokens, which have scales of their own.  Accumulated in fp32 and rounded
+    once, the same from call to call.  Added to ``out`` when it is
     given (bf16 or fp32); ``push`` as in ``gemm.linear_weight_grad``."""
     n, k = dy.shape[-1], x.shape[-1]
     if dy.shape[:-1].numel() != x.shape[:-1].numel():

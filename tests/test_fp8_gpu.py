@@ -137,6 +137,30 @@ def test_rows_that_start_anywhere(dev, dtype, cols):
             assert (buffer == 5).all()
 
 
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,k", [(2304, 2304), (2300, 2200)])  # 81 tiles: 7 are left over on 74 pairs, and split
+def test_weight_grad_of_split_tiles(dev, n, k, out):
+    """The parts of a split tile are added in fp32, in one order, and rounded once."""
+    from elf_b200.ops import fp8
+
+    dy, x = fp8.quantize(activations(4100, n, torch.bfloat16, dev, 1)), fp8.quantize(activations(4100, k, torch.bfloat16, dev, 2))
+    a, b = values(dy).T, values(x)
+    got = fp8.linear_weight_grad(dy, x, out_dtype=out)
+    bound = product_bound(a, b, out)
+    assert ((got.double() - a @ b).abs() <= bound).all()
+    assert (got.double() - a @ b).norm() / (a @ b).norm() < (2.0**-9 if out == torch.bfloat16 else 1e-5)
+    for _ in range(3):
+        assert torch.equal(got, fp8.linear_weight_grad(dy, x, out_dtype=out))
+    # added to a gradient: one more rounding, of the sum
+    results = []
+    for _ in range(4):
+        grad = torch.full((n, k), 3.0, device=dev, dtype=out)
+        results.append(fp8.linear_weight_grad(dy, x, out=grad))
+    assert all(torch.equal(results[0], r) for r in results[1:])
+    want = a @ b + 3.0
+    assert ((results[0].double() - want).abs() <= bound + (want.abs() + 3.0) * torch.finfo(out).eps).all()
+
+
 @pytest.mark.parametrize("n,k", [(1, 1), (7, 33), (40, 129), (33, 1043), (129, 7)])
 def test_weight_grad_of_odd_widths(dev, n, k):
     """Rows of the result start anywhere; operands from 8 bits and as they are."""

@@ -347,8 +347,8 @@ def linear_weight_grad(dy: Union[BlockScaled, torch.Tensor], x: Union[BlockScale
                        out_dtype: torch.dtype = torch.bfloat16, push: Optional[dict] = None) -> torch.Tensor:
     """``dy^T x`` summed over all leading dimensions, from 8-bit checkpoints or 16-bit tensors, on the bf16
     tensor path: the reduction runs over tokens, which have scales of their own.  Accumulated in fp32 and rounded
-    once, the same from call to call.  Added to ``out`` when it is
-    given (bf16 or fp32); ``push`` as in ``gemm.linear_weight_grad``."""
+    once, the same from call to call; fp16 and fp32 operands are taken in bf16.  Added to ``out`` when it is given
+    (bf16 or fp32); ``push`` as in ``gemm.linear_weight_grad``."""
     n, k = dy.shape[-1], x.shape[-1]
     if dy.shape[:-1].numel() != x.shape[:-1].numel():
         raise ValueError("linear_weight_grad: dy and x have different numbers of rows")

@@ -1,5 +1,5 @@
-"""Linear layers, norms and activation checkpoints in 8 bits (kernels in ``elf_b200/csrc/fp8_ops.cu`` and
-``fp8_gemm_sm100.cu``).
+"""Linear layers, norms and activation checkpoints in 8 bits (kernels in ``elf_b200/csrc/fp8_ops.cu``,
+``fp8_gemm_sm100.cu`` and ``fp8_gemm_sm100_2cta.cu``).
 
 A ``BlockScaled`` tensor holds e4m3 values and one power-of-two scale per block of 128 columns,
 for each row (activations, gradients) or for each 128 rows (weights).  A block's scale is the smallest

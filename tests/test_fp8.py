@@ -12,6 +12,7 @@ from elf_b200.ops import fp8
 from elf_b200.ops.fp8 import BlockScaled
 from elf_b200.zb_utils import LinearDW, LinearFP8DW, replace_layer_with_layer_dw, replace_linear_with_linear_fp8
 
+from .dist_utils import _free_port
 from .fp8_oracle import held, product_bound, values
 
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
@@ -318,7 +319,7 @@ def test_command_runs_in_8_bits(partitioner):
     import sys
 
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-    cmd = [sys.executable, "-m", "torch.distributed.run", "--nnodes=1", "--nproc-per-node=2", "--master-addr", "127.0.0.1", "--master-port", "29797",
+    cmd = [sys.executable, "-m", "torch.distributed.run", "--nnodes=1", "--nproc-per-node=2", "--master-addr", "127.0.0.1", "--master-port", str(_free_port()),
            os.path.join(root, "benchmarks", "run_transformer.py"), "--architecture", "llama", "--name", "llama-tiny", "--partitioner", partitioner, "--ffn-fp8",
            "--scheduler", "zbh1", "--nmb", "4", "--mb-size", "1", "--niters", "1", "--warmup", "1", "--backend", "gloo"]
     if partitioner != "handcrafted":

@@ -105,14 +105,16 @@ __device__ __forceinline__ void umma_ss_mxf8_pair(uint32_t tmem_d, uint64_t desc
       : "memory");
 }
 
-// Arrival on a barrier of the other CTA without the release, which waits for every earlier memory operation of
-// the thread at cluster scope: 1250 cycles, against the 1024 that the MMAs of a slot take.  The words it
-// announces are shared memory of this CTA, made visible to the tensor core's copy by the proxy fence before it.
-__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+// Arrival on a barrier that may live in the other CTA, after what this warp has written to this CTA's shared memory (each
+// lane's proxy fence and a __syncwarp come before).  The release covers shared memory only: one that also waits for the
+// warp's global accesses takes longer than the MMAs of a slot (4096 x 4096 x 14336: 287 us against 182).  The MMA thread
+// tests the barrier without ordering anything and then acquires, likewise shared memory only (184 us with an acquiring test).
+__device__ __forceinline__ void mbar_arrive_cluster_smem(uint32_t cluster_addr) {
+  asm volatile("fence.release.sync_restrict::shared::cta.cluster;" ::: "memory");
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // Four accumulating MMAs, a block of K apart by A_STEP and B_STEP in the descriptors' address units; returns whether the
-// barrier's phase had completed when the test, issued before them, came up.
+// barrier's phase had completed when the test, issued before them, came up (the caller acquires what it stands for).
 template <int A_STEP, int B_STEP>
 __device__ __forceinline__ bool umma_x4_then_ready(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t sfa, uint32_t bar, uint32_t parity) {
   uint32_t ready;
@@ -121,7 +123,7 @@ __device__ __forceinline__ bool umma_x4_then_ready(uint32_t tmem_d, uint64_t des
       ".reg .pred p, t;\n\t"
       ".reg .b64 a, b;\n\t"
       "setp.eq.b32 p, 0, 0;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 t, [%7], %8;\n\t"
+      "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 t, [%7], %8;\n\t"
       "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%1], %2, %3, %4, [%5], [%6], p;\n\t"
       "add.s64 a, %2, %9;\n\t"
       "add.s64 b, %3, %10;\n\t"
@@ -460,15 +462,18 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       for (int u = pair_id; u < sched.total_units && ok; u += num_pairs, ++i) {
         const Unit unit = unit_at(u, sched, k_blocks, width);
         const int acc = i & 1;
-        if (i > 0 && !mbar_wait(acc_free_bar, uint32_t(i - 1) & 1u, abort_flag)) break;
+        if (i > 0 && !mbar_wait<true>(acc_free_bar, uint32_t(i - 1) & 1u, abort_flag)) break;
         tc_fence_after_sync();
         const uint32_t tmem_d = tmem_base + acc * ACC1;
         bool ready = false;
         for (int kb = unit.kb0; kb < unit.kb1; kb += 2) {
-          if (!ready && !mbar_wait(full_bar(slot), phase, abort_flag)) {
+          if (ready) {
+            fence_acquire_cluster_smem();
+          } else if (!mbar_wait<true>(full_bar(slot), phase, abort_flag)) {
             ok = false;
             break;
           }
+          tc_fence_after_sync();
           const int next = slot + 1 == SLOTS ? 0 : slot + 1;
           const uint32_t next_phase = phase ^ (next == 0 ? 1u : 0u);
           const uint32_t sfa = tmem_base + SF_COL + (sf_count++ & 1) * 16;
@@ -635,7 +640,7 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         store_scale_words(sf_base + slot * SF_BYTES + 1024, lane, b1);
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(full_bar(slot), 0));
+        if (lane == 0) mbar_arrive_cluster_smem(map_to_cta(full_bar(slot), 0));
         if (++slot == SLOTS) {
           slot = 0;
           phase ^= 1u;

@@ -136,14 +136,40 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
+// What other CTAs of the cluster did to shared memory before their arrivals (released there), ordered behind a relaxed test of
+// the barrier that has succeeded.
+__device__ __forceinline__ void fence_acquire_cluster_smem() {
+  asm volatile("fence.acquire.sync_restrict::shared::cluster.cluster;" ::: "memory");
+}
+__device__ __forceinline__ bool mbar_test_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred P;\n\t"
+      "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 P, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, P;\n\t"
+      "}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
 // Bounded wait.  `abort_flag` lives in shared memory: the first role that gives up raises
 // it and every other waiter of the CTA leaves at its next poll, so the CTA always reaches
-// its common exit path (TMEM dealloc) instead of hanging the SM.
+// its common exit path (TMEM dealloc) instead of hanging the SM.  CLUSTER: the arrivals come from other CTAs as well.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  if (mbar_try_wait(bar, parity)) return true;
+  auto ready = [&] {
+    if (!CLUSTER) return mbar_try_wait(bar, parity);
+    if (!mbar_test_cluster(bar, parity)) return false;
+    fence_acquire_cluster_smem();
+    return true;
+  };
+  if (ready()) return true;
   const unsigned long long t0 = globaltimer_ns();
   for (uint32_t it = 1;; ++it) {
-    if (mbar_try_wait(bar, parity)) return true;
+    if (ready()) return true;
     if ((it & 0xffu) == 0) {
       if (*abort_flag) return false;
       if (globaltimer_ns() - t0 > kWaitLimitNs) {

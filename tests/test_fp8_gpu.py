@@ -465,3 +465,53 @@ def test_split_last_wave(dev):
     assert (y.double() - a @ b).norm() / (a @ b).norm() < 1e-4
     for _ in range(3):
         assert torch.equal(y, fp8.linear_forward(x, w, out_dtype=torch.float32))
+
+
+def loud_and_quiet(rows, cols, dev, block_rows=1, seed=0):
+    """Block-scaled matrix whose neighbouring blocks differ by up to 2^24 in scale, drawn block by block: a block multiplied by
+    the scale of another is far off."""
+    from elf_b200.ops import fp8
+
+    g = torch.Generator(device=dev).manual_seed(seed)
+    q = (fp8.quantize if block_rows == 1 else fp8.quantize_weight)(torch.randn(rows, cols, device=dev, generator=g))
+    scale = torch.randint(115, 140, q.scale.shape, device=dev, generator=g).to(torch.uint8)
+    q.scale.copy_(scale)
+    return q
+
+
+@pytest.mark.parametrize("m,n,k", [(3000, 4100, 4200), (2304, 2304, 14336)])
+def test_scales_belong_to_their_blocks(dev, m, n, k):
+    """Scale words that the tensor core reads are those of the blocks it multiplies, in every tile and at every repetition."""
+    from elf_b200.ops import fp8
+
+    x, w = loud_and_quiet(m, k, dev, seed=1), loud_and_quiet(n, k, dev, 128, seed=2)
+    a, b = values(x), values(w).T
+    want, bound = a @ b, product_bound(a, b, torch.float32)
+    first = fp8.linear_forward(x, w, out_dtype=torch.float32)
+    assert ((first.double() - want).abs() <= bound).all()
+    for _ in range(40):
+        assert torch.equal(fp8.linear_forward(x, w, out_dtype=torch.float32), first)
+    dy = loud_and_quiet(m, n, dev, seed=3)
+    a, b = values(dy), values(w)
+    want, bound = a @ b, product_bound(a, b, torch.float32)
+    first = fp8.linear_input_grad(dy, w, torch.float32)
+    assert ((first.double() - want).abs() <= bound).all()
+    for _ in range(40):
+        assert torch.equal(fp8.linear_input_grad(dy, w, torch.float32), first)
+
+
+def test_gated_forms_repeat_themselves(dev):
+    """Several units for every pair of CTAs, blocks of very different scales: every repetition gives the same bits."""
+    from elf_b200.ops import fp8
+
+    m, d, f = 3000, 1160, 3200
+    x, wg, wd = loud_and_quiet(m, d, dev, seed=1), loud_and_quiet(2 * f, d, dev, 128, seed=2), loud_and_quiet(d, f, dev, 128, seed=3)
+    dy, gate_up = loud_and_quiet(m, d, dev, seed=4), fp8.quantize(activations(m, 2 * f, torch.bfloat16, dev, 5))
+    same_bits = lambda p, q: torch.equal(p.data.view(torch.uint8), q.data.view(torch.uint8)) and torch.equal(p.scale, q.scale)  # noqa: E731
+    act, gu = fp8.gated_forward(x, wg)
+    grad = fp8.gated_backward(dy, wd, gate_up)
+    want, err = projections(x, wg, d)
+    check_held(gu, want, err)
+    for _ in range(40):
+        for got, first in zip((*fp8.gated_forward(x, wg), fp8.gated_backward(dy, wd, gate_up)), (act, gu, grad)):
+            assert same_bits(got, first)

@@ -37,6 +37,7 @@ from __future__ import annotations
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _ext
 from . import gemm as _gemm
@@ -166,6 +167,12 @@ def _matrix(t: torch.Tensor) -> torch.Tensor:
 def _need_float(t: torch.Tensor, name: str) -> None:
     if t.dtype not in _FLOATS:
         raise TypeError(f"{name} must be bf16, fp16 or fp32, got {t.dtype}")
+
+
+def _no_tangent(t: torch.Tensor, what: str) -> None:
+    # a dual tensor need not require grad: past the autograd function its tangent would be lost without a word
+    if _forward_ad.unpack_dual(t).tangent is not None:
+        raise NotImplementedError(f"{what}: forward-mode derivatives are not implemented")
 
 
 def _same_device(name: str, t, other: str, u) -> None:
@@ -459,7 +466,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
 
     ``w_q``: the weight's block-scaled copy (``quantize_weight(w)``), which a training loop makes once per
     optimizer step; without it every call makes its own.  The gradients are those of the product with the
-    rounded operands, passed through the rounding unchanged."""
+    rounded operands, passed through the rounding unchanged; reverse mode only."""
     _check_differentiable("linear", x, w, bias)
     if not (w.dim() == 2 and x.dim() >= 1 and x.shape[-1] == w.shape[1]):
         raise ValueError(f"linear: x {tuple(x.shape)} does not match a weight of shape {tuple(w.shape)}")
@@ -541,5 +548,6 @@ def _check_differentiable(what: str, x: torch.Tensor, *others) -> None:
     for t in (x, *others):
         if t is not None:
             _need_float(t, what)
+            _no_tangent(t, what)
             if t.device != x.device:
                 raise ValueError(f"{what}: all tensors must be on one device, got {t.device} and {x.device}")

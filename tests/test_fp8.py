@@ -180,6 +180,24 @@ def test_gated_ffn_without_elements(m, d, f, out):
         assert g.shape == t.shape and not g.isnan().any()
 
 
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_forward_mode_is_refused(which):
+    """A dual tensor need not require grad: its tangent is refused, not dropped, whichever argument carries it."""
+    from torch.autograd import forward_ad
+
+    calls = ((fp8.linear, [rand(4, 64), rand(8, 64, seed=1), rand(8, seed=2)]), (fp8.gated_ffn, [rand(4, 64), rand(256, 64, seed=1), rand(8, 128, seed=2)]))
+    for f, args in calls:
+        with forward_ad.dual_level():
+            dual = list(args)
+            dual[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                f(*dual)
+            assert torch.equal(f(*args), f(*args))  # without a tangent: as ever
+        call = lambda t: f(*args[:which], t, *args[which + 1 :])  # noqa: B023, E731
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.func.jvp(call, (args[which],), (torch.ones_like(args[which]),))
+
+
 # ------------------------------------------------------------------------------ split-backward layer
 
 

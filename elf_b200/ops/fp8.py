@@ -169,9 +169,11 @@ def _need_float(t: torch.Tensor, name: str) -> None:
         raise TypeError(f"{name} must be bf16, fp16 or fp32, got {t.dtype}")
 
 
-def _no_tangent(t: torch.Tensor, what: str) -> None:
+def _no_tangent(what: str, *tensors) -> None:
     # a dual tensor need not require grad: past the autograd function its tangent would be lost without a word
-    if _forward_ad.unpack_dual(t).tangent is not None:
+    if getattr(_forward_ad, "_current_level", 0) < 0:  # spares small calls a look at every tensor
+        return
+    if any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError(f"{what}: forward-mode derivatives are not implemented")
 
 
@@ -286,9 +288,24 @@ def _norm(x, residual, w, eps):
     return BlockScaled._made(data, scale), rstd, h
 
 
+class _AddNorm(torch.autograd.Function):
+    """``add_rms_norm`` as a node of the graph: the residual stream passes its gradient on to both terms."""
+
+    @staticmethod
+    def forward(ctx, x, residual, w, eps):
+        q, rstd, h = _norm(x, residual, w, eps)
+        ctx.mark_non_differentiable(q.data, q.scale, rstd)
+        ctx.set_materialize_grads(False)
+        return h, q.data, q.scale, rstd
+
+    @staticmethod
+    def backward(ctx, dh, *_):
+        return dh, dh, None, None
+
+
 def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-5) -> Tuple[BlockScaled, torch.Tensor]:
     """``(q, rstd)``: ``x * rstd * w`` in 8 bits with ``rstd = (mean(x^2) + eps)^-1/2`` in fp32, the statistic
-    that ``elf_b200.ops.fused``'s RMSNorm backward takes.  One pass over ``x``; the kernel handles bf16 with a width that
+    that ``elf_b200.ops.fused``'s RMSNorm backward takes; neither is differentiable.  One pass over ``x``; the kernel handles bf16 with a width that
     is a multiple of 8, at most 8192, as ``fused.rms_norm`` does, other inputs take torch operations."""
     q, rstd, _ = _norm(x, None, w, eps)
     return q, rstd
@@ -296,8 +313,12 @@ def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-5) -> Tuple[Block
 
 def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, w: torch.Tensor, eps: float = 1e-5) -> Tuple[BlockScaled, torch.Tensor, torch.Tensor]:
     """``(q, rstd, h)`` with ``h = x + residual`` (rounded to the inputs' type; the norm is that of the
-    rounded sum, which is what later passes read back)."""
-    return _norm(x, residual, w, eps)
+    rounded sum, which is what later passes read back).  ``h`` is differentiable, ``q`` and ``rstd`` are not."""
+    _no_tangent("add_rms_norm", x, residual)
+    if residual is None or not (torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad)):
+        return _norm(x, residual, w, eps)
+    h, data, scale, rstd = _AddNorm.apply(x, residual, w, eps)
+    return BlockScaled._made(data, scale), rstd, h
 
 
 # ------------------------------------------------------------------------------ products
@@ -545,9 +566,9 @@ def gated_ffn(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, ga
 
 
 def _check_differentiable(what: str, x: torch.Tensor, *others) -> None:
+    _no_tangent(what, x, *others)
     for t in (x, *others):
         if t is not None:
             _need_float(t, what)
-            _no_tangent(t, what)
             if t.device != x.device:
                 raise ValueError(f"{what}: all tensors must be on one device, got {t.device} and {x.device}")

@@ -198,6 +198,29 @@ def test_forward_mode_is_refused(which):
             torch.func.jvp(call, (args[which],), (torch.ones_like(args[which]),))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_residual_stream_keeps_its_gradient(dtype):
+    """``h`` of ``add_rms_norm`` passes its gradient to both terms; values and statistic are those without a graph."""
+    x, r, w = rand(3, 5, 64, dtype=dtype), rand(3, 5, 64, dtype=dtype, seed=1), rand(64, dtype=dtype, seed=2)
+    want = fp8.add_rms_norm(x, r, w)
+    dh = rand(3, 5, 64, dtype=dtype, seed=3)
+    for needs in ((True, True), (True, False), (False, True)):
+        leaves = [t.clone().requires_grad_(n) for t, n in zip((x, r), needs)]
+        q, rstd, h = fp8.add_rms_norm(leaves[0], leaves[1], w.clone().requires_grad_())
+        assert torch.equal(h, want[2]) and torch.equal(rstd, want[1]) and not rstd.requires_grad
+        assert torch.equal(values(q), values(want[0])) and torch.equal(q.scale, want[0].scale)
+        h.backward(dh)
+        for t, n in zip(leaves, needs):
+            assert torch.equal(t.grad, dh) if n else t.grad is None
+    both = x.clone().requires_grad_()  # the same tensor twice
+    fp8.add_rms_norm(both, both, w)[2].backward(dh)
+    assert torch.equal(both.grad, dh + dh)
+    with torch.no_grad():
+        assert not fp8.add_rms_norm(x.requires_grad_(), r, w)[2].requires_grad
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda t: fp8.add_rms_norm(t, r, w)[2], (x.detach(),), (dh,))
+
+
 # ------------------------------------------------------------------------------ split-backward layer
 
 

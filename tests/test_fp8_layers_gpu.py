@@ -87,6 +87,22 @@ def test_linear_gradients(dev, m, n, k):
     assert ((leaves[2].grad.double() - dy.double().sum(0)).abs() <= dy.double().sum(0).abs() * 2.0**-8 + m * 2.0**-24 * dy.double().abs().sum(0)).all()
 
 
+def test_residual_stream_keeps_its_gradient(dev):
+    """``h`` of ``add_rms_norm`` between two layers in 8 bits: its gradient reaches both terms."""
+    from elf_b200.ops import fp8
+
+    x, r, g = (activations(200, 256, torch.bfloat16, dev, s) for s in (0, 1, 2))
+    gain, w = activations(1, 256, torch.bfloat16, dev, 3)[0].requires_grad_(), activations(64, 256, torch.bfloat16, dev, 4)
+    plain_q, plain_rstd, plain_h = fp8.add_rms_norm(x, r, gain)
+    assert not plain_h.requires_grad
+    x.requires_grad_(), r.requires_grad_()
+    q, rstd, h = fp8.add_rms_norm(x, r, gain)
+    assert torch.equal(h, plain_h) and torch.equal(rstd, plain_rstd) and same(values(q), values(plain_q)) and not rstd.requires_grad
+    y = fp8.linear(h, w)
+    dx, dr, dh = torch.autograd.grad((y, h), (x, r, h), (torch.ones_like(y), g))
+    assert torch.equal(dx, dh) and torch.equal(dr, dh) and dh.any()
+
+
 def test_gradients_that_are_not_dense(dev):
     """An expanded (stride 0) and a strided output gradient."""
     from elf_b200.ops import fp8

@@ -347,13 +347,34 @@ def _product(a: BlockScaled, b: BlockScaled, transposed: bool, bias, out_dtype) 
     return _ext.get().fp8_gemm(a.data, a.scale, b.data, b.scale, _shift(b), transposed, out_dtype, bias, _gemm.status(a.device))
 
 
+class _Biased(torch.autograd.Function):
+    """``linear_forward`` as a node of the graph: its bias has a gradient, its 8-bit operands have none."""
+
+    @staticmethod
+    def forward(ctx, bias, x, w, out_dtype):
+        ctx.dtype = bias.dtype
+        return _product(x, w, False, bias, out_dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        return _bias_grad(dy, ctx.dtype), None, None, None
+
+
+def _bias_grad(dy: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    return _matrix(dy).float().sum(0).to(dtype)
+
+
 def linear_forward(x: BlockScaled, w: BlockScaled, bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``x W^T (+ bias)`` for ``x [..., K]`` scaled by rows and ``w [N, K]`` scaled by tiles or rows; accumulated in
     fp32 and rounded once.  On the GPU a bias of another type is taken in ``out_dtype``, the type a layer of that type holds
-    it in."""
+    it in.  The result is differentiable with respect to the bias; ``linear`` is the form for all operands."""
     _check_product(x, w, 1, "linear_forward")
     if not (bias is None or (bias.shape == (w.shape[0],) and bias.device == w.device)):
         raise ValueError("linear_forward: the bias must be a vector with one element per output")
+    _no_tangent("linear_forward", bias)
+    if bias is not None and bias.requires_grad and torch.is_grad_enabled():
+        return _Biased.apply(bias, x, w, out_dtype)
     return _product(x, w, False, bias, out_dtype)
 
 
@@ -478,7 +499,7 @@ class _Linear(torch.autograd.Function):
         if ctx.needs_input_grad[1]:
             dw = linear_weight_grad(dyq, BlockScaled._made(data, scale), out_dtype=ctx.w_dtype)
         if ctx.needs_input_grad[2]:
-            db = _matrix(dy).float().sum(0).to(ctx.bias_dtype)
+            db = _bias_grad(dy, ctx.bias_dtype)
         return dx, dw, db, None
 
 

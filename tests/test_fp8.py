@@ -221,6 +221,23 @@ def test_residual_stream_keeps_its_gradient(dtype):
         torch.func.jvp(lambda t: fp8.add_rms_norm(t, r, w)[2], (x.detach(),), (dh,))
 
 
+@pytest.mark.parametrize("lead", [(7,), (2, 3), ()])
+def test_bias_keeps_its_gradient(lead):
+    """The product of 8-bit operands is differentiable with respect to its bias, and to nothing else."""
+    x, w = fp8.quantize(rand(*lead, 200)), fp8.quantize_weight(rand(24, 200, seed=1))
+    bias = rand(24, seed=2)
+    plain = fp8.linear_forward(x, w, bias, torch.float32)
+    y = fp8.linear_forward(x, w, bias.requires_grad_(), torch.float32)
+    assert torch.equal(y, plain) and not plain.requires_grad
+    dy = rand(*lead, 24, seed=3)
+    y.backward(dy)
+    # an fp32 sum of as many terms as there are rows
+    rows = dy.reshape(-1, 24).double()
+    assert ((bias.grad.double() - rows.sum(0)).abs() <= len(rows) * 2.0**-24 * rows.abs().sum(0)).all()
+    with torch.no_grad():
+        assert not fp8.linear_forward(x, w, bias).requires_grad
+
+
 # ------------------------------------------------------------------------------ split-backward layer
 
 

@@ -103,6 +103,25 @@ def test_residual_stream_keeps_its_gradient(dev):
     assert torch.equal(dx, dh) and torch.equal(dr, dh) and dh.any()
 
 
+@pytest.mark.parametrize("lead", [(7,), (2, 3), ()])
+def test_bias_keeps_its_gradient(dev, lead):
+    """The product of 8-bit operands is differentiable with respect to its bias, and to nothing else."""
+    from elf_b200.ops import fp8
+
+    x, w = fp8.quantize(torch.randn(*lead, 200, device=dev)), fp8.quantize_weight(activations(24, 200, torch.float32, dev, 1))
+    bias = activations(1, 24, torch.float32, dev, 2)[0]
+    plain = fp8.linear_forward(x, w, bias, torch.float32)
+    y = fp8.linear_forward(x, w, bias.requires_grad_(), torch.float32)
+    assert torch.equal(y, plain) and not plain.requires_grad
+    dy = torch.randn(*lead, 24, device=dev)
+    y.backward(dy)
+    # an fp32 sum of as many terms as there are rows
+    rows = dy.reshape(-1, 24).double()
+    assert ((bias.grad.double() - rows.sum(0)).abs() <= len(rows) * 2.0**-24 * rows.abs().sum(0)).all()
+    with torch.no_grad():
+        assert not fp8.linear_forward(x, w, bias).requires_grad
+
+
 def test_gradients_that_are_not_dense(dev):
     """An expanded (stride 0) and a strided output gradient."""
     from elf_b200.ops import fp8

@@ -46,6 +46,12 @@ __device__ __forceinline__ float mul_exact(float a, float b) {
   return r;
 }
 
+__device__ __forceinline__ float add_exact(float a, float b) {
+  float r;
+  asm("add.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // Two fp32 operations in one instruction, on a pair in a 64-bit register; subnormal numbers survive.
 __device__ __forceinline__ uint64_t pair_of(float a, float b) {
   uint64_t r;

@@ -384,6 +384,50 @@ __global__ void __launch_bounds__(THREADS) repack_kernel(const uint8_t* __restri
   for (int i = 0; i < 2 * UNITS; ++i) store_raw<uint8_t, TO>(dst + (long long)row[i] * ld_dst + col[i], col[i], have[i], raw[i]);
 }
 
+// ------------------------------------------------------------------------------ 16- and 32-bit values as sums of bf16
+// Operands of the 16-bit product that are not bf16: a value is cut off after 8 significant bits, what is left again.  fp16 has
+// 11 bits and is the sum of two parts, fp32 has 24 and is that of three, both exactly (down to bf16's smallest step, 2^-133).
+// Infinities and NaN are all in the first part.
+template <typename T>
+constexpr int BF16_PARTS = sizeof(T) == 2 ? 2 : 3;
+template <typename T, Access A>
+__global__ void __launch_bounds__(THREADS) bf16_parts_kernel(const T* __restrict__ x, long long ldx, __nv_bfloat16* __restrict__ out, long long ldo,
+                                                             long long part_step, uint32_t total, uint32_t units_per_row, int cols, Span span) {
+  await_previous();
+  Raw<T> raw[UNITS];
+  const T* src[UNITS];
+  uint32_t row[UNITS];
+  int col[UNITS], have[UNITS];
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) {
+    const uint32_t u = (blockIdx.x * UNITS + i) * THREADS + threadIdx.x;
+    row[i] = u / units_per_row;
+    col[i] = int(u - row[i] * units_per_row) * UNIT;
+    have[i] = u < total ? min(cols - col[i], UNIT) : 0;
+    src[i] = x + (long long)row[i] * ldx + col[i];
+  }
+  load_groups<T, A>(src, have, span, raw);
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) {
+    float v[UNIT];
+    unpack<T>(raw[i], v);
+#pragma unroll
+    for (int p = 0; p < BF16_PARTS<T>; ++p) {
+      Raw<__nv_bfloat16> part;
+      __nv_bfloat16* e = reinterpret_cast<__nv_bfloat16*>(part.q);
+#pragma unroll
+      for (int j = 0; j < UNIT; ++j) {
+        const uint32_t bits = __float_as_uint(v[j]);
+        const bool finite = abs_bits(v[j]) < kInfBits;
+        const uint32_t top = abs_bits(v[j]) > kInfBits ? 0x7fc00000u : bits & 0xffff0000u;  // NaN stays NaN without its low bits
+        e[j] = __ushort_as_bfloat16(uint16_t(top >> 16));
+        v[j] = finite ? add_exact(v[j], __uint_as_float(top ^ 0x80000000u)) : 0.f;
+      }
+      store_raw<__nv_bfloat16, Access::kPieces16>(out + p * part_step + (long long)row[i] * ldo + col[i], col[i], have[i], part);
+    }
+  }
+}
+
 // ------------------------------------------------------------------------------ RMSNorm
 // h = x + residual (rounded to bf16, as the next residual addition reads it), y = h * rstd * w, y in
 // 8 bits.  Each thread holds 8 values (16 bytes) of a row per step; the 16 lanes whose values make up a
@@ -666,6 +710,22 @@ cudaError_t dequantize_as(const uint8_t* data, long long ldq, const uint8_t* sca
   return cudaSuccess;
 }
 
+template <typename T>
+cudaError_t bf16_parts_as(const void* x, long long ldx, void* out, long long ldo, long long part_step, long long rows, int cols, cudaStream_t stream) {
+  const Span span = span_of<T>(x, ldx, rows, cols);
+  const uint32_t upr = uint32_t((cols + UNIT - 1) / UNIT);
+  const long long step = rows_per_launch(upr);
+  auto* kern = aligned(x, ldx * sizeof(T), 16) ? bf16_parts_kernel<T, Access::kPieces16> : bf16_parts_kernel<T, Access::kShifted>;
+  for (long long r = 0; r < rows; r += step) {
+    const uint32_t total = uint32_t(std::min(step, rows - r)) * upr;
+    if (cudaError_t e = launch_overlapped(kern, (total + UNITS * THREADS - 1) / (UNITS * THREADS), THREADS, 0, 0, stream, static_cast<const T*>(x) + r * ldx, ldx,
+                                          static_cast<__nv_bfloat16*>(out) + r * ldo, ldo, part_step, total, upr, cols, span);
+        e != cudaSuccess)
+      return e;
+  }
+  return cudaSuccess;
+}
+
 template <int VPT>
 cudaError_t rmsnorm_warps(const NormArgs& p, cudaStream_t stream) {
   auto* kern = p.res ? rmsnorm_fp8_warp_kernel<VPT, true> : rmsnorm_fp8_warp_kernel<VPT, false>;
@@ -733,6 +793,15 @@ cudaError_t fp8_repack(const void* src, long long ld_src, void* dst, long long l
       return e;
   }
   return cudaSuccess;
+}
+
+int bf16_parts(Elem type) { return type == Elem::kBf16 ? 1 : type == Elem::kF16 ? BF16_PARTS<__half> : BF16_PARTS<float>; }
+cudaError_t split_into_bf16_parts(const void* x, Elem type, long long ldx, void* out, long long ldo, long long part_step, long long rows, int cols,
+                                  cudaStream_t stream) {
+  if (rows <= 0 || cols <= 0) return cudaSuccess;
+  if (type == Elem::kBf16) return cudaErrorInvalidValue;
+  if (type == Elem::kF16) return bf16_parts_as<__half>(x, ldx, out, ldo, part_step, rows, cols, stream);
+  return bf16_parts_as<float>(x, ldx, out, ldo, part_step, rows, cols, stream);
 }
 
 cudaError_t fp8_rmsnorm(const void* x, const void* residual, const void* w, void* h, float* rstd, uint8_t* data, long long ldq, uint8_t* scale,

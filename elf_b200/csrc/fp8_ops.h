@@ -22,6 +22,11 @@ cudaError_t fp8_dequantize(const uint8_t* data, long long ldq, const uint8_t* sc
                            long long rows, int cols, cudaStream_t stream);
 // copies rows of bytes to another pitch (pitches in bytes)
 cudaError_t fp8_repack(const void* src, long long ld_src, void* dst, long long ld_dst, long long rows, int row_bytes, cudaStream_t stream);
+// x [rows][cols] (fp16 or fp32, pitch ldx elements) as bf16_parts(type) bf16 matrices whose sum it is, the largest first: part p
+// begins p * part_step elements into `out`, whose rows are ldo elements apart (16-byte aligned, ldo a multiple of 8)
+int bf16_parts(Elem type);
+cudaError_t split_into_bf16_parts(const void* x, Elem type, long long ldx, void* out, long long ldo, long long part_step, long long rows, int cols,
+                                  cudaStream_t stream);
 // h = x + residual (bf16, written when residual is given); data/scale = blocks of h * rstd * w
 cudaError_t fp8_rmsnorm(const void* x, const void* residual, const void* w, void* h, float* rstd, uint8_t* data, long long ldq, uint8_t* scale,
                         long long lds, long long rows, int dim, double eps, int num_sms, cudaStream_t stream);

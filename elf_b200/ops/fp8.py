@@ -388,22 +388,28 @@ def linear_input_grad(dy: BlockScaled, w: BlockScaled, out_dtype: torch.dtype = 
 
 
 def _restored(t: Union[BlockScaled, torch.Tensor]) -> torch.Tensor:
-    """bf16 matrix for the 16-bit weight-gradient product.  Exact for a block-scaled tensor."""
-    return _matrix(t.dequantize() if isinstance(t, BlockScaled) else t.detach().to(torch.bfloat16))
+    """bf16 matrix for the 16-bit weight-gradient product, exact for a block-scaled tensor."""
+    return _matrix(t.dequantize() if isinstance(t, BlockScaled) else t.detach())
 
 
 def linear_weight_grad(dy: Union[BlockScaled, torch.Tensor], x: Union[BlockScaled, torch.Tensor], out: Optional[torch.Tensor] = None,
                        out_dtype: torch.dtype = torch.bfloat16, push: Optional[dict] = None) -> torch.Tensor:
     """``dy^T x`` summed over all leading dimensions, from 8-bit checkpoints or 16-bit tensors, on the bf16
     tensor path: the reduction runs over tokens, which have scales of their own.  Accumulated in fp32 and rounded
-    once, the same from call to call; fp16 and fp32 operands are taken in bf16.  Added to ``out`` when it is given
-    (bf16 or fp32); ``push`` as in ``gemm.linear_weight_grad``."""
+    once, the same from call to call; fp16 and fp32 operands enter whole, as two and three bf16 parts and a product for
+    each.  Added to ``out`` when it is given (bf16 or fp32); ``push`` as in ``gemm.linear_weight_grad``, from 8-bit or
+    bf16 operands."""
     n, k = dy.shape[-1], x.shape[-1]
     if dy.shape[:-1].numel() != x.shape[:-1].numel():
         raise ValueError("linear_weight_grad: dy and x have different numbers of rows")
     if any(isinstance(t, BlockScaled) and t.block_rows != 1 for t in (dy, x)):
         raise ValueError("linear_weight_grad: activations and gradients must be scaled by rows")
     _same_device("dy", dy, "x", x)
+    for name, t in (("dy", dy), ("x", x)):
+        if not isinstance(t, BlockScaled):
+            _need_float(t, name)
+            if push and t.dtype != torch.bfloat16:
+                raise ValueError(f"linear_weight_grad: a push takes 8-bit or bf16 operands, got {name} in {t.dtype}")
     if not (out is None or (out.shape == (n, k) and out.device == x.device and out.dtype in (torch.bfloat16, torch.float32))):
         raise ValueError(f"linear_weight_grad: out must be a bf16 or fp32 matrix [{n}, {k}]")
     if out_dtype not in _FLOATS:

@@ -100,6 +100,19 @@ def test_gated_ffn_matches_its_parts_and_saves_8_bits():
         assert torch.equal(fp8.gated_ffn(x, wg, wd), y)
 
 
+def test_weight_gradient_operands():
+    """Plain operands enter with their own type's bits; a push takes only what is one bf16 matrix."""
+    x = rand(40, 30)
+    for dtype in DTYPES:
+        dy = rand(40, 20, dtype=dtype, seed=1)
+        a, b = dy.double().T, x.double()
+        assert ((fp8.linear_weight_grad(dy, x, out_dtype=torch.float32).double() - a @ b).abs() <= product_bound(a, b, torch.float32)).all()
+    with pytest.raises(TypeError, match="dy must be"):
+        fp8.linear_weight_grad(rand(40, 20).double(), x)
+    with pytest.raises(ValueError, match="push takes"):
+        fp8.linear_weight_grad(rand(40, 20), x.bfloat16(), out=torch.zeros(20, 30, dtype=torch.bfloat16), push={"tag": 1})
+
+
 def test_only_requested_gradients():
     x, w = rand(4, 64), rand(8, 64).requires_grad_()
     fp8.linear(x, w).sum().backward()

@@ -178,6 +178,72 @@ def test_weight_grad_of_odd_widths(dev, n, k):
             assert ((got.double() - want).abs() <= mag * 300 * 2.0**-23 + want.abs() * torch.finfo(out).eps + 2.0**-24).all()
 
 
+def parts_bound(a, b, out, pairs):
+    """Bound on the error of ``a @ b`` as the sum of ``pairs`` products of bf16 parts of the operands, added in fp32: the parts
+    of a value add up to at most 1 + 2^-7 + 2^-15 of its magnitude, which enters once for each operand, and every product after the first
+    adds half a unit of the sum."""
+    return product_bound(a, b, out) * (1 + 2.0**-6 + 2.0**-12) + pairs * 2.0**-24 * (a.abs() @ b.abs()) * (1 + 2.0**-5)
+
+
+@pytest.mark.parametrize("tokens,n,k", [(1, 1, 1), (5, 7, 33), (64, 136, 264), (300, 130, 72), (2304, 264, 1040)])
+@pytest.mark.parametrize("dtype,parts", [(torch.float16, 2), (torch.float32, 3)])
+def test_weight_grad_of_whole_operands(dev, tokens, n, k, dtype, parts):
+    """fp16 and fp32 operands enter with all their bits, at any address and pitch."""
+    from elf_b200.ops import fp8
+
+    wide = activations(tokens, n + 40, dtype, dev, 1)
+    x16 = activations(tokens, k, dtype, dev, 2)
+    xq = fp8.quantize(x16)
+    for dy in (wide[:, :n], wide[:, 3 : n + 3], wide[:, 8 : n + 8].contiguous()):
+        for x, xv, pairs in ((xq, values(xq), parts), (x16, x16.double(), parts * parts), (x16.bfloat16(), x16.bfloat16().double(), parts)):
+            a = dy.double().T
+            for out in DTYPES:
+                got = fp8.linear_weight_grad(dy, x, out_dtype=out)
+                assert got.dtype == out and ((got.double() - a @ xv).abs() <= parts_bound(a, xv, out, pairs)).all()
+                assert torch.equal(got, fp8.linear_weight_grad(dy, x, out_dtype=out))
+            for out in (torch.bfloat16, torch.float32):
+                grad = torch.full((n, k), 3.0, device=dev, dtype=out)
+                assert fp8.linear_weight_grad(dy, x, out=grad).data_ptr() == grad.data_ptr()
+                want = a @ xv + 3.0
+                bound = parts_bound(a, xv, torch.float32, pairs) + (pairs + 1) * 2.0**-23 * (3.0 + (a.abs() @ xv.abs()))
+                assert ((grad.double() - want).abs() <= bound + torch.finfo(out).eps / 2 * (want.abs() + bound)).all()
+        # the other operand in 8 bits
+        dyq = fp8.quantize(dy)
+        a = values(dyq).T
+        assert ((fp8.linear_weight_grad(dyq, x16, out_dtype=torch.float32).double() - a @ x16.double()).abs() <= parts_bound(a, x16.double(), torch.float32, parts)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_weight_grad_of_whole_operands_not_finite(dev, dtype):
+    """An infinity stays one, a NaN as well, also one whose payload is in its low bits; columns do not see each other."""
+    from elf_b200.ops import fp8
+
+    dy, x = activations(40, 72, dtype, dev, 1), fp8.quantize(torch.ones(40, 136, device=dev))
+    clean = fp8.linear_weight_grad(dy, x, out_dtype=torch.float32)
+    bits = torch.int16 if dtype == torch.float16 else torch.int32
+    dy[3, 5], dy[7, 9], dy[0, 70] = float("inf"), float("-inf"), float("nan")
+    dy.view(bits)[2, 33] = 0x7C01 if dtype == torch.float16 else 0x7F800001
+    got = fp8.linear_weight_grad(dy, x, out_dtype=torch.float32)
+    rows = torch.ones(72, dtype=torch.bool, device=dev)
+    rows[[5, 9, 33, 70]] = False
+    assert torch.equal(got[rows], clean[rows])
+    assert (got[5] == float("inf")).all() and (got[9] == float("-inf")).all() and got[70].isnan().all() and got[33].isnan().all()
+
+
+def test_weight_grad_of_the_largest_and_smallest_operands(dev):
+    """fp32 from its largest values to below bf16's smallest normal one."""
+    from elf_b200.ops import fp8
+
+    for scale in (2.0**126, 2.0**-120, 2.0**-128):
+        dy = (torch.rand(3, 40, device=dev, dtype=torch.float64) + 1) * scale
+        dy = dy.float()
+        x = fp8.quantize(torch.ones(3, 16, device=dev) * 2.0**-4)
+        a, b = dy.double().T, values(x)
+        got = fp8.linear_weight_grad(dy, x, out_dtype=torch.float32)
+        # what lies below 2^-133 of a value is not held by bf16, and the tensor core's fp32 sums may drop subnormal ones
+        assert ((got.double() - a @ b).abs() <= parts_bound(a, b, torch.float32, 3) + 3 * 2.0**-126).all()
+
+
 def test_empty_tensors(dev):
     from elf_b200.ops import fp8
 

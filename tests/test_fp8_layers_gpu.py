@@ -68,6 +68,22 @@ def test_gated_ffn_is_its_parts(dev, m, d, f, dtype):
         assert torch.equal(fp8.gated_ffn(x, wg, wd, **held), y)
 
 
+@pytest.mark.parametrize("dtype,parts", [(torch.float16, 2), (torch.float32, 3)])
+def test_gated_ffn_down_gradient_takes_the_whole_output_gradient(dev, dtype, parts):
+    """The down weight's gradient is that of the output's gradient as it is and of the held activation, against 64 bits."""
+    from elf_b200.ops import fp8
+
+    from .test_fp8_gpu import parts_bound
+
+    x, wg, wd, dy = (t.to(dtype) for t in ffn_inputs(70, 136, 256, dev))
+    dy = torch.randn(70, 136, device=dev).to(dtype)
+    leaf = wd.clone().requires_grad_()
+    fp8.gated_ffn(x, wg, leaf).backward(dy)
+    act = values(fp8.gated_forward(fp8.quantize(x), fp8.quantize_weight(wg))[0])
+    want = dy.double().T @ act
+    assert ((leaf.grad.double() - want).abs() <= parts_bound(dy.double().T, act, dtype, parts)).all()
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 8, 8), (200, 136, 264), (33, 130, 72)])
 def test_linear_gradients(dev, m, n, k):
     from elf_b200.ops import fp8

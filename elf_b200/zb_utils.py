@@ -292,10 +292,30 @@ class LinearFP8DW(LinearDW):
 
     def _accumulate_grad_output(self, grad_output) -> None:
         prev = getattr(self, "last_grad_output", None)
-        if prev is not None:  # applied several times in one forward: the sum is kept in 16 bits
-            restored = lambda t: t.dequantize(torch.float32) if isinstance(t, _fp8.BlockScaled) else t.float()
-            grad_output = (restored(prev) + restored(grad_output)).to(torch.bfloat16)
+        if prev is not None:  # applied several times in one forward
+            dims = len(grad_output.shape)
+            total = self._whole(prev, dims) + self._whole(grad_output, dims)
+            grad_output = self._in_bf16(total)
         self.last_grad_output = grad_output
+
+    def _in_bf16(self, total: torch.Tensor) -> torch.Tensor:
+        """A sum of output gradients as the W pass's bf16 product takes it: rounded, like the sum of a 16-bit layer, where the
+        layer is bf16; for an fp16 or fp32 layer two or three bf16 parts under one more leading dimension, which add up to all
+        16 or 24 bits of it."""
+        parts = [total.to(torch.bfloat16)]
+        if self.weight.dtype == torch.bfloat16:
+            return parts[0]
+        for _ in range(1 if self.weight.dtype == torch.float16 else 2):
+            total = torch.where(parts[-1].isfinite(), total - parts[-1].float(), 0.0)
+            parts.append(total.to(torch.bfloat16))
+        return torch.stack(parts)
+
+    @staticmethod
+    def _whole(grad_output, dims: int) -> torch.Tensor:
+        """The fp32 values of a stashed output gradient of ``dims`` dimensions."""
+        if isinstance(grad_output, _fp8.BlockScaled):
+            return grad_output.dequantize(torch.float32)
+        return grad_output.float().sum(0) if grad_output.dim() > dims else grad_output.float()
 
     def forward(self, x, *args, **kwargs):
         return LinearFP8DX.apply(x, self.weight, self.bias, self)
@@ -307,6 +327,9 @@ class LinearFP8DW(LinearDW):
             x = x.to(dev, non_blocking=True)
         if g.device != dev:
             g = g.to(dev, non_blocking=True)
+        dims = len(x.shape)
+        if not isinstance(g, _fp8.BlockScaled) and g.dim() > dims:
+            g = self._whole(g, dims)
         with torch.no_grad():
             grad = self.weight.grad
             if grad is not None and grad.dtype in (torch.bfloat16, torch.float32) and grad.is_contiguous():
@@ -322,8 +345,7 @@ class LinearFP8DW(LinearDW):
                 else:
                     grad.add_(dw)
             if self.bias is not None:
-                g2 = g.dequantize(torch.float32) if isinstance(g, _fp8.BlockScaled) else g.float()
-                db = _flat2d(g2).sum(0)
+                db = _flat2d(self._whole(g, dims)).sum(0)
                 if self.bias.grad is None:
                     self.bias.grad = db.to(self.bias.dtype)
                 else:

@@ -311,6 +311,29 @@ def test_layer_applied_twice_sums_its_output_gradients():
     assert isinstance(layer.last_grad_output, torch.Tensor) and layer.last_grad_output.dtype == torch.bfloat16
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("times", [2, 3])
+def test_layer_applied_to_one_input_several_times(times, dtype):
+    """The gradients of all applications arrive at the weight and the bias with the bits of the layer's type."""
+    layer = LinearFP8DW(torch.nn.Linear(64, 40).to(dtype))
+    x = rand(6, 64, dtype=dtype)
+    dys = [rand(6, 40, dtype=dtype, seed=s + 1) for s in range(times)]
+    torch.autograd.backward([layer(x) for _ in dys], dys)
+    layer.move_last_computed("input", 0)
+    layer.move_last_computed("grad_output", 0)
+    layer.offload_last(0, "cpu")
+    layer.backward(0)
+    xq = held(x)[0]
+    total, mag = sum(held(dy)[0] for dy in dys), sum(held(dy)[0].abs() for dy in dys)
+    # each sum of gradients is rounded to the layer's bits (8 of bf16, 16 in two parts, 24 in three), half a unit of them
+    half = {torch.bfloat16: 2.0**-8, torch.float16: 2.0**-16, torch.float32: 2.0**-23}[dtype]
+    spread = (times - 1) * half * mag
+    bound = product_bound(total.T, xq, dtype) + spread.T @ xq.abs() * (1 + torch.finfo(dtype).eps)
+    assert ((layer.weight.grad.double() - total.T @ xq).abs() <= bound).all()
+    want = total.sum(0)
+    assert ((layer.bias.grad.double() - want).abs() <= spread.sum(0) + 6 * 2.0**-24 * mag.sum(0) + torch.finfo(dtype).eps / 2 * (want.abs() + mag.sum(0) * 2.0**-8)).all()
+
+
 def test_layer_ships_without_its_stash():
     import pickle
 

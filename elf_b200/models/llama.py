@@ -693,6 +693,13 @@ def llama_stage_costs(cfg: LlamaConfig, n_stages: int, placement: Optional[Seque
     return _stage_ranges(cfg, n_stages, placement, split_layers, cost_model)[2]
 
 
+def ffn_layers_in_8_bits(module: nn.Module) -> nn.Module:
+    """In place: the feed-forward projections of the blocks in ``module`` become 8-bit layers."""
+    from ..zb_utils import replace_linear_with_linear_fp8
+
+    return replace_linear_with_linear_fp8(module, lambda name, _: name.rpartition(".")[2] in ("w_gate_up", "w_down"))
+
+
 def build_llama_stages(cfg: LlamaConfig, n_stages: int, only: Optional[Sequence[int]] = None, device=None, dtype=torch.bfloat16, seed: int = 0, split_backward: bool = True, placement: Optional[Sequence[int]] = None, split_layers: bool = False, cost_model=None,
                        fused_head_loss: bool = False) -> List[Optional[LlamaStage]]:
     """Build the stages listed in ``only`` (all by default) directly on ``device``; the
@@ -708,7 +715,7 @@ def build_llama_stages(cfg: LlamaConfig, n_stages: int, only: Optional[Sequence[
     feed-forward layers in 8 bits (``elf_b200.zb_utils.LinearFP8DW``).  With
     ``fused_head_loss`` the last stage ends with the final norm only and the vocabulary projection
     happens inside the loss (``elf_b200.ops.head_loss.ChunkedHeadLoss(stage[-1])`` as loss function)."""
-    from ..zb_utils import replace_layer_with_layer_dw, replace_linear_with_linear_fp8
+    from ..zb_utils import replace_layer_with_layer_dw
 
     if cfg.ffn_fp8 and not split_backward:
         raise ValueError("ffn_fp8 needs split_backward=True: the 8-bit layers compute their weight gradients in W passes")
@@ -731,7 +738,7 @@ def build_llama_stages(cfg: LlamaConfig, n_stages: int, only: Optional[Sequence[
         if split_backward:
             replace_layer_with_layer_dw(stage)
         if cfg.ffn_fp8:
-            replace_linear_with_linear_fp8(stage, lambda name, _: name.rpartition(".")[2] in ("w_gate_up", "w_down"))
+            ffn_layers_in_8_bits(stage)
         stages.append(stage)
     return stages
 

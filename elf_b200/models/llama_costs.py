@@ -67,28 +67,50 @@ def analytic_cost_model(cfg) -> LlamaCostModel:
     """Constants measured on B200 for the Llama-3-8B shape, scaled by FLOPs where a shape differs:
     the attention half takes 20 % of a layer, gate/up + SwiGLU 55 %, the down projection 25 %; the
     head's GEMMs run closer to the tensor-core peak than a layer's mix of GEMMs and bandwidth-bound
-    kernels, so it costs 0.65 of what its FLOP count suggests."""
+    kernels, so it costs 0.65 of what its FLOP count suggests.  Feed-forward layers in 8 bits take 0.75 of
+    their 16-bit time there, the weight gradients, which stay 16-bit products, a third of a layer's."""
     d, hd = cfg.d_model, cfg.head_dim
     layer_flops = 2 * d * (cfg.n_heads + 2 * cfg.n_kv_heads) * hd + 2 * d * d + 6 * d * cfg.ffn + 2 * cfg.seq_len * d  # last term: causal attention
     head = 0.65 * 2 * d * cfg.vocab / layer_flops
+    if cfg.ffn_fp8:
+        layer = 0.2 + 0.75 * 0.8
+        return LlamaCostModel(attention=0.2 / layer, mlp_up=0.75 * 0.55 / layer, mlp_down=0.75 * 0.25 / layer, head=head / layer, embed=0.05 / layer, fbw=(0.29, 0.38, 0.33))
     return LlamaCostModel(attention=0.2, mlp_up=0.55, mlp_down=0.25, head=head, embed=0.05)
+
+
+def _timed_part(cls, cfg, device, dtype):
+    """One block of the kind that a stage of ``cfg`` holds, layers in 8 bits included."""
+    from . import llama as L
+    from ..zb_utils import replace_layer_with_layer_dw
+
+    with torch.device(device):
+        m = cls(cfg).to(dtype)
+    L.init_llama_(m, cfg.init_std, 0)
+    replace_layer_with_layer_dw(m)
+    return L.ffn_layers_in_8_bits(m) if cfg.ffn_fp8 else m
 
 
 class _PartTimer:
     """Runs one module on one micro-batch the way ``PipelineBlock`` runs a stage - the split-backward
     layers stash their operands in the forward and the backward, and compute weight gradients in a
-    pass of their own - with a CUDA event between the passes."""
+    pass of their own, 8-bit layers hold one copy of their weights for all micro-batches - with a CUDA
+    event between the passes."""
 
     def __init__(self, module, make_input, loss=None):
-        from ..zb_utils import LayerDW
+        from ..zb_utils import LayerDW, LinearFP8DW
 
         self.module, self.make_input, self.loss = module, make_input, loss
         self.layers = [m for m in module.modules() if isinstance(m, LayerDW)]
         self.marks = []
+        for layer in self.layers:
+            if isinstance(layer, LinearFP8DW):
+                layer.begin_step()
 
     def _clear(self):
+        from ..zb_utils import LayerDW
+
         for layer in self.layers:
-            layer.clear()
+            LayerDW.clear(layer)  # the stash alone: 8-bit weights stay, as from one micro-batch of a step to the next
 
     def run(self, timed: bool = True) -> None:
         """Enqueue forward, input-gradient and weight-gradient pass; nothing waits for the device."""
@@ -147,7 +169,6 @@ def measure_cost_model(cfg, device=None, dtype=torch.bfloat16, mb_size: int = 1,
     import torch.distributed as dist
 
     from . import llama as L
-    from ..zb_utils import replace_layer_with_layer_dw
 
     device = torch.device(device) if device is not None else (torch.device("cuda", torch.cuda.current_device()) if torch.cuda.is_available() else torch.device("cpu"))
     if device.type != "cuda":
@@ -159,11 +180,7 @@ def measure_cost_model(cfg, device=None, dtype=torch.bfloat16, mb_size: int = 1,
         s, d = cfg.seq_len, cfg.d_model
 
         def build(cls):
-            with torch.device(device):
-                m = cls(cfg).to(dtype)
-            L.init_llama_(m, cfg.init_std, 0)
-            replace_layer_with_layer_dw(m)
-            return m
+            return _timed_part(cls, cfg, device, dtype)
 
         base = torch.randn(mb_size, s, d, device=device, dtype=dtype)
         act = torch.randn(mb_size, s, cfg.ffn, device=device, dtype=dtype)
@@ -180,6 +197,8 @@ def measure_cost_model(cfg, device=None, dtype=torch.bfloat16, mb_size: int = 1,
             "embed": (build(L.LlamaEmbedding), lambda: (ids,), None),
             "head": (build(L.LlamaHead), hidden, lambda logits: L.llama_loss_fn(logits, target, reduction="sum")),
         }
+        if cfg.ffn_fp8:  # both projections together are one node, which keeps less than its parts
+            jobs["mlp"] = (build(L.LlamaMLPBlock), hidden, None)
         timers = {name: _PartTimer(*job) for name, job in jobs.items()}
         # Bring the device to the clock it sustains under load, then time the parts in turn,
         # round after round, with no host synchronisation until the end: the GPU stays loaded the
@@ -203,13 +222,15 @@ def measure_cost_model(cfg, device=None, dtype=torch.bfloat16, mb_size: int = 1,
         del jobs
         torch.cuda.empty_cache()
         total = {k: sum(v) for k, v in t.items()}
-        layer = total["attention"] + total["mlp_up"] + total["mlp_down"]
-        parts = ("attention", "mlp_up", "mlp_down")
+        parts = ("attention", "mlp") if "mlp" in total else ("attention", "mlp_up", "mlp_down")
+        layer = sum(total[k] for k in parts)
+        up_of_mlp = total["mlp_up"] / (total["mlp_up"] + total["mlp_down"])
+        mlp = layer - total["attention"]
         fbw = tuple(sum(t[k][i] for k in parts) / layer for i in range(3))
         model = LlamaCostModel(
             attention=total["attention"] / layer,
-            mlp_up=total["mlp_up"] / layer,
-            mlp_down=total["mlp_down"] / layer,
+            mlp_up=mlp * up_of_mlp / layer,
+            mlp_down=mlp * (1 - up_of_mlp) / layer,
             head=total["head"] / layer,
             embed=total["embed"] / layer,
             layer_ms=layer,

@@ -207,6 +207,27 @@ def test_measured_cost_model_on_the_device(dev):
     assert abs(sum(costs) - (cfg.n_layers + cm.head + cm.embed)) < 1e-6
 
 
+def test_measured_cost_model_times_8_bit_layers(dev, monkeypatch):
+    """With feed-forward layers in 8 bits the timed blocks run in 8 bits, and quantise each weight once."""
+    from elf_b200.models.llama import LlamaConfig
+    from elf_b200.models.llama_costs import measure_cost_model
+    from elf_b200.ops import fp8
+
+    calls = {"gated_forward": 0, "quantize_weight": 0}
+    for name in calls:
+
+        def counted(*args, _name=name, _f=getattr(fp8, name), **kwargs):
+            calls[_name] += 1
+            return _f(*args, **kwargs)
+
+        monkeypatch.setattr(fp8, name, counted)
+    cfg = LlamaConfig(n_layers=8, d_model=512, n_heads=4, n_kv_heads=2, ffn=1536, vocab=4096, seq_len=512, rope_theta=500000.0, ffn_fp8=True)
+    cm = measure_cost_model(cfg, dev, mb_size=2, iters=2, burn_in_s=0.05)
+    assert calls["gated_forward"] == 3 and calls["quantize_weight"] == 4  # one untimed and two timed passes; two parts, and both in one block
+    assert cm.source == "measured" and cm.layer_ms > 0 and abs(cm.attention + cm.mlp_up + cm.mlp_down - 1.0) < 1e-6
+    assert min(cm.attention, cm.mlp_up, cm.mlp_down, cm.head, cm.embed) > 0 and abs(sum(cm.fbw) - 1.0) < 1e-6 and min(cm.fbw) > 0.0
+
+
 def test_stream_order_checker_accepts_the_runtime_and_catches_a_missing_wait(dev):
     """With the stream-order debug mode on, a step that offloads activations, prefetches them and
     copies its outputs to the host raises nothing (every hand-off between streams is preceded by a

@@ -29,6 +29,30 @@ def test_cost_model_roundtrip_and_cpu_fallback():
     assert measure_cost_model(CFG, "cpu").source == "analytic"
 
 
+def test_costs_know_of_8_bit_layers():
+    """The timed blocks and the built-in shares are those of the configuration: feed-forward layers in 8 bits make the layer, and
+    with it the unit, shorter; their weight copies last from one micro-batch to the next."""
+    from dataclasses import replace
+
+    from elf_b200.models.llama import LlamaMLPBlock
+    from elf_b200.models.llama_costs import _PartTimer, _timed_part
+    from elf_b200.zb_utils import LinearDW, LinearFP8DW
+
+    cfg8 = replace(CFG, ffn_fp8=True)
+    cm, cm8 = analytic_cost_model(CFG), analytic_cost_model(cfg8)
+    assert abs(cm8.attention + cm8.mlp - 1.0) < 1e-9 and abs(sum(cm8.fbw) - 1.0) < 1e-9
+    assert cm8.mlp < cm.mlp and cm8.head > cm.head and cm8.mlp_up / cm8.mlp_down == pytest.approx(cm.mlp_up / cm.mlp_down)
+    small = replace(cfg8, n_layers=2, d_model=64, n_heads=4, n_kv_heads=2, ffn=128, vocab=64, seq_len=8)
+    block = _timed_part(LlamaMLPBlock, small, "cpu", torch.float32)
+    assert type(block.w_gate_up) is LinearFP8DW and type(block.w_down) is LinearFP8DW
+    timer = _PartTimer(block, None)
+    held = block.w_down.weight_q()
+    block.w_down.last_input = held
+    timer._clear()
+    assert block.w_down.weight_q() is held and block.w_down.last_input is None
+    assert type(_timed_part(LlamaMLPBlock, replace(small, ffn_fp8=False), "cpu", torch.float32).w_down) is LinearDW
+
+
 def test_a_costlier_embedding_moves_work_off_the_first_rank():
     pl = v(8)
     light = LlamaCostModel(0.2, 0.55, 0.25, head=1.0, embed=0.0)

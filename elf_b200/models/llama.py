@@ -134,7 +134,7 @@ class LlamaDecoderLayer(nn.Module):
     fused = FUSED_LAYERS  # one autograd node with a hand-written backward (elf_b200.models.llama_fused)
 
     def forward(self, x):
-        if self.fused and _fused.fused_apply(x, self.wqkv, self.wo, self.w_gate_up, self.w_down):
+        if self.fused and _fused.fused_apply(x, self.wqkv, self.wo, ffn=(self.w_gate_up, self.w_down)):
             return _fused.decoder_layer(self, x)
         b, s, d = x.shape
         hq, hkv, hd = self.n_heads, self.n_kv_heads, self.head_dim
@@ -194,7 +194,7 @@ class LlamaMLPBlock(nn.Module):
     fused = FUSED_LAYERS
 
     def forward(self, x):
-        if self.fused and _fused.fused_apply(x, self.w_gate_up, self.w_down):
+        if self.fused and _fused.fused_apply(x, ffn=(self.w_gate_up, self.w_down)):
             return _fused.mlp_half(self, x)
         return x + self.w_down(_f.swiglu(self.w_gate_up(self.norm2(x))))
 

@@ -42,26 +42,27 @@ from ..zb_utils import LayerDW, LinearFP8DW, in_partial_replay
 __all__ = ["fused_apply", "attention_half", "mlp_half", "decoder_layer"]
 
 
-def fused_apply(x: torch.Tensor, *linears) -> bool:
+def fused_apply(x: torch.Tensor, *linears, ffn=()) -> bool:
     """Whether the single-node path applies: bf16 CUDA activations ``[batch, seq, d]``, kernels
-    enabled, every projection a bias-free split-backward layer on the tcgen05 path."""
+    enabled, every projection (``linears`` and the feed-forward pair ``ffn``) a bias-free split-backward
+    layer on the tcgen05 path.  Only ``ffn`` may be in 8 bits."""
     from ..zb_utils import LinearDW
 
     if not (_f.kernels_apply(x) and x.dim() == 3 and x.shape[-1] % 8 == 0 and x.shape[-1] <= 8192):
         return False
     if not hasattr(_ext.get(), "residual_add"):
         return False
-    for lin in linears:
+    for lin in (*linears, *ffn):
         if not isinstance(lin, LinearDW) or lin.bias is not None or lin.weight.dtype != x.dtype or not lin.weight.is_cuda:
             return False
         n, k = lin.weight.shape
         if n % 8 or k % 8:
             return False
-    # layers in 8 bits: the feed-forward pair together, its gate and up blocks whole
-    in_8_bits = [isinstance(lin, LinearFP8DW) for lin in linears]
-    if any(in_8_bits):
-        return in_8_bits[-2:] == [True, True] and not any(in_8_bits[:-2]) and len(linears) in (2, 4) and linears[-1].weight.shape[1] % _fp8.BLOCK == 0 and (
-            linears[-2].weight.shape[0] == 2 * linears[-1].weight.shape[1])
+    if any(isinstance(lin, LinearFP8DW) for lin in linears):
+        return False
+    if any(isinstance(lin, LinearFP8DW) for lin in ffn):  # the pair together, its gate and up blocks whole
+        up, down = ffn
+        return isinstance(up, LinearFP8DW) and isinstance(down, LinearFP8DW) and down.weight.shape[1] % _fp8.BLOCK == 0 and up.weight.shape[0] == 2 * down.weight.shape[1]
     return True
 
 

@@ -418,6 +418,23 @@ def test_fused_feed_forward_half_is_its_operators(dev):
     assert torch.equal(blk.w_down.weight.grad, fp8.linear_weight_grad(dyq, act))
 
 
+def test_attention_in_8_bits_runs_in_8_bits(dev):
+    """All four projections converted: with half as many key and value heads as heads the attention pair has the shapes of a
+    feed-forward pair, and is none."""
+    from elf_b200.models.llama import LlamaAttentionBlock, LlamaDecoderLayer, init_llama_
+    from elf_b200.ops.fp8 import BlockScaled
+    from elf_b200.zb_utils import LayerDW, LinearFP8DW, replace_linear_with_linear_fp8
+
+    x = activations(2 * 256, 512, torch.bfloat16, dev).view(2, 256, 512)
+    for cls in (LlamaAttentionBlock, LlamaDecoderLayer):
+        with torch.device(dev):
+            blk = replace_linear_with_linear_fp8(init_llama_(cls(cfg()), 0.05, 1).bfloat16())
+        blk(x.clone().requires_grad_()).sum().backward()
+        layers = [m for m in blk.modules() if isinstance(m, LayerDW)]
+        assert layers and all(type(m) is LinearFP8DW for m in layers)
+        assert all(isinstance(m.last_input, BlockScaled) and isinstance(m.last_grad_output, BlockScaled) for m in layers)
+
+
 def test_decoder_layer_is_its_halves(dev):
     layer, attn, mlp = build_blocks(cfg(), dev)
     x = activations(2 * 256, 512, torch.bfloat16, dev).view(2, 256, 512)

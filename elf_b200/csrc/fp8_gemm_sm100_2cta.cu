@@ -79,21 +79,6 @@ __device__ __forceinline__ Unit unit_at(int u, const Schedule& s, int k_blocks, 
   return r;
 }
 
-// whether `ok` holds for all `threads` threads at the barrier
-__device__ __forceinline__ bool named_barrier_all(uint32_t id, uint32_t threads, bool ok) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t"
-      ".reg .pred P, Q;\n\t"
-      "setp.ne.u32 P, %3, 0;\n\t"
-      "barrier.cta.red.and.pred Q, %1, %2, P;\n\t"
-      "selp.u32 %0, 1, 0, Q;\n\t"
-      "}\n"
-      : "=r"(r)
-      : "r"(id), "r"(threads), "r"(uint32_t(ok))
-      : "memory");
-  return r != 0;
-}
 __device__ __forceinline__ void umma_ss_mxf8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
   asm volatile(
       "{\n\t"

@@ -327,7 +327,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gri
       const bool joined = wu.partial && parts != nullptr;  // fp32 parts in the workspace, added by the last to finish
       const bool add_bias = BIAS && (wu.part == 0 || joined);
       const int n0 = wu.n0;
-      if (!mbar_wait(acc_full_bar(acc), acc_phase, abort_flag)) break;
+      if (!named_barrier_all(1, 128, mbar_wait(acc_full_bar(acc), acc_phase, abort_flag))) break;
       tc_fence_after_sync();
       const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + acc * BN;
       bool finish = true;  // this unit's sums are D's

@@ -243,6 +243,22 @@ __device__ __forceinline__ void tma_store_wait_all() { asm volatile("cp.async.bu
 __device__ __forceinline__ void named_barrier_sync(uint32_t id, uint32_t threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
+// The same; returns whether `ok` holds for all of them.  For waits that may run out: either all go on to the barriers behind
+// one, or none does.
+__device__ __forceinline__ bool named_barrier_all(uint32_t id, uint32_t threads, bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred P, Q;\n\t"
+      "setp.ne.u32 P, %3, 0;\n\t"
+      "barrier.cta.red.and.pred Q, %1, %2, P;\n\t"
+      "selp.u32 %0, 1, 0, Q;\n\t"
+      "}\n"
+      : "=r"(r)
+      : "r"(id), "r"(threads), "r"(uint32_t(ok))
+      : "memory");
+  return r != 0;
+}
 
 // ----------------------------------------------------------------------------------------
 // tcgen05: TMEM allocation, MMA, commit, TMEM loads

@@ -517,7 +517,7 @@ __device__ __forceinline__ double warp_sum(double v) {
 }
 
 // 8 normalised values of column group c (zeros past the row) to 8 bits; all 32 lanes of the warp call this
-__device__ __forceinline__ void store_normalised(const NormArgs& p, long long row, int c, bool live, const float (&v)[8], uint4 gain, InverseRms rs) {
+__device__ __forceinline__ void store_normalised(const NormArgs& p, long long row, int c, const float (&v)[8], uint4 gain, InverseRms rs) {
   float g[8], y[8];
   unpack8(gain, g);
   const uint64_t hi = pair_of(rs.hi, rs.hi), lo = pair_of(rs.lo, rs.lo);
@@ -542,7 +542,7 @@ __device__ __forceinline__ void store_normalised(const NormArgs& p, long long ro
   }
   uint32_t q[2];
   const uint32_t byte = quantize_block<8, 16>(y, abs_bits(top), q);
-  if (live && c < p.dim8) {
+  if (c < p.dim8) {
     *reinterpret_cast<uint2*>(p.data + row * p.ldq + c * 8) = make_uint2(q[0], q[1]);
     if ((c & 15) == 0) p.scale[row * p.lds + c / 16] = uint8_t(byte);
   }
@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(256) rmsnorm_fp8_warp_kernel(const __grid_cons
   for (int i = 0; i < VPT; ++i) {
     const int c = lane + i * 32;
     if (i * 32 >= p.dim8) break;
-    store_normalised(p, row, c, true, v[i], c < p.dim8 ? p.w[c] : make_uint4(0, 0, 0, 0), rs);
+    store_normalised(p, row, c, v[i], c < p.dim8 ? p.w[c] : make_uint4(0, 0, 0, 0), rs);
   }
 }
 
@@ -633,7 +633,7 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_BLOCKS<VPT>) rmsnorm_fp8_bl
     for (int i = 0; i < VPT; ++i) {
       const int c = t + i * threads;
       if ((c & ~31) >= p.dim8) break;  // the whole warp is past the row
-      store_normalised(p, row, c, true, v[i], gain[i], rs);
+      store_normalised(p, row, c, v[i], gain[i], rs);
     }
   }
 }

@@ -33,7 +33,7 @@ import torch.distributed as dist
 from ..ops import _ext
 from ..ops import gemm as _gemm
 from ..optim.flat import FlatGroup
-from ..zb_utils import LinearDW, LinearFP8DW
+from ..zb_utils import LinearDW
 from .symm import SymmetricBuffer
 
 logger = logging.getLogger("dp_sync")
@@ -191,8 +191,7 @@ class SymmetricGradSync:
         self.exchanges: Dict[int, Optional[StageExchange]] = {}
         for block in blocks:
             alloc = lambda n, dt: SymmetricBuffer.allocate(n, dt, dp_group, block.device)
-            # an 8-bit layer's weight gradient comes out of the bf16 product: only into a bf16 gradient can it be pushed
-            layers = [m for m in block.model.modules() if isinstance(m, LinearDW) and not (isinstance(m, LinearFP8DW) and m.weight.dtype != torch.bfloat16)]
+            layers = [m for m in block.model.modules() if isinstance(m, LinearDW)]
             self.exchanges[block.id] = _build_exchange(list(block.model.parameters()), layers, alloc, self.rank, self.world, timeout_ms)
 
     def begin_step(self) -> None:

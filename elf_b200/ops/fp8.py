@@ -416,6 +416,8 @@ def linear_weight_grad(dy: Union[BlockScaled, torch.Tensor], x: Union[BlockScale
         raise TypeError(f"products come in bf16, fp16 or fp32, not {out_dtype}")
     data = x.data if isinstance(x, BlockScaled) else x
     if data.numel() == 0 or n == 0 or not _on_kernels(data):
+        if push:
+            raise ValueError("linear_weight_grad: only the product of CUDA operands that have elements can be pushed")
         plain = lambda t: _values(t) if isinstance(t, BlockScaled) else _matrix(t.detach()).float()  # noqa: E731
         dw = plain(dy).T @ plain(x)
         return dw.to(out_dtype) if out is None else out.add_(dw)

@@ -335,7 +335,7 @@ class LinearFP8DW(LinearDW):
             if grad is not None and grad.dtype in (torch.bfloat16, torch.float32) and grad.is_contiguous():
                 push = None
                 plan = getattr(self, "_push", None)
-                if plan is not None and getattr(self, "_final_pass", False) and grad.dtype == self.weight.dtype and _gemm.usable(grad, self.weight):
+                if plan is not None and getattr(self, "_final_pass", False) and x.numel() and grad.dtype == self.weight.dtype and _gemm.usable(grad, self.weight):
                     push = plan.target()
                 self.weight.grad = _fp8.linear_weight_grad(g, x, out=grad, push=push)
             else:

@@ -74,6 +74,67 @@ def test_fused_dw_push_and_finalize(world):
         assert all(len(ex.pushed) == 3 for ex in exchanges)  # the three matrices went out through GEMM epilogues
 
 
+@pytest.mark.parametrize("world,empty", [(2, False), (4, False), (2, True)])
+def test_8_bit_layers_push_their_gradients(world, empty):
+    """Weight gradients of 8-bit layers leave through the product's epilogue: after the reduction every replica holds the mean, against
+    64 bits.  A last micro-batch without tokens leaves them to the copy."""
+    from elf_b200.ops import fp8, gemm as G
+    from elf_b200.parallel.dp_sync import _build_exchange
+    from elf_b200.parallel.symm import LocalSymmetricGroup
+    from elf_b200.zb_utils import LinearFP8DW, replace_linear_with_linear_fp8
+
+    from .fp8_oracle import product_bound, values
+
+    dev = torch.device("cuda", 0)
+    dims = [(256, 512), (512, 264), (264, 128)]
+    group = LocalSymmetricGroup(world, dev)
+    reps, exchanges = [], []
+    for r in range(world):
+        m = replace_linear_with_linear_fp8(_replica(0, dims, dev))
+        layers = [l for l in m.modules() if isinstance(l, LinearFP8DW)]
+        ex = _build_exchange(list(m.parameters()), layers, group.allocator(r), r, world, timeout_ms=500.0)
+        reps.append(layers)
+        exchanges.append(ex)
+    n_mb = 3
+    for step in range(2):
+        want = [torch.zeros(o, i, device=dev, dtype=torch.float64) for i, o in dims]
+        err = [torch.zeros_like(w) for w in want]
+        for r, (layers, ex) in enumerate(zip(reps, exchanges)):
+            ex.flat.zero_grad()
+            ex.begin_step()
+            local, local_err = [torch.zeros_like(w) for w in want], [torch.zeros_like(w) for w in want]
+            for mb in range(n_mb):
+                tokens = 0 if empty and mb == n_mb - 1 else 200
+                for j, (layer, (i, o)) in enumerate(zip(layers, dims)):
+                    g = torch.Generator(device=dev).manual_seed(1000 * step + 100 * r + 10 * mb + j)
+                    x, dy = (fp8.quantize(torch.randn(tokens, c, device=dev, generator=g)) for c in (i, o))
+                    layer.set("input", mb, x)
+                    layer.set("grad_output", mb, dy)
+                    layer._final_pass = mb == n_mb - 1
+                    layer.backward(mb)
+                    a, b = values(dy).T, values(x)
+                    local[j] += a @ b
+                    # each micro-batch is rounded to bf16 and so is the sum it joins
+                    local_err[j] += product_bound(a, b, torch.bfloat16) + 2.0**-8 * (local[j].abs() + local_err[j])
+            for j in range(len(dims)):
+                want[j] += local[j]
+                err[j] += local_err[j]
+            for layer in layers:
+                layer.clear()
+        scale = 1.0 / world
+        for ex in exchanges:
+            ex.push_rest()
+        for ex in exchanges:
+            ex.reduce(scale)
+        torch.cuda.synchronize()
+        G.check_status()
+        for layers in reps:
+            for layer, w, e in zip(layers, want, err):
+                # the mean is formed in fp32 and rounded
+                assert ((layer.weight.grad.double() - w * scale).abs() <= e * scale + 2.0**-8 * (w.abs() + e) * scale * (1 + 2.0**-10)).all()
+        assert all(len(ex.pushed) == (0 if empty else len(dims)) for ex in exchanges)
+
+
 def test_finalize_wait_is_bounded():
     """A flag that nobody raises: the wait gives up after its limit, reports it in the
     status word, and the context stays usable."""

@@ -111,6 +111,8 @@ def test_weight_gradient_operands():
         fp8.linear_weight_grad(rand(40, 20).double(), x)
     with pytest.raises(ValueError, match="push takes"):
         fp8.linear_weight_grad(rand(40, 20), x.bfloat16(), out=torch.zeros(20, 30, dtype=torch.bfloat16), push={"tag": 1})
+    with pytest.raises(ValueError, match="CUDA operands that have elements"):
+        fp8.linear_weight_grad(fp8.quantize(rand(40, 20)), fp8.quantize(x), out=torch.zeros(20, 30, dtype=torch.bfloat16), push={"tag": 1})
 
 
 def test_only_requested_gradients():

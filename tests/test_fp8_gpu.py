@@ -325,6 +325,29 @@ def test_rms_norm_rounds_once(dev, rows, dim):
         assert torch.equal(values(q), torch.round(y / step) * step)
 
 
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("rows,dim", [(9, 1032), (700, 1304), (65, 1536), (3, 1544), (5, 1800), (7, 2040), (3000, 1800), (2500, 4096), (1800, 5120), (1300, 8192)])
+def test_rms_norm_of_other_widths_and_more_rows(dev, rows, dim, residual):
+    """The widest rows that a warp takes and the narrowest that a block does; more rows than blocks, so that each walks to its next one."""
+    test_rms_norm(dev, rows, dim, residual)
+
+
+@pytest.mark.parametrize("rows,dim", [(3000, 1304), (3000, 1800), (2000, 5120)])
+def test_rms_norm_of_a_sum_rounds_once(dev, rows, dim):
+    from elf_b200.ops import fp8
+
+    for seed in range(6):
+        x, r = activations(rows, dim, torch.bfloat16, dev, seed), activations(rows, dim, torch.bfloat16, dev, 100 + seed)
+        w = (1 + 0.1 * torch.randn(dim, device=dev)).to(torch.bfloat16)
+        hd = (x.double() + r.double()).to(torch.bfloat16).double()
+        y = hd / (hd.square().sum(1, keepdim=True) / dim + 1e-5).sqrt() * w.double()
+        q, _, h = fp8.add_rms_norm(x, r, w, 1e-5)
+        assert same(h, hd)
+        unit = torch.exp2(q.scale.double() - 127).repeat_interleave(128, 1)[:, :dim]
+        step = unit * torch.exp2(torch.floor(torch.log2((y / unit).abs().clamp_min(2.0**-6))) - 3)
+        assert torch.equal(values(q), torch.round(y / step) * step)
+
+
 def test_rms_norm_rows_without_finite_values(dev):
     from elf_b200.ops import fp8
 
@@ -499,6 +522,51 @@ def test_gated_backward(dev, m, d, f):
     err_g = err * fg.abs() + (da * fg).abs() * rel + (da.abs() + err) * (u * s).abs() * (g.abs() + 1) * 2.0**-21 * (1 + g.abs())
     err_u = err * fu.abs() + (da * fu).abs() * rel
     check_held(got, torch.cat([da * fg, da * fu], 1), torch.cat([err_g, err_u], 1) + 1e-37)
+
+
+@pytest.mark.parametrize("m,d,f", [(4000, 528, 5248), (2600, 200, 6272)])  # 16 x 21 and 11 x 25 tiles on 74 pairs
+def test_gated_backward_of_many_tiles(dev, m, d, f):
+    """Three and more units for every pair of CTAs: both accumulators, each barrier's next phase, a last tile of half the columns."""
+    test_gated_backward(dev, m, d, f)
+
+
+@pytest.mark.parametrize("m,d,f", [(300, 200, 640), (4000, 136, 5248)])
+def test_gated_backward_not_finite(dev, m, d, f):
+    """What is not finite in the output's gradient reaches its own row, in the checkpoint its own column of its row, and only as NaN."""
+    from elf_b200.ops import fp8
+
+    _, w = operands(1, d, f, dev, 3)
+    dy, gate_up = activations(m, d, torch.bfloat16, dev, 4), activations(m, 2 * f, torch.bfloat16, dev, 5)
+    rows, cols = [5, 130, m - 1], [3, f // 2 + 7, f - 1]
+    for r, c in zip(rows, cols):  # no block's largest gradient, with or without them
+        gate_up[r, c] = gate_up[r, f + c] = 0
+    clean = fp8.gated_backward(fp8.quantize(dy), w, fp8.quantize(gate_up))
+    inf, nan = float("inf"), float("nan")
+    gate_up[rows[0], cols[0]] = nan  # gate: both gradients
+    gate_up[rows[1], f + cols[1]] = inf  # up: that of gate alone
+    gate_up[rows[2], cols[2]] = -inf
+    dy[7, 3], dy[200, d - 1] = nan, inf
+    got = fp8.gated_backward(fp8.quantize(dy), w, fp8.quantize(gate_up))
+    want = values(clean)
+    want[rows[0], [cols[0], f + cols[0]]] = nan
+    want[rows[1], cols[1]] = nan
+    want[rows[2], [cols[2], f + cols[2]]] = nan
+    whole = torch.zeros(m, dtype=torch.bool, device=dev)
+    whole[[7, 200]] = True
+    assert values(got)[whole].isnan().all()
+    assert same(values(got)[~whole], want[~whole])
+    finite_blocks = ~whole
+    assert torch.equal(got.scale[finite_blocks], clean.scale[finite_blocks])
+
+
+@pytest.mark.parametrize("m,n,k", [*SHAPES, (2047, 264, 528), (4100, 2304, 1040)])
+def test_weight_grad_rounds_once(dev, m, n, k):
+    """bf16 results are fp32 sums rounded once, tiles that are split along the tokens among them."""
+    from elf_b200.ops import fp8
+
+    dy, x = fp8.quantize(activations(m, n, torch.bfloat16, dev, 4) * 1e-3), fp8.quantize(activations(m, k, torch.bfloat16, dev, 5))
+    a, b = values(dy).T, values(x)
+    assert ((fp8.linear_weight_grad(dy, x).double() - a @ b).abs() <= product_bound(a, b, torch.bfloat16)).all()
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 4096, 2048), (16, 1000, 5504), (100, 136, 9000), (128, 264, 4100), (77, 20000, 640), (2, 128, 30000)])

@@ -138,6 +138,41 @@ def test_bias_keeps_its_gradient(dev, lead):
         assert not fp8.linear_forward(x, w, bias).requires_grad
 
 
+@pytest.mark.parametrize("m,n,k", [(200, 136, 264), (33, 130, 72), (1500, 264, 392)])
+def test_linear_weight_gradient_rounds_once(dev, m, n, k):
+    from elf_b200.ops import fp8
+
+    x, w, dy = activations(m, k, torch.bfloat16, dev), activations(n, k, torch.bfloat16, dev, 1).requires_grad_(), activations(m, n, torch.bfloat16, dev, 2)
+    fp8.linear(x, w).backward(dy)
+    a, b = values(fp8.quantize(dy)).T, values(fp8.quantize(x))
+    assert ((w.grad.double() - a @ b).abs() <= product_bound(a, b, torch.bfloat16)).all()
+
+
+def test_training_pass_repeats_itself(dev):
+    """Forward and backward pass of a block with several tiles for every SM: the same bits at every repetition, eager and replayed."""
+    from elf_b200.ops import fp8
+
+    x, wg, wd, dy = ffn_inputs(4000, 1024, 4096, dev)
+    leaves = [t.requires_grad_() for t in (x, wg, wd)]
+    copies = {"gate_up_q": fp8.quantize_weight(wg), "down_q": fp8.quantize_weight(wd)}
+
+    def step():
+        y = fp8.gated_ffn(*leaves, **copies)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    first = step()
+    for _ in range(20):
+        assert all(torch.equal(a, b) for a, b in zip(first, step()))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = step()
+    for _ in range(5):
+        for t in again:
+            t.zero_()
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
 def test_gradients_that_are_not_dense(dev):
     """An expanded (stride 0) and a strided output gradient."""
     from elf_b200.ops import fp8

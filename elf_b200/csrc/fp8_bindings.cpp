@@ -339,49 +339,58 @@ std::vector<c10::optional<at::Tensor>> ffn(const at::Tensor& x, const at::Tensor
   return {y, xq.first, xq.second, act, act_scale, gu, gu_scale};
 }
 
-// bf16 matrices for the 16-bit product, their rows on 16-byte boundaries, whose sum is the operand: the values of a block-scaled
-// tensor or a bf16 one, which are one matrix, or the parts of an fp16 or fp32 one, the largest first
-std::vector<Mat> restored(const at::Tensor& t, const c10::optional<at::Tensor>& scale, const char* name, const at::Device& dev) {
+// One operand of the 16-bit product, rows on 16-byte boundaries.  An operand is the sum of `parts` bf16 matrices (block-scaled and
+// bf16 tensors of one, see split_into_bf16_parts), and each pair of parts of the two has its stretch of the reduction: the
+// matrices lie one behind the other, part p (0: the largest) at stretch (parts - 1 - p) * part_step and, for the other
+// operand's parts, `copies` times copy_step further on.
+Mat stacked(const at::Tensor& t, const c10::optional<at::Tensor>& scale, int parts, int64_t part_step, int copies, int64_t copy_step, const char* name,
+            const at::Device& dev) {
   const Mat m = matrix(t, name, dev);
-  const elfb::Elem type = scale.has_value() ? elfb::Elem::kBf16 : elem_of(t, name);
-  if (!scale.has_value() && type == elfb::Elem::kBf16 && m.aligned(16)) return {m};
-  const int parts = elfb::bf16_parts(type);
-  const int64_t lead[2] = {parts, m.rows}, pitch = round_up(m.cols, 8);
-  if (!scale.has_value() && type == elfb::Elem::kBf16) return {{repacked(m, pitch, dev), m.rows, m.cols, pitch}};
-  const at::Tensor out = new_rows(at::IntArrayRef(lead, 2), m.cols, pitch, at::kBFloat16, dev);
-  if (scale.has_value()) {
-    const Scaled s = scaled(t, *scale, 0, name, dev);
-    check(elfb::fp8_dequantize(s.data.bytes(), s.data.pitch, s.scale.bytes(), s.scale.pitch, 0, out.data_ptr(), elfb::Elem::kBf16, pitch, m.rows, int(m.cols),
-                               cur()),
-          "fp8_dequantize");
-  } else {
-    check(elfb::split_into_bf16_parts(m.t.data_ptr(), type, m.pitch, out.data_ptr(), pitch, m.rows * pitch, m.rows, int(m.cols), cur()), "split_into_bf16_parts");
+  if (parts * copies == 1 && !scale.has_value() && m.aligned(16)) return m;
+  const int64_t pitch = round_up(m.cols, 8), stretch = m.rows * pitch, lead[1] = {m.rows * parts * copies};
+  const at::Tensor out = new_rows(at::IntArrayRef(lead, 1), m.cols, pitch, at::kBFloat16, dev);
+  for (int c = 0; c < copies; ++c) {
+    at::BFloat16* first = out.data_ptr<at::BFloat16>() + c * copy_step * stretch;
+    if (scale.has_value()) {
+      const Scaled s = scaled(t, *scale, 0, name, dev);
+      check(elfb::fp8_dequantize(s.data.bytes(), s.data.pitch, s.scale.bytes(), s.scale.pitch, 0, first, elfb::Elem::kBf16, pitch, m.rows, int(m.cols), cur()),
+            "fp8_dequantize");
+    } else if (parts == 1) {
+      TORCH_CHECK(m.cols * 2 <= INT_MAX - 1024, "rows are too wide to be copied");
+      check(elfb::fp8_repack(m.t.data_ptr(), m.pitch * 2, first, pitch * 2, m.rows, int(m.cols * 2), cur()), "fp8_repack");
+    } else {
+      check(elfb::split_into_bf16_parts(m.t.data_ptr(), elem_of(t, name), m.pitch, first + (parts - 1) * part_step * stretch, pitch, -part_step * stretch, m.rows,
+                                        int(m.cols), cur()),
+            "split_into_bf16_parts");
+    }
   }
-  std::vector<Mat> r;
-  for (int p = 0; p < parts; ++p) r.push_back({out.select(0, p), m.rows, m.cols, pitch});
-  return r;
+  return {out, lead[0], m.cols, pitch};
 }
 
 // dy^T x over all leading dimensions, on the 16-bit tensor path; added to `out` when it is given.  Either operand block-scaled
-// (with its scales) or plain: one product for each pair of bf16 parts of the operands, the small ones first, added in fp32.
+// (with its scales) or plain.  The reduction runs over all pairs of bf16 parts of the operands, the small ones first, so that the
+// large ones' sum is rounded no more often than alone.
 at::Tensor weight_grad(const at::Tensor& dy, const c10::optional<at::Tensor>& dy_scale, const at::Tensor& x, const c10::optional<at::Tensor>& x_scale,
                        const c10::optional<at::Tensor>& out, at::ScalarType dtype, const at::Tensor& status, int64_t variant, bool split_tail) {
   const auto dev = x.device();
   c10::cuda::CUDAGuard guard(dev);
-  const std::vector<Mat> dys = restored(dy, dy_scale, "dy", dev), xs = restored(x, x_scale, "x", dev);
-  const Mat &a = dys[0], &b = xs[0];
-  const bool one = dys.size() * xs.size() == 1;
+  auto parts_of = [](const at::Tensor& t, const c10::optional<at::Tensor>& scale, const char* name) { return scale.has_value() ? 1 : elfb::bf16_parts(elem_of(t, name)); };
+  const int dy_parts = parts_of(dy, dy_scale, "dy"), x_parts = parts_of(x, x_scale, "x");
+  const Mat a = stacked(dy, dy_scale, dy_parts, x_parts, x_parts, 1, "dy", dev), b = stacked(x, x_scale, x_parts, 1, dy_parts, x_parts, "x", dev);
   TORCH_CHECK(a.rows == b.rows && a.rows <= INT_MAX, "dy and x must have the same number of rows");
-  // fp16 results, bf16 sums of several products, and widths whose rows are not on 16-byte boundaries, go through a buffer
-  const bool direct = out.has_value() && (one || out->scalar_type() == at::kFloat) && b.cols % 8 == 0 && out->is_contiguous() && reinterpret_cast<uintptr_t>(out->data_ptr()) % 16 == 0;
+  // fp16 results, whole operands' sums with a bf16 gradient, and widths whose rows are not on 16-byte boundaries, go through a
+  // buffer
+  const bool direct = out.has_value() && (dy_parts * x_parts == 1 || out->scalar_type() == at::kFloat) && b.cols % 8 == 0 && out->is_contiguous() && reinterpret_cast<uintptr_t>(out->data_ptr()) % 16 == 0;
   const int64_t lead[1] = {a.cols};
-  const at::ScalarType held = one && !out.has_value() && dtype == at::kBFloat16 ? at::kBFloat16 : at::kFloat;
+  const at::ScalarType held = !out.has_value() && dtype == at::kBFloat16 ? at::kBFloat16 : at::kFloat;
   at::Tensor dw = direct ? *out : new_rows(at::IntArrayRef(lead, 1), b.cols, round_up(b.cols, 8), held, dev);
   elfb::GemmArgs g;
   g.fmt = 1;
   g.M = int(a.cols);
   g.N = int(b.cols);
   g.K = int(a.rows);
+  g.a = a.t.data_ptr();
+  g.b = b.t.data_ptr();
   g.d = dw.data_ptr();
   g.lda = a.pitch;
   g.ldb = b.pitch;
@@ -398,14 +407,8 @@ at::Tensor weight_grad(const at::Tensor& dy, const c10::optional<at::Tensor>& dy
     workspace = dense({int64_t(bytes)}, at::kByte, dev);
     g.workspace = workspace.data_ptr();
   }
-  for (size_t i = dys.size(); i-- > 0;)
-    for (size_t j = xs.size(); j-- > 0;) {
-      g.a = dys[i].t.data_ptr();
-      g.b = xs[j].t.data_ptr();
-      const char* err = elfb::gemm_tcgen05(g, sm_count(dev), cur());
-      TORCH_CHECK(err == nullptr, "elf_b200 fp8_weight_grad: ", err);
-      g.accumulate = true;
-    }
+  const char* err = elfb::gemm_tcgen05(g, sm_count(dev), cur());
+  TORCH_CHECK(err == nullptr, "elf_b200 fp8_weight_grad: ", err);
   if (direct) return dw;
   if (out.has_value()) {
     at::Tensor sum = *out;

@@ -396,8 +396,8 @@ def linear_weight_grad(dy: Union[BlockScaled, torch.Tensor], x: Union[BlockScale
                        out_dtype: torch.dtype = torch.bfloat16, push: Optional[dict] = None) -> torch.Tensor:
     """``dy^T x`` summed over all leading dimensions, from 8-bit checkpoints or 16-bit tensors, on the bf16
     tensor path: the reduction runs over tokens, which have scales of their own.  Accumulated in fp32 and rounded
-    once, the same from call to call; fp16 and fp32 operands enter whole, as two and three bf16 parts and a product for
-    each.  Added to ``out`` when it is given (bf16 or fp32); ``push`` as in ``gemm.linear_weight_grad``, from 8-bit or
+    once, the same from call to call; fp16 and fp32 operands enter whole, as two and three bf16 parts, each with a
+    stretch of the reduction.  Added to ``out`` when it is given (bf16 or fp32); ``push`` as in ``gemm.linear_weight_grad``, from 8-bit or
     bf16 operands."""
     n, k = dy.shape[-1], x.shape[-1]
     if dy.shape[:-1].numel() != x.shape[:-1].numel():

@@ -3,9 +3,9 @@
 //
 // Why pairs: a 128 x 256 tile on one CTA fetches 48 KiB for 512 cycles of 8-bit MMA, 25 TB/s over the chip,
 // which is more than L2 delivers; the pair fetches 32 KiB per CTA in the same time (each its own 128 rows
-// of A and half of B).  4096 x 4096 x 14336: 176 us; a kernel of single CTAs with 128 x 256 tiles took 249.
-// What bounds it: the tensor pipe, 79 % busy at 180 us there and 84 % in the gradient's form (4096 x 4096 x 28672,
-// 344 us); under a lasting load the chip's power, which takes the clock from 1.9 to 1.1 - 1.4 GHz.
+// of A and half of B).  4096 x 4096 x 14336: 181 us; a kernel of single CTAs with 128 x 256 tiles took 249.
+// What bounds it: the tensor pipe, 76 % busy there and 83 % in the gradient's form (4096 x 4096 x 28672, 348 us); under a
+// lasting load the chip's power, which takes the clock from 1.9 to 1.1 - 1.4 GHz.
 //
 // Roles per CTA as in fp8_gemm_sm100.cu.  The even CTA's MMA thread issues for both.  Barriers, each of a slot of two
 // stages:
@@ -15,7 +15,7 @@
 //                commits per stage instead: 218 us against 200 in the loop alone)
 //   acc_full[a]  one per CTA, committed to both
 //   acc_free     even CTA: the epilogue warps of both arrive once the columns the two accumulators share
-//                have been read (8 arrivals per unit)
+//                have been read (16 arrivals per unit)
 //
 // The tiles of a last, partly filled wave are split along K into units on different pairs.  Every unit but
 // the last to finish leaves its fp32 sums in a workspace; the last one adds all parts in their order, so
@@ -34,7 +34,10 @@ constexpr int EPI_WARPS = 8;     // two per quarter of the TMEM lanes, each with
 constexpr int EPI_THREADS = EPI_WARPS * 32;
 constexpr int NUM_THREADS = 96 + EPI_THREADS;
 constexpr int SF_BYTES = 3 * 512;           // scale words of a slot: 128 rows of A, 256 columns of B
-constexpr int GROUP_M = 4;  // tile rows (of 256) that are swept together before moving to the next columns
+// Tile rows (of 256) that are swept together before moving to the next columns: B is read from DRAM once for each group.
+// In groups of 2, 4, 8 and 16 (us): 4096 x 4096 x 14336 180, 180, 178, 178; gated forward 4096 x 28672 x 4096 397, 375, 362,
+// 355; its backward 266, 266, 262, 260; input gradient 4096 x 4096 x 28672 348, 347, 342, 339.
+constexpr int GROUP_M = 4;
 constexpr int ACC1 = 224;   // first column of the second accumulator: shares 32 with the first
 constexpr int EXCHANGE_BYTES = 3 * 2 * BM * 4;  // block maxima that the two halves of a row tell each other (gated forms)
 constexpr size_t SMEM_BYTES = size_t(STAGES) * STAGE_BYTES + SLOTS * SF_BYTES + EXCHANGE_BYTES + 1024 /*align slack*/ + 256 /*barriers*/;
@@ -136,7 +139,7 @@ __device__ __forceinline__ uint64_t sigmoid2(uint64_t x) {
 // One tile of the gated form: columns 0..127 of the accumulator are gate, 128..255 up.  A thread takes 64 columns
 // of gate and the same of up of one row into registers and gives the accumulator back at once; the maxima of the
 // three blocks (gate, up, activation) are exchanged with the thread that has the row's other half.
-// 4096 x 28672 x 4096: 379 us of 285 at the 8-bit peak (393 before its arithmetic went by fp32 pairs), tensor pipe 71 %
+// 4096 x 28672 x 4096: 375 to 383 us of 285 at the 8-bit peak (393 before its arithmetic went by fp32 pairs), tensor pipe 74 %
 // busy: 32 blocks of K are about as long as this epilogue, and the last of 25 waves is a quarter full.
 template <typename Release>
 __device__ __forceinline__ void gated_tile(uint32_t taddr, int row, int half, int f0, int f, const Params& p, uint32_t* exchange, Release&& release) {
@@ -205,12 +208,12 @@ __device__ __forceinline__ void gated_tile(uint32_t taddr, int row, int half, in
 // One tile of the gated form's backward: the accumulator holds the gradient d of the activation, the thread one row
 // of one block of 128 columns.  gate and up come from their checkpoint.
 //   dgate = d up s (1 + gate (1 - s)),  dup = d gate s,  s = sigmoid(gate)
-// are formed twice, once for the maxima of their blocks and once to be scaled: 256 values per row would not stay in
-// registers.  d stays in TMEM but for the 32 columns shared with the other accumulator, which half of the threads
+// are formed twice, once for the maxima of their blocks and once to be scaled: a thread that has a row's block alone would
+// hold 256 values.  (Two threads to a block, as above, would hold 128 each: not built.)  d stays in TMEM but for the 32 columns shared with the other accumulator, which half of the threads
 // hold.  The checkpoint is read and the result written 32 bytes at a time, whole sectors of a row that is one
 // thread's own: 16-byte accesses cost 40 us more.
 //
-// 4096 x 14336 x 4096: 264 us (180 without this epilogue, 142 at the 8-bit peak); the epilogue of a tile outlasts the
+// 4096 x 14336 x 4096: 264 to 268 us (180 without this epilogue, 142 at the 8-bit peak); the epilogue of a tile outlasts the
 // next tile's MMAs.  Before its arithmetic went by pairs it took 283: arithmetic alone beside the MMAs 243, loads and
 // stores with next to no arithmetic 273, one sweep 250.  Neither 16 epilogue warps (289) nor fetching the next tile's
 // checkpoint into L2 (291) helped.
@@ -672,8 +675,8 @@ Schedule make_schedule(int M, int N, int K, Fp8Form form, int num_pairs) {
     // block of K, and for split tiles 6000 to clear the counters and 200 for each part that is written and read back.
     // N = 4096, whole against split in two (us):  256 rows, K = 4096: 20.5 and 23.2; K = 14336: 45.1 and 35.5 (in four
     // 31.7); 2048 rows (54 of 128 tiles left over), K = 14336: 97 and 110; 4096 rows (34 left over): 188 and 184.
-    // Shorter reductions, where a split would gain 3 us for a tile or two at best, stay whole: a row's result does not
-    // depend on the number of rows then.
+    // Shorter reductions, where a split would gain 3 us for a tile or two at best, stay whole: above 128 rows a row's
+    // result does not depend on their number then (up to 128 another kernel splits K by a rule of its own).
     long long best = 600ll * k_blocks;
     for (int w = 2; w <= 8 && 2 * w <= groups; ++w) {
       const long long waves = ((long long)rem * w + num_pairs - 1) / num_pairs;

@@ -1,6 +1,6 @@
 // Bandwidth-bound kernels that write or read block-scaled 8-bit tensors: quantise, restore, RMSNorm
-// with an 8-bit output.  Each reads its inputs once and writes its outputs once; all arithmetic is
-// fp32.
+// with an 8-bit output, and bf16 parts of wider operands.  Each reads its inputs once and writes its outputs once; arithmetic is
+// fp32, the norm's statistic 64 bits once a thread's squares are added.
 #include "fp8_ops.h"
 
 #include <algorithm>
@@ -473,7 +473,8 @@ __device__ __forceinline__ double square_sum(const float (&v)[N][8]) {
   for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = larger_magnitude(top, v[i][j]);
-  // |v| < 2^(e + 1), the N * 8 <= 32 squares of a thread < 2^(2 e + 7)
+  // |v| < 2^(e + 1): each chain, of even or of odd columns, adds N * 4 squares below 2^(2 e + 2), less than its base 2^(2 e + 7)
+  static_assert(N * 4 * 4 < 128, "a chain of squares must stay below its base");
   const int e = int(abs_bits(top) >> 23) - 127;
   if (e < -50 || e > 58) {  // far from everyday values: in 64 bits
     double sum = 0.0;

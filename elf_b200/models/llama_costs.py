@@ -74,7 +74,8 @@ def analytic_cost_model(cfg) -> LlamaCostModel:
     head = 0.65 * 2 * d * cfg.vocab / layer_flops
     if cfg.ffn_fp8:
         layer = 0.2 + 0.75 * 0.8
-        return LlamaCostModel(attention=0.2 / layer, mlp_up=0.75 * 0.55 / layer, mlp_down=0.75 * 0.25 / layer, head=head / layer, embed=0.05 / layer, fbw=(0.29, 0.38, 0.33))
+        up, down = 0.75 * 0.55 / layer, 0.75 * 0.25 / layer
+        return LlamaCostModel(attention=0.2 / layer, mlp_up=up, mlp_down=down, head=head / layer, embed=0.05 / layer, fbw=(0.29, 0.38, 0.33))
     return LlamaCostModel(attention=0.2, mlp_up=0.55, mlp_down=0.25, head=head, embed=0.05)
 
 

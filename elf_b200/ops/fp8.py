@@ -292,11 +292,14 @@ class _AddNorm(torch.autograd.Function):
     """``add_rms_norm`` as a node of the graph: the residual stream passes its gradient on to both terms."""
 
     @staticmethod
-    def forward(ctx, x, residual, w, eps):
+    def forward(x, residual, w, eps):
         q, rstd, h = _norm(x, residual, w, eps)
-        ctx.mark_non_differentiable(q.data, q.scale, rstd)
-        ctx.set_materialize_grads(False)
         return h, q.data, q.scale, rstd
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        ctx.mark_non_differentiable(*output[1:])
+        ctx.set_materialize_grads(False)
 
     @staticmethod
     def backward(ctx, dh, *_):
@@ -351,12 +354,14 @@ class _Biased(torch.autograd.Function):
     """``linear_forward`` as a node of the graph: its bias has a gradient, its 8-bit operands have none."""
 
     @staticmethod
-    def forward(ctx, bias, x, w, out_dtype):
-        ctx.dtype = bias.dtype
+    def forward(bias, x, w, out_dtype):
         return _product(x, w, False, bias, out_dtype)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    def setup_context(ctx, inputs, output):
+        ctx.dtype = inputs[0].dtype
+
+    @staticmethod
     def backward(ctx, dy):
         return _bias_grad(dy, ctx.dtype), None, None, None
 

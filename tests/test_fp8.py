@@ -232,8 +232,10 @@ def test_residual_stream_keeps_its_gradient(dtype):
     assert torch.equal(both.grad, dh + dh)
     with torch.no_grad():
         assert not fp8.add_rms_norm(x.requires_grad_(), r, w)[2].requires_grad
+    x.requires_grad_(False)
     with pytest.raises(NotImplementedError, match="forward-mode"):
-        torch.func.jvp(lambda t: fp8.add_rms_norm(t, r, w)[2], (x.detach(),), (dh,))
+        torch.func.jvp(lambda t: fp8.add_rms_norm(t, r, w)[2], (x,), (dh,))
+    assert torch.equal(torch.func.grad(lambda t: (fp8.add_rms_norm(t, r, w)[2] * dh).sum())(x), dh)
 
 
 @pytest.mark.parametrize("lead", [(7,), (2, 3), ()])
@@ -251,6 +253,8 @@ def test_bias_keeps_its_gradient(lead):
     assert ((bias.grad.double() - rows.sum(0)).abs() <= len(rows) * 2.0**-24 * rows.abs().sum(0)).all()
     with torch.no_grad():
         assert not fp8.linear_forward(x, w, bias).requires_grad
+    twice = torch.func.grad(lambda b: (fp8.linear_forward(x, w, b, torch.float32) * dy).sum())(bias.detach())
+    assert torch.equal(twice, bias.grad)
 
 
 # ------------------------------------------------------------------------------ split-backward layer
